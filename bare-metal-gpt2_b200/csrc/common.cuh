@@ -22,6 +22,12 @@ enum StatusBits : unsigned {
     ST_KV_BAD_POS = 1u << 9,               // device-side append position outside [0, maxT)
     ST_LINEAR_TIMEOUT = 1u << 11,          // a batched linear layer's stage wait gave up
     ST_MODEL_BAD_TOKEN = 1u << 12,         // a token id outside [0, vocab) reached the embedding
+    ST_KV8_BAD_LEN = 1u << 13,             // 8-bit cache: a length outside the table or the given bound
+    ST_KV8_BAD_PAGE = 1u << 14,            // 8-bit cache: a table entry in use that is no page
+    ST_KV8_NO_PAGE = 1u << 15,             // 8-bit cache: no free page, or a full table row
+    ST_KV8_NONFINITE = 1u << 17,           // 8-bit cache: a K/V value that is not finite was stored
+    ST_KV8_BAD_PARENT = 1u << 18,          // 8-bit cache: a parent outside -1..nRow-1
+    ST_BEAM_LOGIT = 1u << 19,              // beam selection: a NaN or +inf logit
     ST_TEST_WAIT_TIMEOUT = 1u << 16,       // the wait-timeout self-test expired (expected)
 };
 

@@ -29,10 +29,18 @@ ST_KV_BAD_POS = 1 << 9
 ST_DECODE_TIMEOUT = 1 << 10
 ST_LINEAR_TIMEOUT = 1 << 11
 ST_MODEL_BAD_TOKEN = 1 << 12
+ST_KV8_BAD_LEN = 1 << 13
+ST_KV8_BAD_PAGE = 1 << 14
+ST_KV8_NO_PAGE = 1 << 15
 ST_TEST_WAIT_TIMEOUT = 1 << 16
+ST_KV8_NONFINITE = 1 << 17
+ST_KV8_BAD_PARENT = 1 << 18
+ST_BEAM_LOGIT = 1 << 19
 
 LINEAR_STORE, LINEAR_GELU, LINEAR_RESID = 0, 1, 2
 GEN_ATTENTION_ONLY = 1
+KV8_KINDS = {"int8": 0, "e4m3": 1}
+BEAM_HALF, BEAM_FLOAT = 0, 1
 
 # GPT-2-124M (the reference's model/config.h).
 N_LAYER, N_HEAD, N_EMBD, VOCAB, N_CTX = 12, 12, 768, 50257, 1024
@@ -70,6 +78,15 @@ class GPT2Backend(ctypes.Structure):
     ]
 
 
+class GPT2KV8Cache(ctypes.Structure):
+    """The paged 8-bit cache descriptor of include/gpt2_b200.h."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("data", "scale", "ref", "table", "len", "work")] + [
+        ("work_bytes", ctypes.c_size_t)] + [
+        (n, ctypes.c_int) for n in ("nPages", "nRow", "maxPages", "nLayer", "nHead", "headDim", "page",
+                                    "block", "kind")]
+
+
 class GPT2LayerGPU(ctypes.Structure):
     """Same layout as GPT2LayerGPU in the reference's cuda/kernels.cuh:19-23."""
 
@@ -94,6 +111,8 @@ class GPT2WeightsGPU(ctypes.Structure):
 _vp, _ci, _cll, _cu, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_uint, ctypes.c_double
 _kvp = ctypes.POINTER(GPT2KVCache)
 _wp = ctypes.POINTER(GPT2WeightsGPU)
+_k8p = ctypes.POINTER(GPT2KV8Cache)
+_cs = ctypes.c_size_t
 _SIGS = {
     "gpt2_attention_b200": (None, [_vp, _vp, _ci, _ci, _ci, _ci]),
     "gpt2_attention_b200_stream": (_ci, [_vp, _vp, _ci, _ci, _ci, _ci, _vp]),
@@ -125,6 +144,19 @@ _SIGS = {
     "gpt2_b200_linear": (_ci, [_vp, _cll, _vp, _cll, _vp, _vp, _ci, _ci, _ci, _ci, _vp]),
     "gpt2_b200_linear_argmax": (_ci, [_vp, _cll, _vp, _cll, _vp, _ci, _ci, _ci, _vp, _vp]),
     "gpt2_gemv_b200": (None, [_vp, _vp, _vp, _vp, _ci, _ci]),
+    "gpt2_kv8_work_bytes_b200": (_cs, [_k8p, _ci, _ci]),
+    "gpt2_kv8_alloc_b200": (_ci, [_k8p, _ci, _ci]),
+    "gpt2_kv8_free_b200": (None, [_k8p]),
+    "gpt2_kv8_reset_b200": (_ci, [_k8p, _vp]),
+    "gpt2_kv8_store_b200": (_ci, [_k8p, _ci, _ci, _vp, _vp, _cll, _cll, _cll, _vp, _ci, _vp]),
+    "gpt2_kv8_load_b200": (_ci, [_k8p, _ci, _ci, _vp, _vp, _cll, _cll, _cll, _vp, _ci, _vp, _ci, _vp]),
+    "gpt2_kv8_attend_b200": (_ci, [_vp, _cll, _cll, _vp, _cll, _cll, _k8p, _ci, _ci, _ci, _vp, _vp, _ci,
+                                   _ci, _vp]),
+    "gpt2_kv8_reorder_b200": (_ci, [_k8p, _vp, _ci, _ci, _vp]),
+    "gpt2_kv8_compact_b200": (_ci, [_k8p, _vp, _vp]),
+    "gpt2_beam_work_bytes_b200": (_cs, [_ci, _ci]),
+    "gpt2_beam_select_b200": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _cll, _vp, _vp, _ci, _ci, _ci, _ci, _vp,
+                                    _cs, _vp]),
     "gpt2_b200_compose_backend": (None, [ctypes.POINTER(GPT2Backend), ctypes.POINTER(GPT2Backend)]),
     "gpt2_b200_reserve": (_ci, [_ci, _ci, _ci]),
     "gpt2_b200_status": (_cu, [_ci]),
@@ -186,6 +218,23 @@ class Lib:
             d_len.data_ptr() if d_len is not None else None, length, max_len, stream)
         self.check(rc, "gpt2_attn_decode_b200_layers")
 
+    def beam_work(self, torch, B: int, W: int, device):
+        """The zeroed scratch of beam_select for B items of W beams."""
+        return torch.zeros(self.lib.gpt2_beam_work_bytes_b200(B, W), dtype=torch.uint8, device=device)
+
+    def beam_select(self, token, parent, new_score, new_done, logits, score, done, B: int, W: int,
+                    eos: int, work, stream: int = 0) -> None:
+        """The W best continuations of each of B items' W beams: logits [B*W][V] fp16 or fp32 (rows may be
+        strided), score fp32 [B*W], done int32 [B*W] or None; writes token and parent (int32), new_score
+        and new_done (may be score and done; new_done may be None)."""
+        if logits.dtype not in _beam_types() or logits.stride(1) != 1:
+            raise ValueError("beam_select: logits are fp16 or fp32 rows of neighbouring values")
+        rc = self.lib.gpt2_beam_select_b200(
+            token.data_ptr(), parent.data_ptr(), new_score.data_ptr(), _ptr(new_done), logits.data_ptr(),
+            _beam_types()[logits.dtype], logits.stride(0), score.data_ptr(), _ptr(done), B, W,
+            logits.shape[1], eos, work.data_ptr(), work.numel(), stream)
+        self.check(rc, "gpt2_beam_select_b200")
+
     def status(self, clear: bool = True) -> int:
         """The device's status word (bounded-wait timeouts and bad-input bits), cleared if asked."""
         return int(self.lib.gpt2_b200_status(1 if clear else 0))
@@ -203,6 +252,104 @@ def cache_view(data_ptr: int, n_layer: int, max_t: int, n_head: int = 12, head_d
     kv.bytes = 2 * n_layer * n_head * max_t * head_dim * 2
     kv.len = length
     return kv
+
+
+class KV8Cache:
+    """A paged 8-bit KV cache over torch tensors (GPT2KV8Cache and the gpt2_kv8_* entry points).
+
+    data uint8 [pages][layers][2][heads][page][dim], scale fp32 [pages][layers][2][heads][page/block], ref
+    int32 [pages], table int32 [rows][max pages], length int32 [rows]; the tensors stay alive with the
+    cache. q_heads and queries bound what attend() may be called with. create() makes an empty one.
+    """
+
+    def __init__(self, lib: "Lib", torch, data, scale, ref, table, length, kind: str = "int8",
+                 q_heads: int = 0, queries: int = 1):
+        self.lib, self.kind = lib, kind
+        n_pages, n_layer, two, n_head, page, dim = data.shape
+        shapes = (tuple(scale.shape[:4]) == (n_pages, n_layer, 2, n_head) and two == 2
+                  and page % max(1, scale.shape[4]) == 0 and tuple(ref.shape) == (n_pages,)
+                  and tuple(length.shape) == (table.shape[0],))
+        types = (data.dtype == torch.uint8 and scale.dtype == torch.float32
+                 and ref.dtype == table.dtype == length.dtype == torch.int32)
+        if not shapes or not types or not all(t.is_contiguous() for t in (data, scale, ref, table, length)):
+            raise ValueError("KV8Cache: data, scale, ref, table or length has another shape, type or layout")
+        self.data, self.scale, self.ref, self.table, self.length = data, scale, ref, table, length
+        c = GPT2KV8Cache()
+        c.data, c.scale, c.ref = data.data_ptr(), scale.data_ptr(), ref.data_ptr()
+        c.table, c.len = table.data_ptr(), length.data_ptr()
+        c.nPages, c.nLayer, c.nHead, c.headDim, c.page = n_pages, n_layer, n_head, dim, page
+        c.nRow, c.maxPages = table.shape
+        c.block, c.kind = page // max(1, scale.shape[4]), KV8_KINDS[kind]
+        n = lib.gpt2_kv8_work_bytes_b200(ctypes.byref(c), q_heads or n_head, queries)
+        if not n:
+            raise ValueError("KV8Cache: a shape outside the supported ones")
+        self.work = torch.zeros(n, dtype=torch.uint8, device=data.device)
+        c.work, c.work_bytes = self.work.data_ptr(), n
+        self.c, self.ref_c = c, ctypes.byref(c)
+
+    @classmethod
+    def create(cls, lib: "Lib", torch, rows: int, max_pages: int, pages: int, layers: int = N_LAYER,
+               heads: int = N_HEAD, dim: int = 64, page: int = 16, block: int = 16, kind: str = "int8",
+               q_heads: int = 0, queries: int = 1, device="cuda") -> "KV8Cache":
+        """An empty cache: every page free, every row without positions."""
+        z = dict(device=device, dtype=torch.int32)
+        return cls(lib, torch, torch.zeros(pages, layers, 2, heads, page, dim, device=device, dtype=torch.uint8),
+                   torch.zeros(pages, layers, 2, heads, page // block, device=device),
+                   torch.zeros(pages, **z), torch.full((rows, max_pages), -1, **z), torch.zeros(rows, **z),
+                   kind, q_heads, queries)
+
+    def _rows(self, what, k, v):
+        if k.stride() != v.stride() or k.shape != v.shape or k.dim() != 4 or k.stride(3) != 1 or \
+                k.shape[1] != self.c.nRow or k.shape[3] != self.c.nHead * self.c.headDim or \
+                k.element_size() != 2 or not k.dtype.is_floating_point:
+            raise ValueError(f"{what}: k and v are fp16 [layers][rows][tokens][heads * dim], laid out alike")
+
+    def store(self, k, v, layer: int = 0, count=None, stream: int = 0) -> None:
+        """k, v: fp16 [layers][rows][tokens][heads * dim] (strided views are fine), written behind the
+        held positions from `layer` on; count: int32 [rows] or None (all tokens)."""
+        self._rows("store", k, v)
+        s = k.stride()
+        self.lib.check(self.lib.gpt2_kv8_store_b200(
+            self.ref_c, layer, k.shape[0], k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], _ptr(count),
+            k.shape[2], stream), "gpt2_kv8_store_b200")
+
+    def load(self, k, v, layer: int = 0, first=None, count=None, stream: int = 0) -> None:
+        """The inverse: positions first[r].. (0 without first) as fp16 rows, 0 beyond the held ones;
+        count: int32 [rows], an int or None: positions stored but not yet counted in."""
+        self._rows("load", k, v)
+        s = k.stride()
+        n = count if isinstance(count, int) else 0
+        self.lib.check(self.lib.gpt2_kv8_load_b200(
+            self.ref_c, layer, k.shape[0], k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], _ptr(first),
+            k.shape[2], None if isinstance(count, int) else _ptr(count), n, stream), "gpt2_kv8_load_b200")
+
+    def attend(self, out, q, layer: int = 0, count=None, first=None, max_len: int = 0,
+               stream: int = 0) -> None:
+        """q, out: fp16 [rows][queries][q heads * dim]: causal attention of each row's last positions over
+        its keys, counted as load() counts them; keys before first[r] are masked."""
+        if q.shape != out.shape or q.dim() != 3 or q.shape[0] != self.c.nRow or q.stride(2) != 1 or \
+                out.stride(2) != 1 or q.shape[2] % self.c.headDim or q.element_size() != 2:
+            raise ValueError("attend: q and out are fp16 [rows][queries][q heads * dim]")
+        n = count if isinstance(count, int) else 0
+        self.lib.check(self.lib.gpt2_kv8_attend_b200(
+            out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), self.ref_c,
+            layer, q.shape[2] // self.c.headDim, q.shape[1], _ptr(first),
+            None if isinstance(count, int) else _ptr(count), n, max_len, stream), "gpt2_kv8_attend_b200")
+
+    def reorder(self, parent=None, advance: int = 0, reserve: int = 0, stream: int = 0) -> None:
+        """Counts `advance` positions in, makes row r a copy of row parent[r] (int32 [rows]; -1: empty; None:
+        itself) by sharing pages, and makes room for `reserve` more positions."""
+        self.lib.check(self.lib.gpt2_kv8_reorder_b200(self.ref_c, _ptr(parent), advance, reserve, stream),
+                       "gpt2_kv8_reorder_b200")
+
+    def compact(self, live=None, stream: int = 0) -> None:
+        """Moves the live pages to the lowest ids; live: int32 [1] for their number, or None."""
+        self.lib.check(self.lib.gpt2_kv8_compact_b200(self.ref_c, _ptr(live), stream),
+                       "gpt2_kv8_compact_b200")
+
+    def reset(self, stream: int = 0) -> None:
+        """Every page free, every row empty."""
+        self.lib.check(self.lib.gpt2_kv8_reset_b200(self.ref_c, stream), "gpt2_kv8_reset_b200")
 
 
 class ModelWeights:
@@ -297,6 +444,21 @@ class DecodeBatch:
             self.close()
         except Exception:  # noqa: BLE001 - interpreter shutdown
             pass
+
+
+def _ptr(t):
+    """A tensor's device pointer, None for None."""
+    return t.data_ptr() if t is not None else None
+
+
+_TYPES: dict = {}
+
+
+def _beam_types() -> dict:
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float16: BEAM_HALF, torch.float32: BEAM_FLOAT})
+    return _TYPES
 
 
 def _numel(shape) -> int:

@@ -288,6 +288,103 @@ void gpt2_gemv_b200(gpt2_half *C, const gpt2_half *A, const gpt2_half *W, const 
 /* Kernel launches one gpt2_b200_batch_step / one generate step makes (launch accounting). */
 int gpt2_b200_batch_launches_per_step(const gpt2_b200_batch *bt, int flags);
 
+/* ================================================================ beam search over a paged 8-bit cache
+ * Additive extension (the reference decodes one sequence greedily over one fp16 arena). Sequences, or
+ * the beams of a search, hold their K/V in pages of `page` positions that rows can share:
+ *   data  : codes, [nPages][nLayer][K|V][nHead][page][headDim] bytes, so one page of all layers is one
+ *           contiguous run;
+ *   scale : fp32, [nPages][nLayer][K|V][nHead][page/block], one per block of `block` positions and head:
+ *           value = code * scale. kind GPT2_KV8_INT8: codes -127..127; GPT2_KV8_E4M3: e4m3 codes, at
+ *           most 448 in magnitude;
+ *   table : [nRow][maxPages], the page of positions i*page .. i*page + page-1 of each row, -1 = none;
+ *   len   : [nRow], positions held;
+ *   ref   : [nPages], how many table entries name the page (0 = free). A caller that pins pages adds
+ *           its own holds here.
+ *   work  : scratch of at least gpt2_kv8_work_bytes_b200, zeroed once by the owner (gpt2_kv8_alloc_b200 and
+ *           _reset_b200 do); the calls leave its counters at zero.
+ * All six are device pointers, data / scale / ref / table / len / work 16-byte aligned. headDim is 64 or 128, page and
+ * block are 16, 32, 64 or 128 with block <= page, nRow 1..1024. The calls read and write this state and
+ * its work area, so calls on one cache must be ordered on the GPU (one stream, or events); calls on
+ * different caches are independent. No call allocates or synchronises, so all may be captured.
+ * What the device finds wrong (a length outside the table, an entry that is no page, no free page, a
+ * parent outside -1..nRow-1, a K/V value or logit that is not finite) sets bits of gpt2_b200_status(). */
+#define GPT2_KV8_INT8 0
+#define GPT2_KV8_E4M3 1
+typedef struct {
+    void *data;
+    float *scale;
+    int *ref, *table, *len;
+    void *work;
+    size_t work_bytes;
+    int nPages, nRow, maxPages, nLayer, nHead, headDim, page, block, kind;
+} GPT2KV8Cache;
+
+/* Scratch bytes of a cache of this shape whose gpt2_kv8_attend_b200 calls have at most Hq query heads and
+ * Tq queries per row (0 for a bad shape; the pointers are not looked at). */
+size_t gpt2_kv8_work_bytes_b200(const GPT2KV8Cache *kv, int Hq, int Tq);
+/* Allocates all six arrays for the shape fields set in *kv, as gpt2_kv_alloc_b200 does (refused, 1, when
+ * < 64 MiB would stay free; 0 = ok), and resets the cache. */
+int gpt2_kv8_alloc_b200(GPT2KV8Cache *kv, int Hq, int Tq);
+void gpt2_kv8_free_b200(GPT2KV8Cache *kv);
+/* Every page free, every row empty, work area zeroed. */
+int gpt2_kv8_reset_b200(const GPT2KV8Cache *kv, cudaStream_t stream);
+
+/* Writes K and V rows of layers L0 .. L0+nL-1 behind the positions each row holds: row r, token t <
+ * count_r, goes to position len[r] + t, from k + l*layer_stride + r*row_stride + t*tok_stride (halves; v
+ * likewise; head h at h*headDim), where count_r = min(d_count[r], T) if d_count, else T. The pages must be there
+ * (gpt2_kv8_reorder_b200's reserve). A block's scale s becomes max(s_old, amax/qmax) (s_old if the block
+ * held positions before), the codes round(x * (1/s)) to nearest even; where s grew, the block's older codes become
+ * round(code * (s_old/s)). NaN is stored as 0, infinities as the largest fp16 (status bit). len is not
+ * changed: gpt2_kv8_reorder_b200's advance counts the tokens in once all layers have stored them. */
+int gpt2_kv8_store_b200(const GPT2KV8Cache *kv, int L0, int nL, const gpt2_half *k, const gpt2_half *v,
+                        long long layer_stride, long long row_stride, long long tok_stride,
+                        const int *d_count, int T, cudaStream_t stream);
+/* Reads positions first_r .. first_r + T-1 of each row back as fp16 (code * scale, rounded once), to the
+ * same kind of rows; first_r = d_first[r], 0 without d_first. Positions outside 0 .. len[r] + count_r - 1
+ * (stored but not yet counted in: count_r = d_count[r], or count) give 0. */
+int gpt2_kv8_load_b200(const GPT2KV8Cache *kv, int L0, int nL, gpt2_half *k, gpt2_half *v,
+                       long long layer_stride, long long row_stride, long long tok_stride,
+                       const int *d_first, int T, const int *d_count, int count, cudaStream_t stream);
+
+/* Attention over layer L: row r has n = len[r] + count_r keys (count_r as above: the tokens stored in this
+ * step) and its Tq queries are its last positions n-Tq .. n-1; query i sees keys first_r .. n-Tq+i
+ * (d_first NULL: from 0). out = softmax(q K^T / sqrt(headDim)) V, fp32 accumulation, one rounding; a query
+ * that sees no key gives 0. Hq query heads, head h reads K/V head h / (Hq/nHead). q and out: head h at
+ * h*headDim, row r at r*row_stride, query t at t*tok_stride (halves, multiples of 8). max_len bounds n (0 =
+ * the table's capacity) and sizes the split; a row with n outside 0..max_len sets a status bit and gives 0. */
+int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, long long out_tok_stride,
+                         const gpt2_half *q, long long q_row_stride, long long q_tok_stride,
+                         const GPT2KV8Cache *kv, int L, int Hq, int Tq, const int *d_first,
+                         const int *d_count, int count, int max_len, cudaStream_t stream);
+
+/* The state behind a selection. First every row counts in `advance` positions; then row r becomes a copy of
+ * what row parent[r] held (parent NULL: itself; -1: empty) by holding the same pages; then each row gets room
+ * for `reserve` more positions: a partly filled last page that another holder has too is copied to a new
+ * page (its filled part), unless this row is the last in row order that is left with it; the missing pages are added.
+ * New pages are the lowest-numbered free ones, handed out in row order, a row's copy first. Pages no row holds any more are
+ * free. Without enough pages the entry is -1 (status bit). */
+int gpt2_kv8_reorder_b200(const GPT2KV8Cache *kv, const int *parent, int advance, int reserve,
+                          cudaStream_t stream);
+/* Moves the live pages (ref > 0) to the ids 0 .. live-1: the free ids below live, in ascending order, take the live pages
+ * at or above it, in ascending order. Tables and ref follow; *d_live (if not NULL) receives the number of live pages. */
+int gpt2_kv8_compact_b200(const GPT2KV8Cache *kv, int *d_live, cudaStream_t stream);
+
+/* Beam selection. logits: [B*W][ld] of V values, type GPT2_BEAM_HALF or GPT2_BEAM_FLOAT; score [B*W] the beams' log
+ * probabilities so far (-inf: a beam that does not exist, e.g. all but one at the first step); done [B*W] (NULL: none)
+ * marks finished beams. Candidate (w, token) of item b has score[w] + logit - logsumexp(row), a finished beam is
+ * one candidate (w, eos) with its score unchanged; the W largest per item are chosen, equal totals by the lower w, then the
+ * lower token. -inf logits are masked tokens; NaN and +inf set a status bit and count as masked. Outputs, best first: token,
+ * parent (row index b*W + w, as gpt2_kv8_reorder_b200 takes it), new_score, new_done (NULL: not written) = finished
+ * before, or token == eos (eos < 0: none). Where fewer than W candidates exist the rest is a dead beam: token max(eos, 0),
+ * parent its own row, score -inf, done 1. new_score / new_done may be score / done. W 1..32. work: gpt2_beam_work_bytes_b200,
+ * zeroed once by its owner; calls that share it must be ordered. */
+#define GPT2_BEAM_HALF 0
+#define GPT2_BEAM_FLOAT 1
+size_t gpt2_beam_work_bytes_b200(int B, int W);
+int gpt2_beam_select_b200(int *token, int *parent, float *new_score, int *new_done, const void *logits,
+                          int type, long long ld, const float *score, const int *done, int B, int W,
+                          int V, int eos, void *work, size_t work_bytes, cudaStream_t stream);
+
 /* ================================================================ backend, status, set-up */
 
 /* Composes a backend the reference's way (cuda/kernels_fused.cu:157-164): copies *base and installs
