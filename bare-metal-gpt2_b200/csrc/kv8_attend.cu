@@ -1,96 +1,475 @@
 // kv8_attend.cu — attention over the paged 8-bit cache.
 //
-// out = softmax(q K^T / sqrt(D)) V with K = code * scale per block: a block's scale is constant over
-// its keys, so it multiplies the score of a key (K) and the probability (V) instead of every element.
-// Online softmax in base 2: m, l and o are rescaled by 2^(m_old - m_new) per tile of keys.
+// out = softmax(q K^T / sqrt(D)) V with K = code * scale per block of keys: the scale is constant over a
+// block, so it multiplies a key's score (K) and its probability (V), never the D elements. Online
+// softmax in base 2: m, l and o are rescaled by 2^(m_old - m_new) when a row's maximum grows.
 //
-// One warp per (row, query head, query): 32 keys a step, one key per lane for the scores, then D/32
-// output dims per lane over the 32 probabilities.
+// A decode step reads 2 D + 8 / block bytes per key and K/V head once and does 4 D flops per key and query:
+// HBM-bound, if the codes get into the tensor cores cheaply. So:
+//   - the products are mma.m16n8k16 in fp16 with fp32 sums. A code is exact in fp16 and so is q; p is not, and goes
+//     in as hi + lo (two fp16, 22 bits): rounding it to one fp16 alone would add an error of the size of the
+//     output's own rounding. With at most 8 query rows (the decode step) the MMA's rows 8..15 are
+//     free and take lo; with 9 to 16 rows lo is a second MMA. mma.sync's rate is far above what HBM feeds
+//     (32 MMAs per 4 KB of codes), and its operands come from registers: no staging through shared memory, no barriers.
+//   - a warp takes CK keys at a time (32 for D 64, 16 for D 128: 4 KB of K and V), loaded straight into the operand
+//     layout by 16- and 8-byte loads. The sum over dims (QK) may run in any order of dims, so a thread's 16
+//     neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its column order are as
+//     free, so a thread loads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with 16 neighbouring
+//     output dims. The next chunk's loads are in flight while a chunk is computed.
+//   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
+//     shuffles hand them out.
+//   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
+//     vscale the warp has met; o is kept in units of S.
+// A CTA is 4 warps on one (row, K/V head, tile of 16 query rows, span of keys): the warps take chunks in turn and are
+// merged in shared memory; spans (few rows, long contexts) through the work area by the last CTA to arrive, in span order.
 #include "kv8.cuh"
+#include "ptx.cuh"
 
 namespace b200 {
 namespace kv8 {
 
-int attend_max_ctas() { return 2048; }
+constexpr int NW = 4;                // warps per CTA
+constexpr int MAX_SPLIT_CTAS = 2048; // grid of a launch that splits keys, at most
+
+int attend_max_ctas() { return MAX_SPLIT_CTAS; }
 
 struct AttParams {
     const __half *q;
     __half *out;
     long long q_row, q_tok, o_row, o_tok;
     const int *d_first, *d_count;
-    int L, Hq, Tq, count, max_len;
+    long long page_stride;  // bytes from a page to the next
+    long long k_off, v_off; // from a page's start to this layer's K / V runs of head 0
+    float *part;
+    unsigned *arrive;
+    int L, G, Tq, count, max_len;
+    int qtiles, nsplit, span;  // span: keys per split, a multiple of NW * CK
     float scale_log2;
 };
 
-template <int KIND, int D>
-__global__ void __launch_bounds__(128) k_kv8_attend(const View c, const AttParams a) {
-    const int lane = threadIdx.x & 31;
-    const long long w = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (w >= static_cast<long long>(c.nRow) * a.Hq * a.Tq) return;
-    const int t = static_cast<int>(w % a.Tq), hq = static_cast<int>(w / a.Tq % a.Hq), r = static_cast<int>(w / a.Tq / a.Hq);
-    const int h = hq / (a.Hq / c.nHead);
-    __shared__ float qs[4][D];
-    float *q = qs[threadIdx.x >> 5];
-    const __half *qp = a.q + r * a.q_row + t * a.q_tok + static_cast<long long>(hq) * D;
-    for (int d = lane; d < D; d += 32) q[d] = __half2float(qp[d]) * a.scale_log2;
-    __syncwarp();
-    const int n = c.len[r] + (a.d_count ? a.d_count[r] : a.count);
-    int first = a.d_first ? max(a.d_first[r], 0) : 0;
-    int end = n - a.Tq + t + 1;  // keys [first, end)
-    if (n < 0 || n > a.max_len) {
-        if (lane == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
-        end = 0;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+// Two int8 codes (as code + 128) in bytes 0, 2 over 0x64 bytes are the halves 1024 + code + 128: exact.
+__device__ __forceinline__ uint32_t sub1152(uint32_t h) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t two) {
+    uint32_t r;
+    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+// Four neighbouring codes -> their halves, as two packed pairs.
+template <int KIND>
+__device__ __forceinline__ void halves4(uint32_t w, uint32_t &h01, uint32_t &h23) {
+    if (KIND == GPT2_KV8_INT8) {
+        const uint32_t u = w ^ 0x80808080u;
+        h01 = sub1152(__byte_perm(u, 0x64646464u, 0x4140));
+        h23 = sub1152(__byte_perm(u, 0x64646464u, 0x4342));
+    } else {
+        h01 = e4m3x2(w);
+        h23 = e4m3x2(w >> 16);
     }
-    float m = -INFINITY, l = 0.0f, o[D / 32] = {};
-    for (int j0 = first & ~31; j0 < end; j0 += 32) {
-        const int j = j0 + lane;
-        float s = -INFINITY, vs = 0.0f;
-        long long vrow = 0;
-        if (j >= first && j < end) {
-            const int p = c.table[static_cast<long long>(r) * c.maxPages + (j >> c.page_shift)];
-            if (p >= 0 && p < c.nPages) {
-                const int ip = j & (c.page - 1), nb = c.page >> c.block_shift;
-                const long long run = c.run(p, a.L, 0, h), vrun = run + c.nHead;
-                const uint8_t *kp = c.data + ((run << c.page_shift) + ip) * D;
-                float acc = 0.0f;
-                for (int d = 0; d < D; d += 4) {
-                    const unsigned x = *reinterpret_cast<const unsigned *>(kp + d);
+}
+// Codes of the same four dims of two keys -> per dim the pair (key a, key b).
+template <int KIND>
+__device__ __forceinline__ void pairs4(uint32_t a, uint32_t b, uint32_t (&h)[4]) {
+    halves4<KIND>(__byte_perm(a, b, 0x5140), h[0], h[1]);
+    halves4<KIND>(__byte_perm(a, b, 0x7362), h[2], h[3]);
+}
+__device__ __forceinline__ uint32_t pack_hi(float a, float b, float &la, float &lb) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    la = a - f.x;
+    lb = b - f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// One warp's chunk of CK keys: K for 8-key tiles, V for the 4 keys of each 16-key granule a thread holds p of.
+template <int D>
+struct Chunk {
+    static constexpr int CK = 2048 / D, GR = CK / 16;
+    uint4 k[4];
+    uint2 v[8];  // D 64: [granule][key] 8 dims; D 128: [key][half] 16 dims
+};
+
+template <int KIND, int D, int ROWS>
+__global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_attend(const View c, const AttParams a) {
+    using C = Chunk<D>;
+    constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
+    constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
+    __shared__ float so[NW][ROWS][D + 4];
+    __shared__ float sm[NW][ROWS], sl[NW][ROWS];
+    __shared__ int is_last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % a.nsplit;
+    int unit = blockIdx.x / a.nsplit;
+    const int h = unit % c.nHead;
+    unit /= c.nHead;
+    const int qt = unit % a.qtiles, r = unit / a.qtiles;
+    const int R = a.G * a.Tq;
+
+    int n = c.len[r] + (a.d_count ? a.d_count[r] : a.count);
+    if (n < 0 || n > a.max_len) {
+        if (threadIdx.x == 0 && split == 0 && h == 0 && qt == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
+        n = 0;
+    }
+    const int first = a.d_first ? max(a.d_first[r], 0) : 0;
+    // keys that some row of the tile sees: [first, last_end); rows of one token see the same
+    const int last_row = min(qt * ROWS + ROWS, R) - 1;
+    const int last_end = n - a.Tq + last_row / a.G + 1, first_end = n - a.Tq + qt * ROWS / a.G + 1;
+    const int base = first & ~(CK - 1);
+    const int total = last_end > first ? last_end - base : 0;
+    const int active = (total + a.span - 1) / a.span;  // splits with keys
+    if (split >= max(active, 1)) return;
+    const int lo = base + split * a.span, hi = min(lo + a.span, last_end);
+    const int chunks = total ? (hi - lo + CK - 1) / CK : 0;
+
+    // q: thread (g, t) holds dims 64 * (s / 4) + 16 t + 4 (s % 4) .. + 3 of row g (and g + 8) for k-step s
+    uint32_t qa[KS][2 * RR];
+    int end[RR];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc = fmaf(q[d + i], decode<KIND>((x >> (8 * i)) & 0xFFu), acc);
-                }
-                s = acc * c.scale[run * nb + (ip >> c.block_shift)];
-                vs = c.scale[vrun * nb + (ip >> c.block_shift)];
-                vrow = ((vrun << c.page_shift) + ip) * D;
-            } else {
-                atomicOr(c.status, ST_KV8_BAD_PAGE);
+    for (int rr = 0; rr < RR; ++rr) {
+        const int i = qt * ROWS + g + 8 * rr;
+        const bool ok = i < R;
+        const int tok = ok ? i / a.G : 0;
+        end[rr] = ok ? n - a.Tq + tok + 1 : 0;
+        const __half *qp = a.q + r * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + 16 * t;
+#pragma unroll
+        for (int s4 = 0; s4 < KS / 4; ++s4) {
+            uint4 x[2] = {};
+            if (ok) {
+                x[0] = *reinterpret_cast<const uint4 *>(qp + 64 * s4);
+                x[1] = *reinterpret_cast<const uint4 *>(qp + 64 * s4 + 8);
+            }
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(x);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                qa[4 * s4 + s][rr] = w[2 * s];
+                qa[4 * s4 + s][RR + rr] = w[2 * s + 1];
             }
         }
-        float top = s;
+    }
+
+    float o[DT][4];
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-        if (top == -INFINITY) continue;
-        const float mn = fmaxf(m, top), f = exp2f(m - mn);
-        const float p = exp2f(s - mn);
-        m = mn;
-        float sum = p;
+    for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[RR], l[RR], S = 0.0f, invS = 0.0f;
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-        l = l * f + sum;
+    for (int rr = 0; rr < RR; ++rr) m[rr] = -INFINITY, l[rr] = 0.0f;
+
+    // this lane's granule of the current set: its page's byte offset and its scales
+    long long goff = 0;
+    float gks = 0.0f, gvs = 0.0f;
+    unsigned gok = 0;
+    bool bad = false;
+    auto look_up = [&](int set) {
+        const int pos = lo + ((set * SET + lane / GR) * NW + warp) * CK + (lane % GR) * 16;
+        int ok = pos < hi && pos + 16 > first;
+        if (ok) {
+            const int p = c.table[static_cast<long long>(r) * c.maxPages + (pos >> c.page_shift)];
+            if (p < 0 || p >= c.nPages) {
+                bad = true;
+                ok = 0;
+            } else {
+                const int ip = pos & (c.page - 1), nb = c.page >> c.block_shift;
+                const long long run = c.run(p, a.L, 0, h);
+                gks = c.scale[run * nb + (ip >> c.block_shift)] * a.scale_log2;
+                gvs = c.scale[(run + c.nHead) * nb + (ip >> c.block_shift)];
+                goff = p * a.page_stride + static_cast<long long>(h << c.page_shift) * D + ip * D;
+            }
+        }
+        if (!ok) gks = gvs = 0.0f;
+        gok = __ballot_sync(0xFFFFFFFFu, ok);
+    };
+    const uint8_t *kbase = c.data + a.k_off + g * D + 16 * t;
+    const uint8_t *vbase = c.data + a.v_off + 2 * t * D + g * (D / 8);
+    auto load = [&](C &x, int i) {  // chunk i of the set
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] *= f;
-        const float pv = p * vs;
-        for (int jj = 0; jj < 32; ++jj) {
-            const float pj = __shfl_sync(0xFFFFFFFFu, pv, jj);
-            const long long row = __shfl_sync(0xFFFFFFFFu, vrow, jj);
-            if (__shfl_sync(0xFFFFFFFFu, s, jj) == -INFINITY) continue;
+        for (int gi = 0; gi < GR; ++gi) {
+            const long long off = __shfl_sync(0xFFFFFFFFu, goff, i * GR + gi);
+            const bool ok = (gok >> (i * GR + gi)) & 1u;
+            const uint8_t *kp = kbase + off, *vp = vbase + off;
+            if (D == 64) {
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] = fmaf(pj, decode<KIND>(c.data[row + lane + 32 * i]), o[i]);
+                for (int tile = 0; tile < 2; ++tile)
+                    x.k[2 * gi + tile] = ok ? ldg16(kp + 8 * tile * D) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int row = (y & 1) + (y >> 1) * 8;
+                    x.v[4 * gi + y] = ok ? ldg8(vp + row * D) : make_uint2(0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        x.k[2 * tile + hh] = ok ? ldg16(kp + 8 * tile * D + 64 * hh) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int row = (y & 1) + (y >> 1) * 8;
+                    const uint4 w = ok ? ldg16(vp + row * D) : make_uint4(0, 0, 0, 0);
+                    x.v[2 * y] = make_uint2(w.x, w.y);
+                    x.v[2 * y + 1] = make_uint2(w.z, w.w);
+                }
+            }
+        }
+    };
+    auto compute = [&](C &x, int i, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+        float s[NT][4];
+#pragma unroll
+        for (int tile = 0; tile < NT; ++tile) {
+            s[tile][0] = s[tile][1] = s[tile][2] = s[tile][3] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                const uint4 &kw = D == 64 ? x.k[tile] : x.k[2 * tile + st / 4];
+                const uint32_t w = st % 4 == 0 ? kw.x : st % 4 == 1 ? kw.y : st % 4 == 2 ? kw.z : kw.w;
+                uint32_t b0, b1;
+                halves4<KIND>(w, b0, b1);
+                if (ROWS == 8)
+                    mma16816(s[tile], qa[st][0], qa[st][0], qa[st][1], qa[st][1], b0, b1);
+                else
+                    mma16816(s[tile], qa[st][0], qa[st][RR - 1], qa[st][RR], qa[st][2 * RR - 1], b0, b1);
+            }
+        }
+        const bool masked = pos < first || pos + CK > min(first_end, last_end) || ok != (1u << GR) - 1u;
+#pragma unroll
+        for (int tile = 0; tile < NT; ++tile)
+#pragma unroll
+            for (int e = 0; e < 2 * RR; ++e) s[tile][e] *= ks[tile / 2];
+        if (masked) {
+#pragma unroll
+            for (int tile = 0; tile < NT; ++tile)
+#pragma unroll
+                for (int e = 0; e < 2 * RR; ++e) {
+                    const int key = pos + 8 * tile + 2 * t + (e & 1);
+                    if (key < first || key >= end[e >> 1] || !((ok >> (tile / 2)) & 1u)) s[tile][e] = -INFINITY;
+                }
+            if (KIND == GPT2_KV8_E4M3) {  // a code behind the last key may be NaN, and 0 * NaN is not 0
+#pragma unroll
+                for (int y = 0; y < 4 * GR; ++y)
+                    if (pos + 16 * (y / 4) + 2 * t + (y & 1) + ((y >> 1) & 1) * 8 >= n) {
+                        if (D == 64)
+                            x.v[y] = make_uint2(0, 0);
+                        else
+                            x.v[2 * y] = x.v[2 * y + 1] = make_uint2(0, 0);
+                    }
+            }
+        }
+        float ms[RR];
+        bool grew = false;
+#pragma unroll
+        for (int rr = 0; rr < RR; ++rr) {
+            float top = s[0][2 * rr];
+#pragma unroll
+            for (int tile = 0; tile < NT; ++tile) top = fmaxf(top, fmaxf(s[tile][2 * rr], s[tile][2 * rr + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            ms[rr] = fmaxf(m[rr], top);
+            grew |= ms[rr] > m[rr];
+        }
+        float vmax = vs[0];
+#pragma unroll
+        for (int gi = 1; gi < GR; ++gi) vmax = fmaxf(vmax, vs[gi]);
+        if (__any_sync(0xFFFFFFFFu, grew) || vmax > S) {
+            const float Sn = fmaxf(S, vmax), fs = Sn > 0.0f ? S / Sn : 0.0f;
+            float f[RR];
+#pragma unroll
+            for (int rr = 0; rr < RR; ++rr) {
+                f[rr] = ms[rr] > -INFINITY ? ex2(m[rr] - ms[rr]) : 0.0f;
+                l[rr] *= f[rr];
+                m[rr] = ms[rr];
+            }
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] *= f[RR == 1 ? 0 : e >> 1] * fs;
+            S = Sn;
+            invS = Sn > 0.0f ? 1.0f / Sn : 0.0f;
+        }
+        float mm[RR];
+#pragma unroll
+        for (int rr = 0; rr < RR; ++rr) mm[rr] = m[rr] > -INFINITY ? m[rr] : 0.0f;
+#pragma unroll
+        for (int gi = 0; gi < GR; ++gi) {
+            const float w = vs[gi] * invS;
+            uint32_t ph[2 * RR], pl[2 * RR];  // [tile of the granule * RR + rr]
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                for (int rr = 0; rr < RR; ++rr) {
+                    float p0 = ex2(s[2 * gi + tile][2 * rr] - mm[rr]), p1 = ex2(s[2 * gi + tile][2 * rr + 1] - mm[rr]);
+                    l[rr] += p0 + p1;
+                    p0 *= w;
+                    p1 *= w;
+                    float l0, l1;
+                    ph[tile * RR + rr] = pack_hi(p0, p1, l0, l1);
+                    pl[tile * RR + rr] = pack(l0, l1);
+                }
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {  // 4 dims: column tiles 4 q .. 4 q + 3
+                uint32_t wk[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const uint2 vv = D == 64 ? x.v[4 * gi + y] : x.v[2 * y + q / 2];
+                    wk[y] = q & 1 ? vv.y : vv.x;
+                }
+                uint32_t b0[4], b1[4];
+                pairs4<KIND>(wk[0], wk[1], b0);
+                pairs4<KIND>(wk[2], wk[3], b1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (ROWS == 8) {
+                        mma16816(o[4 * q + j], ph[0], pl[0], ph[RR], pl[RR], b0[j], b1[j]);
+                    } else {
+                        mma16816(o[4 * q + j], ph[0], ph[RR - 1], ph[RR], ph[2 * RR - 1], b0[j], b1[j]);
+                        mma16816(o[4 * q + j], pl[0], pl[RR - 1], pl[RR], pl[2 * RR - 1], b0[j], b1[j]);
+                    }
+                }
+            }
+        }
+    };
+
+    const int mine = chunks > warp ? (chunks - warp + NW - 1) / NW : 0;  // chunks warp, warp + NW, ...
+    C buf[2];
+    if (mine > 0) {
+        look_up(0);
+        load(buf[0], 0);
+    }
+    for (int i0 = 0; i0 < mine; i0 += 2) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int i = i0 + b;
+            if (i >= mine) break;
+            float ks[GR], vs[GR];
+            unsigned ok = 0;
+#pragma unroll
+            for (int gi = 0; gi < GR; ++gi) {
+                ks[gi] = __shfl_sync(0xFFFFFFFFu, gks, (i % SET) * GR + gi);
+                vs[gi] = __shfl_sync(0xFFFFFFFFu, gvs, (i % SET) * GR + gi);
+            }
+            ok = (gok >> ((i % SET) * GR)) & ((1u << GR) - 1u);
+            if (i + 1 < mine) {
+                if ((i + 1) % SET == 0) look_up((i + 1) / SET);
+                load(buf[b ^ 1], (i + 1) % SET);
+            }
+            compute(buf[b], i, lo + (i * NW + warp) * CK, ks, vs, ok);
         }
     }
-    __half *op = a.out + r * a.o_row + t * a.o_tok + static_cast<long long>(hq) * D;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(c.status, ST_KV8_BAD_PAGE);
+
+    // the warps' rows: thread (g, t) holds dims 16 t .. (D 64: columns j of tiles 2 t and 2 t + 1)
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) op[lane + 32 * i] = __float2half_rn(o[i] * inv);
+    for (int rr = 0; rr < RR; ++rr) {
+        l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
+        l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
+        if (t == 0) {
+            sm[warp][g + 8 * rr] = m[rr];
+            sl[warp][g + 8 * rr] = l[rr];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < DT; j += 4) {
+                float4 w;
+                float *wf = reinterpret_cast<float *>(&w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
+                *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * t + e) * DT + j]) = w;
+            }
+    }
+    __syncthreads();
+    const int rows = min(ROWS, R - qt * ROWS);
+    auto merged = [&](int row, int d, float &mx, float &lx) {
+        mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+        lx = 0.0f;
+        float x = 0.0f;
+        if (mx > -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = ex2(sm[w][row] - mx);
+                lx = fmaf(f, sl[w][row], lx);
+                x = fmaf(f, so[w][row][d], x);
+            }
+        }
+        return x;
+    };
+    auto put = [&](int row, int d, float x) {
+        const int i = qt * ROWS + row, tok = i / a.G;
+        a.out[r * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
+    };
+    if (active <= 1) {
+        for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
+            float mx, lx;
+            const float x = merged(e / D, e % D, mx, lx);
+            put(e / D, e % D, lx > 0.0f ? x / lx : 0.0f);
+        }
+        return;
+    }
+    const int tile = blockIdx.x / a.nsplit;
+    const int prow = min(ROWS, R);  // rows of a tile in the work area
+    float *part = a.part + static_cast<long long>(blockIdx.x - split) * prow * (D + 2);
+    for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
+        float mx, lx;
+        const float x = merged(e / D, e % D, mx, lx);
+        float *pr = part + (static_cast<long long>(split) * prow + e / D) * (D + 2);
+        pr[e % D] = x;
+        if (e % D == 0) {
+            pr[D] = mx;
+            pr[D + 1] = lx;
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned seen = atomicAdd(&a.arrive[tile], 1u);
+        is_last = seen == static_cast<unsigned>(active - 1);
+        if (is_last) a.arrive[tile] = 0;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
+        const float *pr = part + (e / D) * (D + 2);
+        const long long step = static_cast<long long>(prow) * (D + 2);
+        float mx = -INFINITY;
+        for (int s = 0; s < active; ++s) mx = fmaxf(mx, __ldcg(pr + s * step + D));
+        float lx = 0.0f, x = 0.0f;
+        if (mx > -INFINITY)
+#pragma unroll 4
+            for (int s = 0; s < active; ++s) {
+                const float f = ex2(__ldcg(pr + s * step + D) - mx);
+                lx = fmaf(f, __ldcg(pr + s * step + D + 1), lx);
+                x = fmaf(f, __ldcg(pr + s * step + e % D), x);
+            }
+        put(e / D, e % D, lx > 0.0f ? x / lx : 0.0f);
+    }
 }
 
 }  // namespace kv8
@@ -106,19 +485,58 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
         max_len < 0 || max_len > kv->maxPages * kv->page || count < 0)
         return GPT2_B200_EINVAL;
     if (Tq == 0) return GPT2_B200_OK;
+    const kv8::Work w = kv8::work_layout(kv, Hq, Tq);
     if (!kv8::aligned(out) || !kv8::aligned(q) || (out_row_stride & 7) || (out_tok_stride & 7) || (q_row_stride & 7) ||
-        (q_tok_stride & 7) || kv->work_bytes < kv8::work_layout(kv, Hq, Tq).bytes)
+        (q_tok_stride & 7) || kv->work_bytes < w.bytes)
         return GPT2_B200_EINVAL;
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_EDEVICE;
-    kv8::AttParams a{q, out, q_row_stride, q_tok_stride, out_row_stride, out_tok_stride, d_first, d_count, L, Hq, Tq, count,
-                     max_len ? max_len : kv->maxPages * kv->page,
-                     1.4426950408889634f / sqrtf(static_cast<float>(kv->headDim))};
-    const long long warps = static_cast<long long>(kv->nRow) * Hq * Tq;
-    if ((warps + 3) / 4 > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
-    auto *kern = kv->kind == GPT2_KV8_INT8
-                     ? (kv->headDim == 64 ? kv8::k_kv8_attend<GPT2_KV8_INT8, 64> : kv8::k_kv8_attend<GPT2_KV8_INT8, 128>)
-                     : (kv->headDim == 64 ? kv8::k_kv8_attend<GPT2_KV8_E4M3, 64> : kv8::k_kv8_attend<GPT2_KV8_E4M3, 128>);
-    kern<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, stream>>>(kv8::view(kv, ctx->status), a);
-    return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    kv8::AttParams a;
+    a.q = q;
+    a.out = out;
+    a.q_row = q_row_stride;
+    a.q_tok = q_tok_stride;
+    a.o_row = out_row_stride;
+    a.o_tok = out_tok_stride;
+    a.d_first = d_first;
+    a.d_count = d_count;
+    a.L = L;
+    a.G = Hq / kv->nHead;
+    a.Tq = Tq;
+    a.count = count;
+    a.max_len = max_len ? max_len : kv->maxPages * kv->page;
+    a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(kv->headDim));
+    const long long run = static_cast<long long>(kv->page) * kv->headDim;
+    a.page_stride = run * kv->nHead * 2 * kv->nLayer;
+    a.k_off = run * kv->nHead * 2 * L;
+    a.v_off = a.k_off + run * kv->nHead;
+    a.part = w.part;
+    a.arrive = w.arrive;
+    // Plan: whole (row, head, tile) units while they fill the GPU; else spans of at least NW chunks, about
+    // WAVES CTAs per resident slot.
+    const long long R = static_cast<long long>(a.G) * Tq;
+    const int rows = R <= 8 ? 8 : 16;
+    a.qtiles = static_cast<int>((R + rows - 1) / rows);
+    const long long units = static_cast<long long>(kv->nRow) * kv->nHead * a.qtiles;
+    const int chunk = kv8::NW * (2048 / kv->headDim);
+    const int longest = a.max_len + 2048 / kv->headDim;  // `first` may start inside a chunk
+    const long long target = std::min<long long>(static_cast<long long>(ctx->num_sms) * 6, kv8::MAX_SPLIT_CTAS);
+    long long nsplit = std::max<long long>(1, target / units);
+    nsplit = std::min<long long>(nsplit, (longest + chunk - 1) / chunk);
+    a.span = static_cast<int>((longest + nsplit - 1) / nsplit + chunk - 1) / chunk * chunk;
+    a.nsplit = (longest + a.span - 1) / a.span;
+    if (units * a.nsplit > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
+    const kv8::View c = kv8::view(kv, ctx->status);
+    auto go = [&](auto kern) {
+        kern<<<static_cast<unsigned>(units * a.nsplit), 32 * kv8::NW, 0, stream>>>(c, a);
+        return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    };
+    if (kv->kind == GPT2_KV8_INT8) {
+        if (kv->headDim == 64)
+            return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 16>);
+        return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_INT8, 128, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_INT8, 128, 16>);
+    }
+    if (kv->headDim == 64)
+        return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 64, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 64, 16>);
+    return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 128, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 128, 16>);
 }

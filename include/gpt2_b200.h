@@ -373,7 +373,7 @@ int gpt2_kv8_compact_b200(const GPT2KV8Cache *kv, int *d_live, cudaStream_t stre
  * probabilities so far (-inf: a beam that does not exist, e.g. all but one at the first step); done [B*W] (NULL: none)
  * marks finished beams. Candidate (w, token) of item b has score[w] + logit - logsumexp(row), a finished beam is
  * one candidate (w, eos) with its score unchanged; the W largest per item are chosen, equal totals by the lower w, then the
- * lower token. -inf logits are masked tokens; NaN and +inf set a status bit and count as masked. Outputs, best first: token,
+ * higher logit, then the lower token. -inf logits are masked tokens; NaN and +inf set a status bit and count as masked. Outputs, best first: token,
  * parent (row index b*W + w, as gpt2_kv8_reorder_b200 takes it), new_score, new_done (NULL: not written) = finished
  * before, or token == eos (eos < 0: none). Where fewer than W candidates exist the rest is a dead beam: token max(eos, 0),
  * parent its own row, score -inf, done 1. new_score / new_done may be score / done. W 1..32. work: gpt2_beam_work_bytes_b200,
