@@ -3,32 +3,35 @@
 // total(w, v) = score[w] + (x[w, v] - lse[w]), lse = m + log(sum exp(x - m)); a finished beam is the one candidate
 // (w, eos) with its score. Within a beam totals fall as logits do, so a beam's W largest logits hold all
 // of its candidates that matter: a row is read once, for the running maximum and sum and for its W largest logits.
-// Bound by reading the logits from HBM (2 or 4 bytes each, one exponential per value).
+// Bound by reading the logits from HBM (2 or 4 bytes each; about 8 instructions per value).
 //
-//   - A CTA takes a chunk of a row, tile by tile, a tile in registers (16-byte loads, also of rows that are
-//     not aligned). Each thread keeps its own (m, l).
-//   - The W largest of a tile without a sort: of G >= W disjoint groups of threads each has a maximum, so the smallest of
-//     the G maxima is at most the W-th largest value. Values at least that (about G ln G of them, 22 for 8) go to a
-//     list, and a value's rank is the number of list entries before it. A list that overflows (many equal
-//     values) is replaced by W rounds of a maximum below the last one.
+//   - Every warp streams its own part of a row through a ring of its own in shared memory (cp.async), so the main loop
+//     has no CTA barrier and a warp has up to STAGES - 1 steps in flight. Lanes own values by their index, whatever the
+//     row's alignment: equal rows get equal sums. A row that does not start on a 16-byte boundary is copied in aligned
+//     granules and a lane's values are cut out of two neighbouring ones.
+//   - The warp's W largest so far are a sorted list, lane j holding the j-th; its last entry is the threshold that a value
+//     must pass to be inserted (about W ln(n / W) of n values do). The first step starts from a threshold that at
+//     least W values reach: the W-th largest of the lanes' maxima.
 //   - Logits are compared as 64-bit keys: the value's orderable bits, then the inverted token, so equal logits go to the
 //     lower token whatever the order of arrival.
-//   - The last CTA of an item to arrive (a counter that it re-arms) merges its rows: a key's rank among the sorted
-//     lists of a row's chunks is found by binary search; then the W x W totals the same way, equal
-//     totals by the lower beam.
+//   - Sorted lists are merged by W rounds of a maximum over their heads, a lane per list: the warps' in a CTA, the CTAs' of
+//     a row, and the beams' of an item, the last two by the item's last CTA to arrive (a counter that it re-arms).
 #include <algorithm>
 
 #include "kv8.cuh"
 #include "linear.cuh"
+#include "ptx.cuh"
 
 namespace b200 {
 namespace beam {
 
 constexpr int MAX_W = 32;
-constexpr int NT = 256, NWARP = NT / 32;
-constexpr int MAX_CHUNKS = 64;    // chunks of a row
-constexpr int ROW_KEYS = 256;     // chunks x W of a row, at most
-constexpr int LIST = 1024;        // candidates of a tile
+constexpr int NWARP = 8, NT = 32 * NWARP;
+constexpr int MAX_CHUNKS = 64;  // CTAs of a row: two list heads per lane
+constexpr int ROW_KEYS = 256;   // CTAs x W of a row, at most
+constexpr int VPT = 2;          // 16-byte granules per lane and step
+constexpr int STAGES = 6;
+constexpr int STAGE_BYTES = (32 * VPT + 1) * 16;  // and the granule behind, for rows that are not aligned
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long key_t;
@@ -43,7 +46,7 @@ struct Params {
     long long ld;
     const float *score;
     const int *done;
-    int W, V, eos, chunks, chunk;  // chunk: values per CTA
+    int W, V, eos, chunks, steps;  // steps per warp of a CTA
     key_t *keys;                   // [rows][chunks][W], sorted
     float2 *ml;                    // [rows][chunks]
     unsigned *arrive;              // [items]
@@ -55,23 +58,19 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 __device__ __forceinline__ float key_value(key_t k) {
     const unsigned o = static_cast<unsigned>(k >> 32);
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
-// Entries of the descending list a[0..n) above k.
-__device__ __forceinline__ int above(const key_t *a, int n, key_t k) {
-    int lo = 0;
-    while (n > 0) {
-        const int half = n >> 1;
-        if (a[lo + half] > k) {
-            lo += half + 1;
-            n -= half + 1;
-        } else {
-            n = half;
-        }
-    }
-    return lo;
+__device__ __forceinline__ key_t warp_max(key_t k) {
+    const unsigned hi = __reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(k >> 32));
+    const unsigned lo = __reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(k >> 32) == hi ? static_cast<unsigned>(k) : 0u);
+    return (static_cast<key_t>(hi) << 32) | lo;
 }
 __device__ __forceinline__ void merge_ml(float &m, float &l, float m2, float l2) {
     const float mx = fmaxf(m, m2);
@@ -79,23 +78,79 @@ __device__ __forceinline__ void merge_ml(float &m, float &l, float m2, float l2)
     l = l * ex2((m - mx) * LOG2E) + l2 * ex2((m2 - mx) * LOG2E);
     m = mx;
 }
+// (m, l) over the warp, the same bits in every lane.
+__device__ __forceinline__ void warp_ml(float &m, float &l) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, o);
+        const bool upper = threadIdx.x & o;  // both sides add in the same order
+        float a = upper ? m2 : m, b = upper ? l2 : l;
+        merge_ml(a, b, upper ? m : m2, upper ? l : l2);
+        m = a;
+        l = b;
+    }
+}
+// Merges n <= 64 descending lists of W keys (list i at a + i * W), one or two heads per lane; round j's
+// winner goes to put(j, key, list). Stops when all are used up and returns how many were put.
+template <typename Put>
+__device__ __forceinline__ int merge_lists(const key_t *a, int n, int W, Put put) {
+    const int lane = threadIdx.x & 31;
+    int i0 = 0, i1 = 0;
+    key_t k0 = lane < n ? a[lane * W] : 0, k1 = lane + 32 < n ? a[(lane + 32) * W] : 0;
+    for (int j = 0; j < W; ++j) {
+        const key_t top = warp_max(max(k0, k1));
+        if (!top) return j;
+        if (k0 == top) {  // keys are distinct: one lane pops
+            put(j, top, lane);
+            k0 = ++i0 < W ? a[lane * W + i0] : 0;
+        } else if (k1 == top) {
+            put(j, top, lane + 32);
+            k1 = ++i1 < W ? a[(lane + 32) * W + i1] : 0;
+        }
+    }
+    return W;
+}
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
-// VPT 16-byte vectors per thread and tile.
-template <typename T, int VPT>
+template <typename T>
+__device__ __forceinline__ void unpack(const uint32_t (&w)[4], float *v);
+template <>
+__device__ __forceinline__ void unpack<float>(const uint32_t (&w)[4], float *v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+}
+template <>
+__device__ __forceinline__ void unpack<__half>(const uint32_t (&w)[4], float *v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
-    constexpr int EV = 16 / sizeof(T);  // values per vector
-    constexpr int TILE = NT * VPT * EV;
-    __shared__ key_t list[LIST];
-    __shared__ key_t run[2][MAX_W];
-    __shared__ float gmax[NWARP * 4];
+    constexpr int EV = 16 / sizeof(T);    // values per granule
+    constexpr int STEP = 32 * VPT * EV;   // values per warp and step
+    constexpr int NV = VPT * EV;          // values per lane and step
+    extern __shared__ __align__(16) uint8_t ring_all[];
+    // behind the main loop the rings' memory holds the lists that are merged
+    key_t (*lists)[ROW_KEYS] = reinterpret_cast<key_t (*)[ROW_KEYS]>(ring_all);
+    key_t *totals = reinterpret_cast<key_t *>(ring_all + NWARP * ROW_KEYS * sizeof(key_t));  // [W][W]
+    int *tokens = reinterpret_cast<int *>(totals + MAX_W * MAX_W);                           // [W][W]
+    static_assert(NWARP * ROW_KEYS * 8 + MAX_W * MAX_W * 12 <= NWARP * STAGES * STAGE_BYTES, "lists fit in the rings");
     __shared__ float red_m[NWARP], red_l[NWARP];
-    __shared__ key_t red_k[NWARP];
-    __shared__ int count, is_last;
-    __shared__ key_t rowbuf[NWARP][ROW_KEYS];
+    __shared__ int is_last;
     __shared__ float s_score[MAX_W];
     __shared__ int s_done[MAX_W];
-    __shared__ key_t final_keys[MAX_W * MAX_W];
-    __shared__ int final_token[MAX_W * MAX_W];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int W = p.W, V = p.V;
     const int item = blockIdx.x / (W * p.chunks), rest = blockIdx.x - item * (W * p.chunks);
@@ -104,63 +159,72 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
     const bool alive = p.score[row] > -INFINITY && !(p.done && p.done[row]);
     if (alive) {
         const T *x = static_cast<const T *>(p.logits) + row * p.ld;
-        // Thread and tile own values by their index, whatever the row's alignment: equal rows get equal sums. A row that
-        // starts `shift` values behind a 16-byte boundary is read in aligned granules, and a thread's vector is cut out
-        // of two neighbouring ones (the second comes from L1). Granules that reach over the row's ends are read value by value.
         const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
         const unsigned cut = shift * sizeof(T);
-        const int begin = ch * p.chunk, end = min(begin + p.chunk, V);
-        auto granule = [&](int at) {  // values at .. at + EV - 1, -inf outside the row
-            uint4 g;
+        uint8_t *ring = ring_all + warp * STAGES * STAGE_BYTES;
+        const int begin = (ch * p.steps * NWARP + warp) * STEP;  // step s: values begin + s * NWARP * STEP ..
+        int steps = begin < V ? min(p.steps, (V - begin + NWARP * STEP - 1) / (NWARP * STEP)) : 0;
+        // Granule g of a step holds values base + g * EV - shift ..; outside the row they are -inf. One that
+        // reaches over the row's ends is read value by value.
+        auto fetch = [&](uint8_t *dst, int at) {
             if (at >= 0 && at + EV <= V) {
-                asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w) : "l"(x + at));
+                cp_async16(dst, x + at);
             } else {
-                T part[EV];
 #pragma unroll
-                for (int j = 0; j < EV; ++j) part[j] = at + j >= 0 && at + j < V ? x[at + j] : static_cast<T>(-INFINITY);
-                g = *reinterpret_cast<uint4 *>(part);
+                for (int j = 0; j < EV; ++j)
+                    reinterpret_cast<T *>(dst)[j] = at + j >= 0 && at + j < V ? x[at + j] : static_cast<T>(-INFINITY);
             }
-            return g;
         };
+        auto load = [&](int s) {
+            if (s < steps) {
+                uint8_t *dst = ring + s % STAGES * STAGE_BYTES;
+                const int base = begin + s * (NWARP * STEP) - shift;
+#pragma unroll
+                for (int q = 0; q < VPT; ++q) fetch(dst + (q * 32 + lane) * 16, base + (q * 32 + lane) * EV);
+                if (cut && lane == 0) fetch(dst + 32 * VPT * 16, base + 32 * VPT * EV);
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) load(s);
         float m = -INFINITY, l = 0.0f;
+        key_t mine = 0, worst = 0;  // the j-th largest key in lane j; the W-th
+        float thr = -INFINITY;
         bool bad = false;
-        if (tid < 2 * MAX_W) run[tid / MAX_W][tid % MAX_W] = 0;
-        int cur = 0;
-        for (int base = begin; base < end; base += TILE) {
-            float v[VPT][EV];
-            uint4 raw[VPT], next[VPT];
+        for (int s = 0; s < steps; ++s) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();  // every lane's copies of step s are there, and all are done with step s - 1
+            load(s + STAGES - 1);
+            const uint4 *src = reinterpret_cast<const uint4 *>(ring + s % STAGES * STAGE_BYTES);
+            float v[NV];
 #pragma unroll
             for (int q = 0; q < VPT; ++q) {
-                const int at = base + (q * NT + tid) * EV;
-                raw[q] = granule(at - shift);
-                if (cut) next[q] = granule(at - shift + EV);
-            }
-            if (cut) {
-#pragma unroll
-                for (int q = 0; q < VPT; ++q) {
-                    const uint4 &y = raw[q], &z = next[q];
-                    uint32_t s[5];
+                const uint4 a = src[q * 32 + lane];
+                uint32_t o[4] = {a.x, a.y, a.z, a.w};
+                if (cut) {
+                    const uint4 b = src[q * 32 + lane + 1];
+                    uint32_t c[5];
                     switch (cut >> 2) {
-                        case 0: s[0] = y.x, s[1] = y.y, s[2] = y.z, s[3] = y.w, s[4] = z.x; break;
-                        case 1: s[0] = y.y, s[1] = y.z, s[2] = y.w, s[3] = z.x, s[4] = z.y; break;
-                        case 2: s[0] = y.z, s[1] = y.w, s[2] = z.x, s[3] = z.y, s[4] = z.z; break;
-                        default: s[0] = y.w, s[1] = z.x, s[2] = z.y, s[3] = z.z, s[4] = z.w; break;
+                        case 0: c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w, c[4] = b.x; break;
+                        case 1: c[0] = a.y, c[1] = a.z, c[2] = a.w, c[3] = b.x, c[4] = b.y; break;
+                        case 2: c[0] = a.z, c[1] = a.w, c[2] = b.x, c[3] = b.y, c[4] = b.z; break;
+                        default: c[0] = a.w, c[1] = b.x, c[2] = b.y, c[3] = b.z, c[4] = b.w; break;
                     }
-                    const unsigned bits = (cut & 2) * 8;
-                    raw[q] = make_uint4(__funnelshift_r(s[0], s[1], bits), __funnelshift_r(s[1], s[2], bits),
-                                        __funnelshift_r(s[2], s[3], bits), __funnelshift_r(s[3], s[4], bits));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(c[i], c[i + 1], (cut & 2) * 8);
                 }
+                unpack<T>(o, v + q * EV);
             }
-            float top = -INFINITY;
+            float top = v[0];
 #pragma unroll
-            for (int q = 0; q < VPT; ++q) {
-                const T *e = reinterpret_cast<const T *>(&raw[q]);
+            for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
+            if (!(top < INFINITY)) {  // NaN and +inf count as masked
+                bad = true;
+                top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < EV; ++j) {
-                    const float y = static_cast<float>(e[j]);
-                    v[q][j] = y < INFINITY ? y : -INFINITY;  // NaN and +inf count as masked
-                    bad |= !(y < INFINITY);
-                    top = fmaxf(top, v[q][j]);
+                for (int i = 0; i < NV; ++i) {
+                    v[i] = v[i] < INFINITY ? v[i] : -INFINITY;
+                    top = fmaxf(top, v[i]);
                 }
             }
             if (top > m) {
@@ -169,97 +233,59 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
             }
             if (m > -INFINITY) {
 #pragma unroll
-                for (int q = 0; q < VPT; ++q)
-#pragma unroll
-                    for (int j = 0; j < EV; ++j) l += ex2((v[q][j] - m) * LOG2E);  // m subtracted first: exact near m, where it counts
+                for (int i = 0; i < NV; ++i) l += ex2((v[i] - m) * LOG2E);  // m subtracted first: exact near m, where it counts
             }
-            // the group maxima: groups of 32 threads (W <= 8), of 16 or of 8
-            float gm = top;
-            const int per = W <= 8 ? 32 : W <= 16 ? 16 : 8;
-            for (int o = 1; o < per; o <<= 1) gm = fmaxf(gm, __shfl_xor_sync(0xFFFFFFFFu, gm, o));
-            if (tid % per == 0) gmax[tid / per] = gm;
-            if (tid == 0) count = 0;
-            __syncthreads();
-            // with fewer beams than groups, neighbouring groups are one: G = the power of two at or above W
-            float thr = INFINITY;
-            const int groups = NT / per;
-            int fold = 1;
-            while (groups / (2 * fold) >= W) fold *= 2;
-            for (int i = 0; i < groups; i += fold) {
-                float z = gmax[i];
-                for (int f = 1; f < fold; ++f) z = fmaxf(z, gmax[i + f]);
-                thr = fminf(thr, z);
-            }
-            const key_t worst = run[cur][W - 1];
-            if (worst) thr = fmaxf(thr, key_value(worst));
-            if (top >= thr && top > -INFINITY) {
+            if (s == 0) {  // the W-th largest of the 32 lane maxima: no W values are lost below it
+                int rank = 0;
 #pragma unroll
-                for (int q = 0; q < VPT; ++q)
-#pragma unroll
-                    for (int j = 0; j < EV; ++j)
-                        if (v[q][j] >= thr && v[q][j] > -INFINITY) {
-                            const int at = atomicAdd(&count, 1);
-                            if (at < LIST)
-                                list[at] = lin::argmax_key(v[q][j], static_cast<unsigned>(base + (q * NT + tid) * EV + j));
-                        }
-            }
-            __syncthreads();
-            const int n = count;
-            if (tid < W) run[cur ^ 1][tid] = 0;
-            __syncthreads();
-            if (n <= LIST) {
-                for (int i = tid; i < n + W; i += NT) {
-                    const key_t k = i < n ? list[i] : run[cur][i - n];
-                    if (!k) continue;
-                    int rank = above(run[cur], W, k);
-                    for (int j = 0; j < n && rank < W; ++j) rank += list[j] > k;
-                    if (rank < W) run[cur ^ 1][rank] = k;
+                for (int i = 0; i < 32; ++i) {
+                    const float u = __shfl_sync(0xFFFFFFFFu, top, i);
+                    rank += u > top || (u == top && i < lane);
                 }
-                __syncthreads();
-            } else {
-                key_t prev = ~0ull;
-                for (int s = 0; s < W; ++s) {
-                    key_t best = 0;
-#pragma unroll
-                    for (int q = 0; q < VPT; ++q)
-#pragma unroll
-                        for (int j = 0; j < EV; ++j)
-                            if (v[q][j] > -INFINITY) {
-                                const key_t k = lin::argmax_key(v[q][j], static_cast<unsigned>(base + (q * NT + tid) * EV + j));
-                                if (k < prev && k > best) best = k;
-                            }
-                    if (tid < W && run[cur][tid] < prev && run[cur][tid] > best) best = run[cur][tid];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-                    if (lane == 0) red_k[warp] = best;
-                    __syncthreads();
-                    best = red_k[0];
-#pragma unroll
-                    for (int i = 1; i < NWARP; ++i) best = max(best, red_k[i]);
-                    if (tid == 0) run[cur ^ 1][s] = best;
-                    prev = best;
-                    __syncthreads();
-                }
+                const unsigned who = __ballot_sync(0xFFFFFFFFu, rank == W - 1);
+                thr = __shfl_sync(0xFFFFFFFFu, top, __ffs(who) - 1);
             }
-            cur ^= 1;
-        }
+            if (!__any_sync(0xFFFFFFFFu, top >= thr && top > -INFINITY)) continue;
+            const unsigned first = begin + s * (NWARP * STEP) + lane * EV;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, o);
-            merge_ml(m, l, m2, l2);
+            for (int i = 0; i < NV; ++i) {
+                const bool in = v[i] >= thr && v[i] > -INFINITY;
+                unsigned todo = __ballot_sync(0xFFFFFFFFu, in);
+                if (!todo) continue;
+                const key_t k = lin::argmax_key(v[i], first + i / EV * 32 * EV + i % EV);
+                todo = __ballot_sync(0xFFFFFFFFu, in && k > worst);
+                while (todo) {
+                    const int from = __ffs(todo) - 1;
+                    todo &= todo - 1;
+                    const key_t in_key = __shfl_sync(0xFFFFFFFFu, k, from);
+                    const int rank = __popc(__ballot_sync(0xFFFFFFFFu, mine > in_key));
+                    const key_t up = __shfl_up_sync(0xFFFFFFFFu, mine, 1);
+                    if (lane >= rank && lane < W) mine = lane == rank ? in_key : up;
+                }
+                worst = __shfl_sync(0xFFFFFFFFu, mine, W - 1);
+                if (worst) thr = key_value(worst);
+            }
         }
+        warp_ml(m, l);
         if (lane == 0) {
             red_m[warp] = m;
             red_l[warp] = l;
         }
+        __syncthreads();  // every warp is through its ring
+        if (lane < W) lists[0][warp * W + lane] = mine;
         if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.status, ST_BEAM_LOGIT);
         __syncthreads();
         const long long at = row * p.chunks + ch;
-        if (tid == 0) {
-            for (int i = 1; i < NWARP; ++i) merge_ml(m, l, red_m[i], red_l[i]);
-            p.ml[at] = make_float2(m, l);
+        if (warp == 0) {
+            key_t *out = p.keys + at * W;
+            const int n = merge_lists(lists[0], NWARP, W, [&](int j, key_t k, int) { out[j] = k; });
+            if (lane >= n && lane < W) out[lane] = 0;
+        } else if (warp == 1) {
+            m = lane < NWARP ? red_m[lane] : -INFINITY;
+            l = lane < NWARP ? red_l[lane] : 0.0f;
+            warp_ml(m, l);
+            if (lane == 0) p.ml[at] = make_float2(m, l);
         }
-        if (tid < W) p.keys[at * W + tid] = run[cur][tid];
     }
     // the last CTA of the item goes on
     __threadfence();
@@ -277,7 +303,7 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         s_score[tid] = p.score[first_row + tid];
         s_done[tid] = p.done ? p.done[first_row + tid] : 0;
     }
-    for (int i = tid; i < W * W; i += NT) final_keys[i] = 0;
+    for (int i = tid; i < W * W; i += NT) totals[i] = 0;
     __syncthreads();
     // a warp per beam: lse, the beam's W best logits, their totals
     for (int b = warp; b < W; b += NWARP) {
@@ -285,8 +311,8 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         if (!(sc > -INFINITY)) continue;
         if (s_done[b]) {
             if (lane == 0) {
-                final_keys[b * W] = lin::argmax_key(sc, static_cast<unsigned>(b * W));
-                final_token[b * W] = max(p.eos, 0);
+                totals[b * W] = lin::argmax_key(sc, static_cast<unsigned>(b * W));
+                tokens[b * W] = max(p.eos, 0);
             }
             continue;
         }
@@ -296,61 +322,28 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
             const float2 z = __ldcg(&p.ml[at + i]);
             merge_ml(m, l, z.x, z.y);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, o);
-            // the same operands in the same order on both sides, so all lanes end alike
-            if (lane & o) {
-                float mm = m2, ll = l2;
-                merge_ml(mm, ll, m, l);
-                m = mm;
-                l = ll;
-            } else {
-                merge_ml(m, l, m2, l2);
-            }
-        }
-        const int n = p.chunks * W;
-        for (int i = lane; i < n; i += 32) rowbuf[warp][i] = __ldcg(&p.keys[at * W + i]);
+        for (int i = lane; i < p.chunks * W; i += 32) lists[warp][i] = __ldcg(&p.keys[at * W + i]);
+        warp_ml(m, l);
         __syncwarp();
         const float lse = m + logf(l);
-        for (int i = lane; i < n; i += 32) {
-            const key_t k = rowbuf[warp][i];
-            if (!k) continue;
-            int rank = 0;
-            for (int c = 0; c < p.chunks && rank < W; ++c) rank += above(&rowbuf[warp][c * W], W, k);
-            if (rank < W) {
-                final_keys[b * W + rank] = lin::argmax_key(sc + (key_value(k) - lse), static_cast<unsigned>(b * W + rank));
-                final_token[b * W + rank] = lin::argmax_key_index(k);
-            }
-        }
+        merge_lists(lists[warp], p.chunks, W, [&](int j, key_t k, int) {
+            totals[b * W + j] = lin::argmax_key(sc + (key_value(k) - lse), static_cast<unsigned>(b * W + j));
+            tokens[b * W + j] = lin::argmax_key_index(k);
+        });
         __syncwarp();
     }
     __syncthreads();
-    // the totals of a beam fall (rounding keeps the order; equal ones by rank), so these are sorted lists again
-    for (int i = tid; i < W * W; i += NT) {
-        const key_t k = final_keys[i];
-        if (!k) continue;
-        int rank = 0;
-        for (int b = 0; b < W && rank < W; ++b) rank += above(&final_keys[b * W], W, k);
-        if (rank < W) {
-            const int out = first_row + rank, b = i / W;
-            p.token[out] = final_token[i];
-            p.parent[out] = first_row + b;
-            p.new_score[out] = key_value(k);
-            if (p.new_done) p.new_done[out] = s_done[b] || final_token[i] == p.eos;
-        }
-    }
-    // fewer candidates than beams: the rest are dead
-    int mine = 0;
-    for (int i = tid; i < W * W; i += NT) mine += final_keys[i] != 0;
-    int total = 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-    if (lane == 0) red_l[warp] = static_cast<float>(mine);
-    __syncthreads();
-    for (int i = 0; i < NWARP; ++i) total += static_cast<int>(red_l[i]);
-    if (tid >= total && tid < W) {
-        const int out = first_row + tid;
+    if (warp != 0) return;
+    // a beam's totals fall with its logits (rounding keeps the order; equal ones by rank): sorted lists again
+    const int n = merge_lists(totals, W, W, [&](int j, key_t k, int b) {
+        const int out = first_row + j, token = tokens[lin::argmax_key_index(k)];
+        p.token[out] = token;
+        p.parent[out] = first_row + b;
+        p.new_score[out] = key_value(k);
+        if (p.new_done) p.new_done[out] = s_done[b] || token == p.eos;
+    });
+    if (lane >= n && lane < W) {  // fewer candidates than beams: the rest are dead
+        const int out = first_row + lane;
         p.token[out] = max(p.eos, 0);
         p.parent[out] = out;
         p.new_score[out] = -INFINITY;
@@ -372,22 +365,26 @@ static Layout layout(int B, int W) {
 }
 
 template <typename T>
-static int launch(Params p, int B, int num_sms, cudaStream_t stream) {
-    constexpr int EV = 16 / sizeof(T);
+static int launch(Params p, int B, int num_sms, bool *attr_done, cudaStream_t stream) {
+    constexpr int STEP = 32 * VPT * (16 / static_cast<int>(sizeof(T)));
+    constexpr int SMEM = NWARP * STAGES * STAGE_BYTES;
     const long long rows = static_cast<long long>(B) * p.W;
-    // Tile: 4 vectors per thread where that still gives two CTAs per SM, else fewer, down to one: few rows are bound by
-    // the latency of one CTA's work, many by bandwidth, which wants more loads in flight per thread.
-    auto ctas = [&](int vpt) { return rows * ((p.V + NT * EV * vpt - 1) / (NT * EV * vpt)); };
-    const int vpt = ctas(4) >= 2ll * num_sms ? 4 : ctas(2) >= 2ll * num_sms ? 2 : 1;
-    const int tile = NT * EV * vpt, most = max_chunks(p.W);
-    long long tiles = (p.V + tile - 1) / tile;
-    const long long per = (tiles + most - 1) / most;  // tiles per chunk
-    p.chunk = static_cast<int>(per * tile);
-    p.chunks = static_cast<int>((tiles + per - 1) / per);
+    // CTAs of a row: about four per SM in all; down to one step per warp when rows are few (bound by the latency
+    // of one CTA), the whole row when they are many.
+    const long long groups = (p.V + NWARP * STEP - 1) / (NWARP * STEP);  // steps of a CTA that had the row to itself
+    long long chunks = (4ll * num_sms + rows - 1) / rows;
+    chunks = std::min<long long>({chunks, groups, max_chunks(p.W)});
+    p.steps = static_cast<int>((groups + chunks - 1) / chunks);
+    p.chunks = static_cast<int>((groups + p.steps - 1) / p.steps);
     const long long grid = rows * p.chunks;
     if (grid > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
-    auto *kern = vpt == 4 ? k_beam_select<T, 4> : vpt == 2 ? k_beam_select<T, 2> : k_beam_select<T, 1>;
-    kern<<<static_cast<unsigned>(grid), NT, 0, stream>>>(p);
+    if (!*attr_done) {
+        RelaxedCapture relaxed;
+        if (cudaFuncSetAttribute(k_beam_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+            return GPT2_B200_ECUDA;
+        *attr_done = true;
+    }
+    k_beam_select<T><<<static_cast<unsigned>(grid), NT, SMEM, stream>>>(p);
     return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
@@ -430,6 +427,6 @@ extern "C" int gpt2_beam_select_b200(int *token, int *parent, float *new_score, 
     p.keys = reinterpret_cast<beam::key_t *>(static_cast<char *>(work) + y.o_keys);
     p.ml = reinterpret_cast<float2 *>(static_cast<char *>(work) + y.o_ml);
     p.status = ctx->status;
-    return type == GPT2_BEAM_HALF ? beam::launch<__half>(p, B, ctx->num_sms, stream)
-                                  : beam::launch<float>(p, B, ctx->num_sms, stream);
+    return type == GPT2_BEAM_HALF ? beam::launch<__half>(p, B, ctx->num_sms, &ctx->beam_attr_done[0], stream)
+                                  : beam::launch<float>(p, B, ctx->num_sms, &ctx->beam_attr_done[1], stream);
 }

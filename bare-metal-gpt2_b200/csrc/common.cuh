@@ -44,6 +44,8 @@ struct DeviceContext {
     int pf_active_clusters[5] = {0, 0, 0, 0, 0};  // prefill split clusters of n CTAs that fit (0 = not asked)
     bool prefill_attr_done = false;
     bool decode_attr_done = false;
+    bool beam_attr_done[2] = {false, false};  // beam selection over fp16, fp32 logits
+    bool kv8_attr_done[8] = {};               // 8-bit cache attention, by kernel variant
     int num_sms = 0;
     int device = 0;                 // CUDA device ordinal of this context
 };

@@ -10,12 +10,12 @@
 //     in as hi + lo (two fp16, 22 bits): rounding it to one fp16 alone would add an error of the size of the
 //     output's own rounding. With at most 8 query rows (the decode step) the MMA's rows 8..15 are
 //     free and take lo; with 9 to 16 rows lo is a second MMA. mma.sync's rate is far above what HBM feeds
-//     (32 MMAs per 4 KB of codes), and its operands come from registers: no staging through shared memory, no barriers.
-//   - a warp takes CK keys at a time (32 for D 64, 16 for D 128: 4 KB of K and V), loaded straight into the operand
-//     layout by 16- and 8-byte loads. The sum over dims (QK) may run in any order of dims, so a thread's 16
-//     neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its column order are as
-//     free, so a thread loads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with 16 neighbouring
-//     output dims. The next chunk's loads are in flight while a chunk is computed.
+//     (32 MMAs per 4 KB of codes).
+//   - a warp takes CK keys at a time (32 for D 64, 16 for D 128: 4 KB of K and V) through a ring of its own in shared
+//     memory (cp.async, STAGES - 1 chunks in flight, no CTA barrier). The sum over dims (QK) may run in any order of dims,
+//     so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
+//     column order are as free, so a thread reads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with
+//     16 neighbouring output dims. The 16-byte granules of a chunk are permuted so that neither read has bank conflicts.
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
 //   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
@@ -54,21 +54,18 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 // Two int8 codes (as code + 128) in bytes 0, 2 over 0x64 bytes are the halves 1024 + code + 128: exact.
 __device__ __forceinline__ uint32_t sub1152(uint32_t h) {
@@ -111,20 +108,35 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// One warp's chunk of CK keys: K for 8-key tiles, V for the 4 keys of each 16-key granule a thread holds p of.
+// A warp's chunk of CK keys in shared memory: 2 KB of K rows, then 2 KB of V rows, in 16-byte granules.
+// Reads: K, a quarter warp takes granules 0..3 (then 4..7 for D 128) of two neighbouring rows; V, a half warp takes two
+// granules (8 bytes a lane) or a quarter warp two granules (16 bytes a lane) of rows 0, 2, 4, 6 of an 8-row
+// group. The maps put each such set on 8 different bank groups (granule index mod 8).
 template <int D>
 struct Chunk {
-    static constexpr int CK = 2048 / D, GR = CK / 16;
-    uint4 k[4];
-    uint2 v[8];  // D 64: [granule][key] 8 dims; D 128: [key][half] 16 dims
+    static constexpr int CK = 2048 / D, GR = CK / 16, ROWG = D / 16;  // granules per row
+    __device__ static int k_at(int row, int gr) { return row * ROWG + (D == 64 ? gr : gr ^ ((row & 1) << 2)); }
+    __device__ static int v_at(int row, int gr) {
+        if (D == 64) {  // 8-row groups: row bits (b2 b1 b0) stored as (b2 b0 b1); the granule's high bit flipped by b2
+            const int at = (row & ~3) | ((row & 1) << 1) | ((row >> 1) & 1);
+            return at * ROWG + (gr ^ ((row >> 1) & 2));
+        }
+        return row * ROWG + (gr ^ (row & 6));
+    }
 };
+constexpr int CHUNK_BYTES = 4096;
+// Chunks per warp's ring. Three CTAs of 4 x 4 chunks (192 KB) fill an SM's shared memory.
+constexpr int STAGES = 4;
+constexpr int RING_BYTES = NW * STAGES * CHUNK_BYTES;
 
 template <int KIND, int D, int ROWS>
 __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_attend(const View c, const AttParams a) {
     using C = Chunk<D>;
     constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
     constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
-    __shared__ float so[NW][ROWS][D + 4];
+    extern __shared__ __align__(128) uint8_t ring_all[];
+    float (*so)[ROWS][D + 4] = reinterpret_cast<float (*)[ROWS][D + 4]>(ring_all);  // [NW], behind the main loop
+    static_assert(NW * ROWS * (D + 4) * 4 <= RING_BYTES, "the warps' rows fit in the rings");
     __shared__ float sm[NW][ROWS], sl[NW][ROWS];
     __shared__ int is_last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -208,55 +220,54 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
         if (!ok) gks = gvs = 0.0f;
         gok = __ballot_sync(0xFFFFFFFFu, ok);
     };
-    const uint8_t *kbase = c.data + a.k_off + g * D + 16 * t;
-    const uint8_t *vbase = c.data + a.v_off + 2 * t * D + g * (D / 8);
-    auto load = [&](C &x, int i) {  // chunk i of the set
+    uint8_t *ring = ring_all + warp * STAGES * CHUNK_BYTES;
+    const uint32_t ring_s = smem_u32(ring);
+    // A copy instruction of the warp takes 512 bytes: 8 rows (D 64) or 4. V's rows are dealt to the lanes so that its
+    // stores, too, meet 8 bank groups per 8 lanes.
+    const int krow = lane / C::ROWG;
+    const int vrow = D == 64 ? ((lane >> 2) & 1) * 2 + ((lane >> 3) & 1) + (lane >> 4) * 4 : krow;
+    const int cgr = lane & (C::ROWG - 1);
+    constexpr int CR = 32 / C::ROWG;  // rows per copy instruction
+    auto load = [&](int i, int stage) {  // chunk i of this warp; its set has been looked up
+        const uint32_t dst = ring_s + stage * CHUNK_BYTES;
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
-            const long long off = __shfl_sync(0xFFFFFFFFu, goff, i * GR + gi);
-            const bool ok = (gok >> (i * GR + gi)) & 1u;
-            const uint8_t *kp = kbase + off, *vp = vbase + off;
-            if (D == 64) {
+            const int src_lane = (i % SET) * GR + gi;
+            const long long off = __shfl_sync(0xFFFFFFFFu, goff, src_lane);
+            if (!((gok >> src_lane) & 1u)) continue;
+            const uint8_t *kp = c.data + a.k_off + off + krow * D + cgr * 16;
+            const uint8_t *vp = c.data + a.v_off + off + vrow * D + cgr * 16;
 #pragma unroll
-                for (int tile = 0; tile < 2; ++tile)
-                    x.k[2 * gi + tile] = ok ? ldg16(kp + 8 * tile * D) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int row = (y & 1) + (y >> 1) * 8;
-                    x.v[4 * gi + y] = ok ? ldg8(vp + row * D) : make_uint2(0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int tile = 0; tile < 2; ++tile)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-                        x.k[2 * tile + hh] = ok ? ldg16(kp + 8 * tile * D + 64 * hh) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int row = (y & 1) + (y >> 1) * 8;
-                    const uint4 w = ok ? ldg16(vp + row * D) : make_uint4(0, 0, 0, 0);
-                    x.v[2 * y] = make_uint2(w.x, w.y);
-                    x.v[2 * y + 1] = make_uint2(w.z, w.w);
-                }
+            for (int x = 0; x < 16 / CR; ++x) {
+                const int row = gi * 16 + x * CR;
+                cp_async16(dst + C::k_at(row + krow, cgr) * 16, kp + x * CR * D);
+                cp_async16(dst + 2048 + C::v_at(row + vrow, cgr) * 16, vp + x * CR * D);
             }
         }
     };
-    auto compute = [&](C &x, int i, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+    auto compute = [&](const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+        const uint4 *kb = reinterpret_cast<const uint4 *>(buf), *vb = reinterpret_cast<const uint4 *>(buf + 2048);
         float s[NT][4];
 #pragma unroll
-        for (int tile = 0; tile < NT; ++tile) {
-            s[tile][0] = s[tile][1] = s[tile][2] = s[tile][3] = 0.0f;
+        for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = s[tile][2] = s[tile][3] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                const uint4 &kw = D == 64 ? x.k[tile] : x.k[2 * tile + st / 4];
-                const uint32_t w = st % 4 == 0 ? kw.x : st % 4 == 1 ? kw.y : st % 4 == 2 ? kw.z : kw.w;
-                uint32_t b0, b1;
-                halves4<KIND>(w, b0, b1);
-                if (ROWS == 8)
-                    mma16816(s[tile], qa[st][0], qa[st][0], qa[st][1], qa[st][1], b0, b1);
-                else
-                    mma16816(s[tile], qa[st][0], qa[st][RR - 1], qa[st][RR], qa[st][2 * RR - 1], b0, b1);
-            }
+        for (int s4 = 0; s4 < KS / 4; ++s4) {
+            uint4 kw[NT];
+#pragma unroll
+            for (int tile = 0; tile < NT; ++tile) kw[tile] = kb[C::k_at(8 * tile + g, 4 * s4 + t)];
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int tile = 0; tile < NT; ++tile) {
+                    const uint32_t w = st == 0 ? kw[tile].x : st == 1 ? kw[tile].y : st == 2 ? kw[tile].z : kw[tile].w;
+                    const uint32_t (&qq)[2 * RR] = qa[4 * s4 + st];
+                    uint32_t b0, b1;
+                    halves4<KIND>(w, b0, b1);
+                    if (ROWS == 8)
+                        mma16816(s[tile], qq[0], qq[0], qq[1], qq[1], b0, b1);
+                    else
+                        mma16816(s[tile], qq[0], qq[RR - 1], qq[RR], qq[2 * RR - 1], b0, b1);
+                }
         }
         const bool masked = pos < first || pos + CK > min(first_end, last_end) || ok != (1u << GR) - 1u;
 #pragma unroll
@@ -271,16 +282,6 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
                     const int key = pos + 8 * tile + 2 * t + (e & 1);
                     if (key < first || key >= end[e >> 1] || !((ok >> (tile / 2)) & 1u)) s[tile][e] = -INFINITY;
                 }
-            if (KIND == GPT2_KV8_E4M3) {  // a code behind the last key may be NaN, and 0 * NaN is not 0
-#pragma unroll
-                for (int y = 0; y < 4 * GR; ++y)
-                    if (pos + 16 * (y / 4) + 2 * t + (y & 1) + ((y >> 1) & 1) * 8 >= n) {
-                        if (D == 64)
-                            x.v[y] = make_uint2(0, 0);
-                        else
-                            x.v[2 * y] = x.v[2 * y + 1] = make_uint2(0, 0);
-                    }
-            }
         }
         float ms[RR];
         bool grew = false;
@@ -332,14 +333,30 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
                     ph[tile * RR + rr] = pack_hi(p0, p1, l0, l1);
                     pl[tile * RR + rr] = pack(l0, l1);
                 }
+            uint32_t vw[4][D / 32];  // D / 8 dims of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the granule
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int row = 16 * gi + 2 * t + (y & 1) + (y >> 1) * 8;
+                if (D == 64) {
+                    const uint2 z = reinterpret_cast<const uint2 *>(vb + C::v_at(row, g >> 1))[g & 1];
+                    vw[y][0] = z.x;
+                    vw[y][1] = z.y;
+                } else {
+                    const uint4 z = vb[C::v_at(row, g)];
+                    vw[y][0] = z.x;
+                    vw[y][1] = z.y;
+                    vw[y][D / 32 - 2] = z.z;
+                    vw[y][D / 32 - 1] = z.w;
+                }
+                // A granule that was not loaded holds what the ring held before, and a code behind the last
+                // key may be NaN in e4m3: 0 * NaN is not 0.
+                if (KIND == GPT2_KV8_E4M3 && masked && (pos + row >= n || !((ok >> gi) & 1u)))
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) vw[y][q] = 0;
+            }
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {  // 4 dims: column tiles 4 q .. 4 q + 3
-                uint32_t wk[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const uint2 vv = D == 64 ? x.v[4 * gi + y] : x.v[2 * y + q / 2];
-                    wk[y] = q & 1 ? vv.y : vv.x;
-                }
+                const uint32_t wk[4] = {vw[0][q], vw[1][q], vw[2][q], vw[3][q]};
                 uint32_t b0[4], b1[4];
                 pairs4<KIND>(wk[0], wk[1], b0);
                 pairs4<KIND>(wk[2], wk[3], b1);
@@ -357,33 +374,41 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
     };
 
     const int mine = chunks > warp ? (chunks - warp + NW - 1) / NW : 0;  // chunks warp, warp + NW, ...
-    C buf[2];
-    if (mine > 0) {
-        look_up(0);
-        load(buf[0], 0);
-    }
-    for (int i0 = 0; i0 < mine; i0 += 2) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int i = i0 + b;
-            if (i >= mine) break;
-            float ks[GR], vs[GR];
-            unsigned ok = 0;
-#pragma unroll
-            for (int gi = 0; gi < GR; ++gi) {
-                ks[gi] = __shfl_sync(0xFFFFFFFFu, gks, (i % SET) * GR + gi);
-                vs[gi] = __shfl_sync(0xFFFFFFFFu, gvs, (i % SET) * GR + gi);
+    // The look-up of a set must come before the loads of its chunks but after the last use of the set before: scales
+    // and validity of the chunks in flight are kept in registers, two sets deep.
+    float pks[2] = {}, pvs[2] = {};  // this lane's granule scales of the even and odd set
+    unsigned pok[2] = {};
+    auto fetch = [&](int i) {
+        if (i < mine) {
+            if (i % SET == 0) {
+                look_up(i / SET);
+                const int b = (i / SET) & 1;
+                if (b) pks[1] = gks, pvs[1] = gvs, pok[1] = gok;
+                else pks[0] = gks, pvs[0] = gvs, pok[0] = gok;
             }
-            ok = (gok >> ((i % SET) * GR)) & ((1u << GR) - 1u);
-            if (i + 1 < mine) {
-                if ((i + 1) % SET == 0) look_up((i + 1) / SET);
-                load(buf[b ^ 1], (i + 1) % SET);
-            }
-            compute(buf[b], i, lo + (i * NW + warp) * CK, ks, vs, ok);
+            load(i, i % STAGES);
         }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+    for (int i = 0; i < mine; ++i) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();  // every lane's copies of chunk i are there, and all are done with chunk i - 1
+        fetch(i + STAGES - 1);
+        const bool odd = (i / SET) & 1;
+        float ks[GR], vs[GR];
+#pragma unroll
+        for (int gi = 0; gi < GR; ++gi) {
+            ks[gi] = __shfl_sync(0xFFFFFFFFu, odd ? pks[1] : pks[0], (i % SET) * GR + gi);
+            vs[gi] = __shfl_sync(0xFFFFFFFFu, odd ? pvs[1] : pvs[0], (i % SET) * GR + gi);
+        }
+        const unsigned ok = ((odd ? pok[1] : pok[0]) >> ((i % SET) * GR)) & ((1u << GR) - 1u);
+        compute(ring + i % STAGES * CHUNK_BYTES, lo + (i * NW + warp) * CK, ks, vs, ok);
     }
     if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(c.status, ST_KV8_BAD_PAGE);
 
+    __syncthreads();  // every warp is through its ring
     // the warps' rows: thread (g, t) holds dims 16 t .. (D 64: columns j of tiles 2 t and 2 t + 1)
 #pragma unroll
     for (int rr = 0; rr < RR; ++rr) {
@@ -527,8 +552,15 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     a.nsplit = (longest + a.span - 1) / a.span;
     if (units * a.nsplit > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
     const kv8::View c = kv8::view(kv, ctx->status);
+    bool *attr_done = &ctx->kv8_attr_done[(kv->kind == GPT2_KV8_INT8 ? 0 : 4) + (kv->headDim == 64 ? 0 : 2) + (rows == 8 ? 0 : 1)];
     auto go = [&](auto kern) {
-        kern<<<static_cast<unsigned>(units * a.nsplit), 32 * kv8::NW, 0, stream>>>(c, a);
+        if (!*attr_done) {
+            RelaxedCapture relaxed;
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kv8::RING_BYTES) != cudaSuccess)
+                return GPT2_B200_ECUDA;
+            *attr_done = true;
+        }
+        kern<<<static_cast<unsigned>(units * a.nsplit), 32 * kv8::NW, kv8::RING_BYTES, stream>>>(c, a);
         return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
     };
     if (kv->kind == GPT2_KV8_INT8) {
