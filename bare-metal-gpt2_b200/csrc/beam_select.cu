@@ -3,15 +3,16 @@
 // total(w, v) = score[w] + (x[w, v] - lse[w]), lse = m + log(sum exp(x - m)); a finished beam is the one candidate
 // (w, eos) with its score. Within a beam totals fall as logits do, so a beam's W largest logits hold all
 // of its candidates that matter: a row is read once, for the running maximum and sum and for its W largest logits.
-// Bound by reading the logits from HBM (2 or 4 bytes each; about 8 instructions per value).
+// Bound by reading the logits from HBM (2 or 4 bytes each) and by issuing about 6 instructions per value.
 //
 //   - Every warp streams its own part of a row through a ring of its own in shared memory (cp.async), so the main loop
-//     has no CTA barrier and a warp has up to STAGES - 1 steps in flight. Lanes own values by their index, whatever the
-//     row's alignment: equal rows get equal sums. A row that does not start on a 16-byte boundary is copied in aligned
-//     granules and a lane's values are cut out of two neighbouring ones.
-//   - The warp's W largest so far are a sorted list, lane j holding the j-th; its last entry is the threshold that a value
-//     must pass to be inserted (about W ln(n / W) of n values do). The first step starts from a threshold that at
-//     least W values reach: the W-th largest of the lanes' maxima.
+//     has no CTA barrier and a warp has up to STAGES - 1 steps in flight. Rows are copied in aligned 16-byte
+//     granules; lanes then take values by their index (neighbouring lanes neighbouring words, so that any alignment of
+//     the row is read without bank conflicts), and equal rows get equal sums wherever they lie.
+//   - The warp's W largest so far are a sorted list, lane j holding the j-th. A value is inserted if it reaches a
+//     threshold that at least W values of the row reach: the list's last entry, or the smallest of the CTA's 8
+//     warps' K-th largest, K = ceil(W / 8). The first step, without lists yet, takes the lanes' maxima for that. So about
+//     W ln(n / W) of a CTA's n values are inserted; the others cost no more than their share of a maximum.
 //   - Logits are compared as 64-bit keys: the value's orderable bits, then the inverted token, so equal logits go to the
 //     lower token whatever the order of arrival.
 //   - Sorted lists are merged by W rounds of a maximum over their heads, a lane per list: the warps' in a CTA, the CTAs' of
@@ -29,9 +30,11 @@ constexpr int MAX_W = 32;
 constexpr int NWARP = 8, NT = 32 * NWARP;
 constexpr int MAX_CHUNKS = 64;  // CTAs of a row: two list heads per lane
 constexpr int ROW_KEYS = 256;   // CTAs x W of a row, at most
-constexpr int VPT = 2;          // 16-byte granules per lane and step
-constexpr int STAGES = 6;
-constexpr int STAGE_BYTES = (32 * VPT + 1) * 16;  // and the granule behind, for rows that are not aligned
+constexpr int NV = 16;          // values per lane and step
+constexpr int STAGES = 4;
+// A step's granules, and the one behind for rows that are not aligned.
+template <typename T>
+constexpr int stage_bytes() { return 32 * NV * static_cast<int>(sizeof(T)) + 16; }
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long key_t;
@@ -78,17 +81,20 @@ __device__ __forceinline__ void merge_ml(float &m, float &l, float m2, float l2)
     l = l * ex2((m - mx) * LOG2E) + l2 * ex2((m2 - mx) * LOG2E);
     m = mx;
 }
+__device__ __forceinline__ unsigned ordered(float x) {
+    const unsigned u = __float_as_uint(x);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(unsigned o) {
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
 // (m, l) over the warp, the same bits in every lane.
 __device__ __forceinline__ void warp_ml(float &m, float &l) {
+    const float mx = from_ordered(__reduce_max_sync(0xFFFFFFFFu, ordered(m)));
+    l = m > -INFINITY ? l * ex2((m - mx) * LOG2E) : 0.0f;
+    m = mx;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, o);
-        const bool upper = threadIdx.x & o;  // both sides add in the same order
-        float a = upper ? m2 : m, b = upper ? l2 : l;
-        merge_ml(a, b, upper ? m : m2, upper ? l : l2);
-        m = a;
-        l = b;
-    }
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
 }
 // Merges n <= 64 descending lists of W keys (list i at a + i * W), one or two heads per lane; round j's
 // winner goes to put(j, key, list). Stops when all are used up and returns how many were put.
@@ -119,36 +125,34 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint32_t (&w)[4], float *v);
-template <>
-__device__ __forceinline__ void unpack<float>(const uint32_t (&w)[4], float *v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+// Two fp32 additions / multiplications as one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
-template <>
-__device__ __forceinline__ void unpack<__half>(const uint32_t (&w)[4], float *v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
-
 template <typename T>
 __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
-    constexpr int EV = 16 / sizeof(T);    // values per granule
-    constexpr int STEP = 32 * VPT * EV;   // values per warp and step
-    constexpr int NV = VPT * EV;          // values per lane and step
+    constexpr int EV = 16 / sizeof(T);       // values per granule
+    constexpr int STEP = 32 * NV;            // values per warp and step
+    constexpr int GPL = NV / EV;             // granules per lane and step
+    constexpr int STAGE_BYTES = stage_bytes<T>();
     extern __shared__ __align__(16) uint8_t ring_all[];
     // behind the main loop the rings' memory holds the lists that are merged
     key_t (*lists)[ROW_KEYS] = reinterpret_cast<key_t (*)[ROW_KEYS]>(ring_all);
     key_t *totals = reinterpret_cast<key_t *>(ring_all + NWARP * ROW_KEYS * sizeof(key_t));  // [W][W]
     int *tokens = reinterpret_cast<int *>(totals + MAX_W * MAX_W);                           // [W][W]
-    static_assert(NWARP * ROW_KEYS * 8 + MAX_W * MAX_W * 12 <= NWARP * STAGES * STAGE_BYTES, "lists fit in the rings");
+    static_assert(NWARP * ROW_KEYS * 8 + MAX_W * MAX_W * 12 <= NWARP * STAGES * stage_bytes<T>(), "lists fit in the rings");
     __shared__ float red_m[NWARP], red_l[NWARP];
     __shared__ int is_last;
+    __shared__ float kth[NWARP];  // each warp's K-th largest value so far
     __shared__ float s_score[MAX_W];
     __shared__ int s_done[MAX_W];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -156,104 +160,139 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
     const int item = blockIdx.x / (W * p.chunks), rest = blockIdx.x - item * (W * p.chunks);
     const int w = rest / p.chunks, ch = rest - w * p.chunks;
     const long long row = static_cast<long long>(item) * W + w;
-    const bool alive = p.score[row] > -INFINITY && !(p.done && p.done[row]);
-    if (alive) {
-        const T *x = static_cast<const T *>(p.logits) + row * p.ld;
-        const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-        const unsigned cut = shift * sizeof(T);
-        uint8_t *ring = ring_all + warp * STAGES * STAGE_BYTES;
-        const int begin = (ch * p.steps * NWARP + warp) * STEP;  // step s: values begin + s * NWARP * STEP ..
-        int steps = begin < V ? min(p.steps, (V - begin + NWARP * STEP - 1) / (NWARP * STEP)) : 0;
-        // Granule g of a step holds values base + g * EV - shift ..; outside the row they are -inf. One that
-        // reaches over the row's ends is read value by value.
-        auto fetch = [&](uint8_t *dst, int at) {
-            if (at >= 0 && at + EV <= V) {
-                cp_async16(dst, x + at);
+    const float my_score = p.score[row];
+    const int my_done = p.done ? p.done[row] : 0;
+    const T *x = static_cast<const T *>(p.logits) + row * p.ld;
+    const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    const unsigned cut = shift * sizeof(T);
+    uint8_t *ring = ring_all + warp * STAGES * STAGE_BYTES;
+    const int begin = (ch * p.steps * NWARP + warp) * STEP;  // step s: values begin + s * NWARP * STEP ..
+    int steps = begin < V ? min(p.steps, (V - begin + NWARP * STEP - 1) / (NWARP * STEP)) : 0;
+    // Granule g of a step holds values base + g * EV - shift ..; outside the row they are -inf. One that
+    // reaches over the row's ends is read value by value.
+    auto fetch = [&](uint8_t *dst, int at) {
+        if (at >= 0 && at + EV <= V) {
+            cp_async16(dst, x + at);
+        } else {
+            T part[EV];
+#pragma unroll
+            for (int j = 0; j < EV; ++j) part[j] = at + j >= 0 && at + j < V ? x[at + j] : static_cast<T>(-INFINITY);
+            *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(part);
+        }
+    };
+    auto load = [&](int s) {
+        if (s < max(steps, 1)) {
+            uint8_t *dst = ring + s % STAGES * STAGE_BYTES;
+            const int base = begin + s * (NWARP * STEP) - shift;
+            if (base >= 0 && base + STEP + EV <= V) {  // whole step inside the row
+                const T *src = x + base + lane * EV;
+#pragma unroll
+                for (int q = 0; q < GPL; ++q) cp_async16(dst + (q * 32 + lane) * 16, src + q * 32 * EV);
+                if (lane == 0) cp_async16(dst + 32 * GPL * 16, src + GPL * 32 * EV);
             } else {
-#pragma unroll
-                for (int j = 0; j < EV; ++j)
-                    reinterpret_cast<T *>(dst)[j] = at + j >= 0 && at + j < V ? x[at + j] : static_cast<T>(-INFINITY);
+                for (int q = 0; q < GPL; ++q) fetch(dst + (q * 32 + lane) * 16, base + (q * 32 + lane) * EV);
+                if (lane == 0) fetch(dst + 32 * GPL * 16, base + 32 * GPL * EV);
             }
-        };
-        auto load = [&](int s) {
-            if (s < steps) {
-                uint8_t *dst = ring + s % STAGES * STAGE_BYTES;
-                const int base = begin + s * (NWARP * STEP) - shift;
+        }
+        cp_async_commit();
+    };
 #pragma unroll
-                for (int q = 0; q < VPT; ++q) fetch(dst + (q * 32 + lane) * 16, base + (q * 32 + lane) * EV);
-                if (cut && lane == 0) fetch(dst + 32 * VPT * 16, base + 32 * VPT * EV);
-            }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) load(s);
+    for (int s = 0; s < STAGES - 1; ++s) load(s);  // before the beam's state is there: most beams are alive
+    const bool alive = my_score > -INFINITY && !my_done;
+    if (!alive) cp_async_wait<0>();
+    if (alive) {
         float m = -INFINITY, l = 0.0f;
         key_t mine = 0, worst = 0;  // the j-th largest key in lane j; the W-th
-        float thr = -INFINITY;
+        float thr = -INFINITY, low = -INFINITY;
         bool bad = false;
-        for (int s = 0; s < steps; ++s) {
+        const int K = (W + NWARP - 1) / NWARP;
+        for (int s = 0; s < max(steps, 1); ++s) {  // a warp without values has one step of -inf, for the barrier in it
             cp_async_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of step s are there, and all are done with step s - 1
             load(s + STAGES - 1);
-            const uint4 *src = reinterpret_cast<const uint4 *>(ring + s % STAGES * STAGE_BYTES);
-            float v[NV];
+            // value i of lane: fp32: 32 i + lane; fp16: 64 (i / 2) + 2 lane + i % 2
+            const uint8_t *src = ring + s % STAGES * STAGE_BYTES + (cut & ~3u) + lane * 4;
+            float2 v[NV / 2];
+            float top;
+            if (sizeof(T) == 4) {
 #pragma unroll
-            for (int q = 0; q < VPT; ++q) {
-                const uint4 a = src[q * 32 + lane];
-                uint32_t o[4] = {a.x, a.y, a.z, a.w};
-                if (cut) {
-                    const uint4 b = src[q * 32 + lane + 1];
-                    uint32_t c[5];
-                    switch (cut >> 2) {
-                        case 0: c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w, c[4] = b.x; break;
-                        case 1: c[0] = a.y, c[1] = a.z, c[2] = a.w, c[3] = b.x, c[4] = b.y; break;
-                        case 2: c[0] = a.z, c[1] = a.w, c[2] = b.x, c[3] = b.y, c[4] = b.z; break;
-                        default: c[0] = a.w, c[1] = b.x, c[2] = b.y, c[3] = b.z, c[4] = b.w; break;
-                    }
+                for (int i = 0; i < NV / 2; ++i)
+                    v[i] = make_float2(*reinterpret_cast<const float *>(src + 256 * i), *reinterpret_cast<const float *>(src + 256 * i + 128));
+                top = max_nan(v[0].x, v[0].y);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(c[i], c[i + 1], (cut & 2) * 8);
+                for (int i = 1; i < NV / 2; ++i) top = max_nan(top, max_nan(v[i].x, v[i].y));
+            } else {
+                __half2 h[NV / 2];
+#pragma unroll
+                for (int i = 0; i < NV / 2; ++i) {
+                    uint32_t u = *reinterpret_cast<const uint32_t *>(src + 128 * i);
+                    if (cut & 2) u = __funnelshift_r(u, *reinterpret_cast<const uint32_t *>(src + 128 * i + 4), 16);
+                    h[i] = *reinterpret_cast<const __half2 *>(&u);
+                    v[i] = __half22float2(h[i]);
                 }
-                unpack<T>(o, v + q * EV);
-            }
-            float top = v[0];
 #pragma unroll
-            for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
+                for (int o = NV / 4; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < o; ++i) h[i] = __hmax2_nan(h[i], h[i + o]);
+                const float2 f = __half22float2(h[0]);
+                top = max_nan(f.x, f.y);
+            }
             if (!(top < INFINITY)) {  // NaN and +inf count as masked
                 bad = true;
                 top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    v[i] = v[i] < INFINITY ? v[i] : -INFINITY;
-                    top = fmaxf(top, v[i]);
+                for (int i = 0; i < NV / 2; ++i) {
+                    v[i].x = v[i].x < INFINITY ? v[i].x : -INFINITY;
+                    v[i].y = v[i].y < INFINITY ? v[i].y : -INFINITY;
+                    top = fmaxf(top, fmaxf(v[i].x, v[i].y));
                 }
             }
             if (top > m) {
                 l *= ex2((m - top) * LOG2E);
                 m = top;
             }
-            if (m > -INFINITY) {
+            if (m > -INFINITY) {  // m subtracted first: exact near m, where it counts
+                const float2 mm = make_float2(-m, -m), ll = make_float2(LOG2E, LOG2E);
+                float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) l += ex2((v[i] - m) * LOG2E);  // m subtracted first: exact near m, where it counts
-            }
-            if (s == 0) {  // the W-th largest of the 32 lane maxima: no W values are lost below it
-                int rank = 0;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float u = __shfl_sync(0xFFFFFFFFu, top, i);
-                    rank += u > top || (u == top && i < lane);
+                for (int i = 0; i < NV / 2; ++i) {
+                    const float2 e = mul2(add2(v[i], mm), ll);
+                    sum = add2(sum, make_float2(ex2(e.x), ex2(e.y)));
                 }
-                const unsigned who = __ballot_sync(0xFFFFFFFFu, rank == W - 1);
-                thr = __shfl_sync(0xFFFFFFFFu, top, __ffs(who) - 1);
+                l += sum.x + sum.y;
             }
+            if (s == 0) {
+                unsigned o = ordered(top), mx = 0;
+                for (int j = 0; j < K; ++j) {
+                    mx = __reduce_max_sync(0xFFFFFFFFu, o);
+                    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, o == mx)) - 1) o = 0;
+                }
+                if (lane == 0) kth[warp] = from_ordered(mx);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int i = 0; i < NWARP; i += 4) {
+                const volatile float *kv = kth + i;
+                low = fminf(i ? low : INFINITY, fminf(fminf(kv[0], kv[1]), fminf(kv[2], kv[3])));
+            }
+            thr = fmaxf(thr, low);
             if (!__any_sync(0xFFFFFFFFu, top >= thr && top > -INFINITY)) continue;
-            const unsigned first = begin + s * (NWARP * STEP) + lane * EV;
+            unsigned mask = 0;  // this lane's values that reach the threshold
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const bool in = v[i] >= thr && v[i] > -INFINITY;
-                unsigned todo = __ballot_sync(0xFFFFFFFFu, in);
-                if (!todo) continue;
-                const key_t k = lin::argmax_key(v[i], first + i / EV * 32 * EV + i % EV);
-                todo = __ballot_sync(0xFFFFFFFFu, in && k > worst);
+                const float y = i & 1 ? v[i / 2].y : v[i / 2].x;
+                if (y >= thr && y > -INFINITY) mask |= 1u << i;
+            }
+            while (__any_sync(0xFFFFFFFFu, mask)) {
+                key_t k = 0;
+                if (mask) {
+                    const int i = __ffs(mask) - 1;
+                    mask &= mask - 1;
+                    const unsigned at = sizeof(T) == 4 ? 32 * i + lane : 64 * (i >> 1) + 2 * lane + (i & 1);
+                    const T y = *reinterpret_cast<const T *>(ring + s % STAGES * STAGE_BYTES + cut + at * sizeof(T));
+                    k = lin::argmax_key(static_cast<float>(y), begin + s * (NWARP * STEP) + at);
+                }
+                unsigned todo = __ballot_sync(0xFFFFFFFFu, k > worst);
                 while (todo) {
                     const int from = __ffs(todo) - 1;
                     todo &= todo - 1;
@@ -263,8 +302,9 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
                     if (lane >= rank && lane < W) mine = lane == rank ? in_key : up;
                 }
                 worst = __shfl_sync(0xFFFFFFFFu, mine, W - 1);
-                if (worst) thr = key_value(worst);
             }
+            if (worst) thr = fmaxf(thr, key_value(worst));
+            if (lane == K - 1 && mine) *const_cast<volatile float *>(&kth[warp]) = fmaxf(kth[warp], key_value(mine));
         }
         warp_ml(m, l);
         if (lane == 0) {
@@ -288,21 +328,21 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         }
     }
     // the last CTA of the item goes on
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        const unsigned seen = atomicAdd(&p.arrive[item], 1u);
-        is_last = seen == static_cast<unsigned>(W * p.chunks - 1);
-        if (is_last) p.arrive[item] = 0;
-    }
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
     const int first_row = item * W;
     if (tid < W) {
         s_score[tid] = p.score[first_row + tid];
         s_done[tid] = p.done ? p.done[first_row + tid] : 0;
     }
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();  // the CTA's results, ordered before it by the barrier, are visible with the count
+        const unsigned seen = atomicAdd(&p.arrive[item], 1u);
+        is_last = seen == static_cast<unsigned>(W * p.chunks - 1);
+        if (is_last) p.arrive[item] = 0;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!is_last) return;
     for (int i = tid; i < W * W; i += NT) totals[i] = 0;
     __syncthreads();
     // a warp per beam: lse, the beam's W best logits, their totals
@@ -366,16 +406,25 @@ static Layout layout(int B, int W) {
 
 template <typename T>
 static int launch(Params p, int B, int num_sms, bool *attr_done, cudaStream_t stream) {
-    constexpr int STEP = 32 * VPT * (16 / static_cast<int>(sizeof(T)));
-    constexpr int SMEM = NWARP * STAGES * STAGE_BYTES;
+    constexpr int STEP = 32 * NV;
+    constexpr int SMEM = NWARP * STAGES * stage_bytes<T>();
     const long long rows = static_cast<long long>(B) * p.W;
-    // CTAs of a row: about four per SM in all; down to one step per warp when rows are few (bound by the latency
-    // of one CTA), the whole row when they are many.
+    // CTAs of a row. One pass of all resident CTAs costs a CTA's steps and about as much as FIXED steps to start and to
+    // merge; the number of CTAs per row that makes passes x cost least is taken. Few rows so come down to one step per warp,
+    // and many rows do not leave a last pass with a few CTAs.
+    constexpr long long FIXED = 3;
+    const long long slots = static_cast<long long>(num_sms) * (228 * 1024 / (SMEM + 2048));
     const long long groups = (p.V + NWARP * STEP - 1) / (NWARP * STEP);  // steps of a CTA that had the row to itself
-    long long chunks = (4ll * num_sms + rows - 1) / rows;
-    chunks = std::min<long long>({chunks, groups, max_chunks(p.W)});
-    p.steps = static_cast<int>((groups + chunks - 1) / chunks);
-    p.chunks = static_cast<int>((groups + p.steps - 1) / p.steps);
+    long long best = 0;
+    for (long long c = 1; c <= std::min<long long>(groups, max_chunks(p.W)); ++c) {
+        const long long steps = (groups + c - 1) / c, used = (groups + steps - 1) / steps;
+        const long long cost = (rows * used + slots - 1) / slots * (steps + FIXED);
+        if (used == c && (!best || cost < best)) {
+            best = cost;
+            p.chunks = static_cast<int>(c);
+            p.steps = static_cast<int>(steps);
+        }
+    }
     const long long grid = rows * p.chunks;
     if (grid > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
     if (!*attr_done) {

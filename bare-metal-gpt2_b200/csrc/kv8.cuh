@@ -21,9 +21,6 @@ struct View {
     int nPages, nRow, maxPages, nLayer, nHead, D, page, block, page_shift, block_shift;
     unsigned *status;
 
-    __host__ __device__ long long run(int p, int L, int which, int h) const {  // runs before this one
-        return ((static_cast<long long>(p) * nLayer + L) * 2 + which) * nHead + h;
-    }
 };
 
 // Work area: counters (zero between calls), then the planner's lists, then the attention's partials.
@@ -32,7 +29,7 @@ struct Work {
     unsigned *arrive;    // [attend_max_ctas()] split-merge arrivals, one per tile of query rows
     int4 *copies;        // [nRow] (source, destination, positions, unused)
     int *list;           // [nPages] free pages found / new id of a moved page
-    int *table0, *len0;  // [nRow][maxPages], [nRow]: the state before a reorder
+    int2 *moves;         // [nPages / 2] (source, destination) of a compaction
     float *part;         // split partials
     size_t bytes;
 };
@@ -47,7 +44,10 @@ inline bool shape_ok(const GPT2KV8Cache *kv) {
     return kv && kv->nPages >= 1 && kv->nRow >= 1 && kv->nRow <= MAX_ROWS && kv->maxPages >= 1 &&
            kv->nLayer >= 1 && kv->nHead >= 1 && (kv->headDim == 64 || kv->headDim == 128) &&
            shift_of(kv->page) > 0 && shift_of(kv->block) > 0 && kv->block <= kv->page &&
-           static_cast<long long>(kv->maxPages) * kv->page <= 0x3FFFFFFFll &&
+           static_cast<long long>(kv->maxPages) * kv->page <= 0x3FFFFFFFll && kv->nHead <= 65535 &&
+           static_cast<long long>(kv->nRow) * kv->maxPages <= 0x7FFFFFFFll &&
+           // rows of codes (a position of one page, layer, K|V and head) are counted in 32 bits: 256 GB of them and more
+           static_cast<double>(kv->nPages) * kv->nLayer * 2.0 * kv->nHead * kv->page < 4294967296.0 &&
            (kv->kind == GPT2_KV8_INT8 || kv->kind == GPT2_KV8_E4M3);
 }
 
@@ -59,16 +59,14 @@ inline Work work_layout(const GPT2KV8Cache *kv, int Hq, int Tq) {
     const size_t group_rows = static_cast<size_t>(Tq) * (Hq / kv->nHead);
     const size_t rows = group_rows < ATT_TILE ? group_rows : ATT_TILE;
     const size_t o_arr = 256, o_cop = o_arr + up(attend_max_ctas() * 4ull), o_list = o_cop + up(kv->nRow * sizeof(int4));
-    const size_t o_tab = o_list + up(static_cast<size_t>(kv->nPages) * 4);
-    const size_t o_len = o_tab + up(static_cast<size_t>(kv->nRow) * kv->maxPages * 4);
-    const size_t o_part = o_len + up(kv->nRow * 4ull);
+    const size_t o_mov = o_list + up(static_cast<size_t>(kv->nPages) * 4);
+    const size_t o_part = o_mov + up(static_cast<size_t>(kv->nPages / 2 + 1) * sizeof(int2));
     char *b = static_cast<char *>(kv->work);
     w.misc = reinterpret_cast<unsigned *>(b);
     w.arrive = reinterpret_cast<unsigned *>(b + o_arr);
     w.copies = reinterpret_cast<int4 *>(b + o_cop);
     w.list = reinterpret_cast<int *>(b + o_list);
-    w.table0 = reinterpret_cast<int *>(b + o_tab);
-    w.len0 = reinterpret_cast<int *>(b + o_len);
+    w.moves = reinterpret_cast<int2 *>(b + o_mov);
     w.part = reinterpret_cast<float *>(b + o_part);
     w.bytes = o_part + up(attend_max_ctas() * rows * (kv->headDim + 2) * sizeof(float));
     return w;

@@ -19,9 +19,17 @@
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
 //   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
-//     vscale the warp has met; o is kept in units of S.
-// A CTA is 4 warps on one (row, K/V head, tile of 16 query rows, span of keys): the warps take chunks in turn and are
-// merged in shared memory; spans (few rows, long contexts) through the work area by the last CTA to arrive, in span order.
+//     vscale of the granules looked up so far; o is kept in units of S.
+//   - m is not the maximum but within 2^LAZY of it: p stays below 2^LAZY, far inside fp16 and fp32, and most chunks need
+//     neither the row maximum's shuffles nor a rescaling of o.
+//
+// Work: a unit is (cache row, tile of 8 or 16 query rows, K/V head) with its chunks of keys, and a CTA's 4 warps take chunks
+// in turn. With units in plenty each has a CTA. With fewer units than resident CTAs all chunks of all units form one
+// sequence and every CTA takes an equal piece of it, found from the rows' lengths by a prefix sum, its loads running ahead over
+// unit borders. At a border the warps are merged in shared memory; a unit cut by a piece's end is merged
+// through the work area by the last CTA to arrive, in piece order.
+#include <algorithm>
+
 #include "kv8.cuh"
 #include "ptx.cuh"
 
@@ -29,21 +37,22 @@ namespace b200 {
 namespace kv8 {
 
 constexpr int NW = 4;                // warps per CTA
-constexpr int MAX_SPLIT_CTAS = 2048; // grid of a launch that splits keys, at most
+constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
+constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
+constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
 
-int attend_max_ctas() { return MAX_SPLIT_CTAS; }
+int attend_max_ctas() { return 2 * MAX_PIECES; }  // a piece cuts two units at most
 
 struct AttParams {
     const __half *q;
     __half *out;
     long long q_row, q_tok, o_row, o_tok;
     const int *d_first, *d_count;
-    long long page_stride;  // bytes from a page to the next
-    long long k_off, v_off; // from a page's start to this layer's K / V runs of head 0
+    unsigned page_runs, k_run;  // runs of a page (layers x 2 x heads), of it before this layer's K
     float *part;
     unsigned *arrive;
     int L, G, Tq, count, max_len;
-    int qtiles, nsplit, span;  // span: keys per split, a multiple of NW * CK
+    int qtiles, entries;  // entries: (row, tile) pairs of a launch in equal pieces, 0: one unit per CTA
     float scale_log2;
 };
 
@@ -58,6 +67,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with a zero accumulator.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// A copy that the compiler takes for another value. An MMA's four A operands are neighbouring registers: a value
+// that is two of them would be moved there before every MMA.
+__device__ __forceinline__ uint32_t twin(uint32_t v) {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -134,91 +157,138 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
     using C = Chunk<D>;
     constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
     constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
+    constexpr int SO_BYTES = NW * ROWS * (D + 4) * 4;
     extern __shared__ __align__(128) uint8_t ring_all[];
-    float (*so)[ROWS][D + 4] = reinterpret_cast<float (*)[ROWS][D + 4]>(ring_all);  // [NW], behind the main loop
-    static_assert(NW * ROWS * (D + 4) * 4 <= RING_BYTES, "the warps' rows fit in the rings");
+    float (*so)[ROWS][D + 4] = reinterpret_cast<float (*)[ROWS][D + 4]>(ring_all + RING_BYTES);  // [NW]
+    int *pre = reinterpret_cast<int *>(ring_all + RING_BYTES + SO_BYTES);  // [entries + 1]: chunks before each entry
     __shared__ float sm[NW][ROWS], sl[NW][ROWS];
-    __shared__ int is_last;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % a.nsplit;
-    int unit = blockIdx.x / a.nsplit;
-    const int h = unit % c.nHead;
-    unit /= c.nHead;
-    const int qt = unit % a.qtiles, r = unit / a.qtiles;
+    __shared__ int is_last, warp_sum[NW];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int R = a.G * a.Tq;
+    const bool one = a.Tq == 1;  // then no row needs a division to find its token
 
-    int n = c.len[r] + (a.d_count ? a.d_count[r] : a.count);
-    if (n < 0 || n > a.max_len) {
-        if (threadIdx.x == 0 && split == 0 && h == 0 && qt == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
-        n = 0;
-    }
-    const int first = a.d_first ? max(a.d_first[r], 0) : 0;
-    // keys that some row of the tile sees: [first, last_end); rows of one token see the same
-    const int last_row = min(qt * ROWS + ROWS, R) - 1;
-    const int last_end = n - a.Tq + last_row / a.G + 1, first_end = n - a.Tq + qt * ROWS / a.G + 1;
-    const int base = first & ~(CK - 1);
-    const int total = last_end > first ? last_end - base : 0;
-    const int active = (total + a.span - 1) / a.span;  // splits with keys
-    if (split >= max(active, 1)) return;
-    const int lo = base + split * a.span, hi = min(lo + a.span, last_end);
-    const int chunks = total ? (hi - lo + CK - 1) / CK : 0;
-
-    // q: thread (g, t) holds dims 64 * (s / 4) + 16 t + 4 (s % 4) .. + 3 of row g (and g + 8) for k-step s
-    uint32_t qa[KS][2 * RR];
-    int end[RR];
-#pragma unroll
-    for (int rr = 0; rr < RR; ++rr) {
-        const int i = qt * ROWS + g + 8 * rr;
-        const bool ok = i < R;
-        const int tok = ok ? i / a.G : 0;
-        end[rr] = ok ? n - a.Tq + tok + 1 : 0;
-        const __half *qp = a.q + r * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + 16 * t;
-#pragma unroll
-        for (int s4 = 0; s4 < KS / 4; ++s4) {
-            uint4 x[2] = {};
-            if (ok) {
-                x[0] = *reinterpret_cast<const uint4 *>(qp + 64 * s4);
-                x[1] = *reinterpret_cast<const uint4 *>(qp + 64 * s4 + 8);
-            }
-            const uint32_t *w = reinterpret_cast<const uint32_t *>(x);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                qa[4 * s4 + s][rr] = w[2 * s];
-                qa[4 * s4 + s][RR + rr] = w[2 * s + 1];
-            }
+    // Entry e: row r, its tile qt, the keys [first, last_end) that some query of the tile sees, in chunks from base on.
+    int r, qt, n, first, base, last_end;
+    auto entry = [&](int e) {
+        r = e, qt = 0;
+        if (a.qtiles > 1) {
+            r = e / a.qtiles;
+            qt = e - r * a.qtiles;
         }
+        n = c.len[r] + (a.d_count ? a.d_count[r] : a.count);
+        if (n < 0 || n > a.max_len) n = -1;
+        first = a.d_first ? max(a.d_first[r], 0) : 0;
+        last_end = one ? n : n - a.Tq + (min(qt * ROWS + ROWS, R) - 1) / a.G + 1;
+        base = first & ~(CK - 1);
+        return last_end > first ? (last_end - base + CK - 1) / CK : 0;
+    };
+    auto put = [&](int h, int row, int d, float x) {
+        const int i = qt * ROWS + row, tok = one ? 0 : i / a.G;
+        a.out[r * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
+    };
+    auto no_keys = [&](int h) {
+        for (int x = tid; x < min(ROWS, R - qt * ROWS) * D; x += 32 * NW) put(h, x / D, x % D, 0.0f);
+    };
+
+    int c0, c1, per = 1;  // this CTA's chunks
+    if (a.entries) {
+        const int own = (a.entries + 32 * NW - 1) / (32 * NW), e0 = min(tid * own, a.entries), e1 = min(e0 + own, a.entries);
+        int sum = 0;
+        for (int e = e0; e < e1; ++e) {
+            pre[e] = sum;
+            const int ch = entry(e);
+            sum += ch * c.nHead;
+            if (n < 0 && blockIdx.x == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
+        }
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            if (lane >= o) before += u;
+        }
+        if (lane == 31) warp_sum[warp] = before;
+        before -= sum;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) before += warp_sum[w];
+            total += warp_sum[w];
+        }
+        for (int e = e0; e < e1; ++e) pre[e] += before;
+        if (tid == 0) pre[a.entries] = total;
+        __syncthreads();
+        per = ((total + gridDim.x - 1) / gridDim.x + NW - 1) & ~(NW - 1);
+        c0 = min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total));
+        c1 = min(c0 + per, total);
+        for (int e = blockIdx.x; e < a.entries; e += gridDim.x)
+            if (pre[e] == pre[e + 1]) {
+                entry(e);
+                for (int h = 0; h < c.nHead; ++h) no_keys(h);
+            }
+    } else {
+        c0 = 0;
+        c1 = entry(blockIdx.x);
+        if (n < 0 && tid == 0 && blockIdx.y == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
+        if (c1 == 0) no_keys(blockIdx.y);
     }
+    // The unit of chunk x: sets entry()'s values, h and the unit's first chunk u0; returns its chunks.
+    int h = blockIdx.y, u0 = 0;
+    auto unit_of = [&](int x) {
+        int e = blockIdx.x;
+        if (a.entries) {
+            int lo = 0, hi = a.entries;  // the last entry with pre <= x (entries without chunks come before it)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (pre[mid] <= x) lo = mid;
+                else hi = mid;
+            }
+            e = lo;
+        }
+        const int ch = entry(e);
+        if (a.entries) {
+            h = (x - pre[e]) / ch;
+            u0 = pre[e] + h * ch;
+        }
+        return ch;
+    };
 
-    float o[DT][4];
-#pragma unroll
-    for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-    float m[RR], l[RR], S = 0.0f, invS = 0.0f;
-#pragma unroll
-    for (int rr = 0; rr < RR; ++rr) m[rr] = -INFINITY, l[rr] = 0.0f;
-
-    // this lane's granule of the current set: its page's byte offset and its scales
-    long long goff = 0;
-    float gks = 0.0f, gvs = 0.0f;
+    // this lane's granule of the current set: its first code row of K (rows are counted in 32 bits) and its scales
+    unsigned grow = 0;
+    // A block of zeros has scale 0; TINY in its place keeps -inf (a masked score) times a scale from being NaN.
+    constexpr float TINY = 1e-20f;
+    float gks = TINY, gvs = 0.0f, gvmax = 0.0f;
     unsigned gok = 0;
     bool bad = false;
     auto look_up = [&](int set) {
-        const int pos = lo + ((set * SET + lane / GR) * NW + warp) * CK + (lane % GR) * 16;
-        int ok = pos < hi && pos + 16 > first;
+        const int r_ = r, qt_ = qt, n_ = n, first_ = first, base_ = base, last_end_ = last_end, h_ = h, u0_ = u0;
+        const int x = c0 + (set * SET + lane / GR) * NW + warp;
+        int ok = x < c1, pos = 0;
+        if (ok) {
+            unit_of(x);
+            pos = base + (x - u0) * CK + (lane % GR) * 16;
+            ok = pos < last_end && pos + 16 > first;
+        }
         if (ok) {
             const int p = c.table[static_cast<long long>(r) * c.maxPages + (pos >> c.page_shift)];
             if (p < 0 || p >= c.nPages) {
                 bad = true;
                 ok = 0;
             } else {
-                const int ip = pos & (c.page - 1), nb = c.page >> c.block_shift;
-                const long long run = c.run(p, a.L, 0, h);
-                gks = c.scale[run * nb + (ip >> c.block_shift)] * a.scale_log2;
-                gvs = c.scale[(run + c.nHead) * nb + (ip >> c.block_shift)];
-                goff = p * a.page_stride + static_cast<long long>(h << c.page_shift) * D + ip * D;
+                const unsigned ip = pos & (c.page - 1), run = p * a.page_runs + a.k_run + h;
+                const int sub = c.page_shift - c.block_shift;
+                gks = fmaxf(c.scale[(run << sub) + (ip >> c.block_shift)] * a.scale_log2, TINY);
+                gvs = c.scale[((run + c.nHead) << sub) + (ip >> c.block_shift)];
+                grow = (run << c.page_shift) + ip;
             }
         }
-        if (!ok) gks = gvs = 0.0f;
+        if (!ok) {
+            gks = TINY;
+            gvs = 0.0f;
+        }
         gok = __ballot_sync(0xFFFFFFFFu, ok);
+        gvmax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(gvs)));  // scales are not negative
+        r = r_, qt = qt_, n = n_, first = first_, base = base_, last_end = last_end_, h = h_, u0 = u0_;
     };
     uint8_t *ring = ring_all + warp * STAGES * CHUNK_BYTES;
     const uint32_t ring_s = smem_u32(ring);
@@ -228,52 +298,55 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
     const int vrow = D == 64 ? ((lane >> 2) & 1) * 2 + ((lane >> 3) & 1) + (lane >> 4) * 4 : krow;
     const int cgr = lane & (C::ROWG - 1);
     constexpr int CR = 32 / C::ROWG;  // rows per copy instruction
+    const uint8_t *kbase = c.data + krow * D + cgr * 16;
+    const uint8_t *vbase = c.data + vrow * D + cgr * 16 + (static_cast<size_t>(c.nHead) << c.page_shift) * D;
+    // C::k_at and C::v_at of this lane's granule, without the multiples of 8 (D 64) or 4 rows that are immediates below
+    const int ko = C::k_at(krow, cgr) * 16, vo0 = 2048 + C::v_at(vrow, cgr) * 16, vo1 = 2048 + C::v_at(vrow, cgr ^ (D == 64 ? 0 : 4)) * 16;
     auto load = [&](int i, int stage) {  // chunk i of this warp; its set has been looked up
         const uint32_t dst = ring_s + stage * CHUNK_BYTES;
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
             const int src_lane = (i % SET) * GR + gi;
-            const long long off = __shfl_sync(0xFFFFFFFFu, goff, src_lane);
+            const unsigned row0 = __shfl_sync(0xFFFFFFFFu, grow, src_lane);
             if (!((gok >> src_lane) & 1u)) continue;
-            const uint8_t *kp = c.data + a.k_off + off + krow * D + cgr * 16;
-            const uint8_t *vp = c.data + a.v_off + off + vrow * D + cgr * 16;
+            const uint8_t *kp = kbase + static_cast<size_t>(row0) * D, *vp = vbase + static_cast<size_t>(row0) * D;
 #pragma unroll
             for (int x = 0; x < 16 / CR; ++x) {
-                const int row = gi * 16 + x * CR;
-                cp_async16(dst + C::k_at(row + krow, cgr) * 16, kp + x * CR * D);
-                cp_async16(dst + 2048 + C::v_at(row + vrow, cgr) * 16, vp + x * CR * D);
+                const int at = (gi * 16 + x * CR) * D;
+                cp_async16(dst + ko + at, kp + x * CR * D);
+                cp_async16(dst + (x & 1 ? vo1 : vo0) + at, vp + x * CR * D);
             }
         }
     };
-    auto compute = [&](const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
-        const uint4 *kb = reinterpret_cast<const uint4 *>(buf), *vb = reinterpret_cast<const uint4 *>(buf + 2048);
+    // Shared-memory offsets of this lane's reads, so that all but an immediate is computed once (C::k_at, C::v_at).
+    const int kl0 = (D == 64 ? g * 4 + t : g * 8 + (t ^ ((g & 1) << 2))) * 16;
+    const int kl1 = D == 64 ? 0 : (g * 8 + ((4 + t) ^ ((g & 1) << 2))) * 16;
+    const int vl = 2048 + (D == 64 ? ((((t >> 1) * 4 + (t & 1)) * 4 + ((g >> 1) ^ (t & 2))) * 16 + (g & 1) * 8)
+                                   : (2 * t * 8 + (g ^ (2 * t))) * 16);
+    // The segment at hand: q, m, l, o and the keys its rows see.
+    uint32_t qa[KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
+    int end[RR], full_end = 0;  // keys of every row: [first, full_end)
+    float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
+    // masked is a constant at both calls
+    auto compute = [&](const bool masked, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) __attribute__((always_inline)) {
         float s[NT][4];
-#pragma unroll
-        for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = s[tile][2] = s[tile][3] = 0.0f;
 #pragma unroll
         for (int s4 = 0; s4 < KS / 4; ++s4) {
             uint4 kw[NT];
 #pragma unroll
-            for (int tile = 0; tile < NT; ++tile) kw[tile] = kb[C::k_at(8 * tile + g, 4 * s4 + t)];
+            for (int tile = 0; tile < NT; ++tile) kw[tile] = *reinterpret_cast<const uint4 *>(buf + (s4 ? kl1 : kl0) + tile * 8 * D);
 #pragma unroll
             for (int st = 0; st < 4; ++st)
 #pragma unroll
                 for (int tile = 0; tile < NT; ++tile) {
                     const uint32_t w = st == 0 ? kw[tile].x : st == 1 ? kw[tile].y : st == 2 ? kw[tile].z : kw[tile].w;
-                    const uint32_t (&qq)[2 * RR] = qa[4 * s4 + st];
+                    const uint32_t (&qq)[4] = qa[4 * s4 + st];
                     uint32_t b0, b1;
                     halves4<KIND>(w, b0, b1);
-                    if (ROWS == 8)
-                        mma16816(s[tile], qq[0], qq[0], qq[1], qq[1], b0, b1);
-                    else
-                        mma16816(s[tile], qq[0], qq[RR - 1], qq[RR], qq[2 * RR - 1], b0, b1);
+                    if (s4 == 0 && st == 0) mma16816_first(s[tile], qq[0], qq[1], qq[2], qq[3], b0, b1);
+                    else mma16816(s[tile], qq[0], qq[1], qq[2], qq[3], b0, b1);
                 }
         }
-        const bool masked = pos < first || pos + CK > min(first_end, last_end) || ok != (1u << GR) - 1u;
-#pragma unroll
-        for (int tile = 0; tile < NT; ++tile)
-#pragma unroll
-            for (int e = 0; e < 2 * RR; ++e) s[tile][e] *= ks[tile / 2];
         if (masked) {
 #pragma unroll
             for (int tile = 0; tile < NT; ++tile)
@@ -283,36 +356,35 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
                     if (key < first || key >= end[e >> 1] || !((ok >> (tile / 2)) & 1u)) s[tile][e] = -INFINITY;
                 }
         }
-        float ms[RR];
+        // A granule's scale is one factor of its scores: the largest of them first, then the factor.
+        float top[RR];
         bool grew = false;
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
-            float top = s[0][2 * rr];
+            top[rr] = -INFINITY;
 #pragma unroll
-            for (int tile = 0; tile < NT; ++tile) top = fmaxf(top, fmaxf(s[tile][2 * rr], s[tile][2 * rr + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            ms[rr] = fmaxf(m[rr], top);
-            grew |= ms[rr] > m[rr];
+            for (int gi = 0; gi < GR; ++gi)
+                top[rr] = fmaxf(top[rr], ks[gi] * fmaxf(fmaxf(s[2 * gi][2 * rr], s[2 * gi][2 * rr + 1]), fmaxf(s[2 * gi + 1][2 * rr], s[2 * gi + 1][2 * rr + 1])));
+            grew |= top[rr] > m[rr] + LAZY;  // m -inf: any key
         }
-        float vmax = vs[0];
-#pragma unroll
-        for (int gi = 1; gi < GR; ++gi) vmax = fmaxf(vmax, vs[gi]);
-        if (__any_sync(0xFFFFFFFFu, grew) || vmax > S) {
-            const float Sn = fmaxf(S, vmax), fs = Sn > 0.0f ? S / Sn : 0.0f;
-            float f[RR];
+        if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
             for (int rr = 0; rr < RR; ++rr) {
-                f[rr] = ms[rr] > -INFINITY ? ex2(m[rr] - ms[rr]) : 0.0f;
-                l[rr] *= f[rr];
-                m[rr] = ms[rr];
+                top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xFFFFFFFFu, top[rr], 1));
+                top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xFFFFFFFFu, top[rr], 2));
+                const float mn = fmaxf(m[rr], top[rr]), f = mn > -INFINITY ? ex2(m[rr] - mn) : 0.0f;
+                m[rr] = mn;
+                l[rr] *= f;
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    o[j][RR == 1 ? 0 : 2 * rr] *= f;
+                    o[j][RR == 1 ? 1 : 2 * rr + 1] *= f;
+                    if (RR == 1) {
+                        o[j][2] *= f;
+                        o[j][3] *= f;
+                    }
+                }
             }
-#pragma unroll
-            for (int j = 0; j < DT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] *= f[RR == 1 ? 0 : e >> 1] * fs;
-            S = Sn;
-            invS = Sn > 0.0f ? 1.0f / Sn : 0.0f;
         }
         float mm[RR];
 #pragma unroll
@@ -325,7 +397,8 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
             for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
                 for (int rr = 0; rr < RR; ++rr) {
-                    float p0 = ex2(s[2 * gi + tile][2 * rr] - mm[rr]), p1 = ex2(s[2 * gi + tile][2 * rr + 1] - mm[rr]);
+                    float p0 = ex2(fmaf(s[2 * gi + tile][2 * rr], ks[gi], -mm[rr]));
+                    float p1 = ex2(fmaf(s[2 * gi + tile][2 * rr + 1], ks[gi], -mm[rr]));
                     l[rr] += p0 + p1;
                     p0 *= w;
                     p1 *= w;
@@ -336,30 +409,32 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
             uint32_t vw[4][D / 32];  // D / 8 dims of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the granule
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                const int row = 16 * gi + 2 * t + (y & 1) + (y >> 1) * 8;
+                const uint8_t *vp = buf + vl + (D == 64 ? 16 * gi + 8 * (y >> 1) + 2 * (y & 1) : 16 * gi + 8 * (y >> 1) + (y & 1)) * D;
                 if (D == 64) {
-                    const uint2 z = reinterpret_cast<const uint2 *>(vb + C::v_at(row, g >> 1))[g & 1];
+                    const uint2 z = *reinterpret_cast<const uint2 *>(vp);
                     vw[y][0] = z.x;
                     vw[y][1] = z.y;
                 } else {
-                    const uint4 z = vb[C::v_at(row, g)];
+                    const uint4 z = *reinterpret_cast<const uint4 *>(vp);
                     vw[y][0] = z.x;
                     vw[y][1] = z.y;
                     vw[y][D / 32 - 2] = z.z;
                     vw[y][D / 32 - 1] = z.w;
                 }
-                // A granule that was not loaded holds what the ring held before, and a code behind the last
-                // key may be NaN in e4m3: 0 * NaN is not 0.
-                if (KIND == GPT2_KV8_E4M3 && masked && (pos + row >= n || !((ok >> gi) & 1u)))
-#pragma unroll
-                    for (int q = 0; q < D / 32; ++q) vw[y][q] = 0;
             }
+            // A granule that was not loaded holds what the ring held before, and a code behind the last
+            // key may be NaN in e4m3: 0 * NaN is not 0.
+            if (KIND == GPT2_KV8_E4M3 && masked)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    if (pos + 16 * gi + 2 * t + (y & 1) + (y >> 1) * 8 >= n || !((ok >> gi) & 1u))
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) vw[y][q] = 0;
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {  // 4 dims: column tiles 4 q .. 4 q + 3
-                const uint32_t wk[4] = {vw[0][q], vw[1][q], vw[2][q], vw[3][q]};
                 uint32_t b0[4], b1[4];
-                pairs4<KIND>(wk[0], wk[1], b0);
-                pairs4<KIND>(wk[2], wk[3], b1);
+                pairs4<KIND>(vw[0][q], vw[1][q], b0);
+                pairs4<KIND>(vw[2][q], vw[3][q], b1);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (ROWS == 8) {
@@ -373,18 +448,18 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
         }
     };
 
-    const int mine = chunks > warp ? (chunks - warp + NW - 1) / NW : 0;  // chunks warp, warp + NW, ...
+    const int mine = c1 - c0 > warp ? (c1 - c0 - warp + NW - 1) / NW : 0;  // chunks c0 + warp, c0 + warp + NW, ...
     // The look-up of a set must come before the loads of its chunks but after the last use of the set before: scales
     // and validity of the chunks in flight are kept in registers, two sets deep.
-    float pks[2] = {}, pvs[2] = {};  // this lane's granule scales of the even and odd set
+    float pks[2] = {}, pvs[2] = {}, pmax[2] = {};  // this lane's granule scales of the even and odd set; the set's largest vscale
     unsigned pok[2] = {};
     auto fetch = [&](int i) {
         if (i < mine) {
             if (i % SET == 0) {
                 look_up(i / SET);
                 const int b = (i / SET) & 1;
-                if (b) pks[1] = gks, pvs[1] = gvs, pok[1] = gok;
-                else pks[0] = gks, pvs[0] = gvs, pok[0] = gok;
+                if (b) pks[1] = gks, pvs[1] = gvs, pmax[1] = gvmax, pok[1] = gok;
+                else pks[0] = gks, pvs[0] = gvs, pmax[0] = gvmax, pok[0] = gok;
             }
             load(i, i % STAGES);
         }
@@ -392,11 +467,60 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch(i);
-    for (int i = 0; i < mine; ++i) {
+    int i = 0;
+    for (int x0 = c0; x0 < c1;) {
+        const int u1 = unit_of(x0) + u0, x1 = min(u1, c1);
+        full_end = one ? n : min(n - a.Tq + qt * ROWS / a.G + 1, last_end);
+        // q: thread (g, t) holds dims 64 * (s / 4) + 16 t + 4 (s % 4) .. + 3 of row g (and g + 8) for k-step s
+#pragma unroll
+        for (int rr = 0; rr < RR; ++rr) {
+            const int row = qt * ROWS + g + 8 * rr;
+            const bool ok = row < R;
+            const int tok = ok && !one ? row / a.G : 0;
+            end[rr] = ok ? n - a.Tq + tok + 1 : 0;
+            const __half *qp = a.q + r * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (row - tok * a.G)) * D + 16 * t;
+#pragma unroll
+            for (int s4 = 0; s4 < KS / 4; ++s4) {
+                uint4 x[2] = {};
+                if (ok) {
+                    x[0] = *reinterpret_cast<const uint4 *>(qp + 64 * s4);
+                    x[1] = *reinterpret_cast<const uint4 *>(qp + 64 * s4 + 8);
+                }
+                const uint32_t *w = reinterpret_cast<const uint32_t *>(x);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    qa[4 * s4 + s][rr] = w[2 * s];
+                    qa[4 * s4 + s][2 + rr] = w[2 * s + 1];
+                    if (RR == 1) {
+                        qa[4 * s4 + s][1] = twin(w[2 * s]);
+                        qa[4 * s4 + s][3] = twin(w[2 * s + 1]);
+                    }
+                }
+            }
+            m[rr] = -INFINITY;
+            l[rr] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        S = (i / SET) & 1 ? pmax[1] : pmax[0];
+        invS = S > 0.0f ? 1.0f / S : 0.0f;
+        for (; c0 + i * NW + warp < x1; ++i) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();  // every lane's copies of chunk i are there, and all are done with chunk i - 1
         fetch(i + STAGES - 1);
         const bool odd = (i / SET) & 1;
+        if (i % SET == 0) {
+            const float Sn = fmaxf(S, odd ? pmax[1] : pmax[0]);
+            if (Sn > S) {
+                const float f = S / Sn;
+#pragma unroll
+                for (int j = 0; j < DT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= f;
+                S = Sn;
+                invS = 1.0f / Sn;
+            }
+        }
         float ks[GR], vs[GR];
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
@@ -404,97 +528,104 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
             vs[gi] = __shfl_sync(0xFFFFFFFFu, odd ? pvs[1] : pvs[0], (i % SET) * GR + gi);
         }
         const unsigned ok = ((odd ? pok[1] : pok[0]) >> ((i % SET) * GR)) & ((1u << GR) - 1u);
-        compute(ring + i % STAGES * CHUNK_BYTES, lo + (i * NW + warp) * CK, ks, vs, ok);
+        const int pos = base + (c0 + i * NW + warp - u0) * CK;
+        const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
+        if (pos < first || pos + CK > full_end || ok != (1u << GR) - 1u) compute(true, buf, pos, ks, vs, ok);
+        else compute(false, buf, pos, ks, vs, ok);
+    }
+        // the warps' rows: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and 2 t + 1)
+        if (x0 > c0) __syncthreads();  // the last segment's merge is through
+#pragma unroll
+        for (int rr = 0; rr < RR; ++rr) {
+            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
+            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
+            if (t == 0) {
+                sm[warp][g + 8 * rr] = m[rr];
+                sl[warp][g + 8 * rr] = l[rr];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < DT; j += 4) {
+                    float4 w;
+                    float *wf = reinterpret_cast<float *>(&w);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
+                    *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * t + e) * DT + j]) = w;
+                }
+        }
+        __syncthreads();
+        const int rows = min(ROWS, R - qt * ROWS);
+        const bool whole = u0 >= c0 && u1 <= c1;
+        const int prow = min(ROWS, R);  // rows of a tile in the work area
+        const int slot = 2 * blockIdx.x + (x0 == c0 ? 0 : 1);
+        for (int x = tid; x < rows * D; x += 32 * NW) {
+            const int row = x / D, d = x % D;
+            const float mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+            float lx = 0.0f, y = 0.0f;
+            if (mx > -INFINITY) {
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float f = ex2(sm[w][row] - mx);
+                    lx = fmaf(f, sl[w][row], lx);
+                    y = fmaf(f, so[w][row][d], y);
+                }
+            }
+            if (whole) {
+                put(h, row, d, lx > 0.0f ? y / lx : 0.0f);
+            } else {
+                float *pr = a.part + (static_cast<long long>(slot) * prow + row) * (D + 2);
+                pr[d] = y;
+                if (d == 0) {
+                    pr[D] = mx;
+                    pr[D + 1] = lx;
+                }
+            }
+        }
+        if (!whole) {  // pieces k0 .. k1 share the unit; its first piece's slot names its counter
+            const int k0 = u0 / per, k1 = (u1 - 1) / per, s0 = 2 * k0 + (u0 == k0 * per ? 0 : 1);
+            __syncthreads();
+            if (tid == 0) {
+                __threadfence();  // the CTA's partials, ordered before it by the barrier, are visible with the count
+                const unsigned seen = atomicAdd(&a.arrive[s0], 1u);
+                is_last = seen == static_cast<unsigned>(k1 - k0);
+                if (is_last) a.arrive[s0] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (is_last) {
+                const long long step = static_cast<long long>(prow) * (D + 2);
+                for (int x = tid; x < rows * D; x += 32 * NW) {
+                    const int row = x / D, d = x % D;
+                    const float *p0 = a.part + s0 * step + row * (D + 2), *pk = a.part + 2 * (k0 + 1) * step + row * (D + 2);
+                    float mx = __ldcg(p0 + D), lx = __ldcg(p0 + D + 1), y = __ldcg(p0 + d);
+                    for (int k = 0; k < k1 - k0; k += 4) {  // four pieces' loads at once
+                        float m4[4], l4[4], y4[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const bool in = k + u < k1 - k0;
+                            const float *q = pk + 2 * (in ? k + u : k) * step;
+                            m4[u] = in ? __ldcg(q + D) : -INFINITY;
+                            l4[u] = __ldcg(q + D + 1);
+                            y4[u] = __ldcg(q + d);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const float mn = fmaxf(mx, m4[u]);
+                            if (mn == -INFINITY) continue;
+                            const float f = ex2(mx - mn), f4 = ex2(m4[u] - mn);
+                            lx = fmaf(lx, f, l4[u] * f4);
+                            y = fmaf(y, f, y4[u] * f4);
+                            mx = mn;
+                        }
+                    }
+                    put(h, row, d, lx > 0.0f ? y / lx : 0.0f);
+                }
+            }
+        }
+        x0 = x1;
     }
     if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(c.status, ST_KV8_BAD_PAGE);
-
-    __syncthreads();  // every warp is through its ring
-    // the warps' rows: thread (g, t) holds dims 16 t .. (D 64: columns j of tiles 2 t and 2 t + 1)
-#pragma unroll
-    for (int rr = 0; rr < RR; ++rr) {
-        l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
-        l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
-        if (t == 0) {
-            sm[warp][g + 8 * rr] = m[rr];
-            sl[warp][g + 8 * rr] = l[rr];
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int j = 0; j < DT; j += 4) {
-                float4 w;
-                float *wf = reinterpret_cast<float *>(&w);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
-                *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * t + e) * DT + j]) = w;
-            }
-    }
-    __syncthreads();
-    const int rows = min(ROWS, R - qt * ROWS);
-    auto merged = [&](int row, int d, float &mx, float &lx) {
-        mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
-        lx = 0.0f;
-        float x = 0.0f;
-        if (mx > -INFINITY) {
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float f = ex2(sm[w][row] - mx);
-                lx = fmaf(f, sl[w][row], lx);
-                x = fmaf(f, so[w][row][d], x);
-            }
-        }
-        return x;
-    };
-    auto put = [&](int row, int d, float x) {
-        const int i = qt * ROWS + row, tok = i / a.G;
-        a.out[r * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
-    };
-    if (active <= 1) {
-        for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
-            float mx, lx;
-            const float x = merged(e / D, e % D, mx, lx);
-            put(e / D, e % D, lx > 0.0f ? x / lx : 0.0f);
-        }
-        return;
-    }
-    const int tile = blockIdx.x / a.nsplit;
-    const int prow = min(ROWS, R);  // rows of a tile in the work area
-    float *part = a.part + static_cast<long long>(blockIdx.x - split) * prow * (D + 2);
-    for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
-        float mx, lx;
-        const float x = merged(e / D, e % D, mx, lx);
-        float *pr = part + (static_cast<long long>(split) * prow + e / D) * (D + 2);
-        pr[e % D] = x;
-        if (e % D == 0) {
-            pr[D] = mx;
-            pr[D + 1] = lx;
-        }
-    }
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const unsigned seen = atomicAdd(&a.arrive[tile], 1u);
-        is_last = seen == static_cast<unsigned>(active - 1);
-        if (is_last) a.arrive[tile] = 0;
-    }
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-    for (int e = threadIdx.x; e < rows * D; e += 32 * NW) {
-        const float *pr = part + (e / D) * (D + 2);
-        const long long step = static_cast<long long>(prow) * (D + 2);
-        float mx = -INFINITY;
-        for (int s = 0; s < active; ++s) mx = fmaxf(mx, __ldcg(pr + s * step + D));
-        float lx = 0.0f, x = 0.0f;
-        if (mx > -INFINITY)
-#pragma unroll 4
-            for (int s = 0; s < active; ++s) {
-                const float f = ex2(__ldcg(pr + s * step + D) - mx);
-                lx = fmaf(f, __ldcg(pr + s * step + D + 1), lx);
-                x = fmaf(f, __ldcg(pr + s * step + e % D), x);
-            }
-        put(e / D, e % D, lx > 0.0f ? x / lx : 0.0f);
-    }
 }
 
 }  // namespace kv8
@@ -531,36 +662,38 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     a.count = count;
     a.max_len = max_len ? max_len : kv->maxPages * kv->page;
     a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(kv->headDim));
-    const long long run = static_cast<long long>(kv->page) * kv->headDim;
-    a.page_stride = run * kv->nHead * 2 * kv->nLayer;
-    a.k_off = run * kv->nHead * 2 * L;
-    a.v_off = a.k_off + run * kv->nHead;
+    a.page_runs = static_cast<unsigned>(kv->nLayer * 2 * kv->nHead);
+    a.k_run = static_cast<unsigned>(L * 2 * kv->nHead);
     a.part = w.part;
     a.arrive = w.arrive;
-    // Plan: whole (row, head, tile) units while they fill the GPU; else spans of at least NW chunks, about
-    // WAVES CTAs per resident slot.
     const long long R = static_cast<long long>(a.G) * Tq;
-    const int rows = R <= 8 ? 8 : 16;
+    const int rows = R <= 8 ? 8 : 16, ck = 2048 / kv->headDim;
     a.qtiles = static_cast<int>((R + rows - 1) / rows);
-    const long long units = static_cast<long long>(kv->nRow) * kv->nHead * a.qtiles;
-    const int chunk = kv8::NW * (2048 / kv->headDim);
-    const int longest = a.max_len + 2048 / kv->headDim;  // `first` may start inside a chunk
-    const long long target = std::min<long long>(static_cast<long long>(ctx->num_sms) * 6, kv8::MAX_SPLIT_CTAS);
-    long long nsplit = std::max<long long>(1, target / units);
-    nsplit = std::min<long long>(nsplit, (longest + chunk - 1) / chunk);
-    a.span = static_cast<int>((longest + nsplit - 1) / nsplit + chunk - 1) / chunk * chunk;
-    a.nsplit = (longest + a.span - 1) / a.span;
-    if (units * a.nsplit > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
+    const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
+    const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
+    if (entries > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
+    // Units that fill the GPU once keep their own CTAs: they share no unit and need no prefix sum, which is worth more than
+    // equal pieces as long as a unit is short (64 sequences x 12 heads of 512 to 1023 keys: 27.6 against 30.9 us).
+    const int full = (rows == 8 && kv->headDim == 64 ? 3 : 2) * ctx->num_sms;
+    const bool pieces = entries * kv->nHead < full && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
+    a.entries = pieces ? static_cast<int>(entries) : 0;
+    const int smem = kv8::RING_BYTES + kv8::NW * rows * (kv->headDim + 4) * 4 + (a.entries + 1) * 4;
+    // CTAs that are resident together: registers (the kernel's launch bounds) and 228 KB of shared memory, 1 KB of it per CTA.
+    const int resident = std::min(rows == 8 && kv->headDim == 64 ? 3 : 2, 228 * 1024 / (smem + 1024 + 512));
+    const dim3 grid = pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident,
+                                                                             kv8::MAX_PIECES, (chunks + kv8::NW - 1) / kv8::NW})))
+                             : dim3(static_cast<unsigned>(entries), kv->nHead);
     const kv8::View c = kv8::view(kv, ctx->status);
     bool *attr_done = &ctx->kv8_attr_done[(kv->kind == GPT2_KV8_INT8 ? 0 : 4) + (kv->headDim == 64 ? 0 : 2) + (rows == 8 ? 0 : 1)];
     auto go = [&](auto kern) {
         if (!*attr_done) {
             RelaxedCapture relaxed;
-            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kv8::RING_BYTES) != cudaSuccess)
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     kv8::RING_BYTES + kv8::NW * rows * (kv->headDim + 4) * 4 + (kv8::MAX_ENTRIES + 1) * 4) != cudaSuccess)
                 return GPT2_B200_ECUDA;
             *attr_done = true;
         }
-        kern<<<static_cast<unsigned>(units * a.nsplit), 32 * kv8::NW, kv8::RING_BYTES, stream>>>(c, a);
+        kern<<<grid, 32 * kv8::NW, smem, stream>>>(c, a);
         return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
     };
     if (kv->kind == GPT2_KV8_INT8) {

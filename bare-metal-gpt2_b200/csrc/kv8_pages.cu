@@ -4,15 +4,18 @@
 // A reorder is planned by one CTA (counts, ranks and the scan for free pages are sequential in row
 // order by definition, so the page ids do not depend on timing) and its page copies run on the
 // whole GPU. Compaction is a scan of the reference counts, then copies between disjoint pages.
+#include <algorithm>
 #include <cstdio>
 
 #include "kv8.cuh"
+#include "ptx.cuh"
 
 namespace b200 {
 namespace kv8 {
 
 constexpr int PLAN_NT = 1024;
-enum Misc { M_COPIES = 0, M_LIVE = 1 };
+constexpr int ENTRIES = 8;  // table entries per thread and batch
+enum Misc { M_COPIES = 0, M_LIVE = 1, M_MOVES = 2 };
 
 // Exclusive prefix sum of v over the CTA's PLAN_NT threads; *total receives the sum.
 __device__ int block_scan(int v, int *warp_sums, int *total) {
@@ -43,48 +46,64 @@ __device__ int block_scan(int v, int *warp_sums, int *total) {
 __global__ void __launch_bounds__(PLAN_NT) k_kv8_plan(const View c, const Work w, const int *parent, int advance,
                                                       int reserve) {
     __shared__ int sums[32];
-    __shared__ int tail_page[MAX_ROWS];
+    __shared__ int len0[MAX_ROWS], from0[MAX_ROWS];
+    __shared__ __align__(16) int tail_page[MAX_ROWS];
+    grid_launch_dependents();  // the copies' CTAs wait for this one's end
     const int tid = threadIdx.x, M = c.maxPages, cap = M << c.page_shift;
-    // the state before: table0 (copied by the caller), len0 = len + advance
     if (tid < c.nRow) {
         long long n = static_cast<long long>(c.len[tid]) + advance;
         if (n < 0 || n > cap) {
             atomicOr(c.status, ST_KV8_BAD_LEN);
             n = n < 0 ? 0 : cap;
         }
-        w.len0[tid] = static_cast<int>(n);
-    }
-    __syncthreads();
-    // drop every old hold, take every new one
-    for (long long e = tid; e < static_cast<long long>(c.nRow) * M; e += PLAN_NT) {
-        const int old = w.table0[e];
-        if (old >= 0 && old < c.nPages) atomicSub(&c.ref[old], 1);
-    }
-    for (long long e = tid; e < static_cast<long long>(c.nRow) * M; e += PLAN_NT) {
-        const int r = static_cast<int>(e / M), i = static_cast<int>(e - static_cast<long long>(r) * M);
-        int from = parent ? parent[r] : r;
+        int from = parent ? parent[tid] : tid;
         if (from < -1 || from >= c.nRow) {
-            if (i == 0) atomicOr(c.status, ST_KV8_BAD_PARENT);
+            atomicOr(c.status, ST_KV8_BAD_PARENT);
             from = -1;
         }
-        int p = -1;
-        if (from >= 0 && i < (w.len0[from] + c.page - 1) >> c.page_shift) {
-            p = w.table0[static_cast<long long>(from) * M + i];
-            if (p < 0 || p >= c.nPages) {
-                atomicOr(c.status, ST_KV8_BAD_PAGE);
-                p = -1;
-            } else {
-                atomicAdd(&c.ref[p], 1);
-            }
-        }
-        c.table[e] = p;
+        len0[tid] = static_cast<int>(n);
+        from0[tid] = from;
     }
     __syncthreads();
+    // Every entry's old and new page. A row's new entry comes from another row's old one in the same column, so a batch of
+    // whole columns is read before any of it is written. Beams share most pages with their parent: where old and
+    // new are the same page nothing is done.
+    const int cols = max(1, min(M, PLAN_NT * ENTRIES / c.nRow));
+    for (int c0 = 0; c0 < M; c0 += cols) {
+        const int width = min(cols, M - c0), total = width * c.nRow;
+        int old_page[ENTRIES], new_page[ENTRIES], at[ENTRIES];
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j) {
+            const int e = tid + j * PLAN_NT;
+            at[j] = -1;
+            if (e < total) {
+                const int r = e / width, i = c0 + e - r * width, from = from0[r];
+                at[j] = r * M + i;
+                old_page[j] = c.table[at[j]];
+                new_page[j] = -1;
+                if (from >= 0 && i < (len0[from] + c.page - 1) >> c.page_shift) {
+                    new_page[j] = c.table[from * M + i];
+                    if (new_page[j] < 0 || new_page[j] >= c.nPages) {
+                        atomicOr(c.status, ST_KV8_BAD_PAGE);
+                        new_page[j] = -1;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j)
+            if (at[j] >= 0 && old_page[j] != new_page[j]) {
+                if (old_page[j] >= 0 && old_page[j] < c.nPages) atomicSub(&c.ref[old_page[j]], 1);
+                if (new_page[j] >= 0) atomicAdd(&c.ref[new_page[j]], 1);
+                c.table[at[j]] = new_page[j];
+            }
+        __syncthreads();
+    }
     // what each row needs
     int n = 0, held = 0, last = -1, copy = 0, grow = 0;
     if (tid < c.nRow) {
-        const int from = parent ? parent[tid] : tid;
-        n = from >= 0 && from < c.nRow ? w.len0[from] : 0;
+        n = from0[tid] >= 0 ? len0[from0[tid]] : 0;
         c.len[tid] = n;
         held = (n + c.page - 1) >> c.page_shift;
         if (reserve > 0 && (n & (c.page - 1))) last = c.table[static_cast<long long>(tid) * M + held - 1];
@@ -95,20 +114,38 @@ __global__ void __launch_bounds__(PLAN_NT) k_kv8_plan(const View c, const Work w
     }
     __syncthreads();
     if (last >= 0) {
-        int before = 0;  // earlier rows that continue in the same page
-        for (int q = 0; q < tid; ++q) before += tail_page[q] == last;
-        copy = before < __ldcg(&c.ref[last]) - 1;
+        const int holds = __ldcg(&c.ref[last]);
+        if (holds > 1) {
+            int before = 0;  // earlier rows that continue in the same page
+            const int4 *t4 = reinterpret_cast<const int4 *>(tail_page);
+            for (int q = 0; q < tid >> 2; ++q) {
+                const int4 z = t4[q];
+                before += (z.x == last) + (z.y == last) + (z.z == last) + (z.w == last);
+            }
+            for (int q = tid & ~3; q < tid; ++q) before += tail_page[q] == last;
+            copy = before < holds - 1;
+        }
     }
     int total;
     const int off = block_scan(copy + grow, sums, &total);
-    // the lowest-numbered free pages
+    // the lowest-numbered free pages, four per thread and step
     int found = 0;
-    for (int base = 0; base < c.nPages && found < total; base += PLAN_NT) {
-        const int p = base + tid;
-        const int free_page = p < c.nPages && __ldcg(&c.ref[p]) == 0;
+    for (int base = 0; base < c.nPages && found < total; base += 4 * PLAN_NT) {
+        const int p0 = base + 4 * tid;
+        int is_free[4], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            is_free[i] = p0 + i < c.nPages && __ldcg(&c.ref[p0 + i]) == 0;
+            mine += is_free[i];
+        }
         int some;
-        const int at = found + block_scan(free_page, sums, &some);
-        if (free_page && at < total) w.list[at] = p;
+        int at = found + block_scan(mine, sums, &some);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (is_free[i]) {
+                if (at < total) w.list[at] = p0 + i;
+                ++at;
+            }
         found += some;
     }
     __syncthreads();
@@ -141,25 +178,37 @@ __global__ void __launch_bounds__(PLAN_NT) k_kv8_plan(const View c, const Work w
     if (tid == 0) w.misc[M_COPIES] = copies;
 }
 
-// The filled part of each copied page: every layer, K|V and head, and the scales of its blocks.
-__global__ void __launch_bounds__(256) k_kv8_copy(const View c, const Work w) {
-    const int copies = static_cast<int>(w.misc[M_COPIES]);
-    const int runs = c.nLayer * 2 * c.nHead, nb = c.page >> c.block_shift;
-    for (long long u = blockIdx.x; u < static_cast<long long>(copies) * runs; u += gridDim.x) {
-        const int4 cp = w.copies[u / runs];
+// The filled part of each copied page: every layer, K|V and head, and the scales of its blocks. A warp per run.
+__global__ void __launch_bounds__(256) k_kv8_copy(View c, Work w) {
+    grid_dependency_wait();
+    const int copies = static_cast<int>(__ldcg(&w.misc[M_COPIES]));
+    const int runs = c.nLayer * 2 * c.nHead, sub = c.page_shift - c.block_shift, lane = threadIdx.x & 31;
+    const long long items = static_cast<long long>(copies) * runs;
+    for (long long u = blockIdx.x * 8 + (threadIdx.x >> 5); u < items; u += gridDim.x * 8) {
+        const int which = static_cast<int>(u / runs), i = static_cast<int>(u - static_cast<long long>(which) * runs);
+        const int4 cp = __ldcg(&w.copies[which]);
         if (cp.y < 0) continue;
-        const long long i = u % runs, src = static_cast<long long>(cp.x) * runs + i, dst = static_cast<long long>(cp.y) * runs + i;
-        const uint4 *s = reinterpret_cast<const uint4 *>(c.data + (src << c.page_shift) * c.D);
-        uint4 *d = reinterpret_cast<uint4 *>(c.data + (dst << c.page_shift) * c.D);
-        for (int x = threadIdx.x; x < cp.z * c.D / 16; x += 256) d[x] = s[x];
-        if (static_cast<int>(threadIdx.x) < (cp.z + c.block - 1) >> c.block_shift)
-            c.scale[dst * nb + threadIdx.x] = c.scale[src * nb + threadIdx.x];
+        const unsigned src = static_cast<unsigned>(cp.x) * runs + i, dst = static_cast<unsigned>(cp.y) * runs + i;
+        const uint4 *s = reinterpret_cast<const uint4 *>(c.data + (static_cast<size_t>(src) << c.page_shift) * c.D);
+        uint4 *d = reinterpret_cast<uint4 *>(c.data + (static_cast<size_t>(dst) << c.page_shift) * c.D);
+        const int n = cp.z * c.D / 16;
+        for (int x = lane; x < n; x += 128) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x + 32 * j < n) v[j] = s[x + 32 * j];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x + 32 * j < n) d[x + 32 * j] = v[j];
+        }
+        if (lane < (cp.z + c.block - 1) >> c.block_shift) c.scale[(dst << sub) + lane] = c.scale[(src << sub) + lane];
     }
 }
 
 // Compaction: list[p] = new id of page p (itself below live); copies between disjoint pages.
 __global__ void __launch_bounds__(PLAN_NT) k_kv8_compact_plan(const View c, const Work w, int *d_live) {
     __shared__ int sums[32];
+    grid_launch_dependents();
     const int tid = threadIdx.x;
     int mine = 0, live;
     for (int p = tid; p < c.nPages; p += PLAN_NT) mine += c.ref[p] > 0;
@@ -176,17 +225,18 @@ __global__ void __launch_bounds__(PLAN_NT) k_kv8_compact_plan(const View c, cons
         __syncthreads();
     }
     int seen = 0;
-    for (int base = live & ~(PLAN_NT - 1); base < c.nPages; base += PLAN_NT) {
+    for (int base = live; base < c.nPages; base += PLAN_NT) {
         const int p = base + tid;
-        const int move = p >= live && p < c.nPages && c.ref[p] > 0;
+        const int move = p < c.nPages && c.ref[p] > 0;
         int some;
         const int at = seen + block_scan(move, sums, &some);
         // list[p], p >= live: the new id. Fewer than live holes, so the map does not overlap their list.
-        if (p >= live && p < c.nPages) {
+        if (p < c.nPages) {
             const int to = move ? w.list[at] : -1;
             if (move) {
                 c.ref[to] = c.ref[p];
                 c.ref[p] = 0;
+                w.moves[at] = make_int2(p, to);
             }
             w.list[p] = to;
         }
@@ -194,26 +244,40 @@ __global__ void __launch_bounds__(PLAN_NT) k_kv8_compact_plan(const View c, cons
     }
     if (tid == 0) {
         w.misc[M_LIVE] = live;
+        w.misc[M_MOVES] = seen;
         if (d_live) *d_live = live;
     }
 }
 
-__global__ void __launch_bounds__(256) k_kv8_compact_move(const View c, const Work w) {
-    const int live = static_cast<int>(w.misc[M_LIVE]);
+// The tables' new ids, then the moved pages' bytes, a CTA per SEGMENT of a page at a time.
+constexpr int SEGMENT = 16384;
+__global__ void __launch_bounds__(256) k_kv8_compact_move(View c, Work w) {
+    grid_dependency_wait();
+    const int live = static_cast<int>(__ldcg(&w.misc[M_LIVE])), moves = static_cast<int>(__ldcg(&w.misc[M_MOVES]));
     const long long entries = static_cast<long long>(c.nRow) * c.maxPages;
     for (long long e = blockIdx.x * 256ll + threadIdx.x; e < entries; e += gridDim.x * 256ll) {
         const int p = c.table[e];
-        if (p >= live && p < c.nPages) c.table[e] = w.list[p];
+        if (p >= live && p < c.nPages) c.table[e] = __ldcg(&w.list[p]);
     }
-    const int runs = c.nLayer * 2 * c.nHead, nb = c.page >> c.block_shift;
-    const long long bytes = static_cast<long long>(runs) * c.page * c.D, scales = static_cast<long long>(runs) * nb;
-    for (int p = live + blockIdx.x; p < c.nPages; p += gridDim.x) {
-        const int to = w.list[p];
-        if (to < 0) continue;
-        const uint4 *s = reinterpret_cast<const uint4 *>(c.data + p * bytes);
-        uint4 *d = reinterpret_cast<uint4 *>(c.data + to * bytes);
-        for (long long x = threadIdx.x; x < bytes / 16; x += 256) d[x] = s[x];
-        for (long long x = threadIdx.x; x < scales; x += 256) c.scale[to * scales + x] = c.scale[p * scales + x];
+    const int runs = c.nLayer * 2 * c.nHead;
+    const long long bytes = static_cast<long long>(runs) * c.page * c.D, scales = static_cast<long long>(runs) << (c.page_shift - c.block_shift);
+    const long long segs = (bytes + SEGMENT - 1) / SEGMENT;
+    for (long long u = blockIdx.x; u < moves * segs; u += gridDim.x) {
+        const int m = static_cast<int>(u / segs);
+        const long long from = (u - m * segs) * SEGMENT;
+        const int2 mv = __ldcg(&w.moves[m]);
+        const uint4 *s = reinterpret_cast<const uint4 *>(c.data + mv.x * bytes + from);
+        uint4 *d = reinterpret_cast<uint4 *>(c.data + mv.y * bytes + from);
+        const int n = static_cast<int>(min(static_cast<long long>(SEGMENT), bytes - from) / 16);
+        uint4 v[SEGMENT / 16 / 256];
+#pragma unroll
+        for (int j = 0; j < SEGMENT / 16 / 256; ++j)
+            if (static_cast<int>(threadIdx.x) + 256 * j < n) v[j] = s[threadIdx.x + 256 * j];
+#pragma unroll
+        for (int j = 0; j < SEGMENT / 16 / 256; ++j)
+            if (static_cast<int>(threadIdx.x) + 256 * j < n) d[threadIdx.x + 256 * j] = v[j];
+        if (from == 0)
+            for (long long x = threadIdx.x; x < scales; x += 256) c.scale[mv.y * scales + x] = c.scale[mv.x * scales + x];
     }
 }
 
@@ -222,6 +286,20 @@ __global__ void k_kv8_reset(const View c) {
     if (i < c.nPages) c.ref[i] = 0;
     if (i < c.nRow) c.len[i] = 0;
     if (i < static_cast<long long>(c.nRow) * c.maxPages) c.table[i] = -1;
+}
+
+// A launch whose CTAs start while the plan before it runs (it waits for the plan's end before it reads anything).
+static int launch_after(void (*kern)(View, Work), int grid, cudaStream_t stream, const View &c, const Work &w) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, c, w) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
 static size_t up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -302,12 +380,10 @@ int gpt2_kv8_reorder_b200(const GPT2KV8Cache *kv, const int *parent, int advance
     if (!ctx) return GPT2_B200_EDEVICE;
     const kv8::Work w = kv8::work_layout(kv, kv->nHead, 1);
     const kv8::View c = kv8::view(kv, ctx->status);
-    if (cudaMemcpyAsync(w.table0, kv->table, static_cast<size_t>(kv->nRow) * kv->maxPages * 4, cudaMemcpyDeviceToDevice, stream) !=
-        cudaSuccess)
-        return GPT2_B200_ECUDA;
     kv8::k_kv8_plan<<<1, kv8::PLAN_NT, 0, stream>>>(c, w, parent, advance, reserve);
-    kv8::k_kv8_copy<<<ctx->num_sms * 8, 256, 0, stream>>>(c, w);
-    return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    if (cudaGetLastError() != cudaSuccess) return GPT2_B200_ECUDA;
+    if (reserve == 0) return GPT2_B200_OK;  // nothing is written next: no page is copied
+    return kv8::launch_after(kv8::k_kv8_copy, ctx->num_sms * 4, stream, c, w);
 }
 
 int gpt2_kv8_compact_b200(const GPT2KV8Cache *kv, int *d_live, cudaStream_t stream) {
@@ -317,8 +393,8 @@ int gpt2_kv8_compact_b200(const GPT2KV8Cache *kv, int *d_live, cudaStream_t stre
     const kv8::Work w = kv8::work_layout(kv, kv->nHead, 1);
     const kv8::View c = kv8::view(kv, ctx->status);
     kv8::k_kv8_compact_plan<<<1, kv8::PLAN_NT, 0, stream>>>(c, w, d_live);
-    kv8::k_kv8_compact_move<<<ctx->num_sms * 8, 256, 0, stream>>>(c, w);
-    return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    if (cudaGetLastError() != cudaSuccess) return GPT2_B200_ECUDA;
+    return kv8::launch_after(kv8::k_kv8_compact_move, ctx->num_sms * 8, stream, c, w);
 }
 
 }  // extern "C"

@@ -189,6 +189,7 @@ class Lib:
             fn = getattr(self.lib, name)
             fn.restype = res
             fn.argtypes = args
+        self._beam_select = self.lib.gpt2_beam_select_b200
 
     def __getattr__(self, name):
         return getattr(self.lib, name)
@@ -227,13 +228,17 @@ class Lib:
         """The W best continuations of each of B items' W beams: logits [B*W][V] fp16 or fp32 (rows may be
         strided), score fp32 [B*W], done int32 [B*W] or None; writes token and parent (int32), new_score
         and new_done (may be score and done; new_done may be None)."""
-        if logits.dtype not in _beam_types() or logits.stride(1) != 1:
+        kind = _beam_types().get(logits.dtype)
+        rows, near = logits.stride()
+        if kind is None or near != 1:
             raise ValueError("beam_select: logits are fp16 or fp32 rows of neighbouring values")
-        rc = self.lib.gpt2_beam_select_b200(
-            token.data_ptr(), parent.data_ptr(), new_score.data_ptr(), _ptr(new_done), logits.data_ptr(),
-            _beam_types()[logits.dtype], logits.stride(0), score.data_ptr(), _ptr(done), B, W,
-            logits.shape[1], eos, work.data_ptr(), work.numel(), stream)
-        self.check(rc, "gpt2_beam_select_b200")
+        rc = self._beam_select(
+            token.data_ptr(), parent.data_ptr(), new_score.data_ptr(),
+            new_done.data_ptr() if new_done is not None else None, logits.data_ptr(), kind, rows,
+            score.data_ptr(), done.data_ptr() if done is not None else None, B, W, logits.shape[1], eos,
+            work.data_ptr(), work.numel(), stream)
+        if rc:
+            self.check(rc, "gpt2_beam_select_b200")
 
     def status(self, clear: bool = True) -> int:
         """The device's status word (bounded-wait timeouts and bad-input bits), cleared if asked."""
@@ -286,6 +291,11 @@ class KV8Cache:
         self.work = torch.zeros(n, dtype=torch.uint8, device=data.device)
         c.work, c.work_bytes = self.work.data_ptr(), n
         self.c, self.ref_c = c, ctypes.byref(c)
+        # what every call needs, looked up once: a decoding step makes dozens of calls
+        self._nrow, self._dim, self._width, self._half = int(c.nRow), dim, n_head * dim, torch.float16
+        self._store, self._load = lib.lib.gpt2_kv8_store_b200, lib.lib.gpt2_kv8_load_b200
+        self._attend, self._reorder = lib.lib.gpt2_kv8_attend_b200, lib.lib.gpt2_kv8_reorder_b200
+        self._compact = lib.lib.gpt2_kv8_compact_b200
 
     @classmethod
     def create(cls, lib: "Lib", torch, rows: int, max_pages: int, pages: int, layers: int = N_LAYER,
@@ -299,53 +309,59 @@ class KV8Cache:
                    kind, q_heads, queries)
 
     def _rows(self, what, k, v):
-        if k.stride() != v.stride() or k.shape != v.shape or k.dim() != 4 or k.stride(3) != 1 or \
-                k.shape[1] != self.c.nRow or k.shape[3] != self.c.nHead * self.c.headDim or \
-                k.element_size() != 2 or not k.dtype.is_floating_point:
+        """The three outer strides of k and v and their tokens, after a check of their form."""
+        s, shape = k.stride(), k.shape
+        if s != v.stride() or shape != v.shape or len(s) != 4 or s[3] != 1 or shape[1] != self._nrow or \
+                shape[3] != self._width or k.dtype != self._half or v.dtype != self._half:
             raise ValueError(f"{what}: k and v are fp16 [layers][rows][tokens][heads * dim], laid out alike")
+        return shape[0], s[0], s[1], s[2], shape[2]
 
     def store(self, k, v, layer: int = 0, count=None, stream: int = 0) -> None:
         """k, v: fp16 [layers][rows][tokens][heads * dim] (strided views are fine), written behind the
         held positions from `layer` on; count: int32 [rows] or None (all tokens)."""
-        self._rows("store", k, v)
-        s = k.stride()
-        self.lib.check(self.lib.gpt2_kv8_store_b200(
-            self.ref_c, layer, k.shape[0], k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], _ptr(count),
-            k.shape[2], stream), "gpt2_kv8_store_b200")
+        n, ls, rs, ts, tokens = self._rows("store", k, v)
+        rc = self._store(self.ref_c, layer, n, k.data_ptr(), v.data_ptr(), ls, rs, ts,
+                         count.data_ptr() if count is not None else None, tokens, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_kv8_store_b200")
 
     def load(self, k, v, layer: int = 0, first=None, count=None, stream: int = 0) -> None:
         """The inverse: positions first[r].. (0 without first) as fp16 rows, 0 beyond the held ones;
         count: int32 [rows], an int or None: positions stored but not yet counted in."""
-        self._rows("load", k, v)
-        s = k.stride()
-        n = count if isinstance(count, int) else 0
-        self.lib.check(self.lib.gpt2_kv8_load_b200(
-            self.ref_c, layer, k.shape[0], k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], _ptr(first),
-            k.shape[2], None if isinstance(count, int) else _ptr(count), n, stream), "gpt2_kv8_load_b200")
+        n, ls, rs, ts, tokens = self._rows("load", k, v)
+        add, d_add = _count(count)
+        rc = self._load(self.ref_c, layer, n, k.data_ptr(), v.data_ptr(), ls, rs, ts,
+                        first.data_ptr() if first is not None else None, tokens, d_add, add, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_kv8_load_b200")
 
     def attend(self, out, q, layer: int = 0, count=None, first=None, max_len: int = 0,
                stream: int = 0) -> None:
         """q, out: fp16 [rows][queries][q heads * dim]: causal attention of each row's last positions over
         its keys, counted as load() counts them; keys before first[r] are masked."""
-        if q.shape != out.shape or q.dim() != 3 or q.shape[0] != self.c.nRow or q.stride(2) != 1 or \
-                out.stride(2) != 1 or q.shape[2] % self.c.headDim or q.element_size() != 2:
+        qs, os_, shape = q.stride(), out.stride(), q.shape
+        if shape != out.shape or len(qs) != 3 or shape[0] != self._nrow or qs[2] != 1 or os_[2] != 1 or \
+                shape[2] % self._dim or q.dtype != self._half or out.dtype != self._half:
             raise ValueError("attend: q and out are fp16 [rows][queries][q heads * dim]")
-        n = count if isinstance(count, int) else 0
-        self.lib.check(self.lib.gpt2_kv8_attend_b200(
-            out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), self.ref_c,
-            layer, q.shape[2] // self.c.headDim, q.shape[1], _ptr(first),
-            None if isinstance(count, int) else _ptr(count), n, max_len, stream), "gpt2_kv8_attend_b200")
+        add, d_add = _count(count)
+        rc = self._attend(out.data_ptr(), os_[0], os_[1], q.data_ptr(), qs[0], qs[1], self.ref_c, layer,
+                          shape[2] // self._dim, shape[1], first.data_ptr() if first is not None else None,
+                          d_add, add, max_len, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_kv8_attend_b200")
 
     def reorder(self, parent=None, advance: int = 0, reserve: int = 0, stream: int = 0) -> None:
         """Counts `advance` positions in, makes row r a copy of row parent[r] (int32 [rows]; -1: empty; None:
         itself) by sharing pages, and makes room for `reserve` more positions."""
-        self.lib.check(self.lib.gpt2_kv8_reorder_b200(self.ref_c, _ptr(parent), advance, reserve, stream),
-                       "gpt2_kv8_reorder_b200")
+        rc = self._reorder(self.ref_c, parent.data_ptr() if parent is not None else None, advance, reserve, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_kv8_reorder_b200")
 
     def compact(self, live=None, stream: int = 0) -> None:
         """Moves the live pages to the lowest ids; live: int32 [1] for their number, or None."""
-        self.lib.check(self.lib.gpt2_kv8_compact_b200(self.ref_c, _ptr(live), stream),
-                       "gpt2_kv8_compact_b200")
+        rc = self._compact(self.ref_c, live.data_ptr() if live is not None else None, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_kv8_compact_b200")
 
     def reset(self, stream: int = 0) -> None:
         """Every page free, every row empty."""
@@ -446,9 +462,11 @@ class DecodeBatch:
             pass
 
 
-def _ptr(t):
-    """A tensor's device pointer, None for None."""
-    return t.data_ptr() if t is not None else None
+def _count(count):
+    """(int, device pointer or None) of a count given as an int, an int32 tensor or None."""
+    if count is None:
+        return 0, None
+    return (count, None) if isinstance(count, int) else (0, count.data_ptr())
 
 
 _TYPES: dict = {}
