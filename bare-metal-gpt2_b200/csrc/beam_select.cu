@@ -10,9 +10,9 @@
 //     granules; lanes then take values by their index (neighbouring lanes neighbouring words, so that any alignment of
 //     the row is read without bank conflicts), and equal rows get equal sums wherever they lie.
 //   - The warp's W largest so far are a sorted list, lane j holding the j-th. A value is inserted if it reaches a
-//     threshold that at least W values of the row reach: the list's last entry, or the smallest of the CTA's 8
-//     warps' K-th largest, K = ceil(W / 8). The first step, without lists yet, takes the lanes' maxima for that. So about
-//     W ln(n / W) of a CTA's n values are inserted; the others cost no more than their share of a maximum.
+//     threshold that at least W values of the row reach: the list's last entry, or the smallest of the CTA's 8 warps' K-th
+//     largest, K = ceil(W / 8); in the first step, without lists yet, of their lanes' maxima. About W ln(n / W) of a CTA's
+//     n values are inserted; the others cost no more than their share of a maximum.
 //   - Logits are compared as 64-bit keys: the value's orderable bits, then the inverted token, so equal logits go to the
 //     lower token whatever the order of arrival.
 //   - Sorted lists are merged by W rounds of a maximum over their heads, a lane per list: the warps' in a CTA, the CTAs' of
@@ -31,7 +31,10 @@ constexpr int NWARP = 8, NT = 32 * NWARP;
 constexpr int MAX_CHUNKS = 64;  // CTAs of a row: two list heads per lane
 constexpr int ROW_KEYS = 256;   // CTAs x W of a row, at most
 constexpr int NV = 16;          // values per lane and step
-constexpr int STAGES = 4;
+// Steps in a warp's ring: 4 KB and more in flight per warp, and for fp32 four CTAs per SM (with 4 stages three: a batch of 1024
+// rows then takes three passes instead of two, 56 against 50 us).
+template <typename T>
+constexpr int stages() { return sizeof(T) == 4 ? 3 : 4; }
 // A step's granules, and the one behind for rows that are not aligned.
 template <typename T>
 constexpr int stage_bytes() { return 32 * NV * static_cast<int>(sizeof(T)) + 16; }
@@ -103,6 +106,7 @@ __device__ __forceinline__ int merge_lists(const key_t *a, int n, int W, Put put
     const int lane = threadIdx.x & 31;
     int i0 = 0, i1 = 0;
     key_t k0 = lane < n ? a[lane * W] : 0, k1 = lane + 32 < n ? a[(lane + 32) * W] : 0;
+#pragma unroll 1
     for (int j = 0; j < W; ++j) {
         const key_t top = warp_max(max(k0, k1));
         if (!top) return j;
@@ -143,16 +147,17 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
     constexpr int EV = 16 / sizeof(T);       // values per granule
     constexpr int STEP = 32 * NV;            // values per warp and step
     constexpr int GPL = NV / EV;             // granules per lane and step
-    constexpr int STAGE_BYTES = stage_bytes<T>();
+    constexpr int STAGE_BYTES = stage_bytes<T>(), STAGES = stages<T>();
     extern __shared__ __align__(16) uint8_t ring_all[];
     // behind the main loop the rings' memory holds the lists that are merged
     key_t (*lists)[ROW_KEYS] = reinterpret_cast<key_t (*)[ROW_KEYS]>(ring_all);
     key_t *totals = reinterpret_cast<key_t *>(ring_all + NWARP * ROW_KEYS * sizeof(key_t));  // [W][W]
     int *tokens = reinterpret_cast<int *>(totals + MAX_W * MAX_W);                           // [W][W]
-    static_assert(NWARP * ROW_KEYS * 8 + MAX_W * MAX_W * 12 <= NWARP * STAGES * stage_bytes<T>(), "lists fit in the rings");
+    static_assert(NWARP * ROW_KEYS * 8 + MAX_W * MAX_W * 12 <= NWARP * stages<T>() * stage_bytes<T>(), "lists fit in the rings");
     __shared__ float red_m[NWARP], red_l[NWARP];
     __shared__ int is_last;
-    __shared__ float kth[NWARP];  // each warp's K-th largest value so far
+    __shared__ float kth[NWARP], kth2[NWARP];  // each warp's K-th largest value so far; its K2-th lane maximum
+    __shared__ float cta_low;     // the smallest of them, as last seen
     __shared__ float s_score[MAX_W];
     __shared__ int s_done[MAX_W];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         }
         cp_async_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < STAGES - 1; ++s) load(s);  // before the beam's state is there: most beams are alive
     const bool alive = my_score > -INFINITY && !my_done;
     if (!alive) cp_async_wait<0>();
@@ -205,7 +210,25 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         key_t mine = 0, worst = 0;  // the j-th largest key in lane j; the W-th
         float thr = -INFINITY, low = -INFINITY;
         bool bad = false;
-        const int K = (W + NWARP - 1) / NWARP;
+        // The CTA's warps that have values; K values of each are W in all, and K2 of half of them.
+        const int active = max(1, min(NWARP, (V - ch * p.steps * NWARP * STEP + STEP - 1) / STEP));
+        const int K = (W + active - 1) / active, K2 = (W + (active + 1) / 2 - 1) / ((active + 1) / 2);
+        auto row_low = [&](int i) {
+            const float x = i < active ? *const_cast<volatile float *>(&kth[i & (NWARP - 1)]) : INFINITY;
+            return from_ordered(__reduce_min_sync(0xFFFFFFFFu, ordered(x)));
+        };
+        // The count-th largest of the lanes' x, and the at-th on the way (by lane 0).
+        auto kth_of_warp = [&](float x, int count, int at, float &kept) {
+            unsigned o = ordered(x), mx = 0;
+#pragma unroll 1
+            for (int j = 1; j <= count; ++j) {
+                mx = __reduce_max_sync(0xFFFFFFFFu, o);
+                if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, o == mx)) - 1) o = 0;
+                if (j == at && lane == 0) kept = from_ordered(mx);
+            }
+            return from_ordered(mx);
+        };
+        if (tid == 0) cta_low = -INFINITY;  // before the barrier of step 0
         for (int s = 0; s < max(steps, 1); ++s) {  // a warp without values has one step of -inf, for the barrier in it
             cp_async_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of step s are there, and all are done with step s - 1
@@ -262,49 +285,46 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
                 l += sum.x + sum.y;
             }
             if (s == 0) {
-                unsigned o = ordered(top), mx = 0;
-                for (int j = 0; j < K; ++j) {
-                    mx = __reduce_max_sync(0xFFFFFFFFu, o);
-                    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, o == mx)) - 1) o = 0;
-                }
-                if (lane == 0) kth[warp] = from_ordered(mx);
+                const float kb = kth_of_warp(top, K2, K, kth[warp]);
+                if (lane == 0) kth2[warp] = kb;
                 __syncthreads();
-            }
-#pragma unroll
-            for (int i = 0; i < NWARP; i += 4) {
-                const volatile float *kv = kth + i;
-                low = fminf(i ? low : INFINITY, fminf(fminf(kv[0], kv[1]), fminf(kv[2], kv[3])));
+                low = row_low(lane);
+                // the (A + 1) / 2-th largest of the warps' K2-th: a warp at the row's end, with few values, does not lower it
+                float unused;
+                low = fmaxf(low, kth_of_warp(lane < active ? kth2[lane & (NWARP - 1)] : -INFINITY, (active + 1) / 2, 0, unused));
+            } else {
+                low = *const_cast<volatile float *>(&cta_low);
             }
             thr = fmaxf(thr, low);
-            if (!__any_sync(0xFFFFFFFFu, top >= thr && top > -INFINITY)) continue;
-            unsigned mask = 0;  // this lane's values that reach the threshold
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const float y = i & 1 ? v[i / 2].y : v[i / 2].x;
-                if (y >= thr && y > -INFINITY) mask |= 1u << i;
-            }
-            while (__any_sync(0xFFFFFFFFu, mask)) {
+            // Each lane with such a value: 16 lanes look at its values again, in the ring, and those that reach the
+            // threshold are inserted, which raises it for the lanes that are left.
+            unsigned from = __ballot_sync(0xFFFFFFFFu, top >= thr && top > -INFINITY);
+            if (!from) continue;
+            do {
+                const int who = __ffs(from) - 1;
+                from &= from - 1;
+                const unsigned at = sizeof(T) == 4 ? 32 * lane + who : 64 * (lane >> 1) + 2 * who + (lane & 1);
                 key_t k = 0;
-                if (mask) {
-                    const int i = __ffs(mask) - 1;
-                    mask &= mask - 1;
-                    const unsigned at = sizeof(T) == 4 ? 32 * i + lane : 64 * (i >> 1) + 2 * lane + (i & 1);
-                    const T y = *reinterpret_cast<const T *>(ring + s % STAGES * STAGE_BYTES + cut + at * sizeof(T));
-                    k = lin::argmax_key(static_cast<float>(y), begin + s * (NWARP * STEP) + at);
+                if (lane < NV) {
+                    const float y = static_cast<float>(*reinterpret_cast<const T *>(ring + s % STAGES * STAGE_BYTES + cut + at * sizeof(T)));
+                    if (y >= thr && y > -INFINITY && y < INFINITY) k = lin::argmax_key(y, begin + s * (NWARP * STEP) + at);
                 }
-                unsigned todo = __ballot_sync(0xFFFFFFFFu, k > worst);
-                while (todo) {
-                    const int from = __ffs(todo) - 1;
-                    todo &= todo - 1;
-                    const key_t in_key = __shfl_sync(0xFFFFFFFFu, k, from);
+#pragma unroll 1
+                for (unsigned todo = __ballot_sync(0xFFFFFFFFu, k > worst); todo; todo &= todo - 1) {
+                    const key_t in_key = __shfl_sync(0xFFFFFFFFu, k, __ffs(todo) - 1);
                     const int rank = __popc(__ballot_sync(0xFFFFFFFFu, mine > in_key));
                     const key_t up = __shfl_up_sync(0xFFFFFFFFu, mine, 1);
                     if (lane >= rank && lane < W) mine = lane == rank ? in_key : up;
                 }
                 worst = __shfl_sync(0xFFFFFFFFu, mine, W - 1);
-            }
-            if (worst) thr = fmaxf(thr, key_value(worst));
+                if (worst) thr = fmaxf(thr, key_value(worst));
+                from &= __ballot_sync(0xFFFFFFFFu, top >= thr);
+            } while (from);
+            // the CTA's bound; two warps may write it at once, either value holds
             if (lane == K - 1 && mine) *const_cast<volatile float *>(&kth[warp]) = fmaxf(kth[warp], key_value(mine));
+            __syncwarp();
+            low = row_low(lane);
+            if (lane == 0 && low > *const_cast<volatile float *>(&cta_low)) *const_cast<volatile float *>(&cta_low) = low;
         }
         warp_ml(m, l);
         if (lane == 0) {
@@ -407,7 +427,7 @@ static Layout layout(int B, int W) {
 template <typename T>
 static int launch(Params p, int B, int num_sms, bool *attr_done, cudaStream_t stream) {
     constexpr int STEP = 32 * NV;
-    constexpr int SMEM = NWARP * STAGES * stage_bytes<T>();
+    constexpr int SMEM = NWARP * stages<T>() * stage_bytes<T>();
     const long long rows = static_cast<long long>(B) * p.W;
     // CTAs of a row. One pass of all resident CTAs costs a CTA's steps and about as much as FIXED steps to start and to
     // merge; the number of CTAs per row that makes passes x cost least is taken. Few rows so come down to one step per warp,
