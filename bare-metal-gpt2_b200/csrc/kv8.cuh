@@ -68,7 +68,7 @@ inline Work work_layout(const GPT2KV8Cache *kv, int Hq, int Tq) {
     w.list = reinterpret_cast<int *>(b + o_list);
     w.moves = reinterpret_cast<int2 *>(b + o_mov);
     w.part = reinterpret_cast<float *>(b + o_part);
-    w.bytes = o_part + up(attend_max_ctas() * rows * (kv->headDim + 2) * sizeof(float));
+    w.bytes = o_part + up(attend_max_ctas() * rows * (kv->headDim + 4) * sizeof(float));
     return w;
 }
 

@@ -29,6 +29,7 @@
 // unit borders. At a border the warps are merged in shared memory; a unit cut by a piece's end is merged
 // through the work area by the last CTA to arrive, in piece order.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "ptx.cuh"
@@ -36,7 +37,7 @@
 namespace b200 {
 namespace kv8 {
 
-constexpr int NW = 4;                // warps per CTA
+constexpr int NW_PIECES = 4, NW_UNITS = 2;  // warps per CTA, see the plan in gpt2_kv8_attend_b200
 constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
 constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
 constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
@@ -148,19 +149,35 @@ struct Chunk {
     }
 };
 constexpr int CHUNK_BYTES = 4096;
-// Chunks per warp's ring. Three CTAs of 4 x 4 chunks (192 KB) fill an SM's shared memory.
-constexpr int STAGES = 4;
-constexpr int RING_BYTES = NW * STAGES * CHUNK_BYTES;
 
-template <int KIND, int D, int ROWS>
-__global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_attend(const View c, const AttParams a) {
+// A kernel variant's shape: registers for `resident` CTAs per SM, and the shared memory of a CTA.
+//   D 64, 8 rows: 12 warps per SM, 4 chunks per warp's ring.
+//   else: the accumulators of 128 dims or 16 rows take the registers; q of 128 dims lies in shared memory instead (32
+//   registers), and the warps' rows are merged in two halves of the dims, so that 12 warps fit with 3 chunks per ring
+//   (8 sequences of 8192 to 16384 keys, 8 x 4 heads, 4 queries: 71 us).
+template <int D, int ROWS, int NW>
+struct Shape {
+    static constexpr int RESIDENT = 12 / NW;
+    static constexpr int STAGES = D == 64 && ROWS == 8 ? 4 : 3;
+    static constexpr int RING = NW * STAGES * CHUNK_BYTES;
+    static constexpr int DH = D / 2;                      // dims merged at a time
+    static constexpr int SO = NW * ROWS * (DH + 4) * 4;
+    static constexpr bool Q_SMEM = D == 128;
+    static constexpr int QS = Q_SMEM ? D / 16 * 512 : 0;
+    static constexpr int BYTES = RING + SO + QS;
+};
+
+template <int KIND, int D, int ROWS, int NW>
+__global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_attend(const View c, const AttParams a) {
     using C = Chunk<D>;
+    using SH = Shape<D, ROWS, NW>;
+    constexpr int STAGES = SH::STAGES, RING_BYTES = SH::RING, DH = SH::DH;
     constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
     constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
-    constexpr int SO_BYTES = NW * ROWS * (D + 4) * 4;
     extern __shared__ __align__(128) uint8_t ring_all[];
-    float (*so)[ROWS][D + 4] = reinterpret_cast<float (*)[ROWS][D + 4]>(ring_all + RING_BYTES);  // [NW]
-    int *pre = reinterpret_cast<int *>(ring_all + RING_BYTES + SO_BYTES);  // [entries + 1]: chunks before each entry
+    float (*so)[ROWS][DH + 4] = reinterpret_cast<float (*)[ROWS][DH + 4]>(ring_all + RING_BYTES);  // [NW]
+    uint4 *qs = reinterpret_cast<uint4 *>(ring_all + RING_BYTES + SH::SO);  // [KS][32]: A operands of a k-step
+    int *pre = reinterpret_cast<int *>(ring_all + SH::BYTES);               // [entries + 1]: chunks before each entry
     __shared__ float sm[NW][ROWS], sl[NW][ROWS];
     __shared__ int is_last, warp_sum[NW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -324,7 +341,7 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
     const int vl = 2048 + (D == 64 ? ((((t >> 1) * 4 + (t & 1)) * 4 + ((g >> 1) ^ (t & 2))) * 16 + (g & 1) * 8)
                                    : (2 * t * 8 + (g ^ (2 * t))) * 16);
     // The segment at hand: q, m, l, o and the keys its rows see.
-    uint32_t qa[KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
+    __align__(16) uint32_t qa[SH::Q_SMEM ? 1 : KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
     float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
     // masked is a constant at both calls
@@ -340,7 +357,8 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
 #pragma unroll
                 for (int tile = 0; tile < NT; ++tile) {
                     const uint32_t w = st == 0 ? kw[tile].x : st == 1 ? kw[tile].y : st == 2 ? kw[tile].z : kw[tile].w;
-                    const uint32_t (&qq)[4] = qa[4 * s4 + st];
+                    if (SH::Q_SMEM && tile == 0) *reinterpret_cast<uint4 *>(qa[0]) = qs[(4 * s4 + st) * 32 + lane];
+                    const uint32_t (&qq)[4] = qa[SH::Q_SMEM ? 0 : 4 * s4 + st];
                     uint32_t b0, b1;
                     halves4<KIND>(w, b0, b1);
                     if (s4 == 0 && st == 0) mma16816_first(s[tile], qq[0], qq[1], qq[2], qq[3], b0, b1);
@@ -437,13 +455,12 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
                 pairs4<KIND>(vw[2][q], vw[3][q], b1);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (ROWS == 8) {
-                        mma16816(o[4 * q + j], ph[0], pl[0], ph[RR], pl[RR], b0[j], b1[j]);
-                    } else {
-                        mma16816(o[4 * q + j], ph[0], ph[RR - 1], ph[RR], ph[2 * RR - 1], b0[j], b1[j]);
-                        mma16816(o[4 * q + j], pl[0], pl[RR - 1], pl[RR], pl[2 * RR - 1], b0[j], b1[j]);
-                    }
+                    if (ROWS == 8) mma16816(o[4 * q + j], ph[0], pl[0], ph[RR], pl[RR], b0[j], b1[j]);
+                    else mma16816(o[4 * q + j], ph[0], ph[RR - 1], ph[RR], ph[2 * RR - 1], b0[j], b1[j]);
                 }
+                if (ROWS == 16)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma16816(o[4 * q + j], pl[0], pl[RR - 1], pl[RR], pl[2 * RR - 1], b0[j], b1[j]);
             }
         }
     };
@@ -472,6 +489,7 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
         const int u1 = unit_of(x0) + u0, x1 = min(u1, c1);
         full_end = one ? n : min(n - a.Tq + qt * ROWS / a.G + 1, last_end);
         // q: thread (g, t) holds dims 64 * (s / 4) + 16 t + 4 (s % 4) .. + 3 of row g (and g + 8) for k-step s
+        if (SH::Q_SMEM) __syncthreads();  // every warp is through with the last segment's q
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
             const int row = qt * ROWS + g + 8 * rr;
@@ -481,6 +499,7 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
             const __half *qp = a.q + r * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (row - tok * a.G)) * D + 16 * t;
 #pragma unroll
             for (int s4 = 0; s4 < KS / 4; ++s4) {
+                if (SH::Q_SMEM && s4 % NW != warp) continue;  // the warps share the work
                 uint4 x[2] = {};
                 if (ok) {
                     x[0] = *reinterpret_cast<const uint4 *>(qp + 64 * s4);
@@ -489,17 +508,29 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
                 const uint32_t *w = reinterpret_cast<const uint32_t *>(x);
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    qa[4 * s4 + s][rr] = w[2 * s];
-                    qa[4 * s4 + s][2 + rr] = w[2 * s + 1];
-                    if (RR == 1) {
-                        qa[4 * s4 + s][1] = twin(w[2 * s]);
-                        qa[4 * s4 + s][3] = twin(w[2 * s + 1]);
+                    if (SH::Q_SMEM) {
+                        uint32_t *dst = reinterpret_cast<uint32_t *>(qs + (4 * s4 + s) * 32 + lane);
+                        dst[rr] = w[2 * s];
+                        dst[2 + rr] = w[2 * s + 1];
+                        if (RR == 1) {
+                            dst[1] = w[2 * s];
+                            dst[3] = w[2 * s + 1];
+                        }
+                    } else {
+                        uint32_t (&dst)[4] = qa[SH::Q_SMEM ? 0 : 4 * s4 + s];
+                        dst[rr] = w[2 * s];
+                        dst[2 + rr] = w[2 * s + 1];
+                        if (RR == 1) {
+                            dst[1] = twin(w[2 * s]);
+                            dst[3] = twin(w[2 * s + 1]);
+                        }
                     }
                 }
             }
             m[rr] = -INFINITY;
             l[rr] = 0.0f;
         }
+        if (SH::Q_SMEM) __syncthreads();
 #pragma unroll
         for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
         S = (i / SET) & 1 ? pmax[1] : pmax[0];
@@ -533,52 +564,60 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
         if (pos < first || pos + CK > full_end || ok != (1u << GR) - 1u) compute(true, buf, pos, ks, vs, ok);
         else compute(false, buf, pos, ks, vs, ok);
     }
-        // the warps' rows: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and 2 t + 1)
-        if (x0 > c0) __syncthreads();  // the last segment's merge is through
-#pragma unroll
-        for (int rr = 0; rr < RR; ++rr) {
-            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
-            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
-            if (t == 0) {
-                sm[warp][g + 8 * rr] = m[rr];
-                sl[warp][g + 8 * rr] = l[rr];
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < DT; j += 4) {
-                    float4 w;
-                    float *wf = reinterpret_cast<float *>(&w);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
-                    *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * t + e) * DT + j]) = w;
-                }
-        }
-        __syncthreads();
+        // The warps' rows, half of the dims at a time: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and
+        // 2 t + 1), t 0, 1 the lower half.
         const int rows = min(ROWS, R - qt * ROWS);
         const bool whole = u0 >= c0 && u1 <= c1;
         const int prow = min(ROWS, R);  // rows of a tile in the work area
         const int slot = 2 * blockIdx.x + (x0 == c0 ? 0 : 1);
-        for (int x = tid; x < rows * D; x += 32 * NW) {
-            const int row = x / D, d = x % D;
-            const float mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
-            float lx = 0.0f, y = 0.0f;
-            if (mx > -INFINITY) {
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float f = ex2(sm[w][row] - mx);
-                    lx = fmaf(f, sl[w][row], lx);
-                    y = fmaf(f, so[w][row][d], y);
+        for (int rr = 0; rr < RR; ++rr) {
+            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
+            l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
+        }
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            if (x0 > c0 || half) __syncthreads();  // the last merge is through
+            if (t >> 1 == half) {
+#pragma unroll
+                for (int rr = 0; rr < RR; ++rr) {
+                    if ((t & 1) == 0) {
+                        sm[warp][g + 8 * rr] = m[rr];
+                        sl[warp][g + 8 * rr] = l[rr];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int j = 0; j < DT; j += 4) {
+                            float4 w;
+                            float *wf = reinterpret_cast<float *>(&w);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
+                            *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * (t & 1) + e) * DT + j]) = w;
+                        }
                 }
             }
-            if (whole) {
-                put(h, row, d, lx > 0.0f ? y / lx : 0.0f);
-            } else {
-                float *pr = a.part + (static_cast<long long>(slot) * prow + row) * (D + 2);
-                pr[d] = y;
-                if (d == 0) {
-                    pr[D] = mx;
-                    pr[D + 1] = lx;
+            __syncthreads();
+            for (int x = tid; x < rows * DH; x += 32 * NW) {
+                const int row = x / DH, dh = x % DH, d = half * DH + dh;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w][row]);
+                float lx = 0.0f, y = 0.0f;
+                if (mx > -INFINITY) {
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) {
+                        const float f = ex2(sm[w][row] - mx);
+                        lx = fmaf(f, sl[w][row], lx);
+                        y = fmaf(f, so[w][row][dh], y);
+                    }
+                }
+                if (whole) {
+                    put(h, row, d, lx > 0.0f ? y / lx : 0.0f);
+                } else {
+                    float *pr = a.part + static_cast<long long>(slot) * prow * (D + 4);  // [prow][D] o, [prow][2] m, l, 16-byte steps
+                    pr[row * D + d] = y;
+                    if (d == 0) *reinterpret_cast<float2 *>(pr + prow * D + 2 * row) = make_float2(mx, lx);
                 }
             }
         }
@@ -594,32 +633,42 @@ __global__ void __launch_bounds__(32 * NW, ROWS == 8 && D == 64 ? 3 : 2) k_kv8_a
             }
             __syncthreads();
             if (is_last) {
-                const long long step = static_cast<long long>(prow) * (D + 2);
-                for (int x = tid; x < rows * D; x += 32 * NW) {
-                    const int row = x / D, d = x % D;
-                    const float *p0 = a.part + s0 * step + row * (D + 2), *pk = a.part + 2 * (k0 + 1) * step + row * (D + 2);
-                    float mx = __ldcg(p0 + D), lx = __ldcg(p0 + D + 1), y = __ldcg(p0 + d);
-                    for (int k = 0; k < k1 - k0; k += 4) {  // four pieces' loads at once
-                        float m4[4], l4[4], y4[4];
+                const long long step = static_cast<long long>(prow) * (D + 4);
+                // Four dims per thread and four pieces at a time, all their loads in flight.
+#pragma unroll 2
+                for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
+                    const int row = x / (D / 4), d = x % (D / 4) * 4;
+                    float mx = -INFINITY, lx = 0.0f;
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int k = k0; k <= k1; k += 4) {
+                        float2 ml[4];
+                        float4 yk[4];
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            const bool in = k + u < k1 - k0;
-                            const float *q = pk + 2 * (in ? k + u : k) * step;
-                            m4[u] = in ? __ldcg(q + D) : -INFINITY;
-                            l4[u] = __ldcg(q + D + 1);
-                            y4[u] = __ldcg(q + d);
+                            const int kk = min(k + u, k1);
+                            const float *q = a.part + (kk == k0 ? s0 : 2 * kk) * step;
+                            ml[u] = __ldcg(reinterpret_cast<const float2 *>(q + prow * D + 2 * row));
+                            yk[u] = __ldcg(reinterpret_cast<const float4 *>(q + row * D + d));
+                            if (k + u > k1) ml[u].x = -INFINITY;
                         }
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            const float mn = fmaxf(mx, m4[u]);
+                            const float mn = fmaxf(mx, ml[u].x);
                             if (mn == -INFINITY) continue;
-                            const float f = ex2(mx - mn), f4 = ex2(m4[u] - mn);
-                            lx = fmaf(lx, f, l4[u] * f4);
-                            y = fmaf(y, f, y4[u] * f4);
+                            const float f = ex2(mx - mn), fk = ex2(ml[u].x - mn);
+                            lx = fmaf(lx, f, ml[u].y * fk);
+                            y.x = fmaf(y.x, f, yk[u].x * fk);
+                            y.y = fmaf(y.y, f, yk[u].y * fk);
+                            y.z = fmaf(y.z, f, yk[u].z * fk);
+                            y.w = fmaf(y.w, f, yk[u].w * fk);
                             mx = mn;
                         }
                     }
-                    put(h, row, d, lx > 0.0f ? y / lx : 0.0f);
+                    const float inv = lx > 0.0f ? 1.0f / lx : 0.0f;
+                    put(h, row, d, y.x * inv);
+                    put(h, row, d + 1, y.y * inv);
+                    put(h, row, d + 2, y.z * inv);
+                    put(h, row, d + 3, y.w * inv);
                 }
             }
         }
@@ -672,36 +721,44 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
     const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
     if (entries > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
-    // Units that fill the GPU once keep their own CTAs: they share no unit and need no prefix sum, which is worth more than
-    // equal pieces as long as a unit is short (64 sequences x 12 heads of 512 to 1023 keys: 27.6 against 30.9 us).
-    const int full = (rows == 8 && kv->headDim == 64 ? 3 : 2) * ctx->num_sms;
-    const bool pieces = entries * kv->nHead < full && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
+    // Plan. Units that fill the GPU once have a CTA each: no prefix sum, no shared units; two warps per CTA, so that the
+    // longest unit ends soon after the others (64 sequences x 12 heads of 512 to 1023 keys: 26.9 us, with four warps
+    // 27.7, in equal pieces 30.9). Fewer units: equal pieces, four warps per CTA, which merge their rows before a piece's
+    // partials go through the work area.
+    const bool pieces = entries * kv->nHead < 3ll * ctx->num_sms && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
     a.entries = pieces ? static_cast<int>(entries) : 0;
-    const int smem = kv8::RING_BYTES + kv8::NW * rows * (kv->headDim + 4) * 4 + (a.entries + 1) * 4;
-    // CTAs that are resident together: registers (the kernel's launch bounds) and 228 KB of shared memory, 1 KB of it per CTA.
-    const int resident = std::min(rows == 8 && kv->headDim == 64 ? 3 : 2, 228 * 1024 / (smem + 1024 + 512));
-    const dim3 grid = pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident,
-                                                                             kv8::MAX_PIECES, (chunks + kv8::NW - 1) / kv8::NW})))
-                             : dim3(static_cast<unsigned>(entries), kv->nHead);
     const kv8::View c = kv8::view(kv, ctx->status);
-    bool *attr_done = &ctx->kv8_attr_done[(kv->kind == GPT2_KV8_INT8 ? 0 : 4) + (kv->headDim == 64 ? 0 : 2) + (rows == 8 ? 0 : 1)];
-    auto go = [&](auto kern) {
+    auto go = [&](auto kern, auto shape, int variant) {
+        using SH = decltype(shape);
+        bool *attr_done = &ctx->kv8_attr_done[variant];
         if (!*attr_done) {
             RelaxedCapture relaxed;
-            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kv8::RING_BYTES + kv8::NW * rows * (kv->headDim + 4) * 4 + (kv8::MAX_ENTRIES + 1) * 4) != cudaSuccess)
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::BYTES + (kv8::MAX_ENTRIES + 1) * 4) != cudaSuccess)
                 return GPT2_B200_ECUDA;
             *attr_done = true;
         }
-        kern<<<grid, 32 * kv8::NW, smem, stream>>>(c, a);
+        const int smem = SH::BYTES + (a.entries + 1) * 4;
+        // CTAs that are resident together: registers (the kernel's launch bounds) and 228 KB of shared memory, 1 KB of it per CTA.
+        const int resident = std::min(SH::RESIDENT, 228 * 1024 / (smem + 1024 + 512));
+        const int warps = pieces ? kv8::NW_PIECES : kv8::NW_UNITS;
+        const dim3 grid = pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident,
+                                                                                 kv8::MAX_PIECES, (chunks + warps - 1) / warps})))
+                                 : dim3(static_cast<unsigned>(entries), kv->nHead);
+        kern<<<grid, 32 * warps, smem, stream>>>(c, a);
         return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
     };
-    if (kv->kind == GPT2_KV8_INT8) {
-        if (kv->headDim == 64)
-            return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 16>);
-        return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_INT8, 128, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_INT8, 128, 16>);
-    }
-    if (kv->headDim == 64)
-        return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 64, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 64, 16>);
-    return rows == 8 ? go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 128, 8>) : go(kv8::k_kv8_attend<GPT2_KV8_E4M3, 128, 16>);
+    auto by_rows = [&](auto kind, auto dim) {
+        constexpr int KIND = decltype(kind)::value, D = decltype(dim)::value;
+        constexpr int NP = kv8::NW_PIECES, NU = kv8::NW_UNITS, base = (KIND == GPT2_KV8_INT8 ? 0 : 8) + (D == 64 ? 0 : 4);
+        if (rows == 8)
+            return pieces ? go(kv8::k_kv8_attend<KIND, D, 8, NP>, kv8::Shape<D, 8, NP>(), base)
+                          : go(kv8::k_kv8_attend<KIND, D, 8, NU>, kv8::Shape<D, 8, NU>(), base + 1);
+        return pieces ? go(kv8::k_kv8_attend<KIND, D, 16, NP>, kv8::Shape<D, 16, NP>(), base + 2)
+                      : go(kv8::k_kv8_attend<KIND, D, 16, NU>, kv8::Shape<D, 16, NU>(), base + 3);
+    };
+    auto by_dim = [&](auto kind) {
+        return kv->headDim == 64 ? by_rows(kind, std::integral_constant<int, 64>()) : by_rows(kind, std::integral_constant<int, 128>());
+    };
+    return kv->kind == GPT2_KV8_INT8 ? by_dim(std::integral_constant<int, GPT2_KV8_INT8>())
+                                     : by_dim(std::integral_constant<int, GPT2_KV8_E4M3>());
 }
