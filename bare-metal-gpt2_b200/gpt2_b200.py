@@ -157,6 +157,9 @@ _SIGS = {
     "gpt2_beam_work_bytes_b200": (_cs, [_ci, _ci]),
     "gpt2_beam_select_b200": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _cll, _vp, _vp, _ci, _ci, _ci, _ci, _vp,
                                     _cs, _vp]),
+    "gpt2_b200_beam_create": (_ci, [ctypes.POINTER(_vp), _wp, _k8p, _ci, _ci]),
+    "gpt2_b200_beam_destroy": (None, [_vp]),
+    "gpt2_b200_beam_generate": (_ci, [_vp, _vp, _cll, _vp, _ci, _ci, _vp, _cll, _vp, _vp]),
     "gpt2_b200_compose_backend": (None, [ctypes.POINTER(GPT2Backend), ctypes.POINTER(GPT2Backend)]),
     "gpt2_b200_reserve": (_ci, [_ci, _ci, _ci]),
     "gpt2_b200_status": (_cu, [_ci]),
@@ -453,6 +456,35 @@ class DecodeBatch:
         """Destroys the batch (the library synchronises the device first); safe to call twice."""
         if self.h:
             self.lib.gpt2_b200_batch_destroy(self.h)
+            self.h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+
+class BeamDecoder:
+    """Beam search with GPT-2-124M over a KV8Cache of B * W rows (the gpt2_b200_beam_* entry points)."""
+
+    def __init__(self, lib: "Lib", weights: ModelWeights, cache: KV8Cache, B: int, W: int):
+        self.lib, self.weights, self.cache, self.B, self.W = lib, weights, cache, B, W
+        self.h = ctypes.c_void_p()
+        lib.check(lib.gpt2_b200_beam_create(ctypes.byref(self.h), ctypes.byref(weights.struct), cache.ref_c, B, W),
+                  "gpt2_b200_beam_create")
+
+    def generate(self, prompt, prompt_len, n_steps: int, out, score=None, eos: int = -1, stream: int = 0) -> None:
+        """prompt: int32 [B][P]; prompt_len: int32 [B] (1..P); out: int32 [B * W][>= n_steps+1], each item's
+        hypotheses best first; score: fp32 [B * W] or None."""
+        self.lib.check(self.lib.gpt2_b200_beam_generate(
+            self.h, prompt.data_ptr(), prompt.stride(0), prompt_len.data_ptr(), n_steps, eos, out.data_ptr(),
+            out.stride(0), score.data_ptr() if score is not None else None, stream), "gpt2_b200_beam_generate")
+
+    def close(self) -> None:
+        """Destroys the decoder (the library synchronises the device first); safe to call twice."""
+        if self.h:
+            self.lib.gpt2_b200_beam_destroy(self.h)
             self.h = ctypes.c_void_p()
 
     def __del__(self):

@@ -385,6 +385,21 @@ int gpt2_beam_select_b200(int *token, int *parent, float *new_score, int *new_do
                           int type, long long ld, const float *score, const int *done, int B, int W,
                           int V, int eos, void *work, size_t work_bytes, cudaStream_t stream);
 
+/* Beam search with GPT-2-124M: the decode step of gpt2_b200_batch_step over the 8-bit cache, the selection and the
+ * reorder, captured in one CUDA graph. B prompts, W beams each (W 1..32, B*W <= 256), over a cache of B*W rows in the
+ * GPT-2-124M shape, whose pages must be enough for what the beams hold apart (status bit otherwise); weights and cache
+ * stay owned by the caller. */
+typedef struct gpt2_b200_beam gpt2_b200_beam;
+int gpt2_b200_beam_create(gpt2_b200_beam **out, const GPT2WeightsGPU *w, const GPT2KV8Cache *kv, int B, int W);
+/* Releases the beam decoder; synchronises its device first. */
+void gpt2_b200_beam_destroy(gpt2_b200_beam *bm);
+/* Empties the cache and runs n_steps steps (at most 1024 and the cache's positions): item b consumes its prompt
+ * d_prompt[b][0 .. d_plen[b]-1] one token per step, then its W beams are extended by the W best continuations per step; a
+ * beam that chose eos (-1: none) keeps its score and repeats eos. d_out[b*W+w][0..n_steps] receives hypothesis w of item b,
+ * best first (prompt included), d_score[b*W+w] (if not NULL) the sum of its chosen tokens' log probabilities. */
+int gpt2_b200_beam_generate(gpt2_b200_beam *bm, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps,
+                            int eos, int *d_out, long long out_stride, float *d_score, cudaStream_t stream);
+
 /* ================================================================ backend, status, set-up */
 
 /* Composes a backend the reference's way (cuda/kernels_fused.cu:157-164): copies *base and installs
