@@ -132,13 +132,14 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// A warp's chunk of CK keys in shared memory: 2 KB of K rows, then 2 KB of V rows, in 16-byte granules.
+// A warp's chunk of CK keys in shared memory: K rows, then V rows, half of it each, in 16-byte granules.
 // Reads: K, a quarter warp takes granules 0..3 (then 4..7 for D 128) of two neighbouring rows; V, a half warp takes two
 // granules (8 bytes a lane) or a quarter warp two granules (16 bytes a lane) of rows 0, 2, 4, 6 of an 8-row
 // group. The maps put each such set on 8 different bank groups (granule index mod 8).
+constexpr int CHUNK_BYTES = 8192, HALF = CHUNK_BYTES / 2;
 template <int D>
 struct Chunk {
-    static constexpr int CK = 2048 / D, GR = CK / 16, ROWG = D / 16;  // granules per row
+    static constexpr int CK = CHUNK_BYTES / 2 / D, GR = CK / 16, ROWG = D / 16;  // granules per row
     __device__ static int k_at(int row, int gr) { return row * ROWG + (D == 64 ? gr : gr ^ ((row & 1) << 2)); }
     __device__ static int v_at(int row, int gr) {
         if (D == 64) {  // 8-row groups: row bits (b2 b1 b0) stored as (b2 b0 b1); the granule's high bit flipped by b2
@@ -148,7 +149,6 @@ struct Chunk {
         return row * ROWG + (gr ^ (row & 6));
     }
 };
-constexpr int CHUNK_BYTES = 4096;
 
 // A kernel variant's shape: registers for `resident` CTAs per SM, and the shared memory of a CTA.
 //   D 64, 8 rows: 12 warps per SM, 4 chunks per warp's ring.
@@ -158,7 +158,7 @@ constexpr int CHUNK_BYTES = 4096;
 template <int D, int ROWS, int NW>
 struct Shape {
     static constexpr int RESIDENT = 12 / NW;
-    static constexpr int STAGES = D == 64 && ROWS == 8 ? 4 : 3;
+    static constexpr int STAGES = 2;
     static constexpr int RING = NW * STAGES * CHUNK_BYTES;
     static constexpr int DH = D / 2;                      // dims merged at a time
     static constexpr int SO = NW * ROWS * (DH + 4) * 4;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     const uint8_t *kbase = c.data + krow * D + cgr * 16;
     const uint8_t *vbase = c.data + vrow * D + cgr * 16 + (static_cast<size_t>(c.nHead) << c.page_shift) * D;
     // C::k_at and C::v_at of this lane's granule, without the multiples of 8 (D 64) or 4 rows that are immediates below
-    const int ko = C::k_at(krow, cgr) * 16, vo0 = 2048 + C::v_at(vrow, cgr) * 16, vo1 = 2048 + C::v_at(vrow, cgr ^ (D == 64 ? 0 : 4)) * 16;
+    const int ko = C::k_at(krow, cgr) * 16, vo0 = HALF + C::v_at(vrow, cgr) * 16, vo1 = HALF + C::v_at(vrow, cgr ^ (D == 64 ? 0 : 4)) * 16;
     auto load = [&](int i, int stage) {  // chunk i of this warp; its set has been looked up
         const uint32_t dst = ring_s + stage * CHUNK_BYTES;
 #pragma unroll
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     // Shared-memory offsets of this lane's reads, so that all but an immediate is computed once (C::k_at, C::v_at).
     const int kl0 = (D == 64 ? g * 4 + t : g * 8 + (t ^ ((g & 1) << 2))) * 16;
     const int kl1 = D == 64 ? 0 : (g * 8 + ((4 + t) ^ ((g & 1) << 2))) * 16;
-    const int vl = 2048 + (D == 64 ? ((((t >> 1) * 4 + (t & 1)) * 4 + ((g >> 1) ^ (t & 2))) * 16 + (g & 1) * 8)
+    const int vl = HALF + (D == 64 ? ((((t >> 1) * 4 + (t & 1)) * 4 + ((g >> 1) ^ (t & 2))) * 16 + (g & 1) * 8)
                                    : (2 * t * 8 + (g ^ (2 * t))) * 16);
     // The segment at hand: q, m, l, o and the keys its rows see.
     __align__(16) uint32_t qa[SH::Q_SMEM ? 1 : KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
@@ -716,7 +716,7 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     a.part = w.part;
     a.arrive = w.arrive;
     const long long R = static_cast<long long>(a.G) * Tq;
-    const int rows = R <= 8 ? 8 : 16, ck = 2048 / kv->headDim;
+    const int rows = R <= 8 ? 8 : 16, ck = kv8::HALF / kv->headDim;
     a.qtiles = static_cast<int>((R + rows - 1) / rows);
     const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
     const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
