@@ -355,11 +355,9 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
     }
     __syncthreads();
     if (tid == 0) {
-        __threadfence();  // the CTA's results, ordered before it by the barrier, are visible with the count
-        const unsigned seen = atomicAdd(&p.arrive[item], 1u);
+        const unsigned seen = kv8::arrive_add(&p.arrive[item]);
         is_last = seen == static_cast<unsigned>(W * p.chunks - 1);
         if (is_last) p.arrive[item] = 0;
-        __threadfence();
     }
     __syncthreads();
     if (!is_last) return;

@@ -103,6 +103,15 @@ inline View view(const GPT2KV8Cache *kv, unsigned *status) {
     return v;
 }
 
+// Counts this CTA in at a counter in global memory. Called by one thread behind a CTA barrier and before another: what the
+// CTA wrote before is visible to the CTA that counts last, and what the others wrote is visible to this one (release and
+// acquire at GPU scope; the two barriers carry both to the CTA's other threads).
+__device__ __forceinline__ unsigned arrive_add(unsigned *p) {
+    unsigned v;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
 // ---------------------------------------------------------------- codes
 template <int KIND>
 __device__ __forceinline__ float qmax() {

@@ -37,7 +37,7 @@
 namespace b200 {
 namespace kv8 {
 
-constexpr int NW_PIECES = 4, NW_UNITS = 2;  // warps per CTA, see the plan in gpt2_kv8_attend_b200
+constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces (whole units: 1 or 2, see the plan)
 constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
 constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
 constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
@@ -625,11 +625,9 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             const int k0 = u0 / per, k1 = (u1 - 1) / per, s0 = 2 * k0 + (u0 == k0 * per ? 0 : 1);
             __syncthreads();
             if (tid == 0) {
-                __threadfence();  // the CTA's partials, ordered before it by the barrier, are visible with the count
-                const unsigned seen = atomicAdd(&a.arrive[s0], 1u);
+                const unsigned seen = arrive_add(&a.arrive[s0]);
                 is_last = seen == static_cast<unsigned>(k1 - k0);
                 if (is_last) a.arrive[s0] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (is_last) {
@@ -721,11 +719,14 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
     const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
     if (entries > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
-    // Plan. Units that fill the GPU once have a CTA each: no prefix sum, no shared units; two warps per CTA, so that the
-    // longest unit ends soon after the others (64 sequences x 12 heads of 512 to 1023 keys: 26.9 us, with four warps
-    // 27.7, in equal pieces 30.9). Fewer units: equal pieces, four warps per CTA, which merge their rows before a piece's
-    // partials go through the work area.
-    const bool pieces = entries * kv->nHead < 3ll * ctx->num_sms && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
+    // Plan. Units that fill the GPU have a CTA each: no prefix sum, no shared units. Two warps per CTA (64 sequences x 12 heads
+    // of 512 to 1023 keys: 25.2 us, with one warp 32.7, with four 27.7, in equal pieces 30.9) as long as single warps would leave
+    // a third of the SMs' 12 warps empty, then one (128 x 12 units of 640 to 700 keys: 28.8 against 33.5 us; 256 x 12 of 150 to
+    // 300: 33.3 against 40.0). Fewer units: equal pieces, four warps per CTA, which merge their rows before a piece's partials
+    // go through the work area.
+    const long long units = entries * kv->nHead;
+    const bool pieces = units < 3ll * ctx->num_sms && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
+    const int warps = pieces ? kv8::NW_PIECES : units < 8ll * ctx->num_sms ? 2 : 1;
     a.entries = pieces ? static_cast<int>(entries) : 0;
     const kv8::View c = kv8::view(kv, ctx->status);
     auto go = [&](auto kern, auto shape, int variant) {
@@ -740,7 +741,6 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
         const int smem = SH::BYTES + (a.entries + 1) * 4;
         // CTAs that are resident together: registers (the kernel's launch bounds) and 228 KB of shared memory, 1 KB of it per CTA.
         const int resident = std::min(SH::RESIDENT, 228 * 1024 / (smem + 1024 + 512));
-        const int warps = pieces ? kv8::NW_PIECES : kv8::NW_UNITS;
         const dim3 grid = pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident,
                                                                                  kv8::MAX_PIECES, (chunks + warps - 1) / warps})))
                                  : dim3(static_cast<unsigned>(entries), kv->nHead);
@@ -749,12 +749,15 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     };
     auto by_rows = [&](auto kind, auto dim) {
         constexpr int KIND = decltype(kind)::value, D = decltype(dim)::value;
-        constexpr int NP = kv8::NW_PIECES, NU = kv8::NW_UNITS, base = (KIND == GPT2_KV8_INT8 ? 0 : 8) + (D == 64 ? 0 : 4);
-        if (rows == 8)
-            return pieces ? go(kv8::k_kv8_attend<KIND, D, 8, NP>, kv8::Shape<D, 8, NP>(), base)
-                          : go(kv8::k_kv8_attend<KIND, D, 8, NU>, kv8::Shape<D, 8, NU>(), base + 1);
-        return pieces ? go(kv8::k_kv8_attend<KIND, D, 16, NP>, kv8::Shape<D, 16, NP>(), base + 2)
-                      : go(kv8::k_kv8_attend<KIND, D, 16, NU>, kv8::Shape<D, 16, NU>(), base + 3);
+        constexpr int base = (KIND == GPT2_KV8_INT8 ? 0 : 12) + (D == 64 ? 0 : 6);
+        if (rows == 8) {
+            if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4>, kv8::Shape<D, 8, 4>(), base);
+            if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 2>, kv8::Shape<D, 8, 2>(), base + 1);
+            return go(kv8::k_kv8_attend<KIND, D, 8, 1>, kv8::Shape<D, 8, 1>(), base + 2);
+        }
+        if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 16, 4>, kv8::Shape<D, 16, 4>(), base + 3);
+        if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 16, 2>, kv8::Shape<D, 16, 2>(), base + 4);
+        return go(kv8::k_kv8_attend<KIND, D, 16, 1>, kv8::Shape<D, 16, 1>(), base + 5);
     };
     auto by_dim = [&](auto kind) {
         return kv->headDim == 64 ? by_rows(kind, std::integral_constant<int, 64>()) : by_rows(kind, std::integral_constant<int, 128>());
