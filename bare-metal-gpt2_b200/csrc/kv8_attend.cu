@@ -10,9 +10,9 @@
 //     in as hi + lo (two fp16, 22 bits): rounding it to one fp16 alone would add an error of the size of the
 //     output's own rounding. With at most 8 query rows (the decode step) the MMA's rows 8..15 are
 //     free and take lo; with 9 to 16 rows lo is a second MMA. mma.sync's rate is far above what HBM feeds
-//     (32 MMAs per 4 KB of codes).
-//   - a warp takes CK keys at a time (32 for D 64, 16 for D 128: 4 KB of K and V) through a ring of its own in shared
-//     memory (cp.async, STAGES - 1 chunks in flight, no CTA barrier). The sum over dims (QK) may run in any order of dims,
+//     (64 MMAs of 8 cycles per 8 KB of codes).
+//   - a warp takes CK keys at a time (64 for D 64, 32 for D 128: 8 KB of K and V) through a ring of its own in shared
+//     memory (cp.async, the next chunk in flight while one is computed, no CTA barrier). The sum over dims (QK) may run in any order of dims,
 //     so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
 //     column order are as free, so a thread reads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with
 //     16 neighbouring output dims. The 16-byte granules of a chunk are permuted so that neither read has bank conflicts.
@@ -150,17 +150,15 @@ struct Chunk {
     }
 };
 
-// A kernel variant's shape: registers for `resident` CTAs per SM, and the shared memory of a CTA.
-//   D 64, 8 rows: 12 warps per SM, 4 chunks per warp's ring.
-//   else: the accumulators of 128 dims or 16 rows take the registers; q of 128 dims lies in shared memory instead (32
-//   registers), and the warps' rows are merged in two halves of the dims, so that 12 warps fit with 3 chunks per ring
-//   (8 sequences of 8192 to 16384 keys, 8 x 4 heads, 4 queries: 71 us).
+// A kernel variant's shape: 12 warps per SM, each with two chunks in its ring (192 KB of an SM's shared memory). The accumulators
+// of 128 dims or 16 rows take the registers, so q of 128 dims lies in shared memory instead (32 registers), and the warps'
+// rows are merged in two halves of the dims: the merge area of 16 rows x 128 dims would leave room for 8 warps only.
 template <int D, int ROWS, int NW>
 struct Shape {
     static constexpr int RESIDENT = 12 / NW;
     static constexpr int STAGES = 2;
     static constexpr int RING = NW * STAGES * CHUNK_BYTES;
-    static constexpr int DH = D / 2;                      // dims merged at a time
+    static constexpr int DH = D == 64 && ROWS == 8 ? D : D / 2;  // dims merged at a time
     static constexpr int SO = NW * ROWS * (DH + 4) * 4;
     static constexpr bool Q_SMEM = D == 128;
     static constexpr int QS = Q_SMEM ? D / 16 * 512 : 0;
@@ -344,8 +342,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     __align__(16) uint32_t qa[SH::Q_SMEM ? 1 : KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
     float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
-    // masked is a constant at both calls
-    auto compute = [&](const bool masked, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) __attribute__((always_inline)) {
+    auto compute = [&](const bool masked, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
         float s[NT][4];
 #pragma unroll
         for (int s4 = 0; s4 < KS / 4; ++s4) {
@@ -561,11 +558,10 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
         const unsigned ok = ((odd ? pok[1] : pok[0]) >> ((i % SET) * GR)) & ((1u << GR) - 1u);
         const int pos = base + (c0 + i * NW + warp - u0) * CK;
         const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
-        if (pos < first || pos + CK > full_end || ok != (1u << GR) - 1u) compute(true, buf, pos, ks, vs, ok);
-        else compute(false, buf, pos, ks, vs, ok);
+        compute(pos < first || pos + CK > full_end || ok != (1u << GR) - 1u, buf, pos, ks, vs, ok);
     }
-        // The warps' rows, half of the dims at a time: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and
-        // 2 t + 1), t 0, 1 the lower half.
+        // The warps' rows, DH dims at a time: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and 2 t + 1).
+        constexpr int PARTS = D / DH, TP = 4 / PARTS;  // threads t of a part
         const int rows = min(ROWS, R - qt * ROWS);
         const bool whole = u0 >= c0 && u1 <= c1;
         const int prow = min(ROWS, R);  // rows of a tile in the work area
@@ -576,12 +572,12 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 2);
         }
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-            if (x0 > c0 || half) __syncthreads();  // the last merge is through
-            if (t >> 1 == half) {
+        for (int part = 0; part < PARTS; ++part) {
+            if (x0 > c0 || part) __syncthreads();  // the last merge is through
+            if (t / TP == part) {
 #pragma unroll
                 for (int rr = 0; rr < RR; ++rr) {
-                    if ((t & 1) == 0) {
+                    if (t % TP == 0) {
                         sm[warp][g + 8 * rr] = m[rr];
                         sl[warp][g + 8 * rr] = l[rr];
                     }
@@ -593,13 +589,13 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                             float *wf = reinterpret_cast<float *>(&w);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
-                            *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * (t & 1) + e) * DT + j]) = w;
+                            *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * (t % TP) + e) * DT + j]) = w;
                         }
                 }
             }
             __syncthreads();
             for (int x = tid; x < rows * DH; x += 32 * NW) {
-                const int row = x / DH, dh = x % DH, d = half * DH + dh;
+                const int row = x / DH, dh = x % DH, d = part * DH + dh;
                 float mx = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w][row]);
