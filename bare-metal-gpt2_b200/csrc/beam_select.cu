@@ -384,10 +384,12 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         warp_ml(m, l);
         __syncwarp();
         const float lse = m + logf(l);
-        merge_lists(lists[warp], p.chunks, W, [&](int j, key_t k, int) {
+        auto candidate = [&](int j, key_t k, int) {
             totals[b * W + j] = lin::argmax_key(sc + (key_value(k) - lse), static_cast<unsigned>(b * W + j));
             tokens[b * W + j] = lin::argmax_key_index(k);
-        });
+        };
+        if (p.chunks > 1) merge_lists(lists[warp], p.chunks, W, candidate);
+        else if (lane < W && lists[warp][lane]) candidate(lane, lists[warp][lane], 0);
         __syncwarp();
     }
     __syncthreads();
