@@ -215,6 +215,36 @@ def test_attention_few_rows_many_rows_long_contexts(cuda, lib, kind, rows, heads
     assert lib.status() == 0
 
 
+@pytest.mark.parametrize("kind,dim,group,n,rows", [("int8", 64, 1, 200, 3), ("int8", 64, 1, 20000, 4), ("int8", 64, 1, 90, 400), ("int8", 64, 16, 90, 3),
+                                                  ("int8", 128, 1, 90, 3), ("e4m3", 64, 1, 90, 3)])
+def test_queries_that_are_not_finite_give_nan_in_their_head_alone(cuda, lib, kind, dim, group, n, rows):
+    """And queries of zeros, of the smallest subnormals and of fp16's ends stay within the tolerance."""
+    torch = cuda
+    heads = 4
+    lens = [n] * rows
+    cache = filled(torch, lib, kind, rows, heads, dim, 32, 16, lens, heads * group, 1, seed=1)
+    q = torch.randn(rows, 1, heads * group * dim, device="cuda").half()
+    q[0, 0, 3], q[1, 0, dim * group + 5], q[2, 0, 2 * dim * group] = float("nan"), float("inf"), float("-inf")
+    q[0, 0, dim * group: 2 * dim * group] = 0.0
+    q[1, 0, :dim] = 6e-8
+    q[2, 0, :dim] = 65504.0 * torch.sign(q[2, 0, :dim])
+    out = torch.empty_like(q)
+    cache.attend(out, q)
+    view = out.view(rows, heads * group, dim)
+    for r, h in ((0, 0), (1, group), (2, 2 * group)):
+        assert bool(view[r, h].isnan().all())
+        view[r, h] = 0
+        q.view(rows, heads * group, dim)[r, h] = 0
+    assert bool(out.isfinite().all())
+    again = torch.empty_like(q)
+    cache.attend(again, q)
+    for r, h in ((0, 0), (1, group), (2, 2 * group)):
+        view[r, h] = again.view(rows, heads * group, dim)[r, h]
+    assert torch.equal(out, again)  # the other heads do not see them
+    check_attention(torch, cache, kind, q, again, 0, lens, None)
+    assert lib.status() == 0
+
+
 def test_attention_counts_this_steps_tokens(cuda, lib):
     """count / d_count: keys stored in this step, before reorder() counts them in."""
     torch = cuda
