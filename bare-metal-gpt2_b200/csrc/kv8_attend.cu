@@ -24,7 +24,7 @@
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
 //   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
-//     vscale of the granules looked up so far; o is kept in units of S.
+//     vscale of the unit's granules looked up so far; o is kept in units of S.
 //   - m is not the maximum but within 2^LAZY of it: p stays below 2^LAZY, far inside fp16 and fp32, and most chunks need
 //     neither the row maximum's shuffles nor a rescaling of o.
 //
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
     unsigned grow = 0;
     float gks = 0.0f, gvs = 0.0f;
     unsigned gok = 0;
+    int gof = 0;  // whose chunk: its unit's first chunk
     // A block of zeros has scale 0; TINY in its place keeps -inf (a masked score) times a scale from being NaN.
     constexpr float TINY = 1e-20f;
     bool bad = false;
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         int ok = x < c1, pos = 0;
         if (ok) {
             unit_of(x);
+            gof = u0;
             pos = base + (x - u0) * CK + (lane % GR) * 16;
             ok = pos < last_end && pos + 16 > first;
         }
@@ -594,9 +596,13 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
 
     const int mine = c1 - c0 > warp ? (c1 - c0 - warp + NW - 1) / NW : 0;  // chunks c0 + warp, c0 + warp + NW, ...
     // The look-up of a set comes before the loads of its chunks, while the set before is still in use: pks, pvs and pok are
-    // the set's in use, pmax its largest vscale.
-    float pks = TINY, pvs = 0.0f, pmax = 0.0f;
+    // the set's in use, pof whose they are.
+    float pks = TINY, pvs = 0.0f;
     unsigned pok = 0;
+    int pof = 0;
+    // The set's largest vscale (they are not negative), of this unit's chunks alone: what another unit's values are is no matter
+    // for this one's rounding.
+    auto largest = [&]() { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, NW != NW_PIECES || pof == u0 ? __float_as_uint(pvs) : 0u)); };
     auto fetch = [&](int i) {
         if (i < mine) {
             if (i % SET == 0) look_up(i / SET);
@@ -696,7 +702,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
 #pragma unroll
         for (int j = 0; j < (SH::INT ? DT : 0); ++j) c12[j][0] = c12[j][1] = c12[j][2] = c12[j][3] = c3[j][0] = c3[j][1] = c3[j][2] = c3[j][3] = 0;
-        S = i % SET ? pmax : 0.0f;  // a new set's comes with its first chunk
+        S = i % SET ? largest() : 0.0f;  // a new set's comes with its first chunk
         invS = S > 0.0f ? 1.0f / S : 0.0f;
         for (; c0 + i * NW + warp < x1; ++i) {
         cp_async_wait<STAGES - 2>();
@@ -706,8 +712,8 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             pks = fmaxf(gks * a.scale_log2, TINY);
             pvs = gvs;
             pok = gok;
-            pmax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(pvs)));  // scales are not negative
-            const float Sn = fmaxf(S, pmax);
+            pof = gof;
+            const float Sn = fmaxf(S, largest());
             if (Sn > S) {
                 const float f = S / Sn;
                 if (SH::INT) flush(f);

@@ -215,6 +215,26 @@ def test_attention_few_rows_many_rows_long_contexts(cuda, lib, kind, rows, heads
     assert lib.status() == 0
 
 
+@pytest.mark.parametrize("kind,dim", [("int8", 64), ("e4m3", 64), ("int8", 128), ("e4m3", 128)])
+@pytest.mark.parametrize("rows,heads,group,n", [(5, 3, 1, 200), (16, 6, 2, 700), (9, 3, 12, 300), (60, 12, 1, 300), (100, 12, 2, 150), (100, 12, 1, 500)])
+def test_values_of_another_size_in_other_rows_and_heads(cuda, lib, kind, dim, rows, heads, group, n):
+    """V's magnitude differs 2^20-fold from row to row and head to head: each keeps its own precision."""
+    torch = cuda
+    g = torch.Generator().manual_seed(n)
+    lens = [n - 13 * i % n for i in range(rows)]
+    cache = make(torch, lib, rows, heads, dim, 16, 16, kind, n, q_heads=heads * group)
+    k, v = torch.randn(2, 2, rows, n, heads, dim, generator=g).unbind(0)
+    v = v * 2.0 ** (torch.arange(rows)[:, None, None, None] * 7 + torch.arange(heads)[:, None] * 9).remainder(21).sub(10)
+    k, v = (x.flatten(3).half().cuda() for x in (k, v))
+    cache.store(k, v, count=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    cache.length.copy_(torch.tensor(lens, dtype=torch.int32))
+    q = torch.randn(rows, 1, heads * group * dim, generator=g).half().cuda()
+    out = torch.full_like(q, 9.0)
+    cache.attend(out, q)
+    check_attention(torch, cache, kind, q, out, 0, lens, None)
+    assert lib.status() == 0
+
+
 @pytest.mark.parametrize("kind,dim,group,n,rows", [("int8", 64, 1, 200, 3), ("int8", 64, 1, 20000, 4), ("int8", 64, 1, 90, 400), ("int8", 64, 16, 90, 3),
                                                   ("int8", 128, 1, 90, 3), ("e4m3", 64, 1, 90, 3)])
 def test_queries_that_are_not_finite_give_nan_in_their_head_alone(cuda, lib, kind, dim, group, n, rows):
