@@ -12,11 +12,11 @@
 //     free and take lo; with 9 to 16 rows lo is a second MMA. mma.sync's rate is far above what HBM feeds
 //     (64 MMAs of 8 cycles per 8 KB of codes).
 //   - a warp takes CK keys at a time (64 for D 64, 32 for D 128: 8 KB of K and V) through a ring of its own in shared
-//     memory (cp.async, the next chunk in flight while one is computed, no CTA barrier). The sum over dims (QK) may run in any order of dims,
-//     so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
+//     memory (cp.async, the next chunk in flight while one is computed, no CTA barrier). The sum over dims (QK) may run in any
+//     order of dims, so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
 //     column order are as free, so a thread reads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with
 //     16 neighbouring output dims. The 16-byte granules of a chunk are permuted so that neither read has bank conflicts.
-//   - int8 codes of 64 dims under at most 8 query rows (GPT-2's decode step) need no conversion at all: INT. q is cut into
+//   - int8 codes of 64 dims under at most 8 query rows in long contexts need no conversion at all: INT. q is cut into
 //     three signed 8-bit digits (23 bits below the row's largest element), p * vscale / S into three unsigned ones, and
 //     mma.m16n8k32 multiplies the codes as they are, exactly; rows 8..15 take the second digit, a second MMA the third. What
 //     is left is about half the instructions of the converting path, which is bound by issuing them (16 sequences x 12 heads, 8192
@@ -24,15 +24,22 @@
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
 //   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
-//     vscale of the unit's granules looked up so far; o is kept in units of S.
+//     vscale of the row's granules looked up so far; o is kept in units of S.
 //   - m is not the maximum but within 2^LAZY of it: p stays below 2^LAZY, far inside fp16 and fp32, and most chunks need
 //     neither the row maximum's shuffles nor a rescaling of o.
 //
-// Work: a unit is (cache row, tile of 8 or 16 query rows, K/V head) with its chunks of keys, and a CTA's 4 warps take chunks
-// in turn. With units in plenty each has a CTA. With fewer units than resident CTAs all chunks of all units form one
-// sequence and every CTA takes an equal piece of it, found from the rows' lengths by a prefix sum, its loads running ahead over
-// unit borders. At a border the warps are merged in shared memory; a unit cut by a piece's end is merged
-// through the work area by the last CTA to arrive, in piece order.
+// Work: a unit is (cache row, tile of 8 or 16 query rows, K/V head) with its chunks of keys, which the warps of a CTA (1, 2 or 4)
+// take in turn; at its end they are merged in shared memory. With units in plenty each has a CTA. With fewer units than resident
+// CTAs all chunks of all units form one sequence and every CTA takes an equal piece of it, found from the rows' lengths by a
+// prefix sum, its loads running ahead over unit borders; a unit cut by a piece's end is merged through the work area by the last
+// CTA to arrive, in piece order.
+//
+// Beams share their leading pages, and one query row of each fills an eighth of an MMA tile. With units in plenty and at most 4
+// query rows in each, a CTA so takes 2 or 4 neighbouring cache rows of a head (GROUP). It compares their table rows; the chunks
+// of the pages that all of them hold are read and converted once, for the query rows of all. The rows' own chunks follow, in
+// which the other rows' scores are masked. 32 items x 4 beams x 12 heads of 640 to 700 keys, 640 shared: 15.0 us, each row by
+// itself 29.0. Rows that share nothing gain a little from four warps to deal their chunks to (128 x 12 heads of 2048 to 4096 keys:
+// 128 us, by themselves 146).
 #include <algorithm>
 #include <type_traits>
 
@@ -42,7 +49,7 @@
 namespace b200 {
 namespace kv8 {
 
-constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces (whole units: 1 or 2, see the plan)
+constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces, and of a group
 constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
 // In the integer path p takes 23 bits: P_BITS below 1, LAZY_INT above.
 constexpr float LAZY_INT = 2.0f, P_ONE = 2097152.0f;  // 2^21
@@ -178,12 +185,12 @@ struct Chunk {
 // A kernel variant's shape: 12 warps per SM, each with two chunks in its ring (192 KB of an SM's shared memory). The accumulators
 // of 128 dims or 16 rows take the registers, so q of 128 dims lies in shared memory instead (32 registers), and the warps'
 // rows are merged in two halves of the dims: the merge area of 16 rows x 128 dims would leave room for 8 warps only.
-// INT: the integer accumulators take 64 more registers: 8 or 10 warps per SM.
+// INT: the integer accumulators take 64 more registers: 8 warps per SM.
 template <int D, int ROWS, int NW, bool INT_>
 struct Shape {
     static constexpr bool INT = INT_;
     static_assert(!INT || (D == 64 && ROWS == 8), "the integer path's accumulators fit 64 dims and 8 rows");
-    static constexpr int WARPS = !INT ? 12 : NW == 2 ? 10 : 8;  // per SM
+    static constexpr int WARPS = INT ? 8 : 12;  // per SM
     static constexpr int RESIDENT = WARPS / NW;
     static constexpr int STAGES = 2;
     static constexpr int RING = NW * STAGES * CHUNK_BYTES;
@@ -194,7 +201,8 @@ struct Shape {
     static constexpr int BYTES = RING + SO + QS;
 };
 
-template <int KIND, int D, int ROWS, int NW, bool INT>
+// GROUP: 0, or the cache rows of a CTA that reads their shared pages once (2 or 4)
+template <int KIND, int D, int ROWS, int NW, bool INT, int GROUP>
 __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_kv8_attend(const View c, const AttParams a) {
     using C = Chunk<D>;
     using SH = Shape<D, ROWS, NW, INT>;
@@ -227,8 +235,14 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         return last_end > first ? (last_end - base + CK - 1) / CK : 0;
     };
     auto put = [&](int h, int row, int d, float x) {
-        const int i = qt * ROWS + row, tok = one ? 0 : i / a.G;
-        a.out[r * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
+        int i = qt * ROWS + row, r_ = r;
+        if (GROUP) {
+            const int u = row / R;
+            r_ = GROUP * blockIdx.x + u;
+            i = row - u * R;
+        }
+        const int tok = one ? 0 : i / a.G;
+        a.out[r_ * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
     };
     auto no_keys = [&](int h) {
         for (int x = tid; x < min(ROWS, R - qt * ROWS) * D; x += 32 * NW) put(h, x / D, x % D, 0.0f);
@@ -236,14 +250,58 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
 
     // One unit per CTA: the pages of a warp's first granules, whatever the row's length, so that the table is read while the
     // length is.
-    const bool early = !a.entries && !a.d_first && a.qtiles == 1;
+    const bool early = !GROUP && !a.entries && !a.d_first && a.qtiles == 1;
     int early_page = -1;
     if (early) {
         const int pos = ((lane / GR) * NW + warp) * CK + (lane % GR) * 16;
         if (pos < a.max_len) early_page = c.table[static_cast<long long>(blockIdx.x) * c.maxPages + (pos >> c.page_shift)];
     }
     int c0, c1, per = 1;  // this CTA's chunks
-    if (a.entries) {
+    // A group's chunks: shared ones [0, first_of[0]) for all rows, then row i's own [first_of[i], first_of[i + 1]).
+    __shared__ int first_of[GROUP + 1], len_of[GROUP + 1], differ;
+    const int in_group = GROUP ? min(GROUP, c.nRow - GROUP * static_cast<int>(blockIdx.x)) : 1;
+    if (GROUP) {
+        const int r0 = GROUP * blockIdx.x;
+        if (tid == 0) differ = 0x7FFFFFFF;
+        if (tid < GROUP) {
+            int x = tid < in_group ? c.len[r0 + tid] + (a.d_count ? a.d_count[r0 + tid] : a.count) : 0;
+            if (x < 0 || x > a.max_len) {
+                if (blockIdx.y == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
+                x = 0;
+            }
+            len_of[tid] = x;
+        }
+        __syncthreads();
+        int least = 0x7FFFFFFF;  // keys that every query of every row sees
+        for (int i = 0; i < in_group; ++i) least = min(least, len_of[i] - a.Tq + 1);
+        const int *t0 = c.table + static_cast<long long>(r0) * c.maxPages;
+        const int pages = in_group > 1 && least > 0 ? ((least - 1) >> c.page_shift) + 1 : 0;
+        for (int p = tid; p < pages; p += 32 * NW) {
+            bool same = true;
+            for (int i = 1; i < in_group; ++i) same &= t0[p] == t0[static_cast<long long>(i) * c.maxPages + p];
+            if (!same) {
+                atomicMin(&differ, p);
+                break;
+            }
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int at = in_group > 1 ? max(0, differ < pages ? differ << c.page_shift : least) / CK : 0;
+            const int from = at;
+            for (int i = 0; i < GROUP; ++i) {
+                first_of[i] = at;
+                at += max(0, (len_of[i] + CK - 1) / CK - from);
+            }
+            first_of[GROUP] = at;
+        }
+        __syncthreads();
+        r = r0, qt = 0, first = 0, base = 0;
+        n = last_end = 0x7FFFFFFF;
+        c0 = 0;
+        c1 = first_of[GROUP];
+        if (c1 == 0)
+            for (int x = tid; x < in_group * R * D; x += 32 * NW) put(blockIdx.y, x / D, x % D, 0.0f);
+    } else if (a.entries) {
         const int own = (a.entries + 32 * NW - 1) / (32 * NW), e0 = min(tid * own, a.entries), e1 = min(e0 + own, a.entries);
         int sum = 0;
         for (int e = e0; e < e1; ++e) {
@@ -287,6 +345,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
     // The unit of chunk x: sets entry()'s values, h and the unit's first chunk u0; returns its chunks.
     int h = blockIdx.y, u0 = 0;
     auto unit_of = [&](int x) {
+        if (GROUP) return c1;
         int e = blockIdx.x;
         if (a.entries) {
             int lo = 0, hi = a.entries;  // the last entry with pre <= x (entries without chunks come before it)
@@ -305,12 +364,21 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         return ch;
     };
 
+    // GROUP: the row whose own chunk x is (-1: a shared one), and its first key.
+    auto chunk_of = [&](int x, int &key) {
+        int i = -1;
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u)
+            if (x >= first_of[u] && x < first_of[u + 1]) i = u;
+        key = (i < 0 ? x : x - first_of[i] + first_of[0]) * CK;
+        return i;
+    };
     // This lane's granule of the set looked up last: its first code row of K (rows are counted in 32 bits) and its scales, which
     // nothing waits for before the set's first chunk is computed.
     unsigned grow = 0;
     float gks = 0.0f, gvs = 0.0f;
     unsigned gok = 0;
-    int gof = 0;  // whose chunk: its unit's first chunk
+    int gof = 0;  // whose chunk: its unit's first chunk; GROUP: its row
     // A block of zeros has scale 0; TINY in its place keeps -inf (a masked score) times a scale from being NaN.
     constexpr float TINY = 1e-20f;
     bool bad = false;
@@ -318,7 +386,14 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         const int r_ = r, qt_ = qt, n_ = n, first_ = first, base_ = base, last_end_ = last_end, h_ = h, u0_ = u0;
         const int x = c0 + (set * SET + lane / GR) * NW + warp;
         int ok = x < c1, pos = 0;
-        if (ok) {
+        if (GROUP) {
+            if (ok) {
+                const int own = gof = chunk_of(x, pos);
+                pos += (lane % GR) * 16;
+                ok = own < 0 || pos < len_of[own];
+                r = GROUP * blockIdx.x + max(own, 0);
+            }
+        } else if (ok) {
             unit_of(x);
             gof = u0;
             pos = base + (x - u0) * CK + (lane % GR) * 16;
@@ -379,9 +454,10 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
     uint32_t qd[2][4], qd0[2][2];  // INT: q's first two digits, and the third, per 32 dims
     float qs_row = 0.0f;           // INT: the value of q's last digit
     int c12[SH::INT ? DT : 1][4], c3[SH::INT ? DT : 1][4];  // INT: sums of the digits of p times codes, not yet in o
+    int my_row = 0;  // GROUP: the cache row, in the group, of this lane's query row
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
     float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
-    auto compute = [&](const bool masked, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+    auto compute = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
         float s[NT][4];
 #pragma unroll
         for (int s4 = 0; s4 < KS / 4; ++s4) {
@@ -410,6 +486,9 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                     if (key < first || key >= end[e >> 1] || !((ok >> (tile / 2)) & 1u)) s[tile][e] = -INFINITY;
                 }
         }
+        if (GROUP && other)
+#pragma unroll
+            for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = -INFINITY;
         // A granule's scale is one factor of its scores: the largest of them first, then the factor.
         float top[RR];
         bool grew = false;
@@ -445,7 +524,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         for (int rr = 0; rr < RR; ++rr) mm[rr] = m[rr] > -INFINITY ? m[rr] : 0.0f;
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
-            const float w = vs[gi] * invS;
+            const float w = other ? 0.0f : vs[gi] * invS;
             uint32_t ph[2 * RR], pl[2 * RR];  // [tile of the granule * RR + rr]
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile)
@@ -511,7 +590,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                 c12[j][e] = c12[j][2 + e] = c3[j][e] = 0;
             }
     };
-    auto compute_int = [&](const bool masked, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+    auto compute_int = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
         float s[NT][2];
 #pragma unroll
         for (int tile = 0; tile < NT; ++tile) {
@@ -534,6 +613,9 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                     if (key < first || key >= end[0] || !((ok >> (tile / 2)) & 1u)) s[tile][x] = -INFINITY;
                 }
         }
+        if (GROUP && other)
+#pragma unroll
+            for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = -INFINITY;
         float kq[GR], top = -INFINITY;
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
@@ -555,7 +637,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             uint32_t d0[2], d1[2], d2[2];
 #pragma unroll
             for (int gi = 0; gi < 2; ++gi) {
-                const float w = vs[2 * k2 + gi] * invS * P_ONE;
+                const float w = other ? 0.0f : vs[2 * k2 + gi] * invS * P_ONE;
                 uint32_t x[4];  // 2^23 + p * w: the low bytes are the digits
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -600,9 +682,19 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
     float pks = TINY, pvs = 0.0f;
     unsigned pok = 0;
     int pof = 0;
-    // The set's largest vscale (they are not negative), of this unit's chunks alone: what another unit's values are is no matter
-    // for this one's rounding.
-    auto largest = [&]() { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, NW != NW_PIECES || pof == u0 ? __float_as_uint(pvs) : 0u)); };
+    // The set's largest vscale (they are not negative), of this unit's chunks alone, and in a group of those that this lane's row
+    // sees: what another row's values are is no matter for this one's rounding.
+    auto largest = [&]() {
+        auto over = [&](bool in) { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, in ? __float_as_uint(pvs) : 0u)); };
+        if (!GROUP) return over(NW != NW_PIECES || pof == u0);
+        float of = 0.0f;
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) {
+            const float x = over(pof < 0 || pof == u);
+            if (my_row == u) of = x;
+        }
+        return of;
+    };
     auto fetch = [&](int i) {
         if (i < mine) {
             if (i % SET == 0) look_up(i / SET);
@@ -620,11 +712,18 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         if (SH::Q_SMEM) __syncthreads();  // every warp is through with the last segment's q
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
-            const int row = qt * ROWS + g + 8 * rr;
-            const bool ok = row < R;
+            int row = qt * ROWS + g + 8 * rr, cr = r, keys = n;
+            bool ok = row < R;
+            if (GROUP) {
+                my_row = g / R;
+                ok = my_row < in_group;
+                row = g - my_row * R;
+                cr = r + (ok ? my_row : 0);
+                keys = ok ? len_of[my_row] : 0;
+            }
             const int tok = ok && !one ? row / a.G : 0;
-            end[rr] = ok ? n - a.Tq + tok + 1 : 0;
-            const __half *qp = a.q + r * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (row - tok * a.G)) * D + 16 * t;
+            end[rr] = ok ? keys - a.Tq + tok + 1 : 0;
+            const __half *qp = a.q + cr * a.q_row + tok * a.q_tok + static_cast<long long>(h * a.G + (row - tok * a.G)) * D + 16 * t;
 #pragma unroll
             for (int s4 = 0; s4 < KS / 4; ++s4) {
                 if (SH::Q_SMEM && s4 % NW != warp) continue;  // the warps share the work
@@ -705,47 +804,54 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         S = i % SET ? largest() : 0.0f;  // a new set's comes with its first chunk
         invS = S > 0.0f ? 1.0f / S : 0.0f;
         for (; c0 + i * NW + warp < x1; ++i) {
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();  // every lane's copies of chunk i are there, and all are done with chunk i - 1
-        fetch(i + STAGES - 1);
-        if (i % SET == 0) {
-            pks = fmaxf(gks * a.scale_log2, TINY);
-            pvs = gvs;
-            pok = gok;
-            pof = gof;
-            const float Sn = fmaxf(S, largest());
-            if (Sn > S) {
-                const float f = S / Sn;
-                if (SH::INT) flush(f);
-                else
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();  // every lane's copies of chunk i are there, and all are done with chunk i - 1
+            fetch(i + STAGES - 1);
+            if (i % SET == 0) {
+                pks = fmaxf(gks * a.scale_log2, TINY);
+                pvs = gvs;
+                pok = gok;
+                pof = gof;
+                const float Sn = fmaxf(S, largest());
+                if (Sn > S) {
+                    const float f = S / Sn;
+                    if (SH::INT) flush(f);
+                    else
 #pragma unroll
-                for (int j = 0; j < DT; ++j)
+                        for (int j = 0; j < DT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] *= f;
-                S = Sn;
-                invS = 1.0f / Sn;
+                            for (int e = 0; e < 4; ++e) o[j][e] *= f;
+                    S = Sn;
+                    invS = 1.0f / Sn;
+                }
+            }
+            float ks[GR], vs[GR];
+#pragma unroll
+            for (int gi = 0; gi < GR; ++gi) {
+                ks[gi] = __shfl_sync(0xFFFFFFFFu, pks, (i % SET) * GR + gi);
+                vs[gi] = __shfl_sync(0xFFFFFFFFu, pvs, (i % SET) * GR + gi);
+            }
+            const unsigned ok = (pok >> ((i % SET) * GR)) & ((1u << GR) - 1u);
+            int pos = base + (c0 + i * NW + warp - u0) * CK;
+            bool other = false;  // GROUP: a chunk of another row than this lane's
+            if (GROUP) {
+                const int own = chunk_of(i * NW + warp, pos);
+                other = own >= 0 && own != my_row;
+                n = own < 0 ? 0x7FFFFFFF : len_of[max(own, 0)];
+                full_end = own < 0 ? 0x7FFFFFFF : n - a.Tq + 1;
+            }
+            const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
+            const bool masked = pos < first || pos + CK > full_end || ok != (1u << GR) - 1u;
+            if (SH::INT) {
+                compute_int(masked, other, buf, pos, ks, vs, ok);
+                if ((i & 511) == 511) flush(1.0f);  // 512 chunks: 32768 keys of at most 255 * 127, below 2^31
+            } else {
+                compute(masked, other, buf, pos, ks, vs, ok);
             }
         }
-        float ks[GR], vs[GR];
-#pragma unroll
-        for (int gi = 0; gi < GR; ++gi) {
-            ks[gi] = __shfl_sync(0xFFFFFFFFu, pks, (i % SET) * GR + gi);
-            vs[gi] = __shfl_sync(0xFFFFFFFFu, pvs, (i % SET) * GR + gi);
-        }
-        const unsigned ok = (pok >> ((i % SET) * GR)) & ((1u << GR) - 1u);
-        const int pos = base + (c0 + i * NW + warp - u0) * CK;
-        const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
-        const bool masked = pos < first || pos + CK > full_end || ok != (1u << GR) - 1u;
-        if (SH::INT) {
-            compute_int(masked, buf, pos, ks, vs, ok);
-            if ((i & 511) == 511) flush(1.0f);  // 512 chunks: 32768 keys of at most 255 * 127, below 2^31
-        } else {
-            compute(masked, buf, pos, ks, vs, ok);
-        }
-    }
         // The warps' rows, DH dims at a time: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and 2 t + 1).
         constexpr int PARTS = D / DH, TP = 4 / PARTS;  // threads t of a part
-        const int rows = min(ROWS, R - qt * ROWS);
+        const int rows = GROUP ? in_group * R : min(ROWS, R - qt * ROWS);
         const bool whole = u0 >= c0 && u1 <= c1;
         const int prow = min(ROWS, R);  // rows of a tile in the work area
         const int slot = 2 * blockIdx.x + (x0 == c0 ? 0 : 1);
@@ -901,15 +1007,17 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
     const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
     if (entries > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
-    // Plan. Units that fill the GPU have a CTA each: no prefix sum, no shared units. Two warps per CTA (64 sequences x 12 heads
-    // of 512 to 1023 keys: 25.2 us, with one warp 32.7, with four 27.7, in equal pieces 30.9) as long as single warps would leave
-    // a third of the SMs' 12 warps empty, then one (128 x 12 units of 640 to 700 keys: 28.8 against 33.5 us; 256 x 12 of 150 to
-    // 300: 33.3 against 40.0). Fewer units: equal pieces, four warps per CTA, which merge their rows before a piece's partials
-    // go through the work area.
+    // Plan. Units that fill the GPU have a CTA each: no prefix sum, no shared units. Groups of two rows (64 sequences x 12 heads
+    // of 512 to 1023 keys: 23.0 us; four rows 30.3, two warps per row 24.2, equal pieces 30.9) as long as groups of four would
+    // leave a third of the SMs' 12 warps empty, then of four (128 x 12 units of 640 to 700 keys: 15.0 us, of two 21.4; 256 x 12
+    // of 150 to 300: 31.4 against 35.1). Windows, whose rows need not start together, and more query rows: one or two
+    // warps per row by the same rule (128 x 12 units of 640 to 700 keys: 28.8 us with one, 33.5 with two). Fewer units: equal
+    // pieces, four warps per CTA, which merge their rows before a piece's partials go through the work area.
     const long long units = entries * kv->nHead;
     const bool pieces = units < 3ll * ctx->num_sms && entries <= kv8::MAX_ENTRIES && chunks <= 0x3FFFFFFFll;
     const int warps = pieces ? kv8::NW_PIECES : units < 8ll * ctx->num_sms ? 2 : 1;
     a.entries = pieces ? static_cast<int>(entries) : 0;
+    const int group = pieces || R > 4 || d_first ? 0 : warps == 1 && R <= 2 ? 4 : 2;
     const kv8::View c = kv8::view(kv, ctx->status);
     auto go = [&](auto kern, auto shape, int variant) {
         using SH = decltype(shape);
@@ -923,27 +1031,34 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
         const int smem = SH::BYTES + (a.entries + 1) * 4;
         // CTAs that are resident together: registers (the kernel's launch bounds) and 228 KB of shared memory, 1 KB of it per CTA.
         const int resident = std::min(SH::RESIDENT, 228 * 1024 / (smem + 1024 + 512));
-        const dim3 grid = pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident,
-                                                                                 kv8::MAX_PIECES, (chunks + warps - 1) / warps})))
-                                 : dim3(static_cast<unsigned>(entries), kv->nHead);
-        kern<<<grid, 32 * warps, smem, stream>>>(c, a);
+        const int threads = 32 * (group ? kv8::NW_PIECES : warps);
+        const dim3 grid =
+            group    ? dim3((kv->nRow + group - 1) / group, kv->nHead)
+            : pieces ? dim3(static_cast<unsigned>(std::min<long long>({static_cast<long long>(ctx->num_sms) * resident, kv8::MAX_PIECES,
+                                                                        (chunks + warps - 1) / warps})))
+                     : dim3(static_cast<unsigned>(entries), kv->nHead);
+        kern<<<grid, threads, smem, stream>>>(c, a);
         return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
     };
     auto by_rows = [&](auto kind, auto dim) {
         constexpr int KIND = decltype(kind)::value, D = decltype(dim)::value;
-        constexpr int base = (KIND == GPT2_KV8_INT8 ? 0 : 12) + (D == 64 ? 0 : 6);
-        constexpr bool INT = KIND == GPT2_KV8_INT8 && D == 64;
+        constexpr int base = (KIND == GPT2_KV8_INT8 ? 0 : 16) + (D == 64 ? 0 : 8);
         if (rows == 8) {
-            // The integer path's q costs more to prepare than its few chunks save where a warp has fewer than 8 (one sequence of 1023
-            // keys: 8.2 against 7.1 us; 8 sequences: 14.1 against 12.3; 16 sequences of 16384: 59.5 against 65.6).
-            if (warps == 4 && INT && chunks >= 8ll * 8 * ctx->num_sms) return go(kv8::k_kv8_attend<KIND, D, 8, 4, INT>, kv8::Shape<D, 8, 4, INT>(), 24);
-            if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false>, kv8::Shape<D, 8, 4, false>(), base);
-            if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 2, INT>, kv8::Shape<D, 8, 2, INT>(), base + 1);
-            return go(kv8::k_kv8_attend<KIND, D, 8, 1, INT>, kv8::Shape<D, 8, 1, INT>(), base + 2);
+            if (group == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 4>, kv8::Shape<D, 8, 4, false>(), base);
+            if (group == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 2>, kv8::Shape<D, 8, 4, false>(), base + 1);
+            // The integer path's q costs more to prepare than its chunks save where a warp has fewer than 8 (one sequence of 1023
+            // keys: 8.2 against 7.1 us; 8 sequences: 14.1 against 12.3; 16 sequences of 16384: 59.5 against 65.6). Its registers
+            // leave an SM 8 warps, the conversion 12: with units in plenty the conversion is as fast or faster (128 x 12 units,
+            // windows of 1024 keys: 46.6 against 57.0 us).
+            if (KIND == GPT2_KV8_INT8 && D == 64 && warps == 4 && chunks >= 8ll * 8 * ctx->num_sms)
+                return go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 8, 4, true, 0>, kv8::Shape<64, 8, 4, true>(), 32);
+            if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 0>, kv8::Shape<D, 8, 4, false>(), base + 2);
+            if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 2, false, 0>, kv8::Shape<D, 8, 2, false>(), base + 3);
+            return go(kv8::k_kv8_attend<KIND, D, 8, 1, false, 0>, kv8::Shape<D, 8, 1, false>(), base + 4);
         }
-        if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 16, 4, false>, kv8::Shape<D, 16, 4, false>(), base + 3);
-        if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 16, 2, false>, kv8::Shape<D, 16, 2, false>(), base + 4);
-        return go(kv8::k_kv8_attend<KIND, D, 16, 1, false>, kv8::Shape<D, 16, 1, false>(), base + 5);
+        if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 16, 4, false, 0>, kv8::Shape<D, 16, 4, false>(), base + 5);
+        if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 16, 2, false, 0>, kv8::Shape<D, 16, 2, false>(), base + 6);
+        return go(kv8::k_kv8_attend<KIND, D, 16, 1, false, 0>, kv8::Shape<D, 16, 1, false>(), base + 7);
     };
     auto by_dim = [&](auto kind) {
         return kv->headDim == 64 ? by_rows(kind, std::integral_constant<int, 64>()) : by_rows(kind, std::integral_constant<int, 128>());

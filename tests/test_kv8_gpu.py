@@ -215,6 +215,49 @@ def test_attention_few_rows_many_rows_long_contexts(cuda, lib, kind, rows, heads
     assert lib.status() == 0
 
 
+@pytest.mark.parametrize("kind,page,block,dim", [("int8", 16, 16, 64), ("e4m3", 32, 16, 64), ("int8", 64, 32, 128), ("e4m3", 128, 128, 128)])
+@pytest.mark.parametrize("rows,group,Tq", [(114, 1, 1), (114, 2, 1), (114, 1, 2), (114, 3, 1), (51, 1, 1), (53, 2, 2), (114, 5, 1)])
+def test_attention_of_rows_that_share_pages(cuda, lib, kind, page, block, dim, rows, group, Tq):
+    """Many rows in neighbouring fours that hold no, some, most or all of their pages in common, of equal and unequal lengths
+    (none among them, shorter than the shared part, more queries than keys), and a last group of fewer rows."""
+    torch = cuda
+    heads = 12
+    rng = np.random.default_rng(dim + page)
+    lens, share = [], []
+    for b in range(0, rows, 4):
+        kind_of = b // 4 % 6
+        longest = int(rng.integers(130, 420))
+        same = [0, 64, longest // page * page, longest // 2, longest, 200][kind_of]
+        few = [longest, longest, longest, longest - 70, longest, longest]
+        more = [int(rng.integers(0, longest + 1)) for _ in range(4)] if kind_of == 5 else [longest, few[kind_of], longest, longest]
+        if kind_of == 0 and b % 24 == 0:
+            more = [0, 1, 65, 2]
+        lens += more
+        share += [same] * 4
+    lens, share = lens[:rows], share[:rows]
+    cache = filled(torch, lib, kind, rows, heads, dim, page, block, lens, heads * group, Tq, seed=4)
+    table = cache.table.cpu()
+    for r in range(rows):
+        first = r // 4 * 4
+        n = share[r] // page
+        full = [x // page for x in (lens[first], lens[r])]
+        if r != first and n:
+            table[r, : min(n, *full)] = table[first, : min(n, *full)]  # whole pages, filled in both
+    cache.table.copy_(table)
+    q = torch.randn(rows, Tq, heads * group * dim, device="cuda").half()
+    out = torch.full_like(q, 9.0)
+    cache.attend(out, q)
+    check_attention(torch, cache, kind, q, out, 0, lens, None)
+    before = out.clone()
+    cache.length[5] = cache.c.maxPages * page + 1  # one row of a group is refused, the others stay
+    cache.attend(out, q)
+    assert lib.status() == G.ST_KV8_BAD_LEN
+    assert bool((out[5] == 0).all())
+    lens[5] = 0
+    check_attention(torch, cache, kind, q, out, 0, lens, None, "refused row")
+    assert torch.equal(out[8:], before[8:])
+
+
 @pytest.mark.parametrize("kind,dim", [("int8", 64), ("e4m3", 64), ("int8", 128), ("e4m3", 128)])
 @pytest.mark.parametrize("rows,heads,group,n", [(5, 3, 1, 200), (16, 6, 2, 700), (9, 3, 12, 300), (60, 12, 1, 300), (100, 12, 2, 150), (100, 12, 1, 500)])
 def test_values_of_another_size_in_other_rows_and_heads(cuda, lib, kind, dim, rows, heads, group, n):
