@@ -184,21 +184,24 @@ struct Chunk {
 
 // A kernel variant's shape: 12 warps per SM, each with two chunks in its ring (192 KB of an SM's shared memory). The accumulators
 // of 128 dims or 16 rows take the registers, so q of 128 dims lies in shared memory instead (32 registers), and the warps'
-// rows are merged in two halves of the dims: the merge area of 16 rows x 128 dims would leave room for 8 warps only.
-// INT: the integer accumulators take 64 more registers: 8 warps per SM.
+// rows are merged where the rings were or, in the middle of a piece, DH dims at a time in q's place.
+// 16 rows of 128 dims spill at 12 warps, so 8 (8 sequences x 8 heads of 16384 keys: 62.5 us, 12 warps 68.7; 55.5 since the merge
+// takes four dims per thread and the last CTA has the loads of all its rows in flight). INT: the integer accumulators take 64
+// more registers: 8 warps, too.
 template <int D, int ROWS, int NW, bool INT_>
 struct Shape {
     static constexpr bool INT = INT_;
     static_assert(!INT || (D == 64 && ROWS == 8), "the integer path's accumulators fit 64 dims and 8 rows");
-    static constexpr int WARPS = INT ? 8 : 12;  // per SM
+    static constexpr int WARPS = INT || (D == 128 && ROWS == 16) ? 8 : 12;  // per SM
     static constexpr int RESIDENT = WARPS / NW;
     static constexpr int STAGES = 2;
     static constexpr int RING = NW * STAGES * CHUNK_BYTES;
-    static constexpr int DH = D == 64 && ROWS == 8 ? D : D / 2;  // dims merged at a time
+    static constexpr int DH = 512 / ROWS, LOG_D = D == 64 ? 6 : 7, LOG_DH = ROWS == 8 ? 6 : 5;  // dims merged at a time
     static constexpr int SO = NW * ROWS * (DH + 4) * 4;
     static constexpr bool Q_SMEM = D == 128;
     static constexpr int QS = Q_SMEM ? D / 16 * 512 : 0;
-    static constexpr int BYTES = RING + SO + QS;
+    static constexpr int BYTES = RING + (SO > QS ? SO : QS);
+    static_assert(NW == 1 || RESIDENT * (BYTES + 1024 + 160 * NW) <= 228 * 1024, "shared memory, with the CTA's 1 KB and the static arrays");
 };
 
 // GROUP: 0, or the cache rows of a CTA that reads their shared pages once (2 or 4)
@@ -210,8 +213,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
     constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
     constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
     extern __shared__ __align__(128) uint8_t ring_all[];
-    float (*so)[ROWS][DH + 4] = reinterpret_cast<float (*)[ROWS][DH + 4]>(ring_all + RING_BYTES);  // [NW]
-    uint4 *qs = reinterpret_cast<uint4 *>(ring_all + RING_BYTES + SH::SO);  // [KS][32]: A operands of a k-step
+    uint4 *qs = reinterpret_cast<uint4 *>(ring_all + RING_BYTES);  // [KS][32]: A operands of a k-step
     int *pre = reinterpret_cast<int *>(ring_all + SH::BYTES);               // [entries + 1]: chunks before each entry
     __shared__ float sm[NW][ROWS], sl[NW][ROWS];
     __shared__ int is_last, warp_sum[NW];
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         base = first & ~(CK - 1);
         return last_end > first ? (last_end - base + CK - 1) / CK : 0;
     };
-    auto put = [&](int h, int row, int d, float x) {
+    auto put = [&](int h, int row, int d, float4 y) {  // dims d .. d + 3
         int i = qt * ROWS + row, r_ = r;
         if (GROUP) {
             const int u = row / R;
@@ -242,10 +244,12 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             i = row - u * R;
         }
         const int tok = one ? 0 : i / a.G;
-        a.out[r_ * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d] = __float2half_rn(x);
+        __half2 v[2] = {__floats2half2_rn(y.x, y.y), __floats2half2_rn(y.z, y.w)};
+        *reinterpret_cast<uint2 *>(&a.out[r_ * a.o_row + tok * a.o_tok + static_cast<long long>(h * a.G + (i - tok * a.G)) * D + d]) =
+            *reinterpret_cast<uint2 *>(v);
     };
-    auto no_keys = [&](int h) {
-        for (int x = tid; x < min(ROWS, R - qt * ROWS) * D; x += 32 * NW) put(h, x / D, x % D, 0.0f);
+    auto no_keys = [&](int h, int rows) {
+        for (int x = 4 * tid; x < rows * D; x += 128 * NW) put(h, x / D, x % D, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     };
 
     // One unit per CTA: the pages of a warp's first granules, whatever the row's length, so that the table is read while the
@@ -299,8 +303,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         n = last_end = 0x7FFFFFFF;
         c0 = 0;
         c1 = first_of[GROUP];
-        if (c1 == 0)
-            for (int x = tid; x < in_group * R * D; x += 32 * NW) put(blockIdx.y, x / D, x % D, 0.0f);
+        if (c1 == 0) no_keys(blockIdx.y, in_group * R);
     } else if (a.entries) {
         const int own = (a.entries + 32 * NW - 1) / (32 * NW), e0 = min(tid * own, a.entries), e1 = min(e0 + own, a.entries);
         int sum = 0;
@@ -334,13 +337,13 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         for (int e = blockIdx.x; e < a.entries; e += gridDim.x)
             if (pre[e] == pre[e + 1]) {
                 entry(e);
-                for (int h = 0; h < c.nHead; ++h) no_keys(h);
+                for (int h = 0; h < c.nHead; ++h) no_keys(h, min(ROWS, R - qt * ROWS));
             }
     } else {
         c0 = 0;
         c1 = entry(blockIdx.x);
         if (n < 0 && tid == 0 && blockIdx.y == 0) atomicOr(c.status, ST_KV8_BAD_LEN);
-        if (c1 == 0) no_keys(blockIdx.y);
+        if (c1 == 0) no_keys(blockIdx.y, min(ROWS, R - qt * ROWS));
     }
     // The unit of chunk x: sets entry()'s values, h and the unit's first chunk u0; returns its chunks.
     int h = blockIdx.y, u0 = 0;
@@ -849,10 +852,16 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                 compute(masked, other, buf, pos, ks, vs, ok);
             }
         }
-        // The warps' rows, DH dims at a time: thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and 2 t + 1).
-        constexpr int PARTS = D / DH, TP = 4 / PARTS;  // threads t of a part
+        // The warps' rows: behind the last chunk all dims at a time, each warp's in its own ring; before, when the next unit's
+        // chunks are there or on their way, DH dims at a time. Thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and
+        // 2 t + 1).
+        const bool idle = x1 == c1;
+        const int dlog = idle ? SH::LOG_D : SH::LOG_DH, tlog = dlog - SH::LOG_D + 2;  // threads t of a part
+        float *const merge = reinterpret_cast<float *>(idle ? ring_all : ring_all + RING_BYTES);
+        const int row_step = (1 << dlog) + 4, warp_step = idle ? RING_BYTES / NW / 4 : ROWS * (DH + 4);
         const int rows = GROUP ? in_group * R : min(ROWS, R - qt * ROWS);
-        const bool whole = u0 >= c0 && u1 <= c1;
+        constexpr bool PIECES = NW == NW_PIECES && !GROUP;
+        const bool whole = !PIECES || (u0 >= c0 && u1 <= c1);
         const int prow = min(ROWS, R);  // rows of a tile in the work area
         const int slot = 2 * blockIdx.x + (x0 == c0 ? 0 : 1);
         if (SH::INT) flush(1.0f);
@@ -864,15 +873,18 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             if (l[rr] != l[rr]) m[rr] = fmaxf(m[rr], 0.0f);  // NaN stays: a row without keys (m -inf) is left out of the merge
         }
 #pragma unroll 1
-        for (int part = 0; part < PARTS; ++part) {
-            if (x0 > c0 || part) __syncthreads();  // the last merge is through
-            if (t / TP == part) {
+        for (int part = 0; part < D >> dlog; ++part) {
+            if (x0 > c0 || !idle) __syncthreads();  // the last merge is through, and all warps with q
+            else __syncwarp();
+            if (t >> tlog == part) {
+                const int tp = t - (part << tlog);
 #pragma unroll
                 for (int rr = 0; rr < RR; ++rr) {
-                    if (t % TP == 0) {
+                    if (tp == 0) {
                         sm[warp][g + 8 * rr] = m[rr];
                         sl[warp][g + 8 * rr] = l[rr];
                     }
+                    float *to = merge + warp * warp_step + (g + 8 * rr) * row_step + 2 * tp * DT;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -881,35 +893,38 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                             float *wf = reinterpret_cast<float *>(&w);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * unit;
-                            *reinterpret_cast<float4 *>(&so[warp][g + 8 * rr][(2 * (t % TP) + e) * DT + j]) = w;
+                            *reinterpret_cast<float4 *>(to + e * DT + j) = w;
                         }
                 }
             }
             __syncthreads();
-            for (int x = tid; x < rows * DH; x += 32 * NW) {
-                const int row = x / DH, dh = x % DH, d = part * DH + dh;
+            for (int x = tid; x < rows << (dlog - 2); x += 32 * NW) {
+                const int row = x >> (dlog - 2), dh = 4 * (x - (row << (dlog - 2))), d = (part << dlog) + dh;
                 float mx = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w][row]);
-                float lx = 0.0f, y = 0.0f;
+                float lx = 0.0f;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (mx > -INFINITY) {
 #pragma unroll
                     for (int w = 0; w < NW; ++w) {
                         const float f = ex2(sm[w][row] - mx);
+                        const float4 z = *reinterpret_cast<const float4 *>(merge + w * warp_step + row * row_step + dh);
                         lx = fmaf(f, sl[w][row], lx);
-                        y = fmaf(f, so[w][row][dh], y);
+                        y = make_float4(fmaf(f, z.x, y.x), fmaf(f, z.y, y.y), fmaf(f, z.z, y.z), fmaf(f, z.w, y.w));
                     }
                 }
                 if (whole) {
-                    put(h, row, d, lx != 0.0f ? y / lx : 0.0f);
+                    const float inv = lx != 0.0f ? 1.0f / lx : 0.0f;  // NaN stays NaN
+                    put(h, row, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
                 } else {
                     float *pr = a.part + static_cast<long long>(slot) * prow * (D + 4);  // [prow][D] o, [prow][2] m, l, 16-byte steps
-                    pr[row * D + d] = y;
+                    *reinterpret_cast<float4 *>(pr + row * D + d) = y;
                     if (d == 0) *reinterpret_cast<float2 *>(pr + prow * D + 2 * row) = make_float2(mx, lx);
                 }
             }
         }
-        if (!whole) {  // pieces k0 .. k1 share the unit; its first piece's slot names its counter
+        if (PIECES && !whole) {  // pieces k0 .. k1 share the unit; its first piece's slot names its counter
             const int k0 = u0 / per, k1 = (u1 - 1) / per, s0 = 2 * k0 + (u0 == k0 * per ? 0 : 1);
             __syncthreads();
             if (tid == 0) {
@@ -920,41 +935,49 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             __syncthreads();
             if (is_last) {
                 const long long step = static_cast<long long>(prow) * (D + 4);
-                // Four dims per thread and four pieces at a time, all their loads in flight.
-#pragma unroll 2
-                for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
-                    const int row = x / (D / 4), d = x % (D / 4) * 4;
-                    float mx = -INFINITY, lx = 0.0f;
-                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int k = k0; k <= k1; k += 4) {
-                        float2 ml[4];
-                        float4 yk[4];
+                // Four dims of up to four rows per thread, two or four pieces at a time, all their loads in flight.
+                constexpr int N = PIECES ? ROWS * D / 4 / (32 * NW) : 1, AT = N > 2 ? 2 : 4;
+                const int row0 = tid / (D / 4), d = tid % (D / 4) * 4;
+                float mx[N], lx[N];
+                float4 y[N];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int kk = min(k + u, k1);
-                            const float *q = a.part + (kk == k0 ? s0 : 2 * kk) * step;
-                            ml[u] = __ldcg(reinterpret_cast<const float2 *>(q + prow * D + 2 * row));
-                            yk[u] = __ldcg(reinterpret_cast<const float4 *>(q + row * D + d));
-                            if (k + u > k1) ml[u].x = -INFINITY;
-                        }
+                for (int v = 0; v < N; ++v) mx[v] = -INFINITY, lx[v] = 0.0f, y[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                for (int k = k0; k <= k1; k += AT) {
+                    float2 ml[AT][N];
+                    float4 yk[AT][N];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const float mn = fmaxf(mx, ml[u].x);
-                            if (mn == -INFINITY) continue;
-                            const float f = ex2(mx - mn), fk = ex2(ml[u].x - mn);
-                            lx = fmaf(lx, f, ml[u].y * fk);
-                            y.x = fmaf(y.x, f, yk[u].x * fk);
-                            y.y = fmaf(y.y, f, yk[u].y * fk);
-                            y.z = fmaf(y.z, f, yk[u].z * fk);
-                            y.w = fmaf(y.w, f, yk[u].w * fk);
-                            mx = mn;
+                    for (int u = 0; u < AT; ++u) {
+                        const int kk = min(k + u, k1);
+                        const float *q = a.part + (kk == k0 ? s0 : 2 * kk) * step;
+#pragma unroll
+                        for (int v = 0; v < N; ++v) {
+                            const int row = min(row0 + v * (128 * NW / D), rows - 1);
+                            ml[u][v] = __ldcg(reinterpret_cast<const float2 *>(q + prow * D + 2 * row));
+                            yk[u][v] = __ldcg(reinterpret_cast<const float4 *>(q + row * D + d));
+                            if (k + u > k1) ml[u][v].x = -INFINITY;
                         }
                     }
-                    const float inv = lx != 0.0f ? 1.0f / lx : 0.0f;  // NaN stays NaN
-                    put(h, row, d, y.x * inv);
-                    put(h, row, d + 1, y.y * inv);
-                    put(h, row, d + 2, y.z * inv);
-                    put(h, row, d + 3, y.w * inv);
+#pragma unroll
+                    for (int u = 0; u < AT; ++u)
+#pragma unroll
+                        for (int v = 0; v < N; ++v) {
+                            const float mn = fmaxf(mx[v], ml[u][v].x);
+                            if (mn == -INFINITY) continue;
+                            const float f = ex2(mx[v] - mn), fk = ex2(ml[u][v].x - mn);
+                            lx[v] = fmaf(lx[v], f, ml[u][v].y * fk);
+                            y[v].x = fmaf(y[v].x, f, yk[u][v].x * fk);
+                            y[v].y = fmaf(y[v].y, f, yk[u][v].y * fk);
+                            y[v].z = fmaf(y[v].z, f, yk[u][v].z * fk);
+                            y[v].w = fmaf(y[v].w, f, yk[u][v].w * fk);
+                            mx[v] = mn;
+                        }
+                }
+#pragma unroll
+                for (int v = 0; v < N; ++v) {
+                    const float inv = lx[v] != 0.0f ? 1.0f / lx[v] : 0.0f;
+                    const int row = row0 + v * (128 * NW / D);
+                    if (row < rows) put(h, row, d, make_float4(y[v].x * inv, y[v].y * inv, y[v].z * inv, y[v].w * inv));
                 }
             }
         }
