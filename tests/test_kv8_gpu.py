@@ -324,6 +324,27 @@ def test_attention_counts_this_steps_tokens(cuda, lib):
     assert lib.status() == 0
 
 
+@pytest.mark.parametrize("kind,rows,dim", [("int8", 100, 64), ("e4m3", 41, 128)])
+def test_attention_of_many_rows_counts_this_steps_tokens(cuda, lib, kind, rows, dim):
+    """count / d_count and max_len with rows taken together, whose pages are all shared up to this step's token."""
+    torch = cuda
+    lens = [95 - r % 3 for r in range(rows)]
+    cache = filled(torch, lib, kind, rows, 12, dim, 16, 16, [n + 1 for n in lens], 12, 1, seed=9)
+    table = cache.table.cpu()
+    for r in range(rows):
+        table[r, :5] = table[r // 4 * 4, :5]
+    cache.table.copy_(table)
+    cache.length.copy_(torch.tensor(lens, dtype=torch.int32))
+    q = torch.randn(rows, 1, 12 * dim, device="cuda").half()
+    out = torch.empty_like(q)
+    cache.attend(out, q, count=1, max_len=96)
+    check_attention(torch, cache, kind, q, out, 0, [n + 1 for n in lens], None)
+    some = [r % 2 for r in range(rows)]
+    cache.attend(out, q, count=torch.tensor(some, dtype=torch.int32, device="cuda"))
+    check_attention(torch, cache, kind, q, out, 0, [n + s for n, s in zip(lens, some)], None)
+    assert lib.status() == 0
+
+
 class Pages:
     """The page operators row by row, as the header defines them."""
 
