@@ -45,7 +45,7 @@ struct DeviceContext {
     bool prefill_attr_done = false;
     bool decode_attr_done = false;
     bool beam_attr_done[2] = {false, false};  // beam selection over fp16, fp32 logits
-    bool kv8_attr_done[33] = {};              // 8-bit cache attention, by kernel variant
+    bool kv8_attr_done[32] = {};              // 8-bit cache attention, by kernel variant
     int num_sms = 0;
     int device = 0;                 // CUDA device ordinal of this context
 };

@@ -16,11 +16,6 @@
 //     order of dims, so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
 //     column order are as free, so a thread reads 8 or 16 neighbouring dims of the 4 keys whose p it holds, and ends with
 //     16 neighbouring output dims. The 16-byte granules of a chunk are permuted so that neither read has bank conflicts.
-//   - int8 codes of 64 dims under at most 8 query rows in long contexts need no conversion at all: INT. q is cut into
-//     three signed 8-bit digits (23 bits below the row's largest element), p * vscale / S into three unsigned ones, and
-//     mma.m16n8k32 multiplies the codes as they are, exactly; rows 8..15 take the second digit, a second MMA the third. What
-//     is left is about half the instructions of the converting path, which is bound by issuing them (16 sequences x 12 heads, 8192
-//     to 16384 keys: 59.5 us, 5.1 TB/s; converting: 65.6 us).
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
 //   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
@@ -51,8 +46,6 @@ namespace kv8 {
 
 constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces, and of a group
 constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
-// In the integer path p takes 23 bits: P_BITS below 1, LAZY_INT above.
-constexpr float LAZY_INT = 2.0f, P_ONE = 2097152.0f;  // 2^21
 constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
 constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
 
@@ -89,24 +82,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
-// The same for 8-bit codes, 32 of them per step, sums in int32: A signed or unsigned, B signed.
-__device__ __forceinline__ void imma_ss(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void imma_us(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Bytes 0, 1, 2 of four integers, each as one register.
-__device__ __forceinline__ void bytes3(const uint32_t (&x)[4], uint32_t &d0, uint32_t &d1, uint32_t &d2) {
-    const uint32_t a = __byte_perm(x[0], x[1], 0x5140), b = __byte_perm(x[2], x[3], 0x5140);
-    d0 = __byte_perm(a, b, 0x5410);
-    d1 = __byte_perm(a, b, 0x7632);
-    d2 = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410);
 }
 // A copy that the compiler takes for another value. An MMA's four A operands are neighbouring registers: a value
 // that is two of them would be moved there before every MMA.
@@ -186,13 +161,10 @@ struct Chunk {
 // of 128 dims or 16 rows take the registers, so q of 128 dims lies in shared memory instead (32 registers), and the warps'
 // rows are merged where the rings were or, in the middle of a piece, DH dims at a time in q's place.
 // 16 rows of 128 dims spill at 12 warps, so 8 (8 sequences x 8 heads of 16384 keys: 62.5 us, 12 warps 68.7; 55.5 since the merge
-// takes four dims per thread and the last CTA has the loads of all its rows in flight). INT: the integer accumulators take 64
-// more registers: 8 warps, too.
-template <int D, int ROWS, int NW, bool INT_>
+// takes four dims per thread and the last CTA has the loads of all its rows in flight).
+template <int D, int ROWS, int NW>
 struct Shape {
-    static constexpr bool INT = INT_;
-    static_assert(!INT || (D == 64 && ROWS == 8), "the integer path's accumulators fit 64 dims and 8 rows");
-    static constexpr int WARPS = INT || (D == 128 && ROWS == 16) ? 8 : 12;  // per SM
+    static constexpr int WARPS = D == 128 && ROWS == 16 ? 8 : 12;  // per SM
     static constexpr int RESIDENT = WARPS / NW;
     static constexpr int STAGES = 2;
     static constexpr int RING = NW * STAGES * CHUNK_BYTES;
@@ -205,10 +177,10 @@ struct Shape {
 };
 
 // GROUP: 0, or the cache rows of a CTA that reads their shared pages once (2 or 4)
-template <int KIND, int D, int ROWS, int NW, bool INT, int GROUP>
-__global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_kv8_attend(const View c, const AttParams a) {
+template <int KIND, int D, int ROWS, int NW, int GROUP>
+__global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_attend(const View c, const AttParams a) {
     using C = Chunk<D>;
-    using SH = Shape<D, ROWS, NW, INT>;
+    using SH = Shape<D, ROWS, NW>;
     constexpr int STAGES = SH::STAGES, RING_BYTES = SH::RING, DH = SH::DH;
     constexpr int CK = C::CK, GR = C::GR, NT = CK / 8, KS = D / 16, DT = D / 8, RR = ROWS / 8;
     constexpr int SET = 32 / GR;  // chunks whose granules one look-up covers
@@ -454,9 +426,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                                    : (2 * t * 8 + (g ^ (2 * t))) * 16);
     // The segment at hand: q, m, l, o and the keys its rows see.
     __align__(16) uint32_t qa[SH::Q_SMEM ? 1 : KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
-    uint32_t qd[2][4], qd0[2][2];  // INT: q's first two digits, and the third, per 32 dims
-    float qs_row = 0.0f;           // INT: the value of q's last digit
-    int c12[SH::INT ? DT : 1][4], c3[SH::INT ? DT : 1][4];  // INT: sums of the digits of p times codes, not yet in o
     int my_row = 0;  // GROUP: the cache row, in the group, of this lane's query row
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
     float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
@@ -583,102 +552,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         }
     };
 
-    // INT: the integer sums go to o, which is scaled by f.
-    auto flush = [&](float f) {
-#pragma unroll
-        for (int j = 0; j < (SH::INT ? DT : 0); ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                o[j][e] = (o[j][e] + fmaf(static_cast<float>(c12[j][e]), 65536.0f, fmaf(static_cast<float>(c12[j][2 + e]), 256.0f, static_cast<float>(c3[j][e])))) * f;
-                c12[j][e] = c12[j][2 + e] = c3[j][e] = 0;
-            }
-    };
-    auto compute_int = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
-        float s[NT][2];
-#pragma unroll
-        for (int tile = 0; tile < NT; ++tile) {
-            const uint4 kw = *reinterpret_cast<const uint4 *>(buf + kl0 + tile * 8 * D);
-            int c[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0};
-            imma_ss(c, qd[0][0], qd[0][1], qd[0][2], qd[0][3], kw.x, kw.y);
-            imma_ss(e, qd0[0][0], 0u, qd0[0][1], 0u, kw.x, kw.y);
-            imma_ss(c, qd[1][0], qd[1][1], qd[1][2], qd[1][3], kw.z, kw.w);
-            imma_ss(e, qd0[1][0], 0u, qd0[1][1], 0u, kw.z, kw.w);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)  // |c| <= 2^20: the first two digits fit an int32
-                s[tile][x] = fmaf(static_cast<float>(c[x] * 256 + c[2 + x]), 256.0f, static_cast<float>(e[x]));
-        }
-        if (masked) {
-#pragma unroll
-            for (int tile = 0; tile < NT; ++tile)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int key = pos + 8 * tile + 2 * t + x;
-                    if (key < first || key >= end[0] || !((ok >> (tile / 2)) & 1u)) s[tile][x] = -INFINITY;
-                }
-        }
-        if (GROUP && other)
-#pragma unroll
-            for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = -INFINITY;
-        float kq[GR], top = -INFINITY;
-#pragma unroll
-        for (int gi = 0; gi < GR; ++gi) {
-            kq[gi] = fmaxf(ks[gi] * qs_row, TINY);
-            if (qs_row != qs_row) kq[gi] = qs_row;
-            top = fmaxf(top, kq[gi] * fmaxf(fmaxf(s[2 * gi][0], s[2 * gi][1]), fmaxf(s[2 * gi + 1][0], s[2 * gi + 1][1])));
-        }
-        if (__any_sync(0xFFFFFFFFu, top > m[0] + LAZY_INT)) {
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float mn = fmaxf(m[0], top), f = mn > -INFINITY ? ex2(m[0] - mn) : 0.0f;
-            m[0] = mn;
-            l[0] *= f;
-            flush(f);
-        }
-        const float mm = m[0] > -INFINITY ? m[0] : 0.0f;
-#pragma unroll
-        for (int k2 = 0; k2 < GR / 2; ++k2) {  // 32 keys
-            uint32_t d0[2], d1[2], d2[2];
-#pragma unroll
-            for (int gi = 0; gi < 2; ++gi) {
-                const float w = other ? 0.0f : vs[2 * k2 + gi] * invS * P_ONE;
-                uint32_t x[4];  // 2^23 + p * w: the low bytes are the digits
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float p = ex2(fmaf(s[4 * k2 + 2 * gi + u / 2][u & 1], kq[2 * k2 + gi], -mm));
-                    l[0] += p;
-                    x[u] = __float_as_uint(fmaf(p, w, 8388608.0f));
-                }
-                bytes3(x, d0[gi], d1[gi], d2[gi]);
-            }
-            uint2 vw[2][4];
-#pragma unroll
-            for (int gi = 0; gi < 2; ++gi)
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                    vw[gi][y] = *reinterpret_cast<const uint2 *>(buf + vl + (16 * (2 * k2 + gi) + 8 * (y >> 1) + 2 * (y & 1)) * D);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {  // 4 dims: codes of 4 keys per dim and granule
-                uint32_t b[2][4];
-#pragma unroll
-                for (int gi = 0; gi < 2; ++gi) {
-                    const uint32_t w0 = q ? vw[gi][0].y : vw[gi][0].x, w1 = q ? vw[gi][1].y : vw[gi][1].x;
-                    const uint32_t w2 = q ? vw[gi][2].y : vw[gi][2].x, w3 = q ? vw[gi][3].y : vw[gi][3].x;
-                    const uint32_t a0 = __byte_perm(w0, w1, 0x5140), a1 = __byte_perm(w2, w3, 0x5140);
-                    const uint32_t a2 = __byte_perm(w0, w1, 0x7362), a3 = __byte_perm(w2, w3, 0x7362);
-                    b[gi][0] = __byte_perm(a0, a1, 0x5410);
-                    b[gi][1] = __byte_perm(a0, a1, 0x7632);
-                    b[gi][2] = __byte_perm(a2, a3, 0x5410);
-                    b[gi][3] = __byte_perm(a2, a3, 0x7632);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    imma_us(c12[SH::INT ? 4 * q + j : 0], d2[0], d1[0], d2[1], d1[1], b[0][j], b[1][j]);
-                    imma_us(c3[SH::INT ? 4 * q + j : 0], d0[0], 0u, d0[1], 0u, b[0][j], b[1][j]);
-                }
-            }
-        }
-    };
-
     const int mine = c1 - c0 > warp ? (c1 - c0 - warp + NW - 1) / NW : 0;  // chunks c0 + warp, c0 + warp + NW, ...
     // The look-up of a set comes before the loads of its chunks, while the set before is still in use: pks, pvs and pok are
     // the set's in use, pof whose they are.
@@ -736,45 +609,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                     x[1] = *reinterpret_cast<const uint4 *>(qp + 64 * s4 + 8);
                 }
                 const uint32_t *w = reinterpret_cast<const uint32_t *>(x);
-                if (SH::INT) {  // q = qs_row * (d2 2^16 + d1 2^8 + d0), qs_row a power of two, digits signed
-                    float f[16], big = 0.0f;
-                    bool bad = false;
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        const float2 z = __half22float2(reinterpret_cast<const __half2 *>(w)[y]);
-                        f[2 * y] = z.x;
-                        f[2 * y + 1] = z.y;
-                        bad |= !(fabsf(z.x) < INFINITY) || !(fabsf(z.y) < INFINITY);
-                        big = fmaxf(big, fmaxf(fabsf(z.x), fabsf(z.y)));
-                    }
-                    if (bad) big = INFINITY;
-                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-                    const int ex = static_cast<int>(__float_as_uint(big) >> 23) - 126;  // big < 2^ex
-                    const bool some = big > 0.0f && big < INFINITY;
-                    const float inv = some ? __uint_as_float(static_cast<unsigned>(22 - ex + 127) << 23) : 0.0f;
-                    // a row that is not finite gives NaN
-                    qs_row = some ? __uint_as_float(static_cast<unsigned>(ex - 22 + 127) << 23) : big > 0.0f ? NAN : 0.0f;
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        uint32_t d0[4], d1[4], d2[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int v = some ? __float2int_rn(f[4 * y + u] * inv) : 0;
-                            const int v0 = static_cast<int8_t>(v), r1 = (v - v0) >> 8, v1 = static_cast<int8_t>(r1);
-                            d0[u] = static_cast<uint32_t>(v0);
-                            d1[u] = static_cast<uint32_t>(v1);
-                            d2[u] = static_cast<uint32_t>((r1 - v1) >> 8);
-                        }
-                        auto low = [](const uint32_t (&z)[4]) {
-                            return __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
-                        };
-                        qd[y >> 1][2 * (y & 1)] = low(d2);
-                        qd[y >> 1][2 * (y & 1) + 1] = low(d1);
-                        qd0[y >> 1][y & 1] = low(d0);
-                    }
-                    continue;
-                }
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     if (SH::Q_SMEM) {
@@ -802,8 +636,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         if (SH::Q_SMEM) __syncthreads();
 #pragma unroll
         for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < (SH::INT ? DT : 0); ++j) c12[j][0] = c12[j][1] = c12[j][2] = c12[j][3] = c3[j][0] = c3[j][1] = c3[j][2] = c3[j][3] = 0;
         S = i % SET ? largest() : 0.0f;  // a new set's comes with its first chunk
         invS = S > 0.0f ? 1.0f / S : 0.0f;
         for (; c0 + i * NW + warp < x1; ++i) {
@@ -818,12 +650,10 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                 const float Sn = fmaxf(S, largest());
                 if (Sn > S) {
                     const float f = S / Sn;
-                    if (SH::INT) flush(f);
-                    else
 #pragma unroll
-                        for (int j = 0; j < DT; ++j)
+                    for (int j = 0; j < DT; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[j][e] *= f;
+                        for (int e = 0; e < 4; ++e) o[j][e] *= f;
                     S = Sn;
                     invS = 1.0f / Sn;
                 }
@@ -845,12 +675,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
             }
             const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
             const bool masked = pos < first || pos + CK > full_end || ok != (1u << GR) - 1u;
-            if (SH::INT) {
-                compute_int(masked, other, buf, pos, ks, vs, ok);
-                if ((i & 511) == 511) flush(1.0f);  // 512 chunks: 32768 keys of at most 255 * 127, below 2^31
-            } else {
-                compute(masked, other, buf, pos, ks, vs, ok);
-            }
+            compute(masked, other, buf, pos, ks, vs, ok);
         }
         // The warps' rows: behind the last chunk all dims at a time, each warp's in its own ring; before, when the next unit's
         // chunks are there or on their way, DH dims at a time. Thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and
@@ -864,8 +689,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
         const bool whole = !PIECES || (u0 >= c0 && u1 <= c1);
         const int prow = min(ROWS, R);  // rows of a tile in the work area
         const int slot = 2 * blockIdx.x + (x0 == c0 ? 0 : 1);
-        if (SH::INT) flush(1.0f);
-        const float unit = SH::INT ? S / P_ONE : S;
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
             l[rr] += __shfl_xor_sync(0xFFFFFFFFu, l[rr], 1);
@@ -892,7 +715,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW, INT>::RESIDENT) k_
                             float4 w;
                             float *wf = reinterpret_cast<float *>(&w);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * unit;
+                            for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
                             *reinterpret_cast<float4 *>(to + e * DT + j) = w;
                         }
                 }
@@ -1067,21 +890,15 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
         constexpr int KIND = decltype(kind)::value, D = decltype(dim)::value;
         constexpr int base = (KIND == GPT2_KV8_INT8 ? 0 : 16) + (D == 64 ? 0 : 8);
         if (rows == 8) {
-            if (group == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 4>, kv8::Shape<D, 8, 4, false>(), base);
-            if (group == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 2>, kv8::Shape<D, 8, 4, false>(), base + 1);
-            // The integer path's q costs more to prepare than its chunks save where a warp has fewer than 8 (one sequence of 1023
-            // keys: 8.2 against 7.1 us; 8 sequences: 14.1 against 12.3; 16 sequences of 16384: 59.5 against 65.6). Its registers
-            // leave an SM 8 warps, the conversion 12: with units in plenty the conversion is as fast or faster (128 x 12 units,
-            // windows of 1024 keys: 46.6 against 57.0 us).
-            if (KIND == GPT2_KV8_INT8 && D == 64 && warps == 4 && chunks >= 8ll * 8 * ctx->num_sms)
-                return go(kv8::k_kv8_attend<GPT2_KV8_INT8, 64, 8, 4, true, 0>, kv8::Shape<64, 8, 4, true>(), 32);
-            if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, false, 0>, kv8::Shape<D, 8, 4, false>(), base + 2);
-            if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 2, false, 0>, kv8::Shape<D, 8, 2, false>(), base + 3);
-            return go(kv8::k_kv8_attend<KIND, D, 8, 1, false, 0>, kv8::Shape<D, 8, 1, false>(), base + 4);
+            if (group == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, 4>, kv8::Shape<D, 8, 4>(), base);
+            if (group == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 4, 2>, kv8::Shape<D, 8, 4>(), base + 1);
+            if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 8, 4, 0>, kv8::Shape<D, 8, 4>(), base + 2);
+            if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 8, 2, 0>, kv8::Shape<D, 8, 2>(), base + 3);
+            return go(kv8::k_kv8_attend<KIND, D, 8, 1, 0>, kv8::Shape<D, 8, 1>(), base + 4);
         }
-        if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 16, 4, false, 0>, kv8::Shape<D, 16, 4, false>(), base + 5);
-        if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 16, 2, false, 0>, kv8::Shape<D, 16, 2, false>(), base + 6);
-        return go(kv8::k_kv8_attend<KIND, D, 16, 1, false, 0>, kv8::Shape<D, 16, 1, false>(), base + 7);
+        if (warps == 4) return go(kv8::k_kv8_attend<KIND, D, 16, 4, 0>, kv8::Shape<D, 16, 4>(), base + 5);
+        if (warps == 2) return go(kv8::k_kv8_attend<KIND, D, 16, 2, 0>, kv8::Shape<D, 16, 2>(), base + 6);
+        return go(kv8::k_kv8_attend<KIND, D, 16, 1, 0>, kv8::Shape<D, 16, 1>(), base + 7);
     };
     auto by_dim = [&](auto kind) {
         return kv->headDim == 64 ? by_rows(kind, std::integral_constant<int, 64>()) : by_rows(kind, std::integral_constant<int, 128>());
