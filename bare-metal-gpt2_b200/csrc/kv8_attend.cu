@@ -6,11 +6,11 @@
 //
 // A decode step reads 2 D + 8 / block bytes per key and K/V head once and does 4 D flops per key and query:
 // HBM-bound, if the codes get into the tensor cores cheaply. So:
-//   - the products are mma.m16n8k16 in fp16 with fp32 sums. A code is exact in fp16 and so is q; p is not, and goes
-//     in as hi + lo (two fp16, 22 bits): rounding it to one fp16 alone would add an error of the size of the
-//     output's own rounding. With at most 8 query rows (the decode step) the MMA's rows 8..15 are
-//     free and take lo; with 9 to 16 rows lo is a second MMA. mma.sync's rate is far above what HBM feeds
-//     (64 MMAs of 8 cycles per 8 KB of codes).
+//   - the products are mma.m16n8k16 in fp16 with fp32 sums. A code is exact in fp16 and so is q; p * vscale is not,
+//     and goes in as hi + lo (two fp16): rounding it to one fp16 alone would add an error of the size of the
+//     output's own rounding. hi + lo keep 22 bits, or 2^-34 of the row's largest where that is more (see e below). With at
+//     most 8 query rows (the decode step) the MMA's rows 8..15 are free and take lo; with 9 to 16 rows lo is a second MMA.
+//     mma.sync's rate is far above what HBM feeds (64 MMAs of 8 cycles per 8 KB of codes).
 //   - a warp takes CK keys at a time (64 for D 64, 32 for D 128: 8 KB of K and V) through a ring of its own in shared
 //     memory (cp.async, the next chunk in flight while one is computed, no CTA barrier). The sum over dims (QK) may run in any
 //     order of dims, so a thread's 16 neighbouring code bytes of one key are its operands for 4 k-steps; PV's sum over keys and its
@@ -18,10 +18,12 @@
 //     16 neighbouring output dims. The 16-byte granules of a chunk are permuted so that neither read has bank conflicts.
 //   - a lane looks up the page and the two scales of one 16-key granule for the warp, 32 granules at a time, and
 //     shuffles hand them out.
-//   - p * vscale would leave fp16's range for small scales, so p * (vscale / S) goes in, S the largest
-//     vscale of the row's granules looked up so far; o is kept in units of S.
-//   - m is not the maximum but within 2^LAZY of it: p stays below 2^LAZY, far inside fp16 and fp32, and most chunks need
-//     neither the row maximum's shuffles nor a rescaling of o.
+//   - p * vscale has fp16's range neither where scales are small nor where the keys with large p have small values and the others
+//     count for the output. So p * vscale * 2^(PV_BITS - e) goes in, e following the row's largest log2(p * vscale) as m follows the
+//     largest score, and o is kept in those units: an attention sink of small values, or a block of huge values that nobody
+//     attends, costs the other keys nothing.
+//   - m is not the maximum but within 2^LAZY of it: p stays below 2^LAZY, far inside fp32, and most chunks need neither the row
+//     maximum's shuffles nor a rescaling of o. So with e: p * vscale goes in at up to 2^(LAZY + PV_BITS) = 2^15.
 //
 // Work: a unit is (cache row, tile of 8 or 16 query rows, K/V head) with its chunks of keys, which the warps of a CTA (1, 2 or 4)
 // take in turn; at its end they are merged in shared memory. With units in plenty each has a CTA. With fewer units than resident
@@ -45,7 +47,9 @@ namespace b200 {
 namespace kv8 {
 
 constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces, and of a group
-constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows
+constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows, and its p * vscale e
+constexpr float PV_BITS = 9.0f;      // log2 of what the row's largest p * vscale goes in as
+constexpr float E_LEAST = -100.0f;   // e's least: what is below that is 0 in any fp16 output
 constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
 constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
 
@@ -67,6 +71,11 @@ struct AttParams {
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -353,7 +362,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     unsigned grow = 0;
     float gks = 0.0f, gvs = 0.0f;
     unsigned gok = 0;
-    int gof = 0;  // whose chunk: its unit's first chunk; GROUP: its row
     // A block of zeros has scale 0; TINY in its place keeps -inf (a masked score) times a scale from being NaN.
     constexpr float TINY = 1e-20f;
     bool bad = false;
@@ -363,14 +371,13 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
         int ok = x < c1, pos = 0;
         if (GROUP) {
             if (ok) {
-                const int own = gof = chunk_of(x, pos);
+                const int own = chunk_of(x, pos);
                 pos += (lane % GR) * 16;
                 ok = own < 0 || pos < len_of[own];
                 r = GROUP * blockIdx.x + max(own, 0);
             }
         } else if (ok) {
             unit_of(x);
-            gof = u0;
             pos = base + (x - u0) * CK + (lane % GR) * 16;
             ok = pos < last_end && pos + 16 > first;
         }
@@ -424,12 +431,12 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     const int kl1 = D == 64 ? 0 : (g * 8 + ((4 + t) ^ ((g & 1) << 2))) * 16;
     const int vl = HALF + (D == 64 ? ((((t >> 1) * 4 + (t & 1)) * 4 + ((g >> 1) ^ (t & 2))) * 16 + (g & 1) * 8)
                                    : (2 * t * 8 + (g ^ (2 * t))) * 16);
-    // The segment at hand: q, m, l, o and the keys its rows see.
+    // The segment at hand: q, m, e, l, o and the keys its rows see.
     __align__(16) uint32_t qa[SH::Q_SMEM ? 1 : KS][4];  // A operands: with 8 rows, rows 8..15 are rows 0..7 again
     int my_row = 0;  // GROUP: the cache row, in the group, of this lane's query row
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
-    float o[DT][4], m[RR], l[RR], S = 0.0f, invS = 0.0f;
-    auto compute = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], unsigned ok) {
+    float o[DT][4], m[RR], l[RR], e2[RR], pv[RR];  // e; 2^(PV_BITS - e)
+    auto compute = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], float most, unsigned ok) {
         float s[NT][4];
 #pragma unroll
         for (int s4 = 0; s4 < KS / 4; ++s4) {
@@ -462,24 +469,37 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
 #pragma unroll
             for (int tile = 0; tile < NT; ++tile) s[tile][0] = s[tile][1] = -INFINITY;
         // A granule's scale is one factor of its scores: the largest of them first, then the factor.
+        auto largest = [&](int rr, int gi) {
+            return ks[gi] * fmaxf(fmaxf(s[2 * gi][2 * rr], s[2 * gi][2 * rr + 1]), fmaxf(s[2 * gi + 1][2 * rr], s[2 * gi + 1][2 * rr + 1]));
+        };
         float top[RR];
         bool grew = false;
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
             top[rr] = -INFINITY;
 #pragma unroll
-            for (int gi = 0; gi < GR; ++gi)
-                top[rr] = fmaxf(top[rr], ks[gi] * fmaxf(fmaxf(s[2 * gi][2 * rr], s[2 * gi][2 * rr + 1]), fmaxf(s[2 * gi + 1][2 * rr], s[2 * gi + 1][2 * rr + 1])));
-            grew |= top[rr] > m[rr] + LAZY;  // m -inf: any key
+            for (int gi = 0; gi < GR; ++gi) top[rr] = fmaxf(top[rr], largest(rr, gi));
+            // m -inf: any key. most, the chunk's largest log2(vscale), stands for every granule's: e is looked at closer below
+            grew |= top[rr] + fmaxf(most - e2[rr], 0.0f) > m[rr] + LAZY;
         }
         if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
             for (int rr = 0; rr < RR; ++rr) {
                 top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xFFFFFFFFu, top[rr], 1));
                 top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xFFFFFFFFu, top[rr], 2));
-                const float mn = fmaxf(m[rr], top[rr]), f = mn > -INFINITY ? ex2(m[rr] - mn) : 0.0f;
+                const float mn = fmaxf(m[rr], top[rr]), fell = m[rr] - mn;  // NaN as long as there is no key
+                const bool some = mn > -INFINITY;
+                float en = -INFINITY;
+#pragma unroll
+                for (int gi = 0; gi < GR; ++gi) en = fmaxf(en, (largest(rr, gi) - mn) + lg2(vs[gi]));
+                en = fmaxf(en, __shfl_xor_sync(0xFFFFFFFFu, en, 1));
+                en = fmaxf(en, __shfl_xor_sync(0xFFFFFFFFu, en, 2));
+                en = fmaxf(fmaxf(en, e2[rr] + fell), E_LEAST);
+                const float f = some ? ex2((e2[rr] + fell) - en) : 0.0f;
                 m[rr] = mn;
-                l[rr] *= f;
+                e2[rr] = en;
+                pv[rr] = ex2(PV_BITS - en);
+                l[rr] *= some ? ex2(fell) : 0.0f;
 #pragma unroll
                 for (int j = 0; j < DT; ++j) {
                     o[j][RR == 1 ? 0 : 2 * rr] *= f;
@@ -496,7 +516,6 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
         for (int rr = 0; rr < RR; ++rr) mm[rr] = m[rr] > -INFINITY ? m[rr] : 0.0f;
 #pragma unroll
         for (int gi = 0; gi < GR; ++gi) {
-            const float w = other ? 0.0f : vs[gi] * invS;
             uint32_t ph[2 * RR], pl[2 * RR];  // [tile of the granule * RR + rr]
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile)
@@ -505,6 +524,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                     float p0 = ex2(fmaf(s[2 * gi + tile][2 * rr], ks[gi], -mm[rr]));
                     float p1 = ex2(fmaf(s[2 * gi + tile][2 * rr + 1], ks[gi], -mm[rr]));
                     l[rr] += p0 + p1;
+                    const float w = other ? 0.0f : vs[gi] * pv[rr];
                     p0 *= w;
                     p1 *= w;
                     float l0, l1;
@@ -554,23 +574,9 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
 
     const int mine = c1 - c0 > warp ? (c1 - c0 - warp + NW - 1) / NW : 0;  // chunks c0 + warp, c0 + warp + NW, ...
     // The look-up of a set comes before the loads of its chunks, while the set before is still in use: pks, pvs and pok are
-    // the set's in use, pof whose they are.
-    float pks = TINY, pvs = 0.0f;
+    // the set's in use, pmost the chunk's largest log2(vscale) in the lanes of its granules.
+    float pks = TINY, pvs = 0.0f, pmost = -INFINITY;
     unsigned pok = 0;
-    int pof = 0;
-    // The set's largest vscale (they are not negative), of this unit's chunks alone, and in a group of those that this lane's row
-    // sees: what another row's values are is no matter for this one's rounding.
-    auto largest = [&]() {
-        auto over = [&](bool in) { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, in ? __float_as_uint(pvs) : 0u)); };
-        if (!GROUP) return over(NW != NW_PIECES || pof == u0);
-        float of = 0.0f;
-#pragma unroll
-        for (int u = 0; u < GROUP; ++u) {
-            const float x = over(pof < 0 || pof == u);
-            if (my_row == u) of = x;
-        }
-        return of;
-    };
     auto fetch = [&](int i) {
         if (i < mine) {
             if (i % SET == 0) look_up(i / SET);
@@ -632,12 +638,12 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             }
             m[rr] = -INFINITY;
             l[rr] = 0.0f;
+            e2[rr] = E_LEAST;
+            pv[rr] = 0.0f;
         }
         if (SH::Q_SMEM) __syncthreads();
 #pragma unroll
         for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        S = i % SET ? largest() : 0.0f;  // a new set's comes with its first chunk
-        invS = S > 0.0f ? 1.0f / S : 0.0f;
         for (; c0 + i * NW + warp < x1; ++i) {
             cp_async_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of chunk i are there, and all are done with chunk i - 1
@@ -646,17 +652,10 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                 pks = fmaxf(gks * a.scale_log2, TINY);
                 pvs = gvs;
                 pok = gok;
-                pof = gof;
-                const float Sn = fmaxf(S, largest());
-                if (Sn > S) {
-                    const float f = S / Sn;
+                pmost = gvs;
 #pragma unroll
-                    for (int j = 0; j < DT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] *= f;
-                    S = Sn;
-                    invS = 1.0f / Sn;
-                }
+                for (int x = 1; x < GR; x <<= 1) pmost = fmaxf(pmost, __shfl_xor_sync(0xFFFFFFFFu, pmost, x));
+                pmost = lg2(pmost);
             }
             float ks[GR], vs[GR];
 #pragma unroll
@@ -664,6 +663,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                 ks[gi] = __shfl_sync(0xFFFFFFFFu, pks, (i % SET) * GR + gi);
                 vs[gi] = __shfl_sync(0xFFFFFFFFu, pvs, (i % SET) * GR + gi);
             }
+            const float most = __shfl_sync(0xFFFFFFFFu, pmost, (i % SET) * GR);
             const unsigned ok = (pok >> ((i % SET) * GR)) & ((1u << GR) - 1u);
             int pos = base + (c0 + i * NW + warp - u0) * CK;
             bool other = false;  // GROUP: a chunk of another row than this lane's
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             }
             const uint8_t *buf = ring + i % STAGES * CHUNK_BYTES;
             const bool masked = pos < first || pos + CK > full_end || ok != (1u << GR) - 1u;
-            compute(masked, other, buf, pos, ks, vs, ok);
+            compute(masked, other, buf, pos, ks, vs, most, ok);
         }
         // The warps' rows: behind the last chunk all dims at a time, each warp's in its own ring; before, when the next unit's
         // chunks are there or on their way, DH dims at a time. Thread (g, t) holds dims 2 t DT .. (the columns j of tiles 2 t and
@@ -707,6 +707,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                         sm[warp][g + 8 * rr] = m[rr];
                         sl[warp][g + 8 * rr] = l[rr];
                     }
+                    const float unit = ex2(e2[rr] - PV_BITS);
                     float *to = merge + warp * warp_step + (g + 8 * rr) * row_step + 2 * tp * DT;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                             float4 w;
                             float *wf = reinterpret_cast<float *>(&w);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * S;
+                            for (int k = 0; k < 4; ++k) wf[k] = (RR == 1 ? o[j + k][e] + o[j + k][2 + e] : o[j + k][2 * rr + e]) * unit;
                             *reinterpret_cast<float4 *>(to + e * DT + j) = w;
                         }
                 }
