@@ -49,6 +49,9 @@ namespace kv8 {
 constexpr int NW_PIECES = 4;         // warps per CTA of a launch in equal pieces, and of a group
 constexpr float LAZY = 6.0f;         // log2 of how far a row's scores may pass m before m follows, and its p * vscale e
 constexpr float PV_BITS = 9.0f;      // log2 of what the row's largest p * vscale goes in as
+// Scores are not rounded before m is subtracted (one FMA), m is: beyond 2^28 that alone could be more than fp32's exponents. From
+// STEEP on, where it is still 2^-8, scores are rounded as m is, and m and e follow every chunk.
+constexpr float STEEP = 65536.0f;
 constexpr float E_LEAST = -100.0f;   // e's least: what is below that is 0 in any fp16 output
 constexpr int MAX_ENTRIES = 1024;    // (row, tile) pairs of a launch whose CTAs take equal pieces
 constexpr int MAX_PIECES = 1024;     // CTAs of such a launch
@@ -436,6 +439,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
     int my_row = 0;  // GROUP: the cache row, in the group, of this lane's query row
     int end[RR], full_end = 0;  // keys of every row: [first, full_end)
     float o[DT][4], m[RR], l[RR], e2[RR], pv[RR];  // e; 2^(PV_BITS - e)
+    bool steep = false;  // some row's |m| is over STEEP
     auto compute = [&](const bool masked, const bool other, const uint8_t *buf, int pos, float (&ks)[GR], float (&vs)[GR], float most, unsigned ok) {
         float s[NT][4];
 #pragma unroll
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             return ks[gi] * fmaxf(fmaxf(s[2 * gi][2 * rr], s[2 * gi][2 * rr + 1]), fmaxf(s[2 * gi + 1][2 * rr], s[2 * gi + 1][2 * rr + 1]));
         };
         float top[RR];
-        bool grew = false;
+        bool grew = steep;
 #pragma unroll
         for (int rr = 0; rr < RR; ++rr) {
             top[rr] = -INFINITY;
@@ -508,6 +512,21 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
                         o[j][2] *= f;
                         o[j][3] *= f;
                     }
+                }
+            }
+            bool far = false;
+#pragma unroll
+            for (int rr = 0; rr < RR; ++rr) far |= fabsf(m[rr]) > STEEP && fabsf(m[rr]) < INFINITY;
+            steep = __any_sync(0xFFFFFFFFu, far);
+            if (steep) {  // round the scores as the maximum was
+#pragma unroll
+                for (int gi = 0; gi < GR; ++gi) {
+#pragma unroll
+                    for (int e = 0; e < 2 * RR; ++e) {
+                        s[2 * gi][e] *= ks[gi];
+                        s[2 * gi + 1][e] *= ks[gi];
+                    }
+                    ks[gi] = 1.0f;
                 }
             }
         }
@@ -641,6 +660,7 @@ __global__ void __launch_bounds__(32 * NW, Shape<D, ROWS, NW>::RESIDENT) k_kv8_a
             e2[rr] = E_LEAST;
             pv[rr] = 0.0f;
         }
+        steep = false;
         if (SH::Q_SMEM) __syncthreads();
 #pragma unroll
         for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;

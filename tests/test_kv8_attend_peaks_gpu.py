@@ -13,7 +13,8 @@ import math
 
 import pytest
 
-from test_kv8_gpu import check_attention, make, values
+import gpt2_b200 as G
+from test_kv8_gpu import check_attention, values
 
 pytestmark = pytest.mark.gpu
 
@@ -24,10 +25,12 @@ def peaked(torch, lib, kind, rows, heads, group, Tq, dim, n, octaves, sink_v, bi
     values `factor` times the rest's, which are 0.5 to 1.5."""
     page = max(block, 32)
     lens = [n - 7 * (i % 5) for i in range(rows)]
-    cache = make(torch, lib, rows, heads, dim, page, block, kind, n, layers=1, seed=seed, q_heads=heads * group, queries=Tq)
-    g = torch.Generator().manual_seed(seed + 1)
-    k = (0.1 * torch.randn(rows, n, heads, dim, generator=g)).cuda()
-    v = (0.5 + torch.rand(rows, n, heads, dim, generator=g)).cuda()
+    most = -(-n // page)
+    cache = G.KV8Cache.create(lib, torch, rows, most, rows * most, 1, heads, dim, page, block, kind, heads * group, Tq)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cache.table.copy_(torch.randperm(rows * most, generator=g, device="cuda").view(rows, most))
+    k = 0.1 * torch.randn(rows, n, heads, dim, generator=g, device="cuda")
+    v = 0.5 + torch.rand(rows, n, heads, dim, generator=g, device="cuda")
     k[..., 0] = 0.0
     k[:, 5, :, 0] = octaves * math.log(2.0)
     v[:, 5 // block * block: 5 // block * block + block] *= sink_v
