@@ -46,6 +46,14 @@ typedef unsigned long long key_t;
 
 __host__ __device__ inline int max_chunks(int W) { return ROW_KEYS / W < MAX_CHUNKS ? ROW_KEYS / W : MAX_CHUNKS; }
 
+// A row's part of the work area, of one size for every call, so that no call's lists lie where another's counters are: calls of
+// any batch and width may share an area.
+struct __align__(16) Record {
+    key_t keys[ROW_KEYS];    // [chunks][W], sorted
+    float2 ml[MAX_CHUNKS];   // [chunks]
+    unsigned arrive, pad[3]; // the item's arrivals, in its first row's record; zero between calls
+};
+
 struct Params {
     int *token, *parent;
     float *new_score;
@@ -55,9 +63,7 @@ struct Params {
     const float *score;
     const int *done;
     int W, V, eos, chunks, steps;  // steps per warp of a CTA
-    key_t *keys;                   // [rows][chunks][W], sorted
-    float2 *ml;                    // [rows][chunks]
-    unsigned *arrive;              // [items]
+    Record *work;                  // [rows]
     unsigned *status;
 };
 
@@ -337,16 +343,16 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         if (lane < W) lists[0][warp * W + lane] = mine;
         if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.status, ST_BEAM_LOGIT);
         __syncthreads();
-        const long long at = row * p.chunks + ch;
+        Record *const rec = p.work + row;
         if (warp == 0) {
-            key_t *out = p.keys + at * W;
+            key_t *out = rec->keys + ch * W;
             const int n = merge_lists(lists[0], NWARP, W, [&](int j, key_t k, int) { out[j] = k; });
             if (lane >= n && lane < W) out[lane] = 0;
         } else if (warp == 1) {
             m = lane < NWARP ? red_m[lane] : -INFINITY;
             l = lane < NWARP ? red_l[lane] : 0.0f;
             warp_ml(m, l);
-            if (lane == 0) p.ml[at] = make_float2(m, l);
+            if (lane == 0) rec->ml[ch] = make_float2(m, l);
         }
     }
     // the last CTA of the item goes on
@@ -357,9 +363,10 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
     }
     __syncthreads();
     if (tid == 0) {
-        const unsigned seen = kv8::arrive_add(&p.arrive[item]);
+        unsigned *const arrive = &p.work[first_row].arrive;
+        const unsigned seen = kv8::arrive_add(arrive);
         is_last = seen == static_cast<unsigned>(W * p.chunks - 1);
-        if (is_last) p.arrive[item] = 0;
+        if (is_last) *arrive = 0;
     }
     __syncthreads();
     if (!is_last) return;
@@ -376,13 +383,13 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
             }
             continue;
         }
-        const long long at = static_cast<long long>(first_row + b) * p.chunks;
+        const Record *const rec = p.work + first_row + b;
         float m = -INFINITY, l = 0.0f;
         for (int i = lane; i < p.chunks; i += 32) {
-            const float2 z = __ldcg(&p.ml[at + i]);
+            const float2 z = __ldcg(&rec->ml[i]);
             merge_ml(m, l, z.x, z.y);
         }
-        for (int i = lane; i < p.chunks * W; i += 32) lists[warp][i] = __ldcg(&p.keys[at * W + i]);
+        for (int i = lane; i < p.chunks * W; i += 32) lists[warp][i] = __ldcg(&rec->keys[i]);
         warp_ml(m, l);
         __syncwarp();
         const float lse = m + logf(l);
@@ -411,19 +418,6 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         p.new_score[out] = -INFINITY;
         if (p.new_done) p.new_done[out] = 1;
     }
-}
-
-struct Layout {
-    size_t o_keys, o_ml, bytes;
-};
-static Layout layout(int B, int W) {
-    auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
-    const size_t rows = static_cast<size_t>(B) * W, ch = static_cast<size_t>(max_chunks(W));
-    Layout y;
-    y.o_keys = up(B * sizeof(unsigned));
-    y.o_ml = y.o_keys + up(rows * ch * W * sizeof(key_t));
-    y.bytes = y.o_ml + up(rows * ch * sizeof(float2));
-    return y;
 }
 
 template <typename T>
@@ -466,7 +460,7 @@ using namespace b200;
 
 extern "C" size_t gpt2_beam_work_bytes_b200(int B, int W) {
     if (B < 1 || W < 1 || W > beam::MAX_W) return 0;
-    return beam::layout(B, W).bytes;
+    return static_cast<size_t>(B) * W * sizeof(beam::Record);
 }
 
 extern "C" int gpt2_beam_select_b200(int *token, int *parent, float *new_score, int *new_done, const void *logits,
@@ -478,8 +472,7 @@ extern "C" int gpt2_beam_select_b200(int *token, int *parent, float *new_score, 
         (reinterpret_cast<uintptr_t>(logits) & (type == GPT2_BEAM_HALF ? 1 : 3)))
         return GPT2_B200_EINVAL;
     if (B == 0) return GPT2_B200_OK;
-    const beam::Layout y = beam::layout(B, W);
-    if (work_bytes < y.bytes) return GPT2_B200_EINVAL;
+    if (work_bytes < gpt2_beam_work_bytes_b200(B, W)) return GPT2_B200_EINVAL;
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_EDEVICE;
     beam::Params p;
@@ -494,9 +487,7 @@ extern "C" int gpt2_beam_select_b200(int *token, int *parent, float *new_score, 
     p.W = W;
     p.V = V;
     p.eos = eos;
-    p.arrive = static_cast<unsigned *>(work);
-    p.keys = reinterpret_cast<beam::key_t *>(static_cast<char *>(work) + y.o_keys);
-    p.ml = reinterpret_cast<float2 *>(static_cast<char *>(work) + y.o_ml);
+    p.work = static_cast<beam::Record *>(work);
     p.status = ctx->status;
     return type == GPT2_BEAM_HALF ? beam::launch<__half>(p, B, ctx->num_sms, &ctx->beam_attr_done[0], stream)
                                   : beam::launch<float>(p, B, ctx->num_sms, &ctx->beam_attr_done[1], stream);

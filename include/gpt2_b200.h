@@ -378,8 +378,9 @@ int gpt2_kv8_compact_b200(const GPT2KV8Cache *kv, int *d_live, cudaStream_t stre
  * higher logit, then the lower token. -inf logits are masked tokens; NaN and +inf set a status bit and count as masked. Outputs, best first: token,
  * parent (row index b*W + w, as gpt2_kv8_reorder_b200 takes it), new_score, new_done (NULL: not written) = finished
  * before, or token == eos (eos < 0: none). Where fewer than W candidates exist the rest is a dead beam: token max(eos, 0),
- * parent its own row, score -inf, done 1. new_score / new_done may be score / done. W 1..32. work: gpt2_beam_work_bytes_b200,
- * zeroed once by its owner; calls that share it must be ordered. */
+ * parent its own row, score -inf, done 1. new_score / new_done may be score / done. W 1..32. work: at least
+ * gpt2_beam_work_bytes_b200(B, W) bytes, zeroed once by their owner. One area serves calls of every B and W that it is large enough
+ * for; calls that share it must be ordered. */
 #define GPT2_BEAM_HALF 0
 #define GPT2_BEAM_FLOAT 1
 size_t gpt2_beam_work_bytes_b200(int B, int W);
