@@ -77,6 +77,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+__device__ __forceinline__ key_t key_of(float x, unsigned n) { return lin::argmax_key(x + 0.0f, n); }  // -0 as 0: they are equal
 __device__ __forceinline__ float key_value(key_t k) {
     const unsigned o = static_cast<unsigned>(k >> 32);
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
                 key_t k = 0;
                 if (lane < NV) {
                     const float y = static_cast<float>(*reinterpret_cast<const T *>(ring + s % STAGES * STAGE_BYTES + cut + at * sizeof(T)));
-                    if (y >= thr && y > -INFINITY && y < INFINITY) k = lin::argmax_key(y, begin + s * (NWARP * STEP) + at);
+                    if (y >= thr && y > -INFINITY && y < INFINITY) k = key_of(y, begin + s * (NWARP * STEP) + at);
                 }
 #pragma unroll 1
                 for (unsigned todo = __ballot_sync(0xFFFFFFFFu, k > worst); todo; todo &= todo - 1) {
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         if (!(sc > -INFINITY)) continue;
         if (s_done[b]) {
             if (lane == 0) {
-                totals[b * W] = lin::argmax_key(sc, static_cast<unsigned>(b * W));
+                totals[b * W] = key_of(sc, static_cast<unsigned>(b * W));
                 tokens[b * W] = max(p.eos, 0);
             }
             continue;
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(NT) k_beam_select(const Params p) {
         __syncwarp();
         const float lse = m + logf(l);
         auto candidate = [&](int j, key_t k, int) {
-            totals[b * W + j] = lin::argmax_key(sc + (key_value(k) - lse), static_cast<unsigned>(b * W + j));
+            totals[b * W + j] = key_of(sc + (key_value(k) - lse), static_cast<unsigned>(b * W + j));
             tokens[b * W + j] = lin::argmax_key_index(k);
         };
         if (p.chunks > 1) merge_lists(lists[warp], p.chunks, W, candidate);
