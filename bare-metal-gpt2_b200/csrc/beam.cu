@@ -6,7 +6,7 @@
 //   projection, LayerNorm; head with logits; selection; bookkeeping; reorder of the pages
 // While a prompt lasts its item decodes in row b*W alone (the other rows are kept empty); its last token's
 // selection forks that row's pages into W beams, which hold the whole pages of the prompt in common from then on. The
-// step is captured in one CUDA graph and replayed. Tokens and parents of every step are kept, and the
+// step is captured in one CUDA graph and replayed, up to the last one, which is launched by itself: it makes no room behind it. Tokens and parents of every step are kept, and the
 // hypotheses are read back from their ends.
 #include <algorithm>
 #include <new>
@@ -89,7 +89,8 @@ __global__ void k_beam_trace(int *out, long long out_stride, float *out_score, c
     if (out_score) out_score[r] = score[r];
 }
 
-int enqueue(gpt2_b200_beam *bm, const int *prompt, long long ps, const int *plen, int eos, cudaStream_t st) {
+// One step; reserve: the positions to make room for behind it.
+int enqueue(gpt2_b200_beam *bm, const int *prompt, long long ps, const int *plen, int eos, int reserve, cudaStream_t st) {
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_ECUDA;
     const GPT2WeightsGPU &w = bm->w;
@@ -114,7 +115,7 @@ int enqueue(gpt2_b200_beam *bm, const int *prompt, long long ps, const int *plen
         (rc = launch(k_beam_advance, 1, 256, st, false, bm->tok, bm->parent, bm->score, bm->done, bm->sel_tok, bm->sel_parent, bm->sel_score,
                      bm->sel_done, bm->hist, bm->step, prompt, ps, plen, rows, bm->W)))
         return rc;
-    return gpt2_kv8_reorder_b200(kv, bm->parent, 1, 1, st);
+    return gpt2_kv8_reorder_b200(kv, bm->parent, 1, reserve, st);
 }
 
 int beam_init(gpt2_b200_beam *bm, const GPT2WeightsGPU *w, const GPT2KV8Cache *kv, int B, int W) {
@@ -246,7 +247,7 @@ int gpt2_b200_beam_generate(gpt2_b200_beam *bm, const int *d_prompt, long long p
         if (cudaStreamBeginCapture(cs, cudaStreamCaptureModeThreadLocal) != cudaSuccess) {
             rc = GPT2_B200_ECUDA;
         } else {
-            rc = enqueue(bm, d_prompt, prompt_stride, d_plen, eos, cs);
+            rc = enqueue(bm, d_prompt, prompt_stride, d_plen, eos, 1, cs);
             if (cudaStreamEndCapture(cs, &g) != cudaSuccess && rc == GPT2_B200_OK) rc = GPT2_B200_ECUDA;
         }
         if (rc == GPT2_B200_OK && cudaGraphInstantiate(&bm->graph, g, 0) != cudaSuccess) rc = GPT2_B200_ECUDA;
@@ -261,8 +262,10 @@ int gpt2_b200_beam_generate(gpt2_b200_beam *bm, const int *d_prompt, long long p
     if ((rc = gpt2_kv8_reset_b200(&bm->kv, stream)) || (rc = gpt2_kv8_reorder_b200(&bm->kv, nullptr, 0, 1, stream))) return rc;
     k_beam_init<<<blocks, 128, 0, stream>>>(bm->tok, bm->score, bm->done, bm->step, d_prompt, prompt_stride, bm->rows, bm->W);
     if (cudaGetLastError() != cudaSuccess) return GPT2_B200_ECUDA;
-    for (int s = 0; s < n_steps; ++s)
+    for (int s = 1; s < n_steps; ++s)
         if (cudaGraphLaunch(bm->graph, stream) != cudaSuccess) return GPT2_B200_ECUDA;
+    // The last step leaves no room behind it, for which table and pool need not have pages.
+    if ((rc = enqueue(bm, d_prompt, prompt_stride, d_plen, eos, 0, stream))) return rc;
     k_beam_trace<<<blocks, 128, 0, stream>>>(d_out, out_stride, d_score, bm->score, bm->hist, d_prompt, prompt_stride, n_steps, bm->rows,
                                             bm->W);
     return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
