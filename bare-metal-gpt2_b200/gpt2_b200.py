@@ -231,15 +231,16 @@ class Lib:
         """The W best continuations of each of B items' W beams: logits [B*W][V] fp16 or fp32 (rows may be
         strided), score fp32 [B*W], done int32 [B*W] or None; writes token and parent (int32), new_score
         and new_done (may be score and done; new_done may be None)."""
-        kind = _beam_types().get(logits.dtype)
-        rows, near = logits.stride()
-        if kind is None or near != 1:
-            raise ValueError("beam_select: logits are fp16 or fp32 rows of neighbouring values")
+        i32, f32, kinds, u8 = _types()
+        kind, strides, shape, n = kinds.get(logits.dtype), logits.stride(), logits.shape, B * W
+        if kind is None or len(strides) != 2 or strides[1] != 1 or shape[0] != n:
+            raise ValueError("beam_select: logits are fp16 or fp32, B * W rows of neighbouring values")
+        at, what = logits.device, "beam_select"
         rc = self._beam_select(
-            token.data_ptr(), parent.data_ptr(), new_score.data_ptr(),
-            new_done.data_ptr() if new_done is not None else None, logits.data_ptr(), kind, rows,
-            score.data_ptr(), done.data_ptr() if done is not None else None, B, W, logits.shape[1], eos,
-            work.data_ptr(), work.numel(), stream)
+            _vector(what, token, i32, n, at), _vector(what, parent, i32, n, at), _vector(what, new_score, f32, n, at),
+            _vector(what, new_done, i32, n, at) if new_done is not None else None, logits.data_ptr(), kind, strides[0],
+            _vector(what, score, f32, n, at), _vector(what, done, i32, n, at) if done is not None else None,
+            B, W, shape[1], eos, _vector(what, work, u8, work.numel(), at), work.numel(), stream)
         if rc:
             self.check(rc, "gpt2_beam_select_b200")
 
@@ -279,8 +280,9 @@ class KV8Cache:
                   and tuple(length.shape) == (table.shape[0],))
         types = (data.dtype == torch.uint8 and scale.dtype == torch.float32
                  and ref.dtype == table.dtype == length.dtype == torch.int32)
-        if not shapes or not types or not all(t.is_contiguous() for t in (data, scale, ref, table, length)):
-            raise ValueError("KV8Cache: data, scale, ref, table or length has another shape, type or layout")
+        if not shapes or not types or not all(t.is_contiguous() and t.device == data.device
+                                              for t in (data, scale, ref, table, length)):
+            raise ValueError("KV8Cache: data, scale, ref, table or length has another shape, type, layout or device")
         self.data, self.scale, self.ref, self.table, self.length = data, scale, ref, table, length
         c = GPT2KV8Cache()
         c.data, c.scale, c.ref = data.data_ptr(), scale.data_ptr(), ref.data_ptr()
@@ -296,6 +298,7 @@ class KV8Cache:
         self.c, self.ref_c = c, ctypes.byref(c)
         # what every call needs, looked up once: a decoding step makes dozens of calls
         self._nrow, self._dim, self._width, self._half = int(c.nRow), dim, n_head * dim, torch.float16
+        self._at, self._int = data.device, torch.int32
         self._store, self._load = lib.lib.gpt2_kv8_store_b200, lib.lib.gpt2_kv8_load_b200
         self._attend, self._reorder = lib.lib.gpt2_kv8_attend_b200, lib.lib.gpt2_kv8_reorder_b200
         self._compact = lib.lib.gpt2_kv8_compact_b200
@@ -315,16 +318,27 @@ class KV8Cache:
         """The three outer strides of k and v and their tokens, after a check of their form."""
         s, shape = k.stride(), k.shape
         if s != v.stride() or shape != v.shape or len(s) != 4 or s[3] != 1 or shape[1] != self._nrow or \
-                shape[3] != self._width or k.dtype != self._half or v.dtype != self._half:
-            raise ValueError(f"{what}: k and v are fp16 [layers][rows][tokens][heads * dim], laid out alike")
+                shape[3] != self._width or k.dtype != self._half or v.dtype != self._half or \
+                k.device != self._at or v.device != self._at:
+            raise ValueError(f"{what}: k and v are fp16 [layers][rows][tokens][heads * dim], laid out alike, on the "
+                             "cache's device")
         return shape[0], s[0], s[1], s[2], shape[2]
+
+    def _per_row(self, what, t):
+        return _vector(what, t, self._int, self._nrow, self._at)
+
+    def _count(self, what, count):
+        """(int, device pointer or None) of a count given as an int, an int32 tensor or None."""
+        if count is None:
+            return 0, None
+        return (count, None) if isinstance(count, int) else (0, self._per_row(what, count))
 
     def store(self, k, v, layer: int = 0, count=None, stream: int = 0) -> None:
         """k, v: fp16 [layers][rows][tokens][heads * dim] (strided views are fine), written behind the
         held positions from `layer` on; count: int32 [rows] or None (all tokens)."""
         n, ls, rs, ts, tokens = self._rows("store", k, v)
         rc = self._store(self.ref_c, layer, n, k.data_ptr(), v.data_ptr(), ls, rs, ts,
-                         count.data_ptr() if count is not None else None, tokens, stream)
+                         self._per_row("store", count) if count is not None else None, tokens, stream)
         if rc:
             self.lib.check(rc, "gpt2_kv8_store_b200")
 
@@ -332,9 +346,9 @@ class KV8Cache:
         """The inverse: positions first[r].. (0 without first) as fp16 rows, 0 beyond the held ones;
         count: int32 [rows], an int or None: positions stored but not yet counted in."""
         n, ls, rs, ts, tokens = self._rows("load", k, v)
-        add, d_add = _count(count)
+        add, d_add = self._count("load", count)
         rc = self._load(self.ref_c, layer, n, k.data_ptr(), v.data_ptr(), ls, rs, ts,
-                        first.data_ptr() if first is not None else None, tokens, d_add, add, stream)
+                        self._per_row("load", first) if first is not None else None, tokens, d_add, add, stream)
         if rc:
             self.lib.check(rc, "gpt2_kv8_load_b200")
 
@@ -344,25 +358,28 @@ class KV8Cache:
         its keys, counted as load() counts them; keys before first[r] are masked."""
         qs, os_, shape = q.stride(), out.stride(), q.shape
         if shape != out.shape or len(qs) != 3 or shape[0] != self._nrow or qs[2] != 1 or os_[2] != 1 or \
-                shape[2] % self._dim or q.dtype != self._half or out.dtype != self._half:
-            raise ValueError("attend: q and out are fp16 [rows][queries][q heads * dim]")
-        add, d_add = _count(count)
+                shape[2] % self._dim or q.dtype != self._half or out.dtype != self._half or \
+                q.device != self._at or out.device != self._at:
+            raise ValueError("attend: q and out are fp16 [rows][queries][q heads * dim] on the cache's device")
+        add, d_add = self._count("attend", count)
         rc = self._attend(out.data_ptr(), os_[0], os_[1], q.data_ptr(), qs[0], qs[1], self.ref_c, layer,
-                          shape[2] // self._dim, shape[1], first.data_ptr() if first is not None else None,
-                          d_add, add, max_len, stream)
+                          shape[2] // self._dim, shape[1],
+                          self._per_row("attend", first) if first is not None else None, d_add, add, max_len, stream)
         if rc:
             self.lib.check(rc, "gpt2_kv8_attend_b200")
 
     def reorder(self, parent=None, advance: int = 0, reserve: int = 0, stream: int = 0) -> None:
         """Counts `advance` positions in, makes row r a copy of row parent[r] (int32 [rows]; -1: empty; None:
         itself) by sharing pages, and makes room for `reserve` more positions."""
-        rc = self._reorder(self.ref_c, parent.data_ptr() if parent is not None else None, advance, reserve, stream)
+        rc = self._reorder(self.ref_c, self._per_row("reorder", parent) if parent is not None else None, advance,
+                           reserve, stream)
         if rc:
             self.lib.check(rc, "gpt2_kv8_reorder_b200")
 
     def compact(self, live=None, stream: int = 0) -> None:
         """Moves the live pages to the lowest ids; live: int32 [1] for their number, or None."""
-        rc = self._compact(self.ref_c, live.data_ptr() if live is not None else None, stream)
+        rc = self._compact(self.ref_c, _vector("compact", live, self._int, 1, self._at) if live is not None else None,
+                           stream)
         if rc:
             self.lib.check(rc, "gpt2_kv8_compact_b200")
 
@@ -477,9 +494,16 @@ class BeamDecoder:
     def generate(self, prompt, prompt_len, n_steps: int, out, score=None, eos: int = -1, stream: int = 0) -> None:
         """prompt: int32 [B][P]; prompt_len: int32 [B] (1..P); out: int32 [B * W][>= n_steps+1], each item's
         hypotheses best first; score: fp32 [B * W] or None."""
+        i32, f32, _, _ = _types()
+        at, rows, what = self.cache.data.device, self.B * self.W, "generate"
+        for t, n in ((prompt, self.B), (out, rows)):
+            if t.dim() != 2 or t.dtype is not i32 or t.shape[0] != n or t.shape[1] < 1 or t.stride(1) != 1 or t.device != at:
+                raise ValueError("generate: prompt is int32 [B][P], out int32 [B * W][>= n_steps + 1], on the cache's device")
+        if out.shape[1] <= n_steps < out.stride(0):  # a view whose rows end early: the library sees the stride alone
+            raise ValueError("generate: out is too narrow")
         self.lib.check(self.lib.gpt2_b200_beam_generate(
-            self.h, prompt.data_ptr(), prompt.stride(0), prompt_len.data_ptr(), n_steps, eos, out.data_ptr(),
-            out.stride(0), score.data_ptr() if score is not None else None, stream), "gpt2_b200_beam_generate")
+            self.h, prompt.data_ptr(), prompt.stride(0), _vector(what, prompt_len, i32, self.B, at), n_steps, eos, out.data_ptr(),
+            out.stride(0), _vector(what, score, f32, rows, at) if score is not None else None, stream), "gpt2_b200_beam_generate")
 
     def close(self) -> None:
         """Destroys the decoder (the library synchronises the device first); safe to call twice."""
@@ -494,20 +518,22 @@ class BeamDecoder:
             pass
 
 
-def _count(count):
-    """(int, device pointer or None) of a count given as an int, an int32 tensor or None."""
-    if count is None:
-        return 0, None
-    return (count, None) if isinstance(count, int) else (0, count.data_ptr())
+def _vector(what, t, dtype, n, device):
+    """The address of t, which must hold n neighbouring elements of the type on the device."""
+    if t.dtype is not dtype or t.numel() != n or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expected {n} neighbouring {dtype} on the device of the other tensors, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
-_TYPES: dict = {}
+_TYPES: list = []
 
 
-def _beam_types() -> dict:
+def _types():
+    """torch.int32, torch.float32, and the types of logits."""
     if not _TYPES:
         import torch
-        _TYPES.update({torch.float16: BEAM_HALF, torch.float32: BEAM_FLOAT})
+        _TYPES.extend((torch.int32, torch.float32, {torch.float16: BEAM_HALF, torch.float32: BEAM_FLOAT}, torch.uint8))
     return _TYPES
 
 
