@@ -124,6 +124,10 @@ class _Caps(ctypes.Structure):
                 ("logits_all", ctypes.c_int)]
 
 
+class ReferenceMissing(FileNotFoundError):
+    """The reference's own code has not been built (its sources are not on this machine)."""
+
+
 class RefCPU:
     """The reference's own attention() (cpu/forward_cpu.c:83-116) and whole fp32 forward
     (gpt2_forward_cpu, cpu/forward_cpu.c:118), compiled from its source."""
@@ -131,7 +135,7 @@ class RefCPU:
     def __init__(self, path: str | None = None):
         path = path or os.path.join(REF_DIR, "libref_cpu.so")
         if not os.path.exists(path):
-            raise FileNotFoundError(f"{path} missing: run `make -C oracle ref`")
+            raise ReferenceMissing(f"{path} missing: run `make -C oracle ref`")
         lib = ctypes.CDLL(path)
         lib.ref_cpu_attention.argtypes = [_f32p, _f32p, ctypes.c_int]
         lib.ref_cpu_attention.restype = ctypes.c_int
@@ -177,7 +181,7 @@ class RefGPU:
     def __init__(self, path: str | None = None):
         path = path or os.path.join(REF_DIR, "libref_gpu.so")
         if not os.path.exists(path):
-            raise FileNotFoundError(f"{path} missing: run `make -C oracle ref`")
+            raise ReferenceMissing(f"{path} missing: run `make -C oracle ref`")
         lib = ctypes.CDLL(path)
         vp, ci = ctypes.c_void_p, ctypes.c_int
         for name, args in {
