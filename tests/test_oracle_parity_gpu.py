@@ -99,3 +99,42 @@ def test_decode_attn_step(cuda, lib, oracle, use_dev):
         want = oracle.decode(qkv[L, :O.E].astype(np.float32), k.view(np.float16).astype(np.float32), v.view(np.float16).astype(np.float32), pos + 1)
         assert_close(got[L], want, f"layer {L}")
     assert lib.status() == 0
+
+
+def plain_forward(torch, w, ids):
+    """GPT-2's logits after every token of ids [B][T], in fp32 from the same weights."""
+    t = {k: v.float() for k, v in w.t.items()}
+
+    def norm(x, g, b):
+        return (x - x.mean(-1, keepdim=True)) / torch.sqrt(x.var(-1, unbiased=False, keepdim=True) + 1e-5) * t[g] + t[b]
+
+    B, T = ids.shape
+    x = t["wte"][ids] + t["wpe"][:T]
+    ahead = torch.ones(T, T, dtype=torch.bool, device=x.device).triu(1)
+    for L in range(L_):
+        p = f"h{L}."
+        q, k, v = (norm(x, p + "ln1_g", p + "ln1_b") @ t[p + "qkv_w"].T + t[p + "qkv_b"]).view(B, T, 3, O.H, O.D).permute(2, 0, 3, 1, 4)
+        a = torch.softmax((q @ k.transpose(-1, -2) / O.D ** 0.5).masked_fill(ahead, -np.inf), -1) @ v
+        x = x + a.transpose(1, 2).reshape(B, T, -1) @ t[p + "attn_proj_w"].T + t[p + "attn_proj_b"]
+        h = norm(x, p + "ln2_g", p + "ln2_b") @ t[p + "fc_w"].T + t[p + "fc_b"]
+        h = 0.5 * h * (1 + torch.tanh(0.7978845608028654 * (h + 0.044715 * h ** 3)))
+        x = x + h @ t[p + "proj_w"].T + t[p + "proj_b"]
+    return norm(x, "lnf_g", "lnf_b") @ t["wte"].T
+
+
+@pytest.mark.parametrize("B", [1, 5, 40])
+def test_batched_decode_step(cuda, lib, B):
+    """Teacher-forced steps against a plain fp32 forward, within the bound for fp16 steps against an fp32 forward (tests/test_model_gpu.py: 5e-2)."""
+    torch = cuda
+    T = 9
+    w = G.ModelWeights(torch, "cuda", seed=7, hf_init=False)
+    ids = torch.from_numpy(np.random.default_rng(B).integers(0, G.VOCAB, (B, T))).cuda()
+    want = plain_forward(torch, w, ids)
+    caches = torch.zeros(B, L_, 2, O.H, 16, O.D, dtype=torch.float16, device="cuda")
+    batch = G.DecodeBatch(lib, w, caches)
+    logits = torch.empty(B, 50264, dtype=torch.float16, device="cuda")
+    for t in range(T):
+        batch.step(ids[:, t].int(), torch.full((B,), t, dtype=torch.int32, device="cuda"), logits)
+        torch.cuda.synchronize()
+        assert float((logits[:, :G.VOCAB].float() - want[:, t]).abs().max()) <= 5e-2, f"position {t}"
+    assert lib.status() == 0
