@@ -847,8 +847,6 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     if (!kv8::aligned(out) || !kv8::aligned(q) || (out_row_stride & 7) || (out_tok_stride & 7) || (q_row_stride & 7) ||
         (q_tok_stride & 7) || kv->work_bytes < w.bytes)
         return GPT2_B200_EINVAL;
-    DeviceContext *ctx = device_context();
-    if (!ctx) return GPT2_B200_EDEVICE;
     kv8::AttParams a;
     a.q = q;
     a.out = out;
@@ -873,7 +871,9 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     a.qtiles = static_cast<int>((R + rows - 1) / rows);
     const long long entries = static_cast<long long>(kv->nRow) * a.qtiles;
     const long long chunks = entries * kv->nHead * (a.max_len / ck + 2);  // at most
-    if (entries > 0x7FFFFFFFll) return GPT2_B200_EINVAL;
+    if (entries > 0x7FFFFFFFll || R > 0x7FFFFFFFll - rows) return GPT2_B200_EINVAL;
+    DeviceContext *ctx = device_context();
+    if (!ctx) return GPT2_B200_EDEVICE;
     // Plan. Units that fill the GPU have a CTA each: no prefix sum, no shared units. Groups of two rows (64 sequences x 12 heads
     // of 512 to 1023 keys: 23.0 us; four rows 30.3, two warps per row 24.2, equal pieces 30.9) as long as groups of four would
     // leave a third of the SMs' 12 warps empty, then of four (128 x 12 units of 640 to 700 keys: 15.0 us, of two 21.4; 256 x 12
