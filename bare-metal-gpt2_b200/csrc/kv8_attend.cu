@@ -34,7 +34,7 @@
 // Beams share their leading pages, and one query row of each fills an eighth of an MMA tile. With units in plenty and at most 4
 // query rows in each, a CTA so takes 2 or 4 neighbouring cache rows of a head (GROUP). It compares their table rows; the chunks
 // of the pages that all of them hold are read and converted once, for the query rows of all. The rows' own chunks follow, in
-// which the other rows' scores are masked. 32 items x 4 beams x 12 heads of 640 to 700 keys, 640 shared: 15.0 us, each row by
+// which the other rows' scores are masked. 32 items x 4 beams x 12 heads of 640 to 700 keys, 640 shared: 14.4 us, each row by
 // itself 29.0. Rows that share nothing gain a little from four warps to deal their chunks to (128 x 12 heads of 2048 to 4096 keys:
 // 128 us, by themselves 146).
 #include <algorithm>
@@ -173,7 +173,7 @@ struct Chunk {
 // of 128 dims or 16 rows take the registers, so q of 128 dims lies in shared memory instead (32 registers), and the warps'
 // rows are merged where the rings were or, in the middle of a piece, DH dims at a time in q's place.
 // 16 rows of 128 dims spill at 12 warps, so 8 (8 sequences x 8 heads of 16384 keys: 62.5 us, 12 warps 68.7; 55.5 since the merge
-// takes four dims per thread and the last CTA has the loads of all its rows in flight).
+// takes four dims per thread and the last CTA has the loads of all its rows in flight, 55.8 with e).
 template <int D, int ROWS, int NW>
 struct Shape {
     static constexpr int WARPS = D == 128 && ROWS == 16 ? 8 : 12;  // per SM
@@ -875,8 +875,8 @@ extern "C" int gpt2_kv8_attend_b200(gpt2_half *out, long long out_row_stride, lo
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_EDEVICE;
     // Plan. Units that fill the GPU have a CTA each: no prefix sum, no shared units. Groups of two rows (64 sequences x 12 heads
-    // of 512 to 1023 keys: 23.0 us; four rows 30.3, two warps per row 24.2, equal pieces 30.9) as long as groups of four would
-    // leave a third of the SMs' 12 warps empty, then of four (128 x 12 units of 640 to 700 keys: 15.0 us, of two 21.4; 256 x 12
+    // of 512 to 1023 keys: 23.3 us; four rows 30.3, two warps per row 24.2, equal pieces 30.9) as long as groups of four would
+    // leave a third of the SMs' 12 warps empty, then of four (128 x 12 units of 640 to 700 keys: 14.4 us, of two 21.4; 256 x 12
     // of 150 to 300: 31.4 against 35.1). Windows, whose rows need not start together, and more query rows: one or two
     // warps per row by the same rule (128 x 12 units of 640 to 700 keys: 28.8 us with one, 33.5 with two). Fewer units: equal
     // pieces, four warps per CTA, which merge their rows before a piece's partials go through the work area.

@@ -349,8 +349,9 @@ int gpt2_kv8_load_b200(const GPT2KV8Cache *kv, int L0, int nL, gpt2_half *k, gpt
 /* Attention over layer L: row r has n = len[r] + count_r keys (count_r as above: the tokens stored in this
  * step) and its Tq queries are its last positions n-Tq .. n-1; query i sees keys first_r .. n-Tq+i
  * (d_first NULL: from 0). out = softmax(q K^T / sqrt(headDim)) V, fp32 accumulation, one rounding; a query
- * that sees no key gives 0. Hq query heads, head h reads K/V head h / (Hq/nHead). q and out: head h at
- * h*headDim, row r at r*row_stride, query t at t*tok_stride (halves, multiples of 8). max_len bounds n (0 =
+ * that sees no key gives 0. (Inside, a probability times its value's scale has 22 bits, or 2^-34 of the row's largest
+ * where that is more.) Hq query heads, head h reads K/V head h / (Hq/nHead). q and out: head h at h*headDim, row r at
+ * r*row_stride, query t at t*tok_stride (halves, multiples of 8). max_len bounds n (0 =
  * the table's capacity) and sizes the split; a row with n outside 0..max_len sets a status bit and gives 0.
  * With many rows, the leading pages that rows 4 i .. 4 i + 3 (or 2 i, 2 i + 1) all hold are read once for them: keep an item's
  * beams together. Which pages are shared, and max_len, may change the last bit of a result; the same call twice does not. */
