@@ -28,6 +28,9 @@ enum StatusBits : unsigned {
     ST_KV8_NONFINITE = 1u << 17,           // 8-bit cache: a K/V value that is not finite was stored
     ST_KV8_BAD_PARENT = 1u << 18,          // 8-bit cache: a parent outside -1..nRow-1
     ST_BEAM_LOGIT = 1u << 19,              // beam selection: a NaN or +inf logit
+    ST_W4_NONFINITE = 1u << 20,            // 4-bit weights: a value that is not finite was quantised
+    ST_EDIT_BAD_INPUT = 1u << 21,          // logits edit: a length, prompt, count or mask row outside its bounds
+    ST_EDIT_NO_TOKEN = 1u << 22,           // logits edit: a row with nothing above -inf to choose
     ST_TEST_WAIT_TIMEOUT = 1u << 16,       // the wait-timeout self-test expired (expected)
 };
 
@@ -46,6 +49,7 @@ struct DeviceContext {
     bool decode_attr_done = false;
     bool beam_attr_done[2] = {false, false};  // beam selection over fp16, fp32 logits
     bool kv8_attr_done[32] = {};              // 8-bit cache attention, by kernel variant
+    bool edit_attr_done = false;              // logits edit
     int num_sms = 0;
     int device = 0;                 // CUDA device ordinal of this context
 };

@@ -36,6 +36,9 @@ ST_TEST_WAIT_TIMEOUT = 1 << 16
 ST_KV8_NONFINITE = 1 << 17
 ST_KV8_BAD_PARENT = 1 << 18
 ST_BEAM_LOGIT = 1 << 19
+ST_W4_NONFINITE = 1 << 20
+ST_EDIT_BAD_INPUT = 1 << 21
+ST_EDIT_NO_TOKEN = 1 << 22
 
 LINEAR_STORE, LINEAR_GELU, LINEAR_RESID = 0, 1, 2
 GEN_ATTENTION_ONLY = 1
@@ -87,6 +90,23 @@ class GPT2KV8Cache(ctypes.Structure):
                                     "block", "kind")]
 
 
+class GPT2W4(ctypes.Structure):
+    """A weight in 4 bits (include/gpt2_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scale", "least")] + [(n, ctypes.c_int) for n in ("N", "K", "group")]
+
+
+class GPT2LogitsEdit(ctypes.Structure):
+    """What gpt2_logits_edit_b200 does to each row (include/gpt2_b200.h)."""
+
+    _fields_ = [("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p),
+                ("history", ctypes.c_void_p), ("history_stride", ctypes.c_longlong), ("max_history", ctypes.c_int),
+                ("length", ctypes.c_void_p), ("prompt", ctypes.c_void_p), ("bias_token", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("bias_stride", ctypes.c_longlong), ("max_bias", ctypes.c_int),
+                ("n_bias", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_longlong),
+                ("mask_rows", ctypes.c_int), ("mask_row", ctypes.c_void_p)]
+
+
 class GPT2LayerGPU(ctypes.Structure):
     """Same layout as GPT2LayerGPU in the reference's cuda/kernels.cuh:19-23."""
 
@@ -112,6 +132,8 @@ _vp, _ci, _cll, _cu, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, cty
 _kvp = ctypes.POINTER(GPT2KVCache)
 _wp = ctypes.POINTER(GPT2WeightsGPU)
 _k8p = ctypes.POINTER(GPT2KV8Cache)
+_w4p = ctypes.POINTER(GPT2W4)
+_edp = ctypes.POINTER(GPT2LogitsEdit)
 _cs = ctypes.c_size_t
 _SIGS = {
     "gpt2_attention_b200": (None, [_vp, _vp, _ci, _ci, _ci, _ci]),
@@ -160,6 +182,10 @@ _SIGS = {
     "gpt2_b200_beam_create": (_ci, [ctypes.POINTER(_vp), _wp, _k8p, _ci, _ci]),
     "gpt2_b200_beam_destroy": (None, [_vp]),
     "gpt2_b200_beam_generate": (_ci, [_vp, _vp, _cll, _vp, _ci, _ci, _vp, _cll, _vp, _vp]),
+    "gpt2_w4_quantize_b200": (_ci, [_w4p, _vp, _cll, _vp]),
+    "gpt2_w4_dequantize_b200": (_ci, [_vp, _cll, _w4p, _vp]),
+    "gpt2_w4_linear_b200": (_ci, [_vp, _cll, _vp, _cll, _w4p, _vp, _vp, _cll, _ci, _ci, _vp]),
+    "gpt2_logits_edit_b200": (_ci, [_vp, _cll, _vp, _cll, _ci, _ci, _ci, _edp, _vp, _vp]),
     "gpt2_b200_compose_backend": (None, [ctypes.POINTER(GPT2Backend), ctypes.POINTER(GPT2Backend)]),
     "gpt2_b200_reserve": (_ci, [_ci, _ci, _ci]),
     "gpt2_b200_status": (_cu, [_ci]),
@@ -388,6 +414,152 @@ class KV8Cache:
         self.lib.check(self.lib.gpt2_kv8_reset_b200(self.ref_c, stream), "gpt2_kv8_reset_b200")
 
 
+class W4Weight:
+    """A weight [N][K] in 4 bits over torch tensors (GPT2W4 and the gpt2_w4_* entry points).
+
+    codes uint8 [N][K/2], scale fp16 [K/group][N], least fp16 [K/group][N] or None; the tensors stay alive with the
+    weight. create() makes an empty one, pack() one from an fp16 weight.
+    """
+
+    def __init__(self, lib: "Lib", torch, codes, scale, least=None):
+        tensors = [t for t in (codes, scale, least) if t is not None]
+        if codes.dim() != 2 or scale.dim() != 2 or (least is not None and least.shape != scale.shape) or codes.dtype != torch.uint8 or \
+                any(t.dtype != torch.float16 for t in tensors[1:]) or not all(t.is_contiguous() and t.device == codes.device for t in tensors):
+            raise ValueError("W4Weight: codes are uint8 [N][K/2], scale and least fp16 [K/group][N], contiguous on one device")
+        N, K = codes.shape[0], 2 * codes.shape[1]
+        group = K // max(1, scale.shape[0])
+        if group not in (32, 64, 128) or K % group or scale.shape != (K // group, N) or N < 1:
+            raise ValueError("W4Weight: groups of 32, 64 or 128 neighbouring k, one scale per group and row")
+        self.lib, self.N, self.K, self.group = lib, N, K, group
+        self.codes, self.scale, self.least = codes, scale, least
+        c = GPT2W4()
+        c.codes, c.scale, c.least = codes.data_ptr(), scale.data_ptr(), least.data_ptr() if least is not None else None
+        c.N, c.K, c.group = N, K, group
+        self.c, self.ref_c = c, ctypes.byref(c)
+        self._at, self._half, self._current = codes.device, torch.float16, _current(torch, codes.device)
+        self._linear = lib.lib.gpt2_w4_linear_b200
+
+    @classmethod
+    def create(cls, lib: "Lib", torch, N: int, K: int, group: int = 64, least: bool = False, device="cuda") -> "W4Weight":
+        """An empty weight; least: the form with a smallest value per group."""
+        if group not in (32, 64, 128) or K < 1 or K % group:
+            raise ValueError("W4Weight: K is a multiple of the group, which is 32, 64 or 128")
+        at = dict(device=device, dtype=torch.float16)
+        return cls(lib, torch, torch.zeros(N, K // 2, device=device, dtype=torch.uint8), torch.zeros(K // group, N, **at),
+                   torch.zeros(K // group, N, **at) if least else None)
+
+    @classmethod
+    def pack(cls, lib: "Lib", torch, w, group: int = 64, least: bool = False, stream: int = 0) -> "W4Weight":
+        """The fp16 weight w [N][K] in 4 bits."""
+        q = cls.create(lib, torch, w.shape[0], w.shape[1], group, least, w.device)
+        q.quantize(w, stream)
+        return q
+
+    def _matrix(self, what, w):
+        if w.dtype != self._half or w.dim() != 2 or w.shape != (self.N, self.K) or w.stride(1) != 1 or w.device != self._at:
+            raise ValueError(f"{what}: expected fp16 [{self.N}][{self.K}] on the weight's device")
+        self._current(what)
+        return w.data_ptr(), w.stride(0) if self.N > 1 else max(w.stride(0), self.K)
+
+    def quantize(self, w, stream: int = 0) -> None:
+        """Writes the codes, scales and least values of the fp16 weight w [N][K]."""
+        p, ld = self._matrix("quantize", w)
+        self.lib.check(self.lib.gpt2_w4_quantize_b200(self.ref_c, p, ld, stream), "gpt2_w4_quantize_b200")
+
+    def dequantize(self, w, stream: int = 0) -> None:
+        """Writes the fp16 values that the codes stand for to w [N][K]."""
+        p, ld = self._matrix("dequantize", w)
+        self.lib.check(self.lib.gpt2_w4_dequantize_b200(p, ld, self.ref_c, stream), "gpt2_w4_dequantize_b200")
+
+    def linear(self, out, x, bias=None, epi: int = LINEAR_STORE, residual=None, stream: int = 0) -> None:
+        """out [B][N] = e(x [B][K] W^T + bias [N]), fp16 rows (strided ones are fine); epi LINEAR_RESID adds residual [B][N]
+        (None: what out holds)."""
+        shape, os_, xs, half, at = out.shape, out.stride(), x.stride(), self._half, self._at
+        B = shape[0] if len(shape) == 2 else 0
+        if B < 1 or shape[1] != self.N or x.shape != (B, self.K) or xs[1] != 1 or os_[1] != 1 or x.dtype is not half or \
+                out.dtype is not half or x.device != at or out.device != at:
+            raise ValueError("linear: out is fp16 [B][N] and x fp16 [B][K] on the weight's device")
+        rp, rs = None, 0
+        if epi == LINEAR_RESID:
+            r = out if residual is None else residual
+            rs = r.stride()
+            if r.shape != shape or rs[1] != 1 or r.dtype is not half or r.device != at:
+                raise ValueError("linear: residual is fp16 [B][N] on the weight's device")
+            rp, rs = r.data_ptr(), rs[0] if B > 1 else self.N
+        self._current("linear")
+        rc = self._linear(out.data_ptr(), os_[0] if B > 1 else self.N, x.data_ptr(), xs[0] if B > 1 else self.K, self.ref_c,
+                          _vector("linear", bias, half, self.N, at) if bias is not None else None, rp, rs, B, epi, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_w4_linear_b200")
+
+
+class LogitsEdit:
+    """Penalties, biases and masks of a batch of rows (GPT2LogitsEdit and gpt2_logits_edit_b200), over tensors that the
+    program fills and changes between calls; they stay alive with the edit.
+
+    repetition, frequency, presence fp32 [rows] or None; history int32 [rows][most] (its first length[r] tokens count, all without
+    length; the first prompt[r] of them are the prompt); bias_token int32 and bias fp32 [rows][most] (n_bias int32 [rows] of them, or
+    all); mask int32 [mask rows][>= ceil(vocab / 32)], bit t % 32 of word t / 32 set where t is allowed; mask_row int32
+    [rows] names each row's (-1: none), by default its own, or the only one.
+    """
+
+    def __init__(self, lib: "Lib", torch, rows: int, vocab: int, repetition=None, frequency=None, presence=None, history=None, length=None,
+                 prompt=None, bias_token=None, bias=None, n_bias=None, mask=None, mask_row=None):
+        tensors = (repetition, frequency, presence, history, length, prompt, bias_token, bias, n_bias, mask, mask_row)
+        some = [t for t in tensors if t is not None]
+        self.lib, self.rows, self.vocab, self.tensors = lib, rows, vocab, tensors
+        self._at = some[0].device if some else None
+        i32, f32, self._kinds, _ = _types()
+        e = GPT2LogitsEdit()
+        for name, t, kind in (("repetition", repetition, f32), ("frequency", frequency, f32), ("presence", presence, f32), ("length", length, i32),
+                              ("prompt", prompt, i32), ("n_bias", n_bias, i32), ("mask_row", mask_row, i32)):
+            if t is not None:
+                setattr(e, name, _vector("LogitsEdit", t, kind, rows, self._at))
+
+        def table(name, t, kind, n):
+            if t.dim() != 2 or t.dtype is not kind or t.shape[0] != n or t.device != self._at or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError(f"LogitsEdit: {name} is {kind} with {n} rows of neighbouring values on the others' device")
+            return t.data_ptr(), (t.stride(0) if t.stride(0) >= t.shape[1] or t.stride(0) == 0 else t.shape[1]), t.shape[1]
+
+        if history is not None:
+            e.history, e.history_stride, e.max_history = table("history", history, i32, rows)
+        elif length is not None or prompt is not None:
+            raise ValueError("LogitsEdit: length and prompt belong to a history")
+        if (bias is None) != (bias_token is None) or (bias is None and n_bias is not None):
+            raise ValueError("LogitsEdit: bias_token, bias and n_bias belong together")
+        if bias is not None:
+            if bias.shape != bias_token.shape or bias.stride() != bias_token.stride():
+                raise ValueError("LogitsEdit: bias_token and bias are laid out alike")
+            e.bias_token, e.bias_stride, e.max_bias = table("bias_token", bias_token, i32, rows)
+            e.bias = table("bias", bias, f32, rows)[0]
+        if mask is not None:
+            n = mask.shape[0]
+            e.mask, e.mask_stride, words = table("mask", mask, i32, n)
+            if words < (vocab + 31) // 32 or (mask_row is None and n not in (1, rows)):
+                raise ValueError("LogitsEdit: a mask has a bit for each token, and one row, as many as the edit, or mask_row")
+            e.mask_rows, e.mask_stride = n, max(e.mask_stride, words)
+        elif mask_row is not None:
+            raise ValueError("LogitsEdit: mask_row belongs to a mask")
+        self.c, self.ref_c = e, ctypes.byref(e)
+        self._current = _current(torch, self._at) if some else None
+        self._edit = lib.lib.gpt2_logits_edit_b200
+
+    def apply(self, out, logits, next_tokens=None, stream: int = 0) -> None:
+        """out [rows][vocab] = the edited logits (fp16 or fp32 rows, strided ones are fine; out may be logits); next_tokens int32
+        [rows]: each row's largest, or None."""
+        kind, shape, os_, ls, at = self._kinds.get(logits.dtype), logits.shape, out.stride(), logits.stride(), logits.device
+        rows, vocab = self.rows, self.vocab
+        if kind is None or out.dtype is not logits.dtype or len(shape) != 2 or shape[0] != rows or shape[1] != vocab or out.shape != shape or \
+                (vocab > 1 and (ls[1] != 1 or os_[1] != 1)) or out.device != at or (self._at is not None and at != self._at):
+            raise ValueError("apply: logits and out are fp16 or fp32 [rows][vocab] of one type, on the edit's device")
+        if self._current is not None:
+            self._current("apply")
+        rc = self._edit(out.data_ptr(), os_[0] if rows > 1 else vocab, logits.data_ptr(), ls[0] if rows > 1 else vocab, kind, rows, vocab, self.ref_c,
+                        _vector("apply", next_tokens, _types()[0], rows, at) if next_tokens is not None else None, stream)
+        if rc:
+            self.lib.check(rc, "gpt2_logits_edit_b200")
+
+
 class ModelWeights:
     """Seeded random GPT-2-124M fp16 weights in one device buffer, described by a GPT2WeightsGPU.
 
@@ -516,6 +688,18 @@ class BeamDecoder:
             self.close()
         except Exception:  # noqa: BLE001 - interpreter shutdown
             pass
+
+
+def _current(torch, device):
+    """A check that the calling thread's current device is `device`: the library launches there."""
+    get, index = torch.cuda.current_device, device.index
+    if device.type != "cuda":
+        return lambda what: None
+
+    def check(what):
+        if get() != index:
+            raise ValueError(f"{what}: the tensors are on {device}, the current device is cuda:{get()}")
+    return check
 
 
 def _vector(what, t, dtype, n, device):

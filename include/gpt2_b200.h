@@ -404,6 +404,71 @@ void gpt2_b200_beam_destroy(gpt2_b200_beam *bm);
 int gpt2_b200_beam_generate(gpt2_b200_beam *bm, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps,
                             int eos, int *d_out, long long out_stride, float *d_score, cudaStream_t stream);
 
+/* ================================================================ 4-bit weights
+ * Additive extension (the reference's own quantised slots, matmul_q and gemv_q of cuda/kernels.cuh:80-85, take 8-bit weights of
+ * another form). A weight [N][K] in 4 bits, all arrays on the device and the caller's:
+ *   codes : [N][K/2] bytes, 16-byte aligned. Of the 8 elements of a 32-bit word, element 2 i lies in bits 4 i .. 4 i + 3 and
+ *           element 2 i + 1 in bits 16 + 4 i .. 16 + 4 i + 3;
+ *   scale : [K/group][N], one per `group` (32, 64 or 128) neighbouring k of a row;
+ *   least : [K/group][N], or NULL.
+ * A code c of 0..15 stands for fp16(c * scale + least), without least for fp16((c - 8) * scale), rounded once. K is a multiple of
+ * group, at most 2^24. No call allocates, synchronises or keeps anything of its arguments, so all may be captured. */
+typedef struct {
+    void *codes;
+    gpt2_half *scale, *least;
+    int N, K, group;
+} GPT2W4;
+
+/* Writes codes, scale and least (if not NULL) for the fp16 weight W (row n at W + n*ldw, 16-byte aligned, ldw a multiple of 8). With least:
+ * l = min of the group, s = (max - min) / 15 rounded down to fp16, c = (x - l) * (1 / s) to the nearest, ties to even. Without: s = max|x| / 7
+ * rounded down, c = 8 + x * (1 / s) to the nearest, 1..15. s = 0 gives code 0, or 8. NaN counts as 0, infinities as the largest
+ * fp16 (status bit). Arithmetic in fp32. */
+int gpt2_w4_quantize_b200(const GPT2W4 *w, const gpt2_half *W, long long ldw, cudaStream_t stream);
+/* The fp16 values that the codes stand for, to rows of the same kind. */
+int gpt2_w4_dequantize_b200(gpt2_half *W, long long ldw, const GPT2W4 *w, cudaStream_t stream);
+
+/* gpt2_b200_linear with a 4-bit weight: C[b, n] = e(sum_k A[b, k] * value(n, k) + bias[n]) for b < B (1..256), sums in fp32, e and one
+ * rounding to fp16 behind them: GPT2_B200_LINEAR_STORE the sum, _GELU gelu_new of it, _RESID R[b, n] + the sum (R: rows of stride
+ * ldr >= N, may be C itself; not read otherwise, may be NULL). bias may be NULL. A 16-byte aligned, lda a multiple of 8, ldc >= N;
+ * C must not overlap A. */
+int gpt2_w4_linear_b200(gpt2_half *C, long long ldc, const gpt2_half *A, long long lda, const GPT2W4 *w, const gpt2_half *bias,
+                        const gpt2_half *R, long long ldr, int B, int epi, cudaStream_t stream);
+
+/* ================================================================ logits on their way to a choice
+ * Penalties for repeated tokens, biases and grammar masks, and the greedy choice, in one pass. All pointers are device pointers
+ * and may be NULL where said. Of row r's history the first n = length[r] (NULL: max_history) tokens count, the first prompt[r] (NULL: 0)
+ * of them being the prompt. A token t (a token outside 0..V-1 is passed over) with logit x becomes, in fp32 and this order,
+ *   x > 0 ? x / repetition[r] : x * repetition[r]    where t is among the n tokens             (repetition NULL: no change)
+ *   x - frequency[r] * c - presence[r]               where t is c > 0 times among those behind the prompt (NULL: 0)
+ *   x + the sum of bias[r][i] over bias_token[r][i] = t, i < n_bias[r] (NULL: max_bias), in order of i
+ *   -inf                                             where the mask's bit of t is 0: bit t % 32 of word t / 32
+ * and is rounded once. NaN stays NaN but for masked ones. mask: [mask_rows][mask_stride] words; row r takes row mask_row[r] of it (-1: no
+ * mask; mask_row NULL: row r, or the one row there is if mask_rows is 1). Lengths outside 0..max_history, prompts outside 0..n, counts
+ * outside 0..max_bias are clamped, a mask row outside -1..mask_rows-1 counts as -1 (status bit). */
+typedef struct {
+    const float *repetition, *frequency, *presence; /* [rows] */
+    const int *history;                             /* [rows][history_stride], NULL: none */
+    long long history_stride;
+    int max_history; /* 0..2^20 - 1 */
+    const int *length, *prompt; /* [rows] */
+    const int *bias_token;      /* [rows][bias_stride], NULL: none */
+    const float *bias;
+    long long bias_stride; /* 0: the same list for all rows; likewise history_stride */
+    int max_bias;          /* 0..1024 */
+    const int *n_bias;     /* [rows] */
+    const unsigned *mask;  /* NULL: none */
+    long long mask_stride; /* words, >= ceil(V / 32) */
+    int mask_rows;
+    const int *mask_row; /* [rows] */
+} GPT2LogitsEdit;
+
+/* out[r] = the edited logits[r], r < rows: rows of V values, type GPT2_BEAM_HALF or GPT2_BEAM_FLOAT, at strides ldo and ld >= V
+ * (elements; any alignment). out may be logits itself with ldo = ld (then only what changes is written, and without d_next only that is
+ * read); otherwise the two must not overlap. d_next (if not NULL): the token of the largest written value of each row, the lowest of equal ones; NaN
+ * is never chosen, and a row that has nothing above -inf gives -1 (status bit). */
+int gpt2_logits_edit_b200(void *out, long long ldo, const void *logits, long long ld, int type, int rows, int V, const GPT2LogitsEdit *edit,
+                          int *d_next, cudaStream_t stream);
+
 /* ================================================================ backend, status, set-up */
 
 /* Composes a backend the reference's way (cuda/kernels_fused.cu:157-164): copies *base and installs
