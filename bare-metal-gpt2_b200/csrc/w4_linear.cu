@@ -1,6 +1,7 @@
 // w4_linear.cu — products with 4-bit weights: C[b, n] = e(sum_k x[b, k] * value(n, k) + bias[n]) for the B rows of a
 // decoding step (the format and the values: w4.cuh).
 #include <algorithm>
+#include <type_traits>
 
 #include "w4.cuh"
 
@@ -20,11 +21,19 @@ __device__ __forceinline__ float gelu_new(float v) {
     return __fdividef(v, 1.0f + __expf(-2.0f * u));
 }
 
+// What an output needs beside its sum.
+struct Extra {
+    float bias, resid;
+};
+__device__ __forceinline__ Extra extra_of(const Dest &d, int b, int n) {
+    return {d.bias ? __half2float(d.bias[n]) : 0.0f, d.epi == EPI_RESID ? __half2float(d.resid[b * d.ldr + n]) : 0.0f};
+}
+
 // One output of row b and feature n, both in range; acc holds the whole sum.
-__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc) {
-    if (d.bias) acc += __half2float(d.bias[n]);
+__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc, const Extra &e) {
+    acc += e.bias;
     if (d.epi == EPI_GELU) acc = gelu_new(acc);
-    if (d.epi == EPI_RESID) acc += __half2float(d.resid[b * d.ldr + n]);
+    if (d.epi == EPI_RESID) acc += e.resid;
     const __half h = __float2half_rn(acc);
     if (d.out) d.out[b * d.ldo + n] = h;
     if (d.epi == EPI_QKV && n >= d.E) {
@@ -39,66 +48,211 @@ __device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc) {
     }
     return h;
 }
+__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc) { return put(d, b, n, acc, extra_of(d, b, n)); }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---------------------------------------------------------------- simple form: a warp per 16 features and 8 rows
-// Lane (g, t) = (lane / 4, lane % 4) takes the 16 bytes of codes of features g and g + 8 at 32 neighbouring k; the matrix
-// instructions sum over k in any order, so 4 of a lane's k serve as its share of each 16.
-constexpr int CHUNK = 128;  // k per warp and step: 4 lanes x 32
+// ---------------------------------------------------------------- few rows
+// B <= 16: bound by reading the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
+// feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA, TMEM and
+// their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
+//   - A step is 16 features x 128 k: lane (g, t) = (lane / 4, lane % 4) holds 32 neighbouring k, 16 bytes, of features g and g + 8.
+//     The sum over k may be taken in any order, so 4 of a lane's k serve as its share of each instruction's 16.
+//   - A CTA's 8 warps are WR rows of 16 features x WK = 8 / WR pieces of k, whose sums are added through shared memory in their order. CTAs
+//     stay and take tile after tile: x is there, and the next tile's codes are on their way while a tile's sums are put together.
+constexpr int CHUNK = 128;
+constexpr int ROW_WARPS = 8;
+constexpr int DEPTH = 4;
+constexpr int ROW_CTAS = 2;  // per SM
+constexpr int ROWS_MAX_B = 16;
+constexpr int PANEL_BYTES = 88 * 1024;  // of x in shared memory
 
-template <bool LEAST>
-__global__ void __launch_bounds__(32) k_w4_simple(const uint8_t *codes, const __half *scale, const __half *least, int K, int group, const __half *x, long long ldx,
-                                                  const Dest d) {
-    const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16, b0 = blockIdx.y * 8;
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    grid_dependency_wait();
-    for (int k0 = 0; k0 < K; k0 += CHUNK) {
-        const int k = k0 + 32 * t;
-        uint4 q[2] = {};
-        __half2 s[2] = {}, l[2] = {};
+struct RowParams {
+    const uint8_t *codes;
+    const __half *scale, *least;
+    int K, shift;  // log2 of the group
+    const __half *x;
+    long long ldx;
+    int tiles, steps, panel;  // tiles; steps of a warp per tile, and those whose x is held at once (a multiple of DEPTH)
+    Dest d;
+};
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+// Volatile, so that a load stays where the registers of the step before become free: moved further up, its result would have to be
+// copied, which waits for it.
+__device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+}
+__device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
+template <int NT, int WR, bool LEAST>
+__global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowParams p) {
+    constexpr int WK = ROW_WARPS / WR, COLS = 8 * NT, FEATURES = 16 * WR;
+    extern __shared__ __align__(16) uint8_t xs[];  // [B][panel * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
+    __shared__ float red[2][WK][FEATURES][COLS + 1];
+    const Dest &d = p.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int wr = warp % WR, kg = warp / WR;
+    const int x_row = p.panel * WK * 256 + 64;  // the odd half line keeps neighbouring rows on different banks
+
+    uint4 qa[DEPTH], qb[DEPTH];
+    uint32_t sa[DEPTH], sb[DEPTH], la[DEPTH], lb[DEPTH];
+    // A lane's place in a tile: its first codes and scales of feature g, and the way to those of the other feature. Nothing outside is
+    // read: features past the last are read as the last and dropped, steps past the last k as the lane's last one and multiplied
+    // by zeros.
+    struct Place {
+        const uint8_t *qa, *qb, *sa, *sb;
+    };
+    const int k_lane = kg * CHUNK + 32 * t;
+    const int k_first = k_lane < p.K ? k_lane : 0, last = k_lane < p.K ? (p.K - 1 - k_lane) / (CHUNK * WK) : 0;
+    const auto place = [&](int tile) {
+        const int n = min(tile * FEATURES + wr * 16 + g, d.N - 1), m = min(tile * FEATURES + wr * 16 + g + 8, d.N - 1);
+        const uint8_t *s = reinterpret_cast<const uint8_t *>(p.scale + static_cast<long long>(k_first >> p.shift) * d.N);
+        return Place{p.codes + (static_cast<long long>(n) * p.K + k_first) / 2, p.codes + (static_cast<long long>(m) * p.K + k_first) / 2, s + 2ll * n, s + 2ll * m};
+    };
+    constexpr int Q_STEP = CHUNK * WK / 2;
+    const int s_step = ((CHUNK * WK) >> p.shift) * d.N * 2;
+    const long long to_least = (p.least - p.scale) * 2;
+    const auto fetch = [&](int u, const Place &at, int step) {
+        step = min(step, last);
+        const long long s = static_cast<long long>(step) * s_step;
+        ld_codes(qa[u], at.qa + static_cast<long long>(step) * Q_STEP);
+        ld_codes(qb[u], at.qb + static_cast<long long>(step) * Q_STEP);
+        ld_scale(sa[u], at.sa + s);
+        ld_scale(sb[u], at.sb + s);
+        if (LEAST) {
+            ld_scale(la[u], at.sa + s + to_least);
+            ld_scale(lb[u], at.sb + s + to_least);
+        }
+    };
+    const int full = p.K / (CHUNK * WK);  // steps that are whole for every lane
+    int tile = blockIdx.x;
+    Place here = place(tile), then = here;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int n = n0 + g + 8 * i;
-            if (n < d.N && k < K) {
-                q[i] = *reinterpret_cast<const uint4 *>(codes + (static_cast<long long>(n) * K + k) / 2);
-                const long long at = static_cast<long long>(k / group) * d.N + n;
-                s[i] = __half2half2(scale[at]);
-                if (LEAST) l[i] = __half2half2(least[at]);
+    for (int u = 0; u < DEPTH; ++u) {
+        la[u] = lb[u] = 0;
+        fetch(u, here, u);
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    const auto fill = [&](int first) {
+        const int chunk0 = first * WK, held = min(p.panel, p.steps - first) * WK;  // zeros behind the last k
+        for (int b = 0; b < d.B; ++b)
+            for (int i = tid; i < held * 16; i += ROW_WARPS * 32) {
+                const int k = chunk0 * CHUNK + i * 8;  // piece i & 15 = 4 t + j of its chunk goes to place 4 j + t
+                cp_async16(xs + b * x_row + (i >> 4) * 256 + ((i & 3) * 4 + (i >> 2 & 3)) * 16, p.x + b * p.ldx + min(k, p.K - 8), k < p.K);
+            }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+    };
+    fill(0);
+    // Rows of x past the last are read as the last: the columns are dropped.
+    const uint8_t *xr[NT];
+#pragma unroll
+    for (int q = 0; q < NT; ++q) xr[q] = xs + min(8 * q + g, d.B - 1) * x_row + kg * 256 + t * 16;
+
+    // The outputs of this thread: 16 lanes take 16 neighbouring features of a row of x.
+    const int sub = tid >> 4, f = tid & 15, units = WR * d.B;
+    for (int turn = 0; tile < p.tiles; tile += gridDim.x, turn ^= 1) {
+        const int n0 = tile * FEATURES, next = tile + gridDim.x;
+        Extra early = {0.0f, 0.0f};
+        if (sub < units && n0 + sub % WR * 16 + f < d.N) early = extra_of(d, sub / WR, n0 + sub % WR * 16 + f);
+        float c[NT][4] = {};
+        if (next < p.tiles) then = place(next);
+        for (int first = 0; first < p.steps; first += p.panel) {
+            if (p.panel < p.steps && (first || tile != static_cast<int>(blockIdx.x))) {
+                __syncthreads();
+                fill(first);
+            }
+            const int end = min(p.steps, first + p.panel);
+            int x_at = 0, i0 = first;
+            const auto products = [&](int u, auto any_big) {
+                constexpr bool BIG = decltype(any_big)::value;
+                const Scale ka = scale_of<LEAST, BIG>(sa[u], la[u]), kb = scale_of<LEAST, BIG>(sb[u], lb[u]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t va[4], vb[4];
+                    values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
+                    values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
+                    const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        const uint4 xv = *reinterpret_cast<const uint4 *>(xr[m] + x_at + u * (WK * 256) + j * 64);
+                        mma16816(c[m], a0, xv.x, xv.y);
+                        mma16816(c[m], a1, xv.z, xv.w);
+                    }
+                }
+            };
+            const auto use = [&](int u) {
+                if (__any_sync(0xFFFFFFFFu, big_scale(max(sa[u], sb[u]))))
+                    products(u, std::true_type());
+                else
+                    products(u, std::false_type());
+            };
+            // Whole rounds whose next fetches are of this tile and all there: no checks, addresses a constant apart.
+            if (i0 + 2 * DEPTH <= full) {
+                const uint8_t *pa = here.qa + static_cast<long long>(i0 + DEPTH) * Q_STEP, *pb = here.qb + static_cast<long long>(i0 + DEPTH) * Q_STEP;
+                const uint8_t *ps = here.sa + static_cast<long long>(i0 + DEPTH) * s_step;
+                const long long other = here.sb - here.sa;
+                for (; i0 < end && i0 + 2 * DEPTH <= full; i0 += DEPTH) {
+#pragma unroll
+                    for (int u = 0; u < DEPTH; ++u) {
+                        use(u);
+                        ld_codes(qa[u], pa + u * Q_STEP);
+                        ld_codes(qb[u], pb + u * Q_STEP);
+                        ld_scale(sa[u], ps);
+                        ld_scale(sb[u], ps + other);
+                        if (LEAST) {
+                            ld_scale(la[u], ps + to_least);
+                            ld_scale(lb[u], ps + to_least + other);
+                        }
+                        ps += s_step;
+                    }
+                    pa += DEPTH * Q_STEP;
+                    pb += DEPTH * Q_STEP;
+                    x_at += DEPTH * WK * 256;
+                }
+            }
+            for (; i0 < end; i0 += DEPTH, x_at += DEPTH * WK * 256) {
+#pragma unroll
+                for (int u = 0; u < DEPTH; ++u) {
+                    const int i = i0 + u;
+                    if (i >= end) break;
+                    use(u);
+                    if (i + DEPTH < p.steps)
+                        fetch(u, here, i + DEPTH);
+                    else if (next < p.tiles)
+                        fetch(u, then, u);
+                }
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint4 xv = make_uint4(0, 0, 0, 0);
-            if (b0 + g < d.B && k < K) xv = *reinterpret_cast<const uint4 *>(x + (b0 + g) * ldx + k + 8 * j);
-            uint32_t v[2][4];
+        for (int q = 0; q < NT; ++q)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) values_of<LEAST>((&q[i].x)[j], s[i], l[i], v[i]);
-            const uint32_t a0[4] = {v[0][0], v[1][0], v[0][1], v[1][1]}, a1[4] = {v[0][2], v[1][2], v[0][3], v[1][3]};
-            mma16816(c, a0, xv.x, xv.y);
-            mma16816(c, a1, xv.z, xv.w);
-        }
-    }
+            for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][8 * q + 2 * t + (i & 1)] = c[q][i];
+        here = then;
+        __syncthreads();  // the other half of red is free: its readers came here
+        for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 16) {
+            const int b = unit / WR, n = unit % WR * 16 + f;
+            unsigned long long key = 0;
+            const bool in = unit < units && n0 + n < d.N;
+            if (in) {
+                float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = n0 + g + 8 * (i >> 1), b = b0 + 2 * t + (i & 1);
-        const bool in = n < d.N && b < d.B;
-        unsigned long long key = 0;
-        if (in) {
-            const float h = __half2float(put(d, b, n, c[i]));
-            if (h == h) key = lin::argmax_key(h + 0.0f, static_cast<unsigned>(n));
-        }
-        if (d.epi == EPI_HEAD) {
+                for (int q = 0; q < WK; ++q) sum += red[turn][q][n][b];
+                const float h = __half2float(unit == sub ? put(d, b, n0 + n, sum, early) : put(d, b, n0 + n, sum)) + 0.0f;
+                if (h == h) key = lin::argmax_key(h, static_cast<unsigned>(n0 + n));
+            }
+            if (d.epi == EPI_HEAD) {
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) key = max(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
-            if (g == 0 && b < d.B) {
-                unsigned long long *at = d.amax + static_cast<long long>(b) * d.keys + blockIdx.x;
-                *at = i < 2 ? key : max(key, *at);
+                for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
+                if (in && f == 0) d.amax[static_cast<long long>(b) * d.keys + (n0 + n) / 16] = key;
             }
         }
     }
@@ -213,10 +367,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             atomicOr(p.d.status, ST_LINEAR_TIMEOUT);
         }
     };
+    // Each role counts slots, phases, stages and tiles by hand: one warp's divisions by run-time numbers take longer than a stage.
     if (warp == 0) {
         // Codes: they do not depend on the kernel before this one, so nothing waits for it.
         const bool leader = elect_one();
-        int it = 0;
+        int it = 0, i = 0, n0 = first_tile * BM;
         for (; it < total; ++it) {
             const int slot = it % CODE_RING;
             const bool ok = it < CODE_RING || mbar_wait(&c_empty[slot], (it / CODE_RING - 1) & 1, p.timeout_ns);
@@ -226,55 +381,63 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             }
             if (leader) {
                 mbar_arrive_expect_tx(&c_full[slot], CODE_BYTES);
-                tma_load_2d(smem + slot * CODE_BYTES, &tm_w, &c_full[slot], (s0 + it % ns) * (KS / 2), (first_tile + it / ns * tile_step) * BM);
+                tma_load_2d(smem + slot * CODE_BYTES, &tm_w, &c_full[slot], (s0 + i) * (KS / 2), n0);
+            }
+            if (++i == ns) {
+                i = 0;
+                n0 += tile_step * BM;
             }
             __syncwarp();
         }
         // every copy has landed before this CTA may end, whatever became of the others
-        for (int i = max(0, it - CODE_RING); i < it; ++i) mbar_wait(&c_full[i % CODE_RING], (i / CODE_RING) & 1, p.timeout_ns);
+        for (int j = max(0, it - CODE_RING); j < it; ++j) mbar_wait(&c_full[j % CODE_RING], (j / CODE_RING) & 1, p.timeout_ns);
     } else {
         grid_dependency_wait();
     }
     if (warp == 2) {
         const bool leader = elect_one();
-        int at = 0;
+        int i = 0, slot = 0, at = 0;
+        uint32_t phase = 1;  // of x_empty: passed at once while the ring fills
         for (; at < 2 * total; ++at) {
-            const int slot = at % p.x_ring;
-            const bool ok = at < p.x_ring || mbar_wait(&x_empty[slot], (at / p.x_ring - 1) & 1, p.timeout_ns);
+            const bool ok = mbar_wait(&x_empty[slot], phase, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 fail();
                 break;
             }
             if (leader) {
                 mbar_arrive_expect_tx(&x_full[slot], static_cast<uint32_t>(x_bytes));
-                tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], (s0 + at / 2 % ns) * KS + at % 2 * X_ATOM, 0);
+                tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], s0 * KS + i * X_ATOM, 0);
+            }
+            if (++i == 2 * ns) i = 0;
+            if (++slot == p.x_ring) {
+                slot = 0;
+                phase ^= 1;
             }
             __syncwarp();
         }
-        for (int i = max(0, at - p.x_ring); i < at; ++i) mbar_wait(&x_full[i % p.x_ring], (i / p.x_ring) & 1, p.timeout_ns);
+        for (int j = max(0, at - p.x_ring); j < at; ++j) mbar_wait(&x_full[j % p.x_ring], (j / p.x_ring) & 1, p.timeout_ns);
     }
     if (warp == 1) {
         const bool leader = elect_one();
         const uint32_t idesc = idesc_f16_f32(BM, p.bpad, 0, 0);
         const uint64_t dx = sdesc_sw128(smem_u32(x_smem), 16, 1024);
-        const uint32_t x_lo = static_cast<uint32_t>(dx), x_hi = static_cast<uint32_t>(dx >> 32);
-        int it = 0;
+        const uint32_t x_lo = static_cast<uint32_t>(dx), x_hi = static_cast<uint32_t>(dx >> 32), x_step = static_cast<uint32_t>(x_bytes) >> 4;
+        int it = 0, slot = 0, acc = 0;
+        uint32_t x_phase = 0, acc_phase = 1;  // of acc_empty: passed at once for the first tiles
         bool ok = true;
         for (int j = 0; j < my_tiles && ok; ++j) {
-            const int acc = j % p.nacc;
-            if (j >= p.nacc) ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&acc_empty[acc], (j / p.nacc - 1) & 1, p.timeout_ns));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&acc_empty[acc], acc_phase, p.timeout_ns));
             for (int i = 0; i < ns && ok; ++i, ++it) {
                 const int buf = it % A_BUFS;
                 ok = mbar_wait_spin(&a_full[buf], (it / A_BUFS) & 1, p.timeout_ns);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int at = 2 * it + h, slot = at % p.x_ring;
-                    ok = ok && mbar_wait_spin(&x_full[slot], (at / p.x_ring) & 1, p.timeout_ns);
+                    ok = ok && mbar_wait_spin(&x_full[slot], x_phase, p.timeout_ns);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t off = static_cast<uint32_t>(slot * x_bytes) >> 4;
+                        const uint32_t off = static_cast<uint32_t>(slot) * x_step;
 #pragma unroll
                         for (int kk = 0; kk < X_ATOM / 16; ++kk)
                             umma_f16_ts_lohi(tm_acc + acc * p.bpad, tm_a + buf * A_COLS + h * (X_ATOM / 2) + kk * 8, x_lo + off + kk * 2, x_hi, idesc,
@@ -282,6 +445,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
                         umma_commit(&x_empty[slot]);
                     }
                     __syncwarp();
+                    if (++slot == p.x_ring) {
+                        slot = 0;
+                        x_phase ^= 1;
+                    }
                 }
                 if (!ok) break;
                 if (leader) {
@@ -289,6 +456,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
                     if (i == ns - 1) umma_commit(&acc_full[acc]);
                 }
                 __syncwarp();
+            }
+            if (++acc == p.nacc) {
+                acc = 0;
+                acc_phase ^= 1;
             }
         }
         if (!ok) fail();
@@ -300,19 +471,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
         const uint32_t lanes = static_cast<uint32_t>(warp4 * 32) << 16;
         const int groups = p.K / p.group;
         __half sc[2][GS], lo[2][GS];
-        const auto scales = [&](int it, __half (&s)[GS], __half (&l)[GS]) {
-            const int n = (first_tile + it / ns * tile_step) * BM + row;
-            const int g0 = (s0 + it % ns) * GS;
+        int si = wg, sn = first_tile * BM + row;  // the stage and the feature of the scales that are fetched next
+        const auto settle = [&] {
+            while (si >= ns) {
+                si -= ns;
+                sn += tile_step * BM;
+            }
+        };
+        const auto scales = [&](__half (&s)[GS], __half (&l)[GS]) {
+            settle();
+            const int g0 = (s0 + si) * GS;
 #pragma unroll
             for (int q = 0; q < GS; ++q) {
-                const bool in = it < total && n < p.d.N && g0 + q < groups;
-                const long long at = static_cast<long long>(g0 + q) * p.d.N + n;
+                const bool in = sn < p.d.N && g0 + q < groups;
+                const long long at = static_cast<long long>(g0 + q) * p.d.N + sn;
                 s[q] = in ? p.scale[at] : __float2half_rn(0.0f);
                 if (LEAST) l[q] = in ? p.least[at] : __float2half_rn(0.0f);
             }
+            si += 2;
         };
-        scales(wg, sc[0], lo[0]);
-        scales(wg + 2, sc[1], lo[1]);
+        scales(sc[0], lo[0]);
+        scales(sc[1], lo[1]);
         bool ok = true;
         for (int it0 = wg; it0 < total && ok; it0 += 4) {
 #pragma unroll
@@ -326,25 +505,35 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
                 if (!ok) break;
                 tc_fence_after();
                 const uint8_t *st = smem + slot * CODE_BYTES + row * 64;
+                bool large = false;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t v[32];
+                for (int q = 0; q < GS; ++q) large = large || big_scale(__half_as_ushort(sc[u][q]));
+                const auto convert = [&](auto any_big) {
+                    constexpr bool BIG = decltype(any_big)::value;
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int chunk = h * 2 + q;  // 32 k, 16 bytes: the 64-byte swizzle's place
-                        const uint4 w = *reinterpret_cast<const uint4 *>(st + ((chunk ^ (row >> 1 & 3)) << 4));
-                        const __half2 s2 = __half2half2(sc[u][chunk * GS / 4]), l2 = LEAST ? __half2half2(lo[u][chunk * GS / 4]) : s2;
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[32];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t four[4];
-                            values_of<LEAST>((&w.x)[j], s2, l2, four);
+                        for (int q = 0; q < 2; ++q) {
+                            const int chunk = h * 2 + q;  // 32 k, 16 bytes: the 64-byte swizzle's place
+                            const uint4 w = *reinterpret_cast<const uint4 *>(st + ((chunk ^ (row >> 1 & 3)) << 4));
+                            const Scale k = scale_of<LEAST, BIG>(__half_as_ushort(sc[u][chunk * GS / 4]), LEAST ? __half_as_ushort(lo[u][chunk * GS / 4]) : 0);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[q * 16 + j * 4 + e] = four[e];
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t four[4];
+                                values_of<LEAST, BIG>((&w.x)[j], k, four);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) v[q * 16 + j * 4 + e] = four[e];
+                            }
                         }
+                        tmem_st32(tm_a + lanes + buf * A_COLS + h * 32, v);
                     }
-                    tmem_st32(tm_a + lanes + buf * A_COLS + h * 32, v);
-                }
-                scales(it + 4, sc[u], lo[u]);
+                };
+                if (__any_sync(0xFFFFFFFFu, large))
+                    convert(std::true_type());
+                else
+                    convert(std::false_type());
+                if (it + 4 < total) scales(sc[u], lo[u]);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -418,8 +607,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
 
 namespace {
 
-constexpr int SIMPLE_MAX_B = 0;
-
 typedef void (*TcKernel)(CUtensorMap, CUtensorMap, TcParams);
 template <bool LEAST>
 TcKernel tc_kernel(int group) {
@@ -472,7 +659,7 @@ int prepare_tc(DeviceContext *ctx) {
 
 }  // namespace
 
-int keys_of(const GPT2W4 &w, int B) { return B <= SIMPLE_MAX_B ? (w.N + 15) / 16 : (w.N + BM - 1) / BM * 4; }
+int keys_of(const GPT2W4 &w, int B) { return B <= ROWS_MAX_B ? (w.N + 15) / 16 : (w.N + BM - 1) / BM * 4; }
 
 int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo) {
     if (!weight_ok(&w) || !x || (reinterpret_cast<uintptr_t>(x) & 15) || (ldx & 7) || ldx < w.K || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
@@ -498,19 +685,65 @@ int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int
 
 namespace {
 
-int launch_simple(const Plan &pl, cudaStream_t stream) {
+typedef void (*RowKernel)(RowParams);
+template <int NT, bool LEAST>
+RowKernel row_kernel(int wr) {
+    return wr == 1 ? k_w4_rows<NT, 1, LEAST> : wr == 2 ? k_w4_rows<NT, 2, LEAST> : wr == 4 ? k_w4_rows<NT, 4, LEAST> : k_w4_rows<NT, 8, LEAST>;
+}
+
+int prepare_rows(DeviceContext *ctx) {
+    if (ctx->w4_rows_attr_done) return GPT2_B200_OK;
+    RelaxedCapture relaxed;
+    for (int wr = 1; wr <= 8; wr *= 2)
+        for (const RowKernel k : {row_kernel<1, false>(wr), row_kernel<1, true>(wr), row_kernel<2, false>(wr), row_kernel<2, true>(wr)})
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, PANEL_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
+    ctx->w4_rows_attr_done = true;
+    return GPT2_B200_OK;
+}
+
+int launch_rows(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
+    const int rc = prepare_rows(ctx);
+    if (rc != GPT2_B200_OK) return rc;
+    const GPT2W4 &w = pl.w;
+    const int B = pl.d.B, nt = B <= 8 ? 1 : 2, chunks = (w.K + CHUNK - 1) / CHUNK, slots = ROW_CTAS * ctx->num_sms;
+    RowParams p = {};
+    p.codes = static_cast<const uint8_t *>(w.codes);
+    p.scale = w.scale;
+    p.least = w.least;
+    p.K = w.K;
+    p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+    p.x = pl.x;
+    p.ldx = pl.ldx;
+    p.d = pl.d;
+    // Tile height: the fewest steps of the busiest CTA, a tile's end counted as one.
+    int wr = 1;
+    long long best = 0;
+    for (int h = 1; h <= ROW_WARPS; h *= 2) {
+        const long long tiles = (static_cast<long long>(w.N) + 16 * h - 1) / (16 * h), rounds = (tiles + slots - 1) / slots;
+        const int wk = ROW_WARPS / h, steps = (chunks + wk - 1) / wk;
+        const long long cost = rounds * (steps + 1);
+        if ((PANEL_BYTES / B - 64) / (256 * wk) < DEPTH) continue;  // x has room for a round of the buffers
+        if (!best || cost < best) {
+            best = cost;
+            wr = h;
+            p.tiles = static_cast<int>(tiles);
+            p.steps = steps;
+        }
+    }
+    const int wk = ROW_WARPS / wr, fit = (PANEL_BYTES / B - 64) / (256 * wk);  // steps whose x fits
+    p.panel = std::min((p.steps + DEPTH - 1) / DEPTH, fit / DEPTH) * DEPTH;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((pl.d.N + 15) / 16, (pl.d.B + 7) / 8, 1);
-    cfg.blockDim = dim3(32, 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tiles, slots)), 1, 1);
+    cfg.blockDim = dim3(ROW_WARPS * 32, 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(B) * (p.panel * wk * 256 + 64);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pl.pdl ? 1 : 0;
-    const uint8_t *codes = static_cast<const uint8_t *>(pl.w.codes);
-    const auto go = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, codes, static_cast<const __half *>(pl.w.scale), static_cast<const __half *>(pl.w.least), pl.w.K, pl.w.group, pl.x, pl.ldx, pl.d); };
-    return (pl.w.least ? go(k_w4_simple<true>) : go(k_w4_simple<false>)) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    const RowKernel k = nt == 1 ? (w.least ? row_kernel<1, true>(wr) : row_kernel<1, false>(wr)) : (w.least ? row_kernel<2, true>(wr) : row_kernel<2, false>(wr));
+    return cudaLaunchKernelEx(&cfg, k, p) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
 int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
@@ -569,13 +802,13 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
 int prepare(const Plan &pl) {
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_ECUDA;
-    return pl.d.B <= SIMPLE_MAX_B ? GPT2_B200_OK : prepare_tc(ctx);
+    return pl.d.B <= ROWS_MAX_B ? prepare_rows(ctx) : prepare_tc(ctx);
 }
 
 int launch(const Plan &pl, cudaStream_t stream) {
     DeviceContext *ctx = device_context();
     if (!ctx) return GPT2_B200_ECUDA;
-    return pl.d.B <= SIMPLE_MAX_B ? launch_simple(pl, stream) : launch_tc(ctx, pl, stream);
+    return pl.d.B <= ROWS_MAX_B ? launch_rows(ctx, pl, stream) : launch_tc(ctx, pl, stream);
 }
 
 }  // namespace w4

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(WARPS * 32)
         const long long n = n0 + warp * PER + i;
         if (n >= N) break;
         uint32_t v[4];
-        values_of<LEAST>(word[i], __half2half2(s[i]), __half2half2(LEAST ? l[i] : s[i]), v);
+        values_of<LEAST, true>(word[i], scale_of<LEAST, true>(__half_as_ushort(s[i]), LEAST ? __half_as_ushort(l[i]) : 0), v);
         __stcs(reinterpret_cast<uint4 *>(W + n * ldw + k), make_uint4(v[0], v[1], v[2], v[3]));
     }
 }
