@@ -1,10 +1,13 @@
 // logits_edit.cu — penalties for repeated tokens, biases and masks on logits, and the greedy choice, in one launch.
 //
-// A row is read and written once: 2 x 2 or 2 x 4 bytes per logit, its history once per segment from L2. Of a segment of tokens a CTA
-// keeps one word each in shared memory: whether the prompt holds the token, how often the rest of the history does, and the first
-// bias entry that names it. The counts are whole numbers added by atomics, so their order does not matter; biases of the same token
-// are summed in the order of their list. A cluster of up to 8 CTAs shares a row when there are few rows; the choice is the
-// maximum of (value, inverted token) keys, which no order changes either.
+// A row is read and written once: 2 x 2 or 2 x 4 bytes per logit. Most logits change by the mask alone, so a CTA works on a segment of
+// tokens in two passes: the dense one copies, masks and looks for the largest; the sparse one takes the tokens of the history and of
+// the bias list, a few hundred, each once. Between them stands one word per token of the segment in shared memory: whether the
+// prompt holds it, how often the rest of the history does, and the first bias entry that names it; a list of the tokens that have one; and
+// one bit per token, by which the dense pass leaves those out of the choice. (Edits within the dense pass took 190 instructions per 16 bytes, which cost three times the
+// bytes.) The counts are whole numbers added by atomics, so their order does not matter; biases of the same token are summed in
+// the order of their list; the choice is the maximum of (value, inverted token), which no order changes either. A cluster of up to 8
+// CTAs shares a row when there are few rows.
 //
 // Rows may start anywhere: a row is cut at the 16-byte boundaries of its input; the vectors at its ends are taken element by
 // element, and so are stores to an output that is aligned otherwise.
@@ -19,9 +22,10 @@ namespace edit {
 namespace {
 
 constexpr int NT = 512;
-constexpr int SEG = 16384;  // tokens of a segment: 64 KB of words
+constexpr int SEG = 16384;  // tokens of a segment: 64 KB of words, two CTAs per SM
 constexpr int MAX_CLUSTER = 8;
-constexpr int BATCH = 2;  // vectors per thread in flight
+constexpr int BATCH = 4;  // vectors per thread in flight
+constexpr int AHEAD = 8;  // tokens of the history per thread in flight
 
 // A token's word: bit 31 in the prompt; bits 20..30 MAX_BIAS - i of its first bias entry i (0: none); below, how often it occurs behind
 // the prompt.
@@ -37,6 +41,7 @@ struct Params {
     long long ldo, ld;
     int V, cluster;
     int seg;      // tokens per segment
+    int list;     // touched tokens of a segment at most
     int len_add;  // added to every length (the decoder's positions)
     int in_place;
     GPT2LogitsEdit e;
@@ -57,6 +62,21 @@ __device__ __forceinline__ float top_of(const uint4 &v, __half) {
 }
 __device__ __forceinline__ float top_of(const uint4 &v, float) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+
+// -inf where a vector's bit is 0.
+__device__ __forceinline__ void cut(uint4 &v, uint32_t allowed, __half) {
+    uint32_t *w = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t keep = (allowed >> (2 * i) & 1) * 0xFFFFu + (allowed >> (2 * i + 1) & 1) * 0xFFFF0000u;
+        w[i] = (w[i] & keep) | (0xFC00FC00u & ~keep);
+    }
+}
+__device__ __forceinline__ void cut(uint4 &v, uint32_t allowed, float) {
+    uint32_t *w = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = allowed >> i & 1 ? w[i] : 0xFF800000u;
 }
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi, bool tell, unsigned *status) {
@@ -88,55 +108,50 @@ __device__ __forceinline__ float edited(float x, uint32_t word, const Row &r) {
     return x;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT) k_logits_edit(const Params p) {
+// MASK, NEXT: there is a mask, a choice is asked for.
+template <typename T, bool MASK, bool NEXT>
+__global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
     constexpr int VEC = 16 / sizeof(T);
-    extern __shared__ __align__(16) uint32_t words[];  // a segment's words, the bias list behind them
+    constexpr uint32_t ALL = (1u << VEC) - 1;
+    extern __shared__ __align__(16) uint32_t words[];  // a segment's words, bits, mask and list, the bias list
     __shared__ unsigned long long best[NT / 32], row_best[MAX_CLUSTER];
-    __shared__ int dups;
+    __shared__ int dups, n_touched;
+    __shared__ uint32_t gather[NT / 32][32 * AHEAD];
     const long long row = blockIdx.x / p.cluster;
     const int rank = static_cast<int>(blockIdx.x % p.cluster);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const GPT2LogitsEdit &e = p.e;
-    int *btok = reinterpret_cast<int *>(words + p.seg);
+    uint32_t *bits = words + p.seg;         // touched tokens
+    uint32_t *allow = bits + p.seg / 32;    // the mask, from the segment's first word on
+    uint16_t *touched = reinterpret_cast<uint16_t *>(allow + p.seg / 32);  // in any order: nothing depends on it
+    int *btok = reinterpret_cast<int *>(touched + p.list);
     float *bval = reinterpret_cast<float *>(btok + e.max_bias);
-    if (p.cluster > 1) cluster_arrive_relaxed();  // waited for before the first write to another CTA
-    for (int i = tid; i < p.seg / 4; i += NT) reinterpret_cast<uint4 *>(words)[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) dups = 0;
+    if (NEXT && p.cluster > 1) cluster_arrive_relaxed();  // waited for before the first write to another CTA
     grid_dependency_wait();
 
     const T *in = static_cast<const T *>(p.in) + row * p.ld;
     T *out = static_cast<T *>(p.out) + row * p.ldo;
     const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));  // elements from the boundary to the row
     const bool same = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const bool lean = p.in_place && !p.next;  // vectors without an edit stay where they are, unread
     const bool tell = tid == 0 && rank == 0;
 
     int n = 0, from = 0;
     const int *hist = nullptr;
     if (e.history && e.max_history > 0) {
         hist = e.history + row * e.history_stride;
-        n = clamped(e.length ? e.length[row] + p.len_add : e.max_history, 0, e.max_history, tell, p.status);
-        if (e.prompt) from = clamped(e.prompt[row], 0, n, tell, p.status);
+        n = e.length ? e.length[row] + p.len_add : e.max_history;
+        if (e.prompt) from = e.prompt[row];
     }
     Row r;
     r.rep = e.repetition ? e.repetition[row] : 1.0f;
     r.freq = e.frequency ? e.frequency[row] : 0.0f;
     r.pres = e.presence ? e.presence[row] : 0.0f;
-    r.nb = 0;
+    r.nb = e.bias_token && e.max_bias > 0 ? (e.n_bias ? e.n_bias[row] : e.max_bias) : 0;
     r.btok = btok;
     r.bval = bval;
     r.dups = &dups;
-    if (e.bias_token && e.max_bias > 0) {
-        r.nb = e.n_bias ? clamped(e.n_bias[row], 0, e.max_bias, tell, p.status) : e.max_bias;
-        for (int i = tid; i < r.nb; i += NT) {
-            btok[i] = e.bias_token[row * e.bias_stride + i];
-            bval[i] = e.bias[row * e.bias_stride + i];
-        }
-    }
-    const unsigned *mask = nullptr;
-    const int mask_words = (p.V + 31) / 32;
-    if (e.mask) {
+    const unsigned *mask = nullptr;  // of this row
+    if (MASK) {
         int m = e.mask_row ? e.mask_row[row] : e.mask_rows == 1 ? 0 : static_cast<int>(row);
         if (m < -1 || m >= e.mask_rows) {
             if (tell) atomicOr(p.status, ST_EDIT_BAD_INPUT);
@@ -145,114 +160,179 @@ __global__ void __launch_bounds__(NT) k_logits_edit(const Params p) {
         if (m >= 0) mask = e.mask + m * e.mask_stride;
     }
 
+    // Vector v of a row holds tokens v * VEC - shift .. + VEC - 1; those from f0 to f1 - 1 are whole.
+    const int f0 = shift ? 1 : 0, f1 = (p.V + shift) / VEC, vectors = (p.V + shift + VEC - 1) / VEC;
+    const int per = (vectors + p.cluster - 1) / p.cluster, v0 = rank * per, v1 = min(vectors, v0 + per), seg = p.seg / VEC;
+    // The dense pass has something to do unless the logits stay in place and nothing asks for the mask or the largest.
+    const bool dense = MASK || NEXT || !p.in_place;
+    n = clamped(n, 0, hist ? e.max_history : 0, tell, p.status);
+    from = clamped(from, 0, n, tell, p.status);
+    r.nb = clamped(r.nb, 0, e.max_bias, tell, p.status);
+    int h[AHEAD];
+    const auto tokens = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) h[k] = i0 + k * NT + lane < n ? hist[i0 + k * NT + lane] : -1;
+    };
+    tokens(warp * 32);
+    for (int i = tid; i < r.nb; i += NT) {
+        btok[i] = e.bias_token[row * e.bias_stride + i];
+        bval[i] = e.bias[row * e.bias_stride + i];
+    }
+    if (n | r.nb)
+        for (int i = tid; i < (p.seg + p.seg / 32) / 4; i += NT) reinterpret_cast<uint4 *>(words)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dups = n_touched = 0;
+
     float top = -INFINITY;
     int at = -1;
-    const int vectors = (p.V + shift + VEC - 1) / VEC, per = (vectors + p.cluster - 1) / p.cluster;
-    const int v1 = min(vectors, (rank + 1) * per);
-    for (int base = rank * per; base < v1; base += p.seg / VEC) {
-        const int m = min(p.seg / VEC, v1 - base);
-        const int t0 = base * VEC - shift;  // the token of the segment's first word: below 0 in a row's first vector
-        const auto whole = [&](int v) { return t0 + v * VEC >= 0 && t0 + v * VEC + VEC <= p.V; };
-        uint4 x[BATCH];
-        const auto fetch = [&](int v) {
-#pragma unroll
-            for (int j = 0; j < BATCH; ++j)
-                if (v + j * NT < m && whole(v + j * NT)) x[j] = *reinterpret_cast<const uint4 *>(in + t0 + (v + j * NT) * VEC);
-        };
-        if (!lean) fetch(tid);  // on its way while the history is counted
-        __syncthreads();
-        for (int i = tid; i < r.nb; i += NT) {
-            const int t = btok[i];
-            if (t >= 0 && t < p.V && static_cast<unsigned>(t - t0) < static_cast<unsigned>(m * VEC))
-                if (atomicMax(&words[t - t0], static_cast<uint32_t>(MAX_BIAS - i) << BIAS_AT)) dups = 1;
+    const auto better = [&](float y, int t) {
+        if (y > top || (y == top && at >= 0 && t < at)) {
+            top = y;
+            at = t;
         }
-        if (r.nb) __syncthreads();  // the counts below go under the entries
-        for (int i = tid; i < n; i += NT) {
-            const int t = hist[i];
-            if (t >= 0 && t < p.V && static_cast<unsigned>(t - t0) < static_cast<unsigned>(m * VEC)) {
-                if (i < from)
-                    atomicOr(&words[t - t0], SEEN);
-                else
-                    atomicAdd(&words[t - t0], 1u);
+    };
+    for (int base = v0; base < v1; base += seg) {
+        const int end = min(base + seg, v1), t0 = base * VEC - shift;  // t0: the token of the first word, below 0 in a row's first vector
+        const int lo = max(t0, 0), span = min(end * VEC - shift, p.V) - lo;
+        const int d0 = max(base, f0) + tid, d1 = min(end, f1);
+        const auto inside = [&](int t) { return static_cast<unsigned>(t - lo) < static_cast<unsigned>(span); };
+        if (base != v0) {
+            if (n > NT * AHEAD) tokens(warp * 32);
+            __syncthreads();  // the words before were read
+            if (tid == 0) n_touched = 0;
+        }
+        if (MASK)
+            for (int i = tid; i < p.seg / 32; i += NT) {
+                const int t = t0 + i * 32, k = t >> 5, last = (p.V - 1) >> 5;  // k is -1 in front of a row that starts inside a vector
+                allow[i] = mask ? __funnelshift_r(k >= 0 ? mask[min(k, last)] : 0u, mask[min(k + 1, last)], t & 31) : 0xFFFFFFFFu;
             }
-        }
-        __syncthreads();
-        for (int v = tid; v < m; v += NT * BATCH) {
-            if (v != tid && !lean) fetch(v);
+        const auto masked = [&](int t) { return MASK && !(allow[(t - t0) >> 5] >> ((t - t0) & 31) & 1); };
+        __syncthreads();  // the words and the counter are 0, the lists are there
+
+        // The first vectors come while the history is counted. One that is masked whole is not read.
+        uint4 x[BATCH];
+        uint32_t allowed[BATCH];
+        const uint4 *src = reinterpret_cast<const uint4 *>(in - shift);
+        const int place32 = (d0 - base) * VEC & 31;  // the same for all vectors of a thread
+        const auto fetch = [&](int v) {
+            const uint32_t *mine = allow + ((v - base) * VEC >> 5);
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const int u = v + j * NT;
-                if (u >= m) break;
-                const int t = t0 + u * VEC;
-                uint32_t w[VEC], any = 0;
+                if (v + j * NT >= d1) break;
+                if (MASK) allowed[j] = mine[j * (NT * VEC / 32)] >> place32 & ALL;
+                if (!MASK || allowed[j]) x[j] = src[v + j * NT];
+            }
+        };
+        if (dense) fetch(d0);
+        const auto dense_pass = [&](int n_edit) {
+            for (int v = d0; v < d1; v += NT * BATCH) {
+                if (v != d0) fetch(v);
 #pragma unroll
-                for (int i = 0; i < VEC; i += 4) {
-                    const uint4 q = *reinterpret_cast<const uint4 *>(words + u * VEC + i);
-                    w[i] = q.x;
-                    w[i + 1] = q.y;
-                    w[i + 2] = q.z;
-                    w[i + 3] = q.w;
-                    any |= q.x | q.y | q.z | q.w;
-                }
-                if (any) {
+                for (int j = 0; j < BATCH; ++j) {
+                    const int u = v + j * NT, t = u * VEC - shift;
+                    if (u >= d1) break;
+                    if (MASK) cut(x[j], allowed[j], T());
+                    if (!p.in_place || (MASK && allowed[j] != ALL)) {
+                        if (same) {
+                            reinterpret_cast<uint4 *>(out - shift)[u] = x[j];
+                        } else {
 #pragma unroll
-                    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<uint4 *>(words + u * VEC + i) = make_uint4(0, 0, 0, 0);
-                }
-                if (!whole(u)) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        if (t + i < 0 || t + i >= p.V) continue;
-                        const bool masked = mask && !(mask[(t + i) >> 5] >> ((t + i) & 31) & 1);
-                        T h = in[t + i];
-                        if (w[i]) from_f(edited(to_f(h), w[i], r), h);
-                        if (masked) from_f(-INFINITY, h);
-                        if (w[i] || masked || !p.in_place) out[t + i] = h;
-                        if (to_f(h) > top) {
-                            top = to_f(h);
-                            at = t + i;
+                            for (int i = 0; i < VEC; ++i) out[t + i] = reinterpret_cast<const T *>(&x[j])[i];
                         }
                     }
-                    continue;
-                }
-                uint32_t allowed = (1u << VEC) - 1;
-                if (mask) {
-                    const int k = t >> 5, s = t & 31;
-                    const unsigned lo = mask[k], hi = s > 32 - VEC && k + 1 < mask_words ? mask[k + 1] : 0u;
-                    allowed &= __funnelshift_r(lo, hi, s);
-                }
-                const bool changed = any || allowed != (1u << VEC) - 1;
-                if (lean) {
-                    if (!changed) continue;
-                    x[j] = *reinterpret_cast<const uint4 *>(in + t);
-                }
-                T *h = reinterpret_cast<T *>(&x[j]);
-                if (changed) {
+                    if (NEXT && (!MASK || allowed[j]) && top_of(x[j], T()) > top) {
+                        const int w = t - t0;
+                        const uint32_t skip = n_edit ? bits[w >> 5] >> (w & 31) : 0u;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        if (w[i]) from_f(edited(to_f(h[i]), w[i], r), h[i]);
-                        if (!(allowed >> i & 1)) from_f(-INFINITY, h[i]);
-                    }
-                }
-                if (same) {
-                    if (changed || !p.in_place) *reinterpret_cast<uint4 *>(out + t) = x[j];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) out[t + i] = h[i];
-                }
-                if (p.next && top_of(x[j], T()) > top) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i)
-                        if (to_f(h[i]) > top) {
-                            top = to_f(h[i]);
-                            at = t + i;
+                        for (int i = 0; i < VEC; ++i) {
+                            const float y = to_f(reinterpret_cast<const T *>(&x[j])[i]);
+                            if (y > top && !(skip >> i & 1)) {
+                                top = y;
+                                at = t + i;
+                            }
                         }
+                    }
                 }
             }
+            // the tokens of a row's first and last vector where those are not whole
+            const int t = tid < VEC ? tid - shift : f1 * VEC - shift + tid - VEC;
+            if (tid < 2 * VEC && inside(t) && (tid < VEC ? shift != 0 && t < VEC - shift : f1 >= f0)) {
+                T y = in[t];
+                const bool gone = masked(t);
+                if (gone) from_f(-INFINITY, y);
+                if (gone || !p.in_place) out[t] = y;
+                if (NEXT && !(n_edit && (bits[(t - t0) >> 5] >> ((t - t0) & 31) & 1))) better(to_f(y), t);
+            }
+        };
+        // Without a choice the pass needs nothing of the history, whose loads it then covers.
+        if (!NEXT && dense) dense_pass(0);
+
+        // Marks a token; the first to do so puts it on the list. The whole warp comes here.
+        const auto mark = [&](bool in_here, int w, uint32_t before) {
+            const bool first = in_here && before == 0;
+            const unsigned all = __ballot_sync(0xFFFFFFFFu, first);
+            if (!all) return;
+            int place = 0;
+            if (lane == 0) place = atomicAdd(&n_touched, __popc(all));
+            place = __shfl_sync(0xFFFFFFFFu, place, 0) + __popc(all & ((1u << lane) - 1));
+            if (first) {
+                touched[place] = static_cast<uint16_t>(w);
+                if (NEXT) atomicOr(&bits[w >> 5], 1u << (w & 31));
+            }
+        };
+        for (int i0 = warp * 32; i0 < r.nb; i0 += NT) {
+            const int i = i0 + lane, t = i < r.nb ? btok[i] : -1;
+            const bool here = inside(t);
+            uint32_t before = 0;
+            if (here) before = atomicMax(&words[t - t0], static_cast<uint32_t>(MAX_BIAS - i) << BIAS_AT);
+            if (before) dups = 1;
+            mark(here, t - t0, before);
+        }
+        if (r.nb) __syncthreads();  // the counts go below the entries
+        // Of the history, a warp first gathers what lies in the segment: with 8 CTAs to a row that is an eighth.
+        uint32_t *gathered = gather[warp];
+        for (int i0 = warp * 32; i0 < n; i0 += NT * AHEAD) {
+            if (i0 != warp * 32) tokens(i0);
+            int got = 0;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const bool here = inside(h[k]);
+                const unsigned all = __ballot_sync(0xFFFFFFFFu, here);
+                if (here) gathered[got + __popc(all & ((1u << lane) - 1))] = static_cast<uint32_t>(h[k] - t0) | (i0 + k * NT + lane < from ? SEEN : 0u);
+                got += __popc(all);
+            }
+            __syncwarp();
+            for (int i = 0; i < got; i += 32) {
+                const bool here = i + lane < got;
+                const uint32_t g = here ? gathered[i + lane] : 0u;
+                const int w = static_cast<int>(g & ~SEEN);
+                uint32_t before = 0;
+                if (here) before = g & SEEN ? atomicOr(&words[w], SEEN) : atomicAdd(&words[w], 1u);
+                mark(here, w, before);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+        const int n_edit = n_touched;
+        const float early = tid < n_edit ? to_f(in[t0 + touched[tid]]) : 0.0f;  // what the sparse pass needs first
+        if (NEXT) {
+            dense_pass(n_edit);
+            __syncthreads();  // an edited logit replaces what the vectors wrote
+        }
+
+        for (int i = tid; i < n_edit; i += NT) {
+            const int w = touched[i], t = t0 + w;
+            const uint32_t word = words[w];
+            words[w] = bits[w >> 5] = 0;
+            if (masked(t)) continue;
+            T y;
+            from_f(edited(i == tid ? early : to_f(in[t]), word, r), y);
+            out[t] = y;
+            if (NEXT) better(to_f(y), t);
         }
     }
     __syncwarp();
-    if (p.cluster > 1) cluster_wait();
-    if (p.next) {
+    if (NEXT && p.cluster > 1) cluster_wait();
+    if (NEXT) {
         // 0.0 + top: equal zeros have equal keys
         unsigned long long key = at < 0 ? 0ull : lin::argmax_key(top + 0.0f, static_cast<unsigned>(at));
 #pragma unroll
@@ -269,8 +349,8 @@ __global__ void __launch_bounds__(NT) k_logits_edit(const Params p) {
         }
     }
     __syncwarp();
-    if (p.cluster > 1) cluster_sync_all();
-    if (p.next && tell) {
+    if (NEXT && p.cluster > 1) cluster_sync_all();
+    if (NEXT && tell) {
         unsigned long long key = row_best[0];
         for (int i = 1; i < p.cluster; ++i) key = max(key, row_best[i]);
         if (!key) atomicOr(p.status, ST_EDIT_NO_TOKEN);
@@ -278,9 +358,10 @@ __global__ void __launch_bounds__(NT) k_logits_edit(const Params p) {
     }
 }
 
+typedef void (*Kernel)(Params);
 template <typename T>
-int set_attr() {
-    return cudaFuncSetAttribute(k_logits_edit<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SEG + 2 * MAX_BIAS) * 4) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+Kernel kernel(bool mask, bool next) {
+    return mask ? (next ? k_logits_edit<T, true, true> : k_logits_edit<T, true, false>) : (next ? k_logits_edit<T, false, true> : k_logits_edit<T, false, false>);
 }
 
 }  // namespace
@@ -302,7 +383,9 @@ int check(const GPT2LogitsEdit *e, int rows, int V) {
 int prepare(DeviceContext *ctx) {
     if (ctx->edit_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
-    if (set_attr<__half>() != GPT2_B200_OK || set_attr<float>() != GPT2_B200_OK) return GPT2_B200_ECUDA;
+    for (int i = 0; i < 4; ++i)
+        for (const Kernel k : {kernel<__half>(i & 1, i & 2), kernel<float>(i & 1, i & 2)})
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (SEG + SEG / 16 + SEG / 2 + 2 * MAX_BIAS) * 4) != cudaSuccess) return GPT2_B200_ECUDA;
     ctx->edit_attr_done = true;
     return GPT2_B200_OK;
 }
@@ -325,18 +408,20 @@ int launch(DeviceContext *ctx, void *out, long long ldo, const void *in, long lo
     p.next = next;
     p.status = ctx->status;
     const long long vectors = (V + 2ll * (vec - 1)) / vec;
-    int c = MAX_CLUSTER;
-    while (c > 1 && (static_cast<long long>(rows) * c > 4ll * ctx->num_sms || vectors < c * 64)) c /= 2;
+    // A row's CTAs: as many as run at once, and so many that a segment is all a CTA has, since each segment reads the history again.
+    int c = 1;
+    while (c < MAX_CLUSTER && vectors >= c * 128 && (static_cast<long long>(rows) * c * 2 <= 2ll * ctx->num_sms || vectors * vec > 1ll * c * SEG)) c *= 2;
     p.cluster = c;
-    p.seg = static_cast<int>(std::min<long long>(SEG, (vectors + c - 1) / c * vec));
+    p.seg = static_cast<int>(std::min<long long>(SEG, ((vectors + c - 1) / c * vec + 127) / 128 * 128));  // what a warp looks at at once
+    p.list = static_cast<int>(std::min<long long>(p.seg, ((e.history ? e.max_history : 0) + p.e.max_bias + 7ll) / 8 * 8));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * c, 1, 1);
     cfg.blockDim = dim3(NT, 1, 1);
-    cfg.dynamicSmemBytes = static_cast<size_t>(p.seg + 2 * p.e.max_bias) * 4;
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.seg + p.seg / 16 + p.list / 2 + 2 * p.e.max_bias) * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int na = 0;
-    if (c > 1) {
+    if (c > 1 && next) {  // a row's CTAs meet only over its choice
         attr[na].id = cudaLaunchAttributeClusterDimension;
         attr[na].val.clusterDim.x = static_cast<unsigned>(c);
         attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
@@ -349,8 +434,8 @@ int launch(DeviceContext *ctx, void *out, long long ldo, const void *in, long lo
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    const cudaError_t err = type == GPT2_BEAM_HALF ? cudaLaunchKernelEx(&cfg, k_logits_edit<__half>, p) : cudaLaunchKernelEx(&cfg, k_logits_edit<float>, p);
-    return err == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    const Kernel k = type == GPT2_BEAM_HALF ? kernel<__half>(e.mask, next) : kernel<float>(e.mask, next);
+    return cudaLaunchKernelEx(&cfg, k, p) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
 }  // namespace edit

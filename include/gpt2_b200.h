@@ -463,9 +463,9 @@ typedef struct {
 } GPT2LogitsEdit;
 
 /* out[r] = the edited logits[r], r < rows: rows of V values, type GPT2_BEAM_HALF or GPT2_BEAM_FLOAT, at strides ldo and ld >= V
- * (elements; any alignment). out may be logits itself with ldo = ld (then only what changes is written, and without d_next only that is
- * read); otherwise the two must not overlap. d_next (if not NULL): the token of the largest written value of each row, the lowest of equal ones; NaN
- * is never chosen, and a row that has nothing above -inf gives -1 (status bit). */
+ * (elements; any alignment). out may be logits itself with ldo = ld (then only what changes is written; without a mask and d_next
+ * only that is read); otherwise the two must not overlap. d_next (if not NULL): the token of the largest written value of each row, the lowest
+ * of equal ones; NaN is never chosen, and a row that has nothing above -inf gives -1 (status bit). */
 int gpt2_logits_edit_b200(void *out, long long ldo, const void *logits, long long ld, int type, int rows, int V, const GPT2LogitsEdit *edit,
                           int *d_next, cudaStream_t stream);
 
