@@ -25,30 +25,35 @@ __device__ __forceinline__ float gelu_new(float v) {
 struct Extra {
     float bias, resid;
 };
+__device__ __forceinline__ float bias_of(const Dest &d, int n) { return d.bias && n < d.N ? __half2float(d.bias[n]) : 0.0f; }
 __device__ __forceinline__ Extra extra_of(const Dest &d, int b, int n) {
-    return {d.bias ? __half2float(d.bias[n]) : 0.0f, d.epi == EPI_RESID ? __half2float(d.resid[b * d.ldr + n]) : 0.0f};
+    return {bias_of(d, n), d.epi == EPI_RESID ? __half2float(d.resid[b * d.ldr + n]) : 0.0f};
 }
 
-// One output of row b and feature n, both in range; acc holds the whole sum.
-__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc, const Extra &e) {
+// The output of a sum, and its place in the K/V cache if it has one.
+__device__ __forceinline__ __half shaped(const Dest &d, float acc, const Extra &e) {
     acc += e.bias;
     if (d.epi == EPI_GELU) acc = gelu_new(acc);
     if (d.epi == EPI_RESID) acc += e.resid;
-    const __half h = __float2half_rn(acc);
+    return __float2half_rn(acc);
+}
+__device__ __forceinline__ void to_cache(const Dest &d, int b, int n, __half h) {
+    if (d.epi != EPI_QKV || n < d.E) return;
+    int m = n - d.E;
+    const bool is_v = m >= d.E;
+    if (is_v) m -= d.E;
+    const int pos = d.d_pos[b];
+    if (pos < 0 || pos >= d.maxT)
+        atomicOr(d.status, ST_KV_BAD_POS);
+    else
+        (is_v ? d.v_dst[b] : d.k_dst[b])[(static_cast<long long>(m >> 6) * d.maxT + pos) * 64 + (m & 63)] = h;
+}
+__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc, const Extra &e) {
+    const __half h = shaped(d, acc, e);
     if (d.out) d.out[b * d.ldo + n] = h;
-    if (d.epi == EPI_QKV && n >= d.E) {
-        int m = n - d.E;
-        const bool is_v = m >= d.E;
-        if (is_v) m -= d.E;
-        const int pos = d.d_pos[b];
-        if (pos < 0 || pos >= d.maxT)
-            atomicOr(d.status, ST_KV_BAD_POS);
-        else
-            (is_v ? d.v_dst[b] : d.k_dst[b])[(static_cast<long long>(m >> 6) * d.maxT + pos) * 64 + (m & 63)] = h;
-    }
+    to_cache(d, b, n, h);
     return h;
 }
-__device__ __forceinline__ __half put(const Dest &d, int b, int n, float acc) { return put(d, b, n, acc, extra_of(d, b, n)); }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -68,7 +73,7 @@ constexpr int CHUNK = 128;
 constexpr int ROW_WARPS = 8;
 constexpr int DEPTH = 4;
 constexpr int ROW_CTAS = 2;  // per SM
-constexpr int ROWS_MAX_B = 16;
+constexpr int ROWS_MAX_B = 8;
 constexpr int PANEL_BYTES = 88 * 1024;  // of x in shared memory
 
 struct RowParams {
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
                 float sum = 0.0f;
 #pragma unroll
                 for (int q = 0; q < WK; ++q) sum += red[turn][q][n][b];
-                const float h = __half2float(unit == sub ? put(d, b, n0 + n, sum, early) : put(d, b, n0 + n, sum)) + 0.0f;
+                const float h = __half2float(put(d, b, n0 + n, sum, unit == sub ? early : extra_of(d, b, n0 + n))) + 0.0f;
                 if (h == h) key = lin::argmax_key(h, static_cast<unsigned>(n0 + n));
             }
             if (d.epi == EPI_HEAD) {
@@ -258,54 +263,85 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
     }
 }
 
-// ---------------------------------------------------------------- tensor-core form
-constexpr int BM = 128;                  // features of a tile: the MMA's M, one TMEM lane each
-constexpr int KS = 128;                  // k of a stage
-constexpr int CODE_BYTES = BM * KS / 2;  // 8 KB of codes
-constexpr int CODE_RING = 8;             // stages of codes in flight (even: each warpgroup has slots of its own)
-constexpr int X_ATOM = 64;               // k of a piece of x: one 128-byte swizzle row
-constexpr int MAX_X_RING = 16;           // pieces of x in flight
-constexpr int A_BUFS = 4;                // converted stages: TMEM columns of 64 each
-constexpr int A_COLS = KS / 2;
+// ---------------------------------------------------------------- many rows
+// B > 16, on tcgen05: 256 features x up to 128 rows of x per CTA, as two MMAs of 128 features that share x; more rows are
+// several column blocks. Sums of 128 k at a time:
+//   warp 0       TMA of the codes, 2 x 128 features x 64 bytes (64-byte swizzle), as they lie;
+//   warp 2       TMA of x, 128-byte swizzle, K-major: the MMAs' B operand;
+//   warps 4-11   a warpgroup per 128 features: a thread converts the 128 codes of one feature into 64 TMEM columns, the MMA's A operand;
+//   warp 1       16 MMAs (K 16) from TMEM and shared memory, accumulators in TMEM;
+//   warps 12-15  the epilogue of a finished tile, while the others are at the next; at the last tile all three warpgroups.
+// A hand-over through an mbarrier costs each role 200 to 400 cycles, and HBM delivers the codes of a stage in 700: so a stage is 32768
+// codes and each role passes one barrier per stage. Two tiles of features per x halve what x costs the L2: at 128 rows of x, 16 KB
+// of codes come with 32 KB of x (one tile of 128 x 256: 8 with 64, 10 TB/s from the L2 and no more).
+// A few features and a long k: the CTAs of a cluster share a tile's k and add their sums through distributed shared memory, in rank order.
+constexpr int BM = 128;                      // features of an MMA, one TMEM lane each
+constexpr int TILES = 2;                     // MMAs side by side
+constexpr int FEATURES = BM * TILES;
+constexpr int KS = 128;                      // k of a stage
+constexpr int CODE_BYTES = FEATURES * KS / 2;
+constexpr int CODE_RING = 4;
+constexpr int MAX_X_RING = 8;
+constexpr int MAX_COLS = 128;                // rows of x per block
+constexpr int PUSH_COLS = 64;                // columns up to which the rings leave room for the cluster's sums
+constexpr int A_BUFS = 2;                    // converted stages
+constexpr int A_COLS = KS / 2;               // TMEM columns of one
 constexpr int TC_THREADS = 512;
-constexpr size_t TC_SMEM = 227 * 1024;  // the SM for itself: no other CTA's TMEM allocation meets this one's
+constexpr size_t TC_SMEM = 226 * 1024;       // the SM for itself: no other CTA's TMEM allocation meets this one's
 
 struct TcParams {
     const __half *scale, *least;
     int K, group;
     int stages, cs, tiles;   // per tile; CTAs that share a tile's k; tiles
-    int x_ring, bpad, nacc;  // pieces of x in flight; columns; accumulators
+    int x_ring, bpad, nacc;  // stages of x in flight; columns; accumulators
+    int push, share;         // split k: sums are pushed to the CTA that adds them (else pulled); columns that each adds
     Dest d;
     unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ float dsmem_ld_f32(uint32_t cluster_saddr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_saddr) : "memory");
+__device__ __forceinline__ float4 dsmem_ld_v4(uint32_t cluster_saddr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_saddr) : "memory");
     return v;
 }
+__device__ __forceinline__ void dsmem_st_f32(uint32_t cluster_saddr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_saddr), "f"(v) : "memory");
+}
 
-// Columns [c0, c1) of this warp's 32 features out of TMEM, through the epilogue. acc: the accumulator's first column.
-__device__ __forceinline__ void epilogue(const Dest &d, uint32_t acc, int warp4, int lane, int n0, int tile, int c0, int c1) {
-    const int n = n0 + warp4 * 32 + lane;
-    const uint32_t row = acc + (static_cast<uint32_t>(warp4 * 32) << 16);
-    for (int c = c0; c < c1; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(row + c, r);
-        tmem_wait_ld();
+// 16 columns from c on of this warp's 32 features out of TMEM, through the epilogue. acc: the accumulator's first column; n: this lane's
+// feature; b0: the block's first row of x. Everything is read before the first output is written: the compiler cannot know that
+// an output is no input of the next, and would wait for each.
+__device__ __forceinline__ void epilogue(const Dest &d, uint32_t acc, int warp4, int lane, int n, float bias, int b0, int c) {
+    uint32_t r[16];
+    tmem_ld16(acc + (static_cast<uint32_t>(warp4 * 32) << 16) + c, r);
+    const int first = b0 + c, many = min(16, d.B - first);
+    float resid[16];
+    if (d.epi == EPI_RESID) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) resid[j] = j < many && n < d.N ? __half2float(d.resid[(first + j) * d.ldr + n]) : 0.0f;
+    }
+    tmem_wait_ld();
+    __half h[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) h[j] = shaped(d, __uint_as_float(r[j]), {bias, d.epi == EPI_RESID ? resid[j] : 0.0f});
+    if (d.out && n < d.N) {
+        __half *out = d.out + first * d.ldo + n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < many) out[j * d.ldo] = h[j];
+    }
+    if (d.epi == EPI_QKV && n < d.N)
+        for (int j = 0; j < 16; ++j)
+            if (j < many) to_cache(d, first + j, n, h[j]);
+    if (d.epi == EPI_HEAD) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int b = c + j;
-            if (b >= d.B) break;
-            __half h = __float2half_rn(0.0f);
-            if (n < d.N) h = put(d, b, n, __uint_as_float(r[j]));
-            if (d.epi == EPI_HEAD) {
-                const float v = __half2float(h) + 0.0f;
-                const unsigned long long key = n < d.N && v == v ? lin::argmax_key(v, static_cast<unsigned>(n)) : 0ull;
-                const unsigned hi = static_cast<unsigned>(key >> 32), mhi = __reduce_max_sync(0xFFFFFFFFu, hi);
-                const unsigned mlo = __reduce_max_sync(0xFFFFFFFFu, hi == mhi ? static_cast<unsigned>(key) : 0u);
-                if (lane == 0) d.amax[static_cast<long long>(b) * d.keys + tile * 4 + warp4] = static_cast<unsigned long long>(mhi) << 32 | mlo;
-            }
+            if (j >= many) break;
+            const float v = __half2float(h[j]) + 0.0f;
+            const unsigned long long key = n < d.N && v == v ? lin::argmax_key(v, static_cast<unsigned>(n)) : 0ull;
+            const unsigned hi = static_cast<unsigned>(key >> 32), mhi = __reduce_max_sync(0xFFFFFFFFu, hi);
+            const unsigned mlo = __reduce_max_sync(0xFFFFFFFFu, hi == mhi ? static_cast<unsigned>(key) : 0u);
+            if (lane == 0) d.amax[static_cast<long long>(first + j) * d.keys + n / 32] = static_cast<unsigned long long>(mhi) << 32 | mlo;
         }
     }
 }
@@ -321,36 +357,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     __shared__ int bad;  // a wait gave up: nothing more is written
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const x_smem = smem + CODE_RING * CODE_BYTES;
-    const int x_bytes = p.bpad * 2 * X_ATOM;
+    const int x_bytes = p.bpad * 2 * KS;
     const int rank = static_cast<int>(cluster_rank());
-    const int first_tile = blockIdx.x / p.cs, tile_step = gridDim.x / p.cs;
+    const int first_tile = blockIdx.x / p.cs, tile_step = gridDim.x / p.cs, b0 = blockIdx.y * p.bpad;
     const int my_tiles = (p.tiles - first_tile + tile_step - 1) / tile_step;
     const int s0 = rank * p.stages / p.cs, ns = (rank + 1) * p.stages / p.cs - s0;  // this CTA's stages of each tile
     const int total = my_tiles * ns;
 
-    if (tid == 0) {
-        for (int i = 0; i < CODE_RING; ++i) {
-            mbar_init(&c_full[i], 1);
-            mbar_init(&c_empty[i], 4);
+    if (warp == 0) {  // one after the other they would take as long as the first copy
+        if (lane < CODE_RING) {
+            mbar_init(&c_full[lane], 1);
+            mbar_init(&c_empty[lane], 8);
         }
-        for (int i = 0; i < MAX_X_RING; ++i) {
-            mbar_init(&x_full[i], 1);
-            mbar_init(&x_empty[i], 1);
+        if (lane < MAX_X_RING) {
+            mbar_init(&x_full[lane], 1);
+            mbar_init(&x_empty[lane], 1);
         }
-        for (int i = 0; i < A_BUFS; ++i) {
-            mbar_init(&a_full[i], 4);
-            mbar_init(&a_empty[i], 1);
+        if (lane < A_BUFS) {
+            mbar_init(&a_full[lane], 8);
+            mbar_init(&a_empty[lane], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 4);
+        if (lane < 2) {
+            mbar_init(&acc_full[lane], 1);
+            mbar_init(&acc_empty[lane], 4);
         }
-        mbar_init(&last_full, 1);
-        bad = 0;
+        if (lane == 31) {
+            mbar_init(&last_full, 1);
+            bad = 0;
+            tma_prefetch_desc(&tm_w);
+        }
+        if (lane == 30) tma_prefetch_desc(&tm_x);
         fence_mbar_init();
-        tma_prefetch_desc(&tm_w);
-        tma_prefetch_desc(&tm_x);
     }
+    if (p.cs > 1) cluster_arrive_relaxed();  // waited for before the first write to another CTA
     if (warp == 1) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
@@ -358,7 +397,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm_a = tmem_slot, tm_acc = tmem_slot + A_BUFS * A_COLS;
+    const uint32_t tm_a = tmem_slot, tm_acc = tmem_slot + A_BUFS * TILES * A_COLS;
     grid_launch_dependents();
 
     const auto fail = [&] {
@@ -371,7 +410,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     if (warp == 0) {
         // Codes: they do not depend on the kernel before this one, so nothing waits for it.
         const bool leader = elect_one();
-        int it = 0, i = 0, n0 = first_tile * BM;
+        int it = 0, i = 0, n0 = first_tile * FEATURES;
         for (; it < total; ++it) {
             const int slot = it % CODE_RING;
             const bool ok = it < CODE_RING || mbar_wait(&c_empty[slot], (it / CODE_RING - 1) & 1, p.timeout_ns);
@@ -381,11 +420,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             }
             if (leader) {
                 mbar_arrive_expect_tx(&c_full[slot], CODE_BYTES);
-                tma_load_2d(smem + slot * CODE_BYTES, &tm_w, &c_full[slot], (s0 + i) * (KS / 2), n0);
+#pragma unroll
+                for (int w = 0; w < TILES; ++w)
+                    tma_load_2d(smem + slot * CODE_BYTES + w * (CODE_BYTES / TILES), &tm_w, &c_full[slot], (s0 + i) * (KS / 2), n0 + w * BM);
             }
             if (++i == ns) {
                 i = 0;
-                n0 += tile_step * BM;
+                n0 += tile_step * FEATURES;
             }
             __syncwarp();
         }
@@ -398,7 +439,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
         const bool leader = elect_one();
         int i = 0, slot = 0, at = 0;
         uint32_t phase = 1;  // of x_empty: passed at once while the ring fills
-        for (; at < 2 * total; ++at) {
+        for (; at < total; ++at) {
             const bool ok = mbar_wait(&x_empty[slot], phase, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 fail();
@@ -406,9 +447,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             }
             if (leader) {
                 mbar_arrive_expect_tx(&x_full[slot], static_cast<uint32_t>(x_bytes));
-                tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], s0 * KS + i * X_ATOM, 0);
+                tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], (s0 + i) * KS, b0);
+                tma_load_2d(x_smem + slot * x_bytes + x_bytes / 2, &tm_x, &x_full[slot], (s0 + i) * KS + 64, b0);
             }
-            if (++i == 2 * ns) i = 0;
+            if (++i == ns) i = 0;
             if (++slot == p.x_ring) {
                 slot = 0;
                 phase ^= 1;
@@ -429,33 +471,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&acc_empty[acc], acc_phase, p.timeout_ns));
             for (int i = 0; i < ns && ok; ++i, ++it) {
                 const int buf = it % A_BUFS;
-                ok = mbar_wait_spin(&a_full[buf], (it / A_BUFS) & 1, p.timeout_ns);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    ok = ok && mbar_wait_spin(&x_full[slot], x_phase, p.timeout_ns);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint32_t off = static_cast<uint32_t>(slot) * x_step;
-#pragma unroll
-                        for (int kk = 0; kk < X_ATOM / 16; ++kk)
-                            umma_f16_ts_lohi(tm_acc + acc * p.bpad, tm_a + buf * A_COLS + h * (X_ATOM / 2) + kk * 8, x_lo + off + kk * 2, x_hi, idesc,
-                                             i > 0 || h > 0 || kk > 0 ? 1u : 0u);
-                        umma_commit(&x_empty[slot]);
-                    }
-                    __syncwarp();
-                    if (++slot == p.x_ring) {
-                        slot = 0;
-                        x_phase ^= 1;
-                    }
-                }
+                ok = mbar_wait_spin(&x_full[slot], x_phase, p.timeout_ns) && mbar_wait_spin(&a_full[buf], (it / A_BUFS) & 1, p.timeout_ns);
+                ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
+                tc_fence_after();
                 if (leader) {
+                    const uint32_t off = static_cast<uint32_t>(slot) * x_step;
+#pragma unroll
+                    for (int w = 0; w < TILES; ++w)
+#pragma unroll
+                        for (int kk = 0; kk < KS / 16; ++kk)
+                            umma_f16_ts_lohi(tm_acc + (acc * TILES + w) * p.bpad, tm_a + (buf * TILES + w) * A_COLS + kk * 8,
+                                             x_lo + off + kk / 4 * (x_step / 2) + kk % 4 * 2, x_hi, idesc, i > 0 || kk > 0 ? 1u : 0u);
                     umma_commit(&a_empty[buf]);
+                    umma_commit(&x_empty[slot]);
                     if (i == ns - 1) umma_commit(&acc_full[acc]);
                 }
                 __syncwarp();
+                if (++slot == p.x_ring) {
+                    slot = 0;
+                    x_phase ^= 1;
+                }
             }
             if (++acc == p.nacc) {
                 acc = 0;
@@ -466,20 +502,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
         __syncwarp();
         if (leader) umma_commit(&last_full);  // arrives when all that was issued is done
     } else if (warp >= 4 && warp < 12) {
-        // Two warpgroups take every other stage: a thread converts the 128 codes of one feature, 64 TMEM columns.
         const int wg = (warp - 4) >> 2, warp4 = warp & 3, row = warp4 * 32 + lane;
-        const uint32_t lanes = static_cast<uint32_t>(warp4 * 32) << 16;
+        const uint32_t to = tm_a + wg * A_COLS + (static_cast<uint32_t>(warp4 * 32) << 16);
+        const uint8_t *from = smem + wg * (CODE_BYTES / TILES) + row * 64;
         const int groups = p.K / p.group;
         __half sc[2][GS], lo[2][GS];
-        int si = wg, sn = first_tile * BM + row;  // the stage and the feature of the scales that are fetched next
-        const auto settle = [&] {
-            while (si >= ns) {
-                si -= ns;
-                sn += tile_step * BM;
-            }
-        };
+        int si = 0, sn = first_tile * FEATURES + wg * BM + row;  // the stage and the feature of the scales that are fetched next
         const auto scales = [&](__half (&s)[GS], __half (&l)[GS]) {
-            settle();
             const int g0 = (s0 + si) * GS;
 #pragma unroll
             for (int q = 0; q < GS; ++q) {
@@ -488,23 +517,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
                 s[q] = in ? p.scale[at] : __float2half_rn(0.0f);
                 if (LEAST) l[q] = in ? p.least[at] : __float2half_rn(0.0f);
             }
-            si += 2;
+            if (++si == ns) {
+                si = 0;
+                sn += tile_step * FEATURES;
+            }
         };
         scales(sc[0], lo[0]);
         scales(sc[1], lo[1]);
         bool ok = true;
-        for (int it0 = wg; it0 < total && ok; it0 += 4) {
+        for (int it0 = 0; it0 < total && ok; it0 += 2) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int it = it0 + 2 * u;
+            for (int u = 0; u < 2; ++u) {  // u: the buffer
+                const int it = it0 + u;
                 if (it >= total || !ok) break;
-                const int slot = it % CODE_RING, buf = it % A_BUFS;
+                const int slot = it % CODE_RING;
                 ok = mbar_wait(&c_full[slot], (it / CODE_RING) & 1, p.timeout_ns);
-                if (it >= A_BUFS) ok = ok && mbar_wait(&a_empty[buf], (it / A_BUFS - 1) & 1, p.timeout_ns);
+                if (it >= A_BUFS) ok = ok && mbar_wait(&a_empty[u], (it / A_BUFS - 1) & 1, p.timeout_ns);
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint8_t *st = smem + slot * CODE_BYTES + row * 64;
+                const uint8_t *st = from + slot * CODE_BYTES;
                 bool large = false;
 #pragma unroll
                 for (int q = 0; q < GS; ++q) large = large || big_scale(__half_as_ushort(sc[u][q]));
@@ -526,20 +558,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
                                 for (int e = 0; e < 4; ++e) v[q * 16 + j * 4 + e] = four[e];
                             }
                         }
-                        tmem_st32(tm_a + lanes + buf * A_COLS + h * 32, v);
+                        tmem_st32(to + u * (TILES * A_COLS) + h * 32, v);
                     }
                 };
                 if (__any_sync(0xFFFFFFFFu, large))
                     convert(std::true_type());
                 else
                     convert(std::false_type());
-                if (it + 4 < total) scales(sc[u], lo[u]);
+                if (it + 2 < total) scales(sc[u], lo[u]);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&c_empty[slot]);
-                    mbar_arrive(&a_full[buf]);
+                    mbar_arrive(&a_full[u]);
                 }
             }
         }
@@ -547,30 +579,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     }
     __syncwarp();
 
-    // The epilogue warps take each tile as it is done; at the last one, when nothing is left to convert, the others help.
+    // Sums that another CTA of the cluster adds: pushed into a buffer of its own there, or left where the rings were.
+    const uint32_t parts = smem_u32(smem) + (p.push ? CODE_RING * CODE_BYTES + p.x_ring * x_bytes : 0);
+    if (p.cs > 1) cluster_wait();
     if (warp >= 4) {
         const int wg = (warp - 4) >> 2, warp4 = warp & 3;  // 2: the epilogue's own
         for (int j = wg == 2 ? 0 : my_tiles - 1; j < my_tiles; ++j) {
-            const int acc = j % p.nacc, tile = first_tile + j * tile_step;
-            const int cols = p.bpad / 16;
+            const int acc = j % p.nacc, n0 = (first_tile + j * tile_step) * FEATURES;
             const bool last = j == my_tiles - 1;
             const bool ok = last ? mbar_wait(&last_full, 0, p.timeout_ns) : mbar_wait(&acc_full[acc], (j / p.nacc) & 1, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) fail();
             __syncwarp();
             if (*reinterpret_cast<volatile int *>(&bad)) break;
             tc_fence_after();
-            const int c0 = last ? wg * cols / 3 * 16 : 0, c1 = last ? (wg + 1) * cols / 3 * 16 : p.bpad;
-            if (p.cs == 1) {
-                epilogue(p.d, tm_acc + acc * p.bpad, warp4, lane, tile * BM, tile, c0, c1);
-            } else {
-                float *part = reinterpret_cast<float *>(smem);  // the ring has been read: [column][feature]
-                const uint32_t row = tm_acc + acc * p.bpad + (static_cast<uint32_t>(warp4 * 32) << 16);
-                for (int c = c0; c < c1; c += 16) {
+            const int pieces = p.bpad / 16 * TILES;  // w for every 16 columns; a warp's part keeps to one w where it can
+            const int first = last ? wg * pieces / 3 : 0, behind = last ? (wg + 1) * pieces / 3 : pieces;
+            for (int piece = first; piece < behind; ++piece) {
+                const int w = piece / (pieces / TILES), c = piece % (pieces / TILES) * 16, f = w * BM + warp4 * 32 + lane;
+                const uint32_t from = tm_acc + (acc * TILES + w) * p.bpad;
+                if (p.cs == 1) {
+                    epilogue(p.d, from, warp4, lane, n0 + f, bias_of(p.d, n0 + f), b0, c);
+                } else {
                     uint32_t r[16];
-                    tmem_ld16(row + c, r);
+                    tmem_ld16(from + (static_cast<uint32_t>(warp4 * 32) << 16) + c, r);
                     tmem_wait_ld();
+                    if (p.push) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) part[(c + i) * BM + warp4 * 32 + lane] = __uint_as_float(r[i]);
+                        for (int i = 0; i < 16; ++i) {
+                            const int q = (c + i) / p.share, at = ((rank * p.share + c + i - q * p.share) * FEATURES + f) * 4;
+                            dsmem_st_f32(dsmem_addr(parts + at, static_cast<uint32_t>(q)), __uint_as_float(r[i]));
+                        }
+                    } else {
+                        float *part = reinterpret_cast<float *>(smem);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) part[(c + i) * FEATURES + f] = __uint_as_float(r[i]);
+                    }
                 }
             }
             tc_fence_before();
@@ -580,23 +623,54 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     }
     __syncwarp();
     if (p.cs > 1) {
-        // Each CTA of the cluster sums its share of the columns over the ranks, in their order.
+        // Every CTA of the cluster has `share` of the columns, and adds them over the ranks in their order: 4 features a thread.
+        const int f = tid % (FEATURES / 4) * 4, n = first_tile * FEATURES + f, c0 = rank * p.share + tid / (FEATURES / 4);
+        const int c1 = min(min(p.d.B - b0, p.bpad), (rank + 1) * p.share);
+        float bias[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bias[i] = bias_of(p.d, n + i);
         cluster_sync_all();
-        const uint32_t part = smem_u32(smem) + (tid & (BM - 1)) * 4;
-        const int n = first_tile * BM + (tid & (BM - 1));
-        const int b1 = min(p.d.B, (rank + 1) * p.bpad / p.cs);
-        for (int b = rank * p.bpad / p.cs + tid / BM; b < b1; b += TC_THREADS / BM) {
-            float v[lin::MAX_CLUSTER];
+        for (int c = c0; c < c1; c += TC_THREADS / (FEATURES / 4)) {
+            const int b = b0 + c;
+            float4 v[lin::MAX_CLUSTER];
 #pragma unroll
-            for (int q = 0; q < lin::MAX_CLUSTER; ++q)
-                if (q < p.cs) v[q] = dsmem_ld_f32(dsmem_addr(part + b * BM * 4, static_cast<uint32_t>(q)));
-            float sum = v[0];
+            for (int q = 0; q < lin::MAX_CLUSTER; ++q) {
+                if (q >= p.cs) break;
+                v[q] = p.push ? lds_v4(parts + ((q * p.share + c - rank * p.share) * FEATURES + f) * 4)
+                              : dsmem_ld_v4(dsmem_addr(parts + (c * FEATURES + f) * 4, static_cast<uint32_t>(q)));
+            }
+            float resid[4] = {};
+            if (p.d.epi == EPI_RESID) {
 #pragma unroll
-            for (int q = 1; q < lin::MAX_CLUSTER; ++q)
-                if (q < p.cs) sum += v[q];
-            if (n < p.d.N && !*reinterpret_cast<volatile int *>(&bad)) put(p.d, b, n, sum);
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.d.N) resid[i] = __half2float(p.d.resid[b * p.d.ldr + n + i]);
+            }
+            float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int q = 1; q < lin::MAX_CLUSTER; ++q) {
+                if (q >= p.cs) break;
+                sum[0] += v[q].x;
+                sum[1] += v[q].y;
+                sum[2] += v[q].z;
+                sum[3] += v[q].w;
+            }
+            if (*reinterpret_cast<volatile int *>(&bad)) break;
+            __half h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = shaped(p.d, sum[i], {bias[i], resid[i]});
+            __half *out = p.d.out + b * p.d.ldo + n;
+            if (n + 3 < p.d.N && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+                *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(h);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.d.N) out[i] = h[i];
+            }
+            if (p.d.epi == EPI_QKV)
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.d.N) to_cache(p.d, b, n + i, h[i]);
         }
-        cluster_sync_all();
+        if (!p.push) cluster_sync_all();  // the others may still be reading this CTA's sums
     }
     tc_fence_before();
     __syncthreads();
@@ -633,7 +707,7 @@ int active_clusters(DeviceContext *ctx, int cs) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(cs) * 64, 1, 1);
     cfg.blockDim = dim3(TC_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = TC_SMEM - 1024;
+    cfg.dynamicSmemBytes = TC_SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(cs);
@@ -652,14 +726,14 @@ int prepare_tc(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
     for (const TcKernel k : {k_w4_tc<1, false>, k_w4_tc<2, false>, k_w4_tc<4, false>, k_w4_tc<1, true>, k_w4_tc<2, true>, k_w4_tc<4, true>})
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM - 1024)) != cudaSuccess) return GPT2_B200_ECUDA;
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
     ctx->w4_attr_done = true;
     return GPT2_B200_OK;
 }
 
 }  // namespace
 
-int keys_of(const GPT2W4 &w, int B) { return B <= ROWS_MAX_B ? (w.N + 15) / 16 : (w.N + BM - 1) / BM * 4; }
+int keys_of(const GPT2W4 &w, int B) { return B <= ROWS_MAX_B ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * 8; }
 
 int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo) {
     if (!weight_ok(&w) || !x || (reinterpret_cast<uintptr_t>(x) & 15) || (ldx & 7) || ldx < w.K || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
@@ -756,28 +830,32 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     p.K = w.K;
     p.group = w.group;
     p.stages = (w.K + KS - 1) / KS;
-    p.tiles = (w.N + BM - 1) / BM;
-    p.bpad = (pl.d.B + 15) / 16 * 16;
-    p.nacc = p.bpad <= 128 ? 2 : 1;
+    p.tiles = (w.N + FEATURES - 1) / FEATURES;
+    const int blocks = (pl.d.B + MAX_COLS - 1) / MAX_COLS;  // of equal width
+    p.bpad = ((pl.d.B + blocks - 1) / blocks + 15) / 16 * 16;
+    p.nacc = p.bpad <= 64 ? 2 : 1;
     p.d = pl.d;
     p.timeout_ns = wait_timeout_ns();
-    p.x_ring = std::min<int>(MAX_X_RING, static_cast<int>((TC_SMEM - 3072 - CODE_RING * CODE_BYTES) / (p.bpad * 2 * X_ATOM)));
     // The widest split of k whose clusters all run at once.
     p.cs = 1;
     if (pl.d.epi != EPI_HEAD)
         for (int c = std::min(lin::MAX_CLUSTER, p.stages); c > 1; --c)
-            if (p.tiles <= active_clusters(ctx, c)) {
+            if (p.tiles * blocks <= active_clusters(ctx, c)) {
                 p.cs = c;
                 break;
             }
+    p.share = (p.bpad + p.cs - 1) / p.cs;
+    p.push = p.cs > 1 && p.bpad <= PUSH_COLS;
+    const size_t rest = TC_SMEM - 1024 - CODE_RING * CODE_BYTES - (p.push ? static_cast<size_t>(p.cs) * p.share * FEATURES * 4 : 0);
+    p.x_ring = std::min<int>(MAX_X_RING, static_cast<int>(rest / (p.bpad * 2 * KS)));
     CUtensorMap tm_w, tm_x;
     if (!encode(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, w.K / 2, w.N, w.K / 2, KS / 2, BM, CU_TENSOR_MAP_SWIZZLE_64B) ||
         !encode(&tm_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, pl.x, w.K, pl.d.B, pl.ldx * 2, 64, p.bpad, CU_TENSOR_MAP_SWIZZLE_128B))
         return GPT2_B200_EDEVICE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.cs > 1 ? p.tiles * p.cs : std::min(p.tiles, ctx->num_sms)), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.cs > 1 ? p.tiles * p.cs : std::min(p.tiles, std::max(1, ctx->num_sms / blocks))), blocks, 1);
     cfg.blockDim = dim3(TC_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = TC_SMEM - 1024;
+    cfg.dynamicSmemBytes = TC_SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int na = 0;
