@@ -268,9 +268,9 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
 // several column blocks. Sums of 128 k at a time:
 //   warp 0       TMA of the codes, 2 x 128 features x 64 bytes (64-byte swizzle), as they lie;
 //   warp 2       TMA of x, 128-byte swizzle, K-major: the MMAs' B operand;
-//   warps 4-11   a warpgroup per 128 features: a thread converts the 128 codes of one feature into 64 TMEM columns, the MMA's A operand;
-//   warp 1       16 MMAs (K 16) from TMEM and shared memory, accumulators in TMEM;
-//   warps 12-15  the epilogue of a finished tile, while the others are at the next; at the last tile all three warpgroups.
+//   warps 4-19   two warpgroups per 128 features, at alternate stages: a thread converts the 128 codes of one feature into 64 TMEM
+//                columns, the MMA's A operand; they also take the finished tiles out of TMEM, once two stages of the next one are there;
+//   warps 1, 3   8 MMAs (K 16) each, from TMEM and shared memory, accumulators in TMEM: one waits while the other's run.
 // A hand-over through an mbarrier costs each role 200 to 400 cycles, and HBM delivers the codes of a stage in 700: so a stage is 32768
 // codes and each role passes one barrier per stage. Two tiles of features per x halve what x costs the L2: at 128 rows of x, 16 KB
 // of codes come with 32 KB of x (one tile of 128 x 256: 8 with 64, 10 TB/s from the L2 and no more).
@@ -286,12 +286,13 @@ constexpr int MAX_COLS = 128;                // rows of x per block
 constexpr int PUSH_COLS = 64;                // columns up to which the rings leave room for the cluster's sums
 constexpr int A_BUFS = 2;                    // converted stages
 constexpr int A_COLS = KS / 2;               // TMEM columns of one
-constexpr int TC_THREADS = 512;
+constexpr int TC_THREADS = 640;
+constexpr int CONVERTERS = 16;               // warps
 constexpr size_t TC_SMEM = 226 * 1024;       // the SM for itself: no other CTA's TMEM allocation meets this one's
 
 struct TcParams {
     const __half *scale, *least;
-    int K, group;
+    int K, shift;            // shift: log2 of the group
     int stages, cs, tiles;   // per tile; CTAs that share a tile's k; tiles
     int x_ring, bpad, nacc;  // stages of x in flight; columns; accumulators
     int push, share;         // split k: sums are pushed to the CTA that adds them (else pulled); columns that each adds
@@ -311,29 +312,44 @@ __device__ __forceinline__ void dsmem_st_f32(uint32_t cluster_saddr, float v) {
 // 16 columns from c on of this warp's 32 features out of TMEM, through the epilogue. acc: the accumulator's first column; n: this lane's
 // feature; b0: the block's first row of x. Everything is read before the first output is written: the compiler cannot know that
 // an output is no input of the next, and would wait for each.
-__device__ __forceinline__ void epilogue(const Dest &d, uint32_t acc, int warp4, int lane, int n, float bias, int b0, int c) {
+template <int EPI>
+__device__ __forceinline__ void epilogue(const Dest &d, uint32_t acc, int warp4, int lane, int n, int b0, int c) {
     uint32_t r[16];
     tmem_ld16(acc + (static_cast<uint32_t>(warp4 * 32) << 16) + c, r);
     const int first = b0 + c, many = min(16, d.B - first);
+    const float bias = bias_of(d, n);
     float resid[16];
-    if (d.epi == EPI_RESID) {
+    if (EPI == EPI_RESID) {
+        const __half *from = d.resid + first * d.ldr + n;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) resid[j] = j < many && n < d.N ? __half2float(d.resid[(first + j) * d.ldr + n]) : 0.0f;
+        for (int j = 0; j < 16; ++j) resid[j] = j < many && n < d.N ? __half2float(from[j * d.ldr]) : 0.0f;
     }
     tmem_wait_ld();
     __half h[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) h[j] = shaped(d, __uint_as_float(r[j]), {bias, d.epi == EPI_RESID ? resid[j] : 0.0f});
+    for (int j = 0; j < 16; ++j) {
+        float v = __uint_as_float(r[j]) + bias;
+        if (EPI == EPI_GELU) v = gelu_new(v);
+        if (EPI == EPI_RESID) v += resid[j];
+        h[j] = __float2half_rn(v);
+    }
     if (d.out && n < d.N) {
         __half *out = d.out + first * d.ldo + n;
+        if (many == 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j, out += d.ldo) *out = h[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j, out += d.ldo)
+                if (j < many) *out = h[j];
+        }
+    }
+    if (EPI == EPI_QKV && n < d.N) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if (j < many) out[j * d.ldo] = h[j];
-    }
-    if (d.epi == EPI_QKV && n < d.N)
-        for (int j = 0; j < 16; ++j)
             if (j < many) to_cache(d, first + j, n, h[j]);
-    if (d.epi == EPI_HEAD) {
+    }
+    if (EPI == EPI_HEAD) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             if (j >= many) break;
@@ -351,7 +367,7 @@ template <int GS, bool LEAST>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const TcParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t c_full[CODE_RING], c_empty[CODE_RING], x_full[MAX_X_RING], x_empty[MAX_X_RING], a_full[A_BUFS], a_empty[A_BUFS], acc_full[2],
+    __shared__ uint64_t c_full[CODE_RING], c_empty[CODE_RING], x_full[MAX_X_RING], x_empty[MAX_X_RING], a_full[TILES][A_BUFS], a_empty[TILES][A_BUFS], acc_full[2],
         acc_empty[2], last_full;
     __shared__ uint32_t tmem_slot;
     __shared__ int bad;  // a wait gave up: nothing more is written
@@ -364,40 +380,65 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     const int s0 = rank * p.stages / p.cs, ns = (rank + 1) * p.stages / p.cs - s0;  // this CTA's stages of each tile
     const int total = my_tiles * ns;
 
-    if (warp == 0) {  // one after the other they would take as long as the first copy
+    // The producers set up their own barriers and start; the others meet behind the allocation.
+    const auto code_copy = [&](int slot, int k, int n0) {
+        mbar_arrive_expect_tx(&c_full[slot], CODE_BYTES);
+#pragma unroll
+        for (int w = 0; w < TILES; ++w) tma_load_2d(smem + slot * CODE_BYTES + w * (CODE_BYTES / TILES), &tm_w, &c_full[slot], k / 2, n0 + w * BM);
+    };
+    // Codes do not depend on the kernel before this one, so nothing waits for it.
+    const int early = min(min(total, ns), CODE_RING), early_x = min(min(total, ns), p.x_ring);
+    const auto x_copy = [&](int slot, int stage) {
+        mbar_arrive_expect_tx(&x_full[slot], static_cast<uint32_t>(x_bytes));
+        tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], stage * KS, b0);
+        tma_load_2d(x_smem + slot * x_bytes + x_bytes / 2, &tm_x, &x_full[slot], stage * KS + 64, b0);
+    };
+    if (warp == 0) {
         if (lane < CODE_RING) {
             mbar_init(&c_full[lane], 1);
-            mbar_init(&c_empty[lane], 8);
+            mbar_init(&c_empty[lane], CONVERTERS / A_BUFS);
         }
-        if (lane < MAX_X_RING) {
-            mbar_init(&x_full[lane], 1);
-            mbar_init(&x_empty[lane], 1);
-        }
-        if (lane < A_BUFS) {
-            mbar_init(&a_full[lane], 8);
-            mbar_init(&a_empty[lane], 1);
+        fence_mbar_init();
+        __syncwarp();
+        if (elect_one())
+            for (int i = 0; i < early; ++i) code_copy(i, (s0 + i) * KS, first_tile * FEATURES);
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane < TILES * A_BUFS) {
+            mbar_init(&a_full[0][lane], 4);
+            mbar_init(&a_empty[0][lane], 1);
         }
         if (lane < 2) {
-            mbar_init(&acc_full[lane], 1);
-            mbar_init(&acc_empty[lane], 4);
+            mbar_init(&acc_full[lane], TILES);
+            mbar_init(&acc_empty[lane], CONVERTERS);
         }
-        if (lane == 31) {
-            mbar_init(&last_full, 1);
-            bad = 0;
-            tma_prefetch_desc(&tm_w);
-        }
-        if (lane == 30) tma_prefetch_desc(&tm_x);
+        if (lane == 31) mbar_init(&last_full, TILES);
         fence_mbar_init();
-    }
-    if (p.cs > 1) cluster_arrive_relaxed();  // waited for before the first write to another CTA
-    if (warp == 1) {
+        __syncwarp();
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
+    } else if (warp == 2) {
+        if (lane < MAX_X_RING) {
+            mbar_init(&x_full[lane], 1);
+            mbar_init(&x_empty[lane], TILES);
+        }
+        fence_mbar_init();
+        __syncwarp();
+        grid_dependency_wait();
+        if (elect_one())
+            for (int i = 0; i < early_x; ++i) x_copy(i, s0 + i);
+        __syncwarp();
+    } else if (tid == 96) {
+        bad = 0;
     }
+    __syncwarp();
+    if (p.cs > 1) cluster_arrive_relaxed();  // waited for before the first write to another CTA
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm_a = tmem_slot, tm_acc = tmem_slot + A_BUFS * TILES * A_COLS;
+    // All of the SM's columns are this CTA's, from 0 on; as constants they cost the MMAs nothing (out of a register, each operand of each
+    // MMA is moved to a uniform one).
+    constexpr uint32_t tm_a = 0, tm_acc = A_BUFS * TILES * A_COLS;
     grid_launch_dependents();
 
     const auto fail = [&] {
@@ -406,28 +447,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             atomicOr(p.d.status, ST_LINEAR_TIMEOUT);
         }
     };
+    if (tid == 0 && tmem_slot != 0) bad = 1;  // cannot be
     // Each role counts slots, phases, stages and tiles by hand: one warp's divisions by run-time numbers take longer than a stage.
     if (warp == 0) {
-        // Codes: they do not depend on the kernel before this one, so nothing waits for it.
         const bool leader = elect_one();
-        int it = 0, i = 0, n0 = first_tile * FEATURES;
+        int it = early, i = early, n0 = first_tile * FEATURES;
         for (; it < total; ++it) {
+            if (i == ns) {
+                i = 0;
+                n0 += tile_step * FEATURES;
+            }
             const int slot = it % CODE_RING;
             const bool ok = it < CODE_RING || mbar_wait(&c_empty[slot], (it / CODE_RING - 1) & 1, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 fail();
                 break;
             }
-            if (leader) {
-                mbar_arrive_expect_tx(&c_full[slot], CODE_BYTES);
-#pragma unroll
-                for (int w = 0; w < TILES; ++w)
-                    tma_load_2d(smem + slot * CODE_BYTES + w * (CODE_BYTES / TILES), &tm_w, &c_full[slot], (s0 + i) * (KS / 2), n0 + w * BM);
-            }
-            if (++i == ns) {
-                i = 0;
-                n0 += tile_step * FEATURES;
-            }
+            if (leader) code_copy(slot, (s0 + i) * KS, n0);
+            ++i;
             __syncwarp();
         }
         // every copy has landed before this CTA may end, whatever became of the others
@@ -437,20 +474,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     }
     if (warp == 2) {
         const bool leader = elect_one();
-        int i = 0, slot = 0, at = 0;
-        uint32_t phase = 1;  // of x_empty: passed at once while the ring fills
+        int i = early_x, slot = early_x == p.x_ring ? 0 : early_x, at = early_x;
+        uint32_t phase = early_x == p.x_ring ? 0 : 1;  // of x_empty: passed at once while the ring fills
         for (; at < total; ++at) {
+            if (i == ns) i = 0;
             const bool ok = mbar_wait(&x_empty[slot], phase, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 fail();
                 break;
             }
-            if (leader) {
-                mbar_arrive_expect_tx(&x_full[slot], static_cast<uint32_t>(x_bytes));
-                tma_load_2d(x_smem + slot * x_bytes, &tm_x, &x_full[slot], (s0 + i) * KS, b0);
-                tma_load_2d(x_smem + slot * x_bytes + x_bytes / 2, &tm_x, &x_full[slot], (s0 + i) * KS + 64, b0);
-            }
-            if (++i == ns) i = 0;
+            if (leader) x_copy(slot, s0 + i);
+            ++i;
             if (++slot == p.x_ring) {
                 slot = 0;
                 phase ^= 1;
@@ -459,155 +493,117 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
         }
         for (int j = max(0, at - p.x_ring); j < at; ++j) mbar_wait(&x_full[j % p.x_ring], (j / p.x_ring) & 1, p.timeout_ns);
     }
-    if (warp == 1) {
+    if (warp == 1 || warp == 3) {
+        const int w = warp >> 1;  // its 128 features
         const bool leader = elect_one();
         const uint32_t idesc = idesc_f16_f32(BM, p.bpad, 0, 0);
         const uint64_t dx = sdesc_sw128(smem_u32(x_smem), 16, 1024);
         const uint32_t x_lo = static_cast<uint32_t>(dx), x_hi = static_cast<uint32_t>(dx >> 32), x_step = static_cast<uint32_t>(x_bytes) >> 4;
-        int it = 0, slot = 0, acc = 0;
-        uint32_t x_phase = 0, acc_phase = 1;  // of acc_empty: passed at once for the first tiles
+        // One flat loop whose only exits are votes: what the MMAs take stays in uniform registers (32 cycles per MMA of 64 columns; 56 with
+        // the waits' results carried through nested loops).
+        int i = 0, buf = 0, slot = 0, acc = 0;
+        uint32_t x_phase = 0, a_phase = 0, acc_phase = 1;  // of acc_empty: passed at once for the first tiles
         bool ok = true;
-        for (int j = 0; j < my_tiles && ok; ++j) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&acc_empty[acc], acc_phase, p.timeout_ns));
-            for (int i = 0; i < ns && ok; ++i, ++it) {
-                const int buf = it % A_BUFS;
-                ok = mbar_wait_spin(&x_full[slot], x_phase, p.timeout_ns) && mbar_wait_spin(&a_full[buf], (it / A_BUFS) & 1, p.timeout_ns);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+        for (int it = 0; it < total; ++it) {
+            if (i == 0) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&acc_empty[acc], acc_phase, p.timeout_ns));
                 if (!ok) break;
-                tc_fence_after();
-                if (leader) {
-                    const uint32_t off = static_cast<uint32_t>(slot) * x_step;
-#pragma unroll
-                    for (int w = 0; w < TILES; ++w)
-#pragma unroll
-                        for (int kk = 0; kk < KS / 16; ++kk)
-                            umma_f16_ts_lohi(tm_acc + (acc * TILES + w) * p.bpad, tm_a + (buf * TILES + w) * A_COLS + kk * 8,
-                                             x_lo + off + kk / 4 * (x_step / 2) + kk % 4 * 2, x_hi, idesc, i > 0 || kk > 0 ? 1u : 0u);
-                    umma_commit(&a_empty[buf]);
-                    umma_commit(&x_empty[slot]);
-                    if (i == ns - 1) umma_commit(&acc_full[acc]);
-                }
-                __syncwarp();
-                if (++slot == p.x_ring) {
-                    slot = 0;
-                    x_phase ^= 1;
-                }
             }
-            if (++acc == p.nacc) {
-                acc = 0;
-                acc_phase ^= 1;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&x_full[slot], x_phase, p.timeout_ns));
+            if (!ok) break;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(&a_full[w][buf], a_phase, p.timeout_ns));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t b_lo = x_lo + static_cast<uint32_t>(slot) * x_step, from = tm_a + (buf * TILES + w) * A_COLS, to = tm_acc + (acc * TILES + w) * p.bpad;
+            if (leader) {
+                umma_f16_ts_lohi(to, from, b_lo, x_hi, idesc, i > 0 ? 1u : 0u);
+#pragma unroll
+                for (int kk = 1; kk < KS / 16; ++kk) umma_f16_ts_lohi(to, from + kk * 8, b_lo + kk / 4 * (x_step / 2) + kk % 4 * 2, x_hi, idesc, 1u);
+                umma_commit(&a_empty[w][buf]);
+                umma_commit(&x_empty[slot]);
+                if (i == ns - 1) umma_commit(&acc_full[acc]);
+            }
+            __syncwarp();
+            buf ^= 1;
+            if (buf == 0) a_phase ^= 1;
+            if (++slot == p.x_ring) {
+                slot = 0;
+                x_phase ^= 1;
+            }
+            if (++i == ns) {
+                i = 0;
+                if (++acc == p.nacc) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
             }
         }
         if (!ok) fail();
         __syncwarp();
         if (leader) umma_commit(&last_full);  // arrives when all that was issued is done
-    } else if (warp >= 4 && warp < 12) {
-        const int wg = (warp - 4) >> 2, warp4 = warp & 3, row = warp4 * 32 + lane;
-        const uint32_t to = tm_a + wg * A_COLS + (static_cast<uint32_t>(warp4 * 32) << 16);
-        const uint8_t *from = smem + wg * (CODE_BYTES / TILES) + row * 64;
-        const int groups = p.K / p.group;
-        __half sc[2][GS], lo[2][GS];
-        int si = 0, sn = first_tile * FEATURES + wg * BM + row;  // the stage and the feature of the scales that are fetched next
-        const auto scales = [&](__half (&s)[GS], __half (&l)[GS]) {
-            const int g0 = (s0 + si) * GS;
-#pragma unroll
-            for (int q = 0; q < GS; ++q) {
-                const bool in = sn < p.d.N && g0 + q < groups;
-                const long long at = static_cast<long long>(g0 + q) * p.d.N + sn;
-                s[q] = in ? p.scale[at] : __float2half_rn(0.0f);
-                if (LEAST) l[q] = in ? p.least[at] : __float2half_rn(0.0f);
-            }
-            if (++si == ns) {
-                si = 0;
-                sn += tile_step * FEATURES;
-            }
-        };
-        scales(sc[0], lo[0]);
-        scales(sc[1], lo[1]);
-        bool ok = true;
-        for (int it0 = 0; it0 < total && ok; it0 += 2) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {  // u: the buffer
-                const int it = it0 + u;
-                if (it >= total || !ok) break;
-                const int slot = it % CODE_RING;
-                ok = mbar_wait(&c_full[slot], (it / CODE_RING) & 1, p.timeout_ns);
-                if (it >= A_BUFS) ok = ok && mbar_wait(&a_empty[u], (it / A_BUFS - 1) & 1, p.timeout_ns);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                const uint8_t *st = from + slot * CODE_BYTES;
-                bool large = false;
-#pragma unroll
-                for (int q = 0; q < GS; ++q) large = large || big_scale(__half_as_ushort(sc[u][q]));
-                const auto convert = [&](auto any_big) {
-                    constexpr bool BIG = decltype(any_big)::value;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t v[32];
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const int chunk = h * 2 + q;  // 32 k, 16 bytes: the 64-byte swizzle's place
-                            const uint4 w = *reinterpret_cast<const uint4 *>(st + ((chunk ^ (row >> 1 & 3)) << 4));
-                            const Scale k = scale_of<LEAST, BIG>(__half_as_ushort(sc[u][chunk * GS / 4]), LEAST ? __half_as_ushort(lo[u][chunk * GS / 4]) : 0);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t four[4];
-                                values_of<LEAST, BIG>((&w.x)[j], k, four);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) v[q * 16 + j * 4 + e] = four[e];
-                            }
-                        }
-                        tmem_st32(to + u * (TILES * A_COLS) + h * 32, v);
-                    }
-                };
-                if (__any_sync(0xFFFFFFFFu, large))
-                    convert(std::true_type());
-                else
-                    convert(std::false_type());
-                if (it + 2 < total) scales(sc[u], lo[u]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&c_empty[slot]);
-                    mbar_arrive(&a_full[u]);
-                }
-            }
-        }
-        if (!ok) fail();
     }
-    __syncwarp();
-
     // Sums that another CTA of the cluster adds: pushed into a buffer of its own there, or left where the rings were.
     const uint32_t parts = smem_u32(smem) + (p.push ? CODE_RING * CODE_BYTES + p.x_ring * x_bytes : 0);
-    if (p.cs > 1) cluster_wait();
     if (warp >= 4) {
-        const int wg = (warp - 4) >> 2, warp4 = warp & 3;  // 2: the epilogue's own
-        for (int j = wg == 2 ? 0 : my_tiles - 1; j < my_tiles; ++j) {
-            const int acc = j % p.nacc, n0 = (first_tile + j * tile_step) * FEATURES;
-            const bool last = j == my_tiles - 1;
-            const bool ok = last ? mbar_wait(&last_full, 0, p.timeout_ns) : mbar_wait(&acc_full[acc], (j / p.nacc) & 1, p.timeout_ns);
+        const int wg = (warp - 4) >> 2, warp4 = warp & 3, row = warp4 * 32 + lane;
+        const int tile_w = wg & 1, turn = wg >> 1;  // its 128 features; its stages are the even or the odd ones, in A buffer `turn`
+        const uint32_t lanes = static_cast<uint32_t>(warp4 * 32) << 16;
+        const uint32_t to = tm_a + lanes + (turn * TILES + tile_w) * A_COLS;
+        const uint8_t *from = smem + tile_w * (CODE_BYTES / TILES) + row * 64;
+        // Scales are fetched for the warpgroup's next stage, two ahead, when this one's have been used.
+        __half sc[GS], lo[GS];
+        int si = turn, sn = first_tile * FEATURES + tile_w * BM + row;  // stage of the tile, and feature, of the next
+        const auto scales = [&] {
+            while (si >= ns) {
+                si -= ns;
+                sn += tile_step * FEATURES;
+            }
+#pragma unroll
+            for (int q = 0; q < GS; ++q) {
+                const int k = (s0 + si) * KS + q * (KS / GS);
+                const bool in = sn < p.d.N && k < p.K;
+                const long long at = static_cast<long long>(k >> p.shift) * p.d.N + sn;
+                sc[q] = in ? p.scale[at] : __float2half_rn(0.0f);
+                if (LEAST) lo[q] = in ? p.least[at] : __float2half_rn(0.0f);
+            }
+            si += 2;
+        };
+        // Takes tile j out of TMEM; the pieces of 16 columns of its two accumulators are shared by the warpgroups.
+        int taken = 0;
+        const auto take = [&] {
+            const int j = taken++, acc = p.nacc == 2 ? j & 1 : 0, round = p.nacc == 2 ? j >> 1 : j, n0 = (first_tile + j * tile_step) * FEATURES;
+            const bool ok = j == my_tiles - 1 ? mbar_wait(&last_full, 0, p.timeout_ns) : mbar_wait(&acc_full[acc], round & 1, p.timeout_ns);
             if (!__all_sync(0xFFFFFFFFu, ok)) fail();
             __syncwarp();
-            if (*reinterpret_cast<volatile int *>(&bad)) break;
+            if (*reinterpret_cast<volatile int *>(&bad)) return;
             tc_fence_after();
-            const int pieces = p.bpad / 16 * TILES;  // w for every 16 columns; a warp's part keeps to one w where it can
-            const int first = last ? wg * pieces / 3 : 0, behind = last ? (wg + 1) * pieces / 3 : pieces;
-            for (int piece = first; piece < behind; ++piece) {
-                const int w = piece / (pieces / TILES), c = piece % (pieces / TILES) * 16, f = w * BM + warp4 * 32 + lane;
-                const uint32_t from = tm_acc + (acc * TILES + w) * p.bpad;
+            const int per = p.bpad / 16;
+            for (int piece = turn; piece < per; piece += 2) {
+                const int c = piece * 16, f = tile_w * BM + row;
+                const uint32_t at = tm_acc + (acc * TILES + tile_w) * p.bpad;
                 if (p.cs == 1) {
-                    epilogue(p.d, from, warp4, lane, n0 + f, bias_of(p.d, n0 + f), b0, c);
+                    switch (p.d.epi) {
+                        case EPI_STORE: epilogue<EPI_STORE>(p.d, at, warp4, lane, n0 + f, b0, c); break;
+                        case EPI_GELU: epilogue<EPI_GELU>(p.d, at, warp4, lane, n0 + f, b0, c); break;
+                        case EPI_RESID: epilogue<EPI_RESID>(p.d, at, warp4, lane, n0 + f, b0, c); break;
+                        case EPI_QKV: epilogue<EPI_QKV>(p.d, at, warp4, lane, n0 + f, b0, c); break;
+                        default: epilogue<EPI_HEAD>(p.d, at, warp4, lane, n0 + f, b0, c);
+                    }
                 } else {
                     uint32_t r[16];
-                    tmem_ld16(from + (static_cast<uint32_t>(warp4 * 32) << 16) + c, r);
+                    tmem_ld16(at + lanes + c, r);
                     tmem_wait_ld();
                     if (p.push) {
+                        int q = c / p.share, left = (q + 1) * p.share - c;  // the CTA that adds column c, and its columns from there on
+                        uint32_t there = dsmem_addr(parts + ((rank * p.share + p.share - left) * FEATURES + f) * 4, static_cast<uint32_t>(q));
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int q = (c + i) / p.share, at = ((rank * p.share + c + i - q * p.share) * FEATURES + f) * 4;
-                            dsmem_st_f32(dsmem_addr(parts + at, static_cast<uint32_t>(q)), __uint_as_float(r[i]));
+                            dsmem_st_f32(there, __uint_as_float(r[i]));
+                            there += FEATURES * 4;
+                            if (--left == 0) {
+                                left = p.share;
+                                there = dsmem_addr(parts + (rank * p.share * FEATURES + f) * 4, static_cast<uint32_t>(min(++q, p.cs - 1)));
+                            }
                         }
                     } else {
                         float *part = reinterpret_cast<float *>(smem);
@@ -618,8 +614,76 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
             }
             tc_fence_before();
             __syncwarp();
-            if (!last && lane == 0) mbar_arrive(&acc_empty[acc]);
+            if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        };
+        scales();
+        bool ok = true;
+        int due = ns + 2;  // from this stage on the first tile is taken: it is converted, and two stages of the next
+        uint32_t a_phase = 1;  // of a_empty: passed at once for the first stage
+        for (int it = turn; it < total; it += 2) {
+            while (it >= due) {
+                take();
+                due += ns;
+            }
+            const int slot = it % CODE_RING;
+            ok = mbar_wait(&c_full[slot], (it / CODE_RING) & 1, p.timeout_ns);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            const uint8_t *st = from + slot * CODE_BYTES;
+            uint4 codes[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) codes[q] = *reinterpret_cast<const uint4 *>(st + ((q ^ (row >> 1 & 3)) << 4));  // 32 k: the 64-byte swizzle's place
+            bool large = false;
+#pragma unroll
+            for (int q = 0; q < GS; ++q) large = large || big_scale(__half_as_ushort(sc[q]));
+            const auto convert = [&](auto any_big) {
+                constexpr bool BIG = decltype(any_big)::value;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int g = (2 * h + q) * GS / 4;
+                        const uint4 &w = codes[2 * h + q];
+                        const Scale k = scale_of<LEAST, BIG>(__half_as_ushort(sc[g]), LEAST ? __half_as_ushort(lo[g]) : 0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t four[4];
+                            values_of<LEAST, BIG>((&w.x)[j], k, four);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[q * 16 + j * 4 + e] = four[e];
+                        }
+                    }
+                    if (h == 0) {  // half a stage is converted before its buffer has to be free
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&a_empty[tile_w][turn], a_phase, p.timeout_ns));
+                        if (!ok) return;
+                        tc_fence_after();
+                    }
+                    tmem_st32(to + h * 32, v);
+                }
+            };
+            if (__any_sync(0xFFFFFFFFu, large))
+                convert(std::true_type());
+            else
+                convert(std::false_type());
+            if (!ok) break;
+            a_phase ^= 1;
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&a_full[tile_w][turn]);
+                mbar_arrive(&c_empty[slot]);
+            }
+            if (it + 2 < total) scales();
         }
+        if (!ok) fail();
+        __syncwarp();
+        if (p.cs > 1) cluster_wait();
+        while (taken < my_tiles && !*reinterpret_cast<volatile int *>(&bad)) take();
+    } else {
+        __syncwarp();
+        if (p.cs > 1) cluster_wait();
     }
     __syncwarp();
     if (p.cs > 1) {
@@ -725,7 +789,7 @@ int active_clusters(DeviceContext *ctx, int cs) {
 int prepare_tc(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
-    for (const TcKernel k : {k_w4_tc<1, false>, k_w4_tc<2, false>, k_w4_tc<4, false>, k_w4_tc<1, true>, k_w4_tc<2, true>, k_w4_tc<4, true>})
+    for (const TcKernel k : {tc_kernel<false>(32), tc_kernel<false>(64), tc_kernel<false>(128), tc_kernel<true>(32), tc_kernel<true>(64), tc_kernel<true>(128)})
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
     ctx->w4_attr_done = true;
     return GPT2_B200_OK;
@@ -828,7 +892,7 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     p.scale = w.scale;
     p.least = w.least;
     p.K = w.K;
-    p.group = w.group;
+    p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.stages = (w.K + KS - 1) / KS;
     p.tiles = (w.N + FEATURES - 1) / FEATURES;
     const int blocks = (pl.d.B + MAX_COLS - 1) / MAX_COLS;  // of equal width
