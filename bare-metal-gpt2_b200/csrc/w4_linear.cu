@@ -895,19 +895,31 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.stages = (w.K + KS - 1) / KS;
     p.tiles = (w.N + FEATURES - 1) / FEATURES;
-    const int blocks = (pl.d.B + MAX_COLS - 1) / MAX_COLS;  // of equal width
-    p.bpad = ((pl.d.B + blocks - 1) / blocks + 15) / 16 * 16;
+    // Column blocks and CTAs per tile, by the cycles that they are seen to take: 3300 to the first codes, 1000 a stage (or the MMAs, 8 a
+    // column), 2000 and 90 a column for the sums of a cluster, 40 a column for a tile's outputs without one. Blocks read the weights
+    // again, from the L2, and convert them again, on SMs that have nothing else to do: with a few features and a short k that is
+    // cheaper than adding wide sums (64 x 2304 x 768).
+    int blocks = 0;
+    long long best = 0;
+    for (int n = (pl.d.B + MAX_COLS - 1) / MAX_COLS; n <= (pl.d.B + 15) / 16; ++n) {
+        const int cols = ((pl.d.B + n - 1) / n + 15) / 16 * 16;
+        if ((pl.d.B + cols - 1) / cols != n) continue;  // an empty block
+        const long long stage = std::max(1000, 8 * cols);
+        for (int c = 1; c <= std::min(lin::MAX_CLUSTER, p.stages); ++c) {
+            if (c > 1 && (pl.d.epi == EPI_HEAD || p.tiles > active_clusters(ctx, c) / n)) continue;
+            const long long each = std::max(1, ctx->num_sms / n), rounds = c > 1 ? 1 : (p.tiles + each - 1) / each;
+            const long long cost = 3300 + rounds * ((p.stages + c - 1) / c * stage + (c > 1 ? 2000 + 90 * cols : 40 * cols));
+            if (!blocks || cost < best) {
+                best = cost;
+                blocks = n;
+                p.cs = c;
+                p.bpad = cols;
+            }
+        }
+    }
     p.nacc = p.bpad <= 64 ? 2 : 1;
     p.d = pl.d;
     p.timeout_ns = wait_timeout_ns();
-    // The widest split of k whose clusters all run at once.
-    p.cs = 1;
-    if (pl.d.epi != EPI_HEAD)
-        for (int c = std::min(lin::MAX_CLUSTER, p.stages); c > 1; --c)
-            if (p.tiles * blocks <= active_clusters(ctx, c)) {
-                p.cs = c;
-                break;
-            }
     p.share = (p.bpad + p.cs - 1) / p.cs;
     p.push = p.cs > 1 && p.bpad <= PUSH_COLS;
     const size_t rest = TC_SMEM - 1024 - CODE_RING * CODE_BYTES - (p.push ? static_cast<size_t>(p.cs) * p.share * FEATURES * 4 : 0);
