@@ -49,8 +49,7 @@ struct DeviceContext {
     bool decode_attr_done = false;
     bool beam_attr_done[2] = {false, false};  // beam selection over fp16, fp32 logits
     bool kv8_attr_done[32] = {};              // 8-bit cache attention, by kernel variant
-    bool w4_attr_done = false;                // 4-bit products, many rows
-    bool w4_rows_attr_done = false;           // 4-bit products, few rows
+    bool w4_attr_done = false;                // 4-bit products
     int w4_clusters[9] = {};                  // 4-bit products: clusters of n CTAs that run at once (0 = not asked)
     bool edit_attr_done = false;              // logits edit
     int num_sms = 0;

@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
     // The dense pass has something to do unless the logits stay in place and nothing asks for the mask or the largest.
     const bool dense = MASK || NEXT || !p.in_place;
     n = clamped(n, 0, hist ? e.max_history : 0, tell, p.status);
-    from = clamped(from, 0, n, tell, p.status);
+    from = p.len_add ? min(max(from, 0), n) : clamped(from, 0, n, tell, p.status);  // the decoder edits within the prompt too
     r.nb = clamped(r.nb, 0, e.max_bias, tell, p.status);
     int h[AHEAD];
     const auto tokens = [&](int i0) {

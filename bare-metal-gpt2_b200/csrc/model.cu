@@ -13,7 +13,8 @@
 //   LayerNorm 1 of the next layer (or the final one)
 // The embedding kernel also applies layer 0's LayerNorm, and the head's epilogue turns the logits
 // into per-tile argmax keys that one small kernel reduces to the next token: 1 + 12 x 7 + 2 = 87
-// launches per step (gpt2_b200_batch_launches_per_step reports the count). A lock-step greedy
+// launches per step (gpt2_b200_batch_launches_per_step reports the count). Over 4-bit weights the linear layers are
+// w4_linear.cu's, with the same epilogues. A lock-step greedy
 // generator captures the whole step, token selection included, in one CUDA graph.
 //
 // Arithmetic follows the reference's fp16 path: activations stored in fp16, fp32 accumulation,
@@ -27,7 +28,9 @@
 #include <new>
 
 #include "common.cuh"
+#include "logits_edit.cuh"
 #include "model.cuh"
+#include "w4.cuh"
 
 namespace b200 {
 
@@ -87,6 +90,21 @@ __global__ void __launch_bounds__(128) k_advance(int *tok, int *pos, int *out, l
     pos[b] = p + 1;
 }
 
+// The same after an edit of the logits, which has chosen (-1: there was nothing to choose; it is recorded, and the embedding reports it).
+__global__ void k_advance_chosen(int *tok, int *pos, int *out, long long out_stride, const int *prompt, long long prompt_stride, const int *plen,
+                                 const int *chosen, int B) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b >= B) return;
+    const int p = pos[b];
+    const long long pi = min(static_cast<long long>(min(p + 1, max(plen[b] - 1, 0))), prompt_stride - 1);
+    const int nxt = p + 1 < plen[b] ? prompt[b * prompt_stride + pi] : chosen[b];
+    out[b * out_stride + p + 1] = nxt;
+    tok[b] = nxt;
+    pos[b] = p + 1;
+}
+
 __global__ void k_gen_init(int *tok, int *pos, int *out, long long out_stride, const int *prompt,
                            long long prompt_stride, int B) {
     const int b = blockIdx.x * blockDim.x + threadIdx.x;
@@ -113,13 +131,21 @@ struct gpt2_b200_batch {
     int *tok = nullptr, *pos = nullptr;           // generation state [B]
     unsigned long long *amax = nullptr;           // [B][head tiles]
     lin::Plan qkv_p[NL], proj_p[NL], fc_p[NL], proj2_p[NL], head_p;
-    cudaGraphExec_t graph[2] = {nullptr, nullptr};  // generate step: full, attention only
+    bool w4 = false, w4_head = false;  // the matmuls, the head over 4-bit weights: their plans instead
+    w4::Plan qkv_4[NL], proj_4[NL], fc_4[NL], proj2_4[NL], head_4;
+    int head_keys = 0;  // argmax keys per row
+    int *chosen = nullptr;       // edited generation: the choice [B]
+    __half *logits = nullptr;    // and the logits [B][LDL], allocated by its first call
+    cudaGraphExec_t graph[3] = {nullptr, nullptr, nullptr};  // generate step: full, attention only, with edited logits
+    GPT2LogitsEdit g_edit = {};
     const int *g_prompt = nullptr, *g_plen = nullptr;
     int *g_out = nullptr;
     long long g_ps = 0, g_os = 0;
 };
 
 namespace {
+
+constexpr int LDL = (V + 7) / 8 * 8;  // row stride of the batch's own logits
 
 // Enqueues one decode step for all B sequences (tokens/positions on the device).
 int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half *logits,
@@ -140,9 +166,15 @@ int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half
     for (int L = 0; L < NL; ++L) {
         int rc;
         if (!attention_only) {
-            lin::Plan p = bt->qkv_p[L];
-            p.p.d_pos = d_pos;
-            if ((rc = lin::launch_linear(p, st)) != GPT2_B200_OK) return rc;
+            if (bt->w4) {
+                bt->qkv_4[L].d.d_pos = d_pos;
+                rc = w4::launch(bt->qkv_4[L], st);
+            } else {
+                lin::Plan p = bt->qkv_p[L];
+                p.p.d_pos = d_pos;
+                rc = lin::launch_linear(p, st);
+            }
+            if (rc != GPT2_B200_OK) return rc;
         }
         // The attention joins the launch chain only with few (sequence, head) pairs (one CTA per
         // pair per SM); with many pairs its small-CTA shape runs faster as an ordinary launch
@@ -155,12 +187,12 @@ int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half
                            bt->maxT, st, attn_pdl, attn_pdl);
         if (rc != GPT2_B200_OK) return rc;
         if (attention_only) continue;
-        if ((rc = lin::launch_linear(bt->proj_p[L], st)) != GPT2_B200_OK) return rc;
+        if ((rc = bt->w4 ? w4::launch(bt->proj_4[L], st) : lin::launch_linear(bt->proj_p[L], st)) != GPT2_B200_OK) return rc;
         if ((rc = launch(k_layernorm, B, LN_THREADS, st, bt->pdl, bt->ln, bt->x, w.layers[L].ln2_g,
                          w.layers[L].ln2_b)) != GPT2_B200_OK)
             return rc;
-        if ((rc = lin::launch_linear(bt->fc_p[L], st)) != GPT2_B200_OK) return rc;
-        if ((rc = lin::launch_linear(bt->proj2_p[L], st)) != GPT2_B200_OK) return rc;
+        if ((rc = bt->w4 ? w4::launch(bt->fc_4[L], st) : lin::launch_linear(bt->fc_p[L], st)) != GPT2_B200_OK) return rc;
+        if ((rc = bt->w4 ? w4::launch(bt->proj2_4[L], st) : lin::launch_linear(bt->proj2_p[L], st)) != GPT2_B200_OK) return rc;
         if (caps && cudaMemcpyAsync(caps + L * E, bt->x, E * sizeof(__half),
                                     cudaMemcpyDeviceToDevice, st) != cudaSuccess)
             return GPT2_B200_ECUDA;
@@ -174,16 +206,59 @@ int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half
     if (caps && cudaMemcpyAsync(caps + NL * E, bt->ln, E * sizeof(__half), cudaMemcpyDeviceToDevice,
                                 st) != cudaSuccess)
         return GPT2_B200_ECUDA;
-    lin::Plan hp = bt->head_p;
-    hp.p.out = logits;
-    hp.p.ldo = logits_stride;
-    const int rc = lin::launch_linear(hp, st);
+    int rc;
+    if (bt->w4_head) {
+        bt->head_4.d.out = logits;
+        bt->head_4.d.ldo = logits_stride;
+        rc = w4::launch(bt->head_4, st);
+    } else {
+        lin::Plan hp = bt->head_p;
+        hp.p.out = logits;
+        hp.p.ldo = logits_stride;
+        rc = lin::launch_linear(hp, st);
+    }
     if (rc != GPT2_B200_OK) return rc;
     return cudaGetLastError() == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
-int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *kvs, int B) {
-    if (!weights_ok(w) || !kvs || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
+bool shaped(const GPT2W4 &q, int n, int k) { return w4::weight_ok(&q) && q.N == n && q.K == k; }
+
+// Plans over 4-bit weights in the place of the fp16 ones.
+int plan_w4(gpt2_b200_batch *bt, const GPT2W4Weights &q) {
+    const int B = bt->B;
+    int rc = GPT2_B200_OK;
+    for (int L = 0; L < NL && rc == GPT2_B200_OK; ++L) {
+        const GPT2LayerGPU &l = bt->w.layers[L];
+        if ((rc = w4::plan(&bt->qkv_4[L], lin::EPI_QKV, q.qkv[L], bt->ln, E, B, l.qkv_b, bt->qkv, Q, nullptr, 0)) ||
+            (rc = w4::plan(&bt->proj_4[L], lin::EPI_RESID, q.attn_proj[L], bt->att, E, B, l.attn_proj_b, bt->x, E, bt->x, E)) ||
+            (rc = w4::plan(&bt->fc_4[L], lin::EPI_GELU, q.fc[L], bt->ln, E, B, l.fc_b, bt->fc, F, nullptr, 0)) ||
+            (rc = w4::plan(&bt->proj2_4[L], lin::EPI_RESID, q.proj[L], bt->fc, F, B, l.proj_b, bt->x, E, bt->x, E)))
+            return rc;
+        w4::Dest &d = bt->qkv_4[L].d;
+        d.k_dst = bt->kslab + static_cast<size_t>(L) * B;
+        d.v_dst = bt->vslab + static_cast<size_t>(L) * B;
+        d.maxT = bt->maxT;
+        d.E = E;
+        bt->qkv_4[L].pdl = bt->proj_4[L].pdl = bt->fc_4[L].pdl = bt->proj2_4[L].pdl = bt->pdl;
+    }
+    if (bt->w4_head) {
+        if ((rc = w4::plan(&bt->head_4, lin::EPI_HEAD, q.head, bt->ln, E, B, nullptr, nullptr, 0, nullptr, 0))) return rc;
+        bt->head_4.d.amax = bt->amax;
+        bt->head_4.pdl = bt->pdl;
+        bt->head_keys = bt->head_4.d.keys;
+    }
+    return rc;
+}
+
+int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B) {
+    if (!weights_ok(w, !q) || !kvs || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
+    if (q) {
+        for (int L = 0; L < NL; ++L)
+            if (!shaped(q->qkv[L], Q, E) || !shaped(q->attn_proj[L], E, E) || !shaped(q->fc[L], F, E) || !shaped(q->proj[L], E, F)) return GPT2_B200_EINVAL;
+        if (q->head.codes && !shaped(q->head, V, E)) return GPT2_B200_EINVAL;
+        bt->w4 = true;
+        bt->w4_head = q->head.codes != nullptr;
+    }
     const int maxT = kvs[0].maxT;
     for (int b = 0; b < B; ++b) {
         const GPT2KVCache &kv = kvs[b];
@@ -197,7 +272,7 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
     bt->maxT = maxT;
     bt->device = ctx->device;
     bt->w = *w;
-    const int head_tiles = (V + lin::BM - 1) / lin::BM;
+    const int head_tiles = (V + 15) / 16;  // as many argmax keys per row as any head kernel writes
     // One arena: activations (16-byte aligned rows), slab pointer arrays, state, argmax keys.
     auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     const size_t o_x = 0, o_ln = o_x + up(sizeof(__half) * B * E), o_qkv = o_ln + up(sizeof(__half) * B * E);
@@ -205,7 +280,8 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
     const size_t o_ks = o_fc + up(sizeof(__half) * B * F), o_vs = o_ks + up(sizeof(void *) * NL * B);
     const size_t o_tok = o_vs + up(sizeof(void *) * NL * B), o_pos = o_tok + up(sizeof(int) * B);
     const size_t o_am = o_pos + up(sizeof(int) * B);
-    const size_t total = o_am + up(sizeof(unsigned long long) * B * head_tiles);
+    const size_t o_ch = o_am + up(sizeof(unsigned long long) * B * head_tiles);
+    const size_t total = o_ch + up(sizeof(int) * B);
     if (cudaMalloc(&bt->arena, total) != cudaSuccess) return GPT2_B200_ENOMEM;
     if (cudaMemset(bt->arena, 0, total) != cudaSuccess) return GPT2_B200_ECUDA;
     char *a = static_cast<char *>(bt->arena);
@@ -219,6 +295,7 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
     bt->tok = reinterpret_cast<int *>(a + o_tok);
     bt->pos = reinterpret_cast<int *>(a + o_pos);
     bt->amax = reinterpret_cast<unsigned long long *>(a + o_am);
+    bt->chosen = reinterpret_cast<int *>(a + o_ch);
     // Slab pointers: layer L of sequence b, K at (2L) and V at (2L+1) slabs (cuda/kvcache.cuh:61-66).
     const size_t slab = static_cast<size_t>(NH) * maxT * HD;
     __half **hk = new (std::nothrow) __half *[2 * NL * B];
@@ -235,7 +312,7 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
     delete[] hk;
     if (!ok) return GPT2_B200_ECUDA;
     const int sms = ctx->num_sms;
-    for (int L = 0; L < NL; ++L) {
+    for (int L = 0; L < NL && !bt->w4; ++L) {
         const GPT2LayerGPU &l = w->layers[L];
         int rc = lin::plan_linear(&bt->qkv_p[L], lin::EPI_QKV, l.qkv_w, Q, E, bt->ln, E, B, l.qkv_b,
                                   bt->qkv, Q, 0, sms);
@@ -258,12 +335,14 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
                               nullptr, 0, 1, sms);
     if (rc) return rc;
     bt->head_p.p.amax = bt->amax;
+    bt->head_keys = bt->head_p.p.n_tiles;
+    if (bt->w4 && (rc = plan_w4(bt, *q))) return rc;
     for (int L = 0; L < NL; ++L)
         bt->qkv_p[L].pdl = bt->proj_p[L].pdl = bt->fc_p[L].pdl = bt->proj2_p[L].pdl = bt->pdl;
     bt->head_p.pdl = bt->pdl;
     // Kernel attributes and the decode workspace for B sequences x 12 heads up to maxT keys, so
     // that a captured step makes no configuration call and never allocates.
-    for (int L = 0; L < NL; ++L)
+    for (int L = 0; L < NL && !bt->w4; ++L)
         if ((rc = lin::prepare_linear(bt->qkv_p[L])) || (rc = lin::prepare_linear(bt->proj_p[L])) ||
             (rc = lin::prepare_linear(bt->fc_p[L])) || (rc = lin::prepare_linear(bt->proj2_p[L])))
             return rc;
@@ -273,23 +352,12 @@ int batch_init(gpt2_b200_batch *bt, const GPT2WeightsGPU *w, const GPT2KVCache *
     return ensure_decode_workspace(ctx, floats, words, 0);
 }
 
-int check_device(const gpt2_b200_batch *bt) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return GPT2_B200_ECUDA;
-    return dev == bt->device ? GPT2_B200_OK : GPT2_B200_EINVAL;
-}
-
-}  // namespace
-
-extern "C" {
-
-int gpt2_b200_batch_create(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2KVCache *kvs,
-                           int B) {
+int batch_new(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B) {
     if (!out) return GPT2_B200_EINVAL;
     *out = nullptr;
     gpt2_b200_batch *bt = new (std::nothrow) gpt2_b200_batch();
     if (!bt) return GPT2_B200_ENOMEM;
-    const int rc = batch_init(bt, w, kvs, B);
+    const int rc = batch_init(bt, w, q, kvs, B);
     if (rc != GPT2_B200_OK) {
         gpt2_b200_batch_destroy(bt);
         return rc;
@@ -298,57 +366,42 @@ int gpt2_b200_batch_create(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const
     return GPT2_B200_OK;
 }
 
-void gpt2_b200_batch_destroy(gpt2_b200_batch *bt) {
-    if (!bt) return;
-    // replays queued on any stream may still be running: drain the device before releasing them
-    int prev = -1;
-    if (cudaGetDevice(&prev) == cudaSuccess && prev != bt->device) cudaSetDevice(bt->device);
-    cudaDeviceSynchronize();
-    for (cudaGraphExec_t &g : bt->graph)
-        if (g) cudaGraphExecDestroy(g);
-    if (bt->arena) cudaFree(bt->arena);
-    if (prev >= 0 && prev != bt->device) cudaSetDevice(prev);
-    delete bt;
+int check_device(const gpt2_b200_batch *bt) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GPT2_B200_ECUDA;
+    return dev == bt->device ? GPT2_B200_OK : GPT2_B200_EINVAL;
 }
 
-int gpt2_b200_batch_step(gpt2_b200_batch *bt, const int *d_tokens, const int *d_pos,
-                         gpt2_half *logits, long long logits_stride, int *d_next,
-                         cudaStream_t stream) {
-    if (!bt || !d_tokens || !d_pos) return GPT2_B200_EINVAL;
-    if (logits && (logits_stride < V || !aligned16(logits))) return GPT2_B200_EINVAL;
-    int rc = check_device(bt);
-    if (rc) return rc;
-    if ((rc = enqueue_step(bt, d_tokens, d_pos, logits, logits_stride, nullptr, false, stream)))
-        return rc;
-    if (d_next) {
-        if ((rc = launch(k_argmax, bt->B, 128, stream, bt->pdl, d_next, bt->amax,
-                         bt->head_p.p.n_tiles)) != GPT2_B200_OK)
-            return rc;
-    }
-    return GPT2_B200_OK;
-}
-
-int gpt2_b200_batch_launches_per_step(const gpt2_b200_batch *bt, int flags) {
-    if (!bt) return -1;
-    // attention only: 12 attention launches + the bookkeeping kernel
-    if (flags & GPT2_B200_GEN_ATTENTION_ONLY) return NL + 1;
-    // embed+LN, 12 x (QKV, attention, proj, LN2, FC, proj2, LN), head, bookkeeping
-    return 1 + NL * 7 + 1 + 1;
-}
-
-int gpt2_b200_batch_generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride,
-                             const int *d_plen, int n_steps, int *d_out, long long out_stride,
-                             int flags, cudaStream_t stream) {
+// Lock-step generation with graph gi: 0 greedy, 1 the attention alone, 2 with edited logits.
+int generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps, int *d_out, long long out_stride, int gi,
+             const GPT2LogitsEdit *edit, cudaStream_t stream) {
     if (!bt || !d_prompt || !d_plen || !d_out || n_steps < 1 || n_steps > bt->maxT ||
         out_stride < n_steps + 1 || prompt_stride < 1)
         return GPT2_B200_EINVAL;
     int rc = check_device(bt);
     if (rc) return rc;
-    const bool attn_only = (flags & GPT2_B200_GEN_ATTENTION_ONLY) != 0;
-    const int gi = attn_only ? 1 : 0;
-    // The graph bakes in the generation buffers; re-capture when they change.
-    if (bt->graph[gi] && (bt->g_prompt != d_prompt || bt->g_plen != d_plen || bt->g_out != d_out ||
-                          bt->g_ps != prompt_stride || bt->g_os != out_stride)) {
+    const bool attn_only = gi == 1;
+    DeviceContext *ctx = device_context();
+    if (!ctx) return GPT2_B200_ECUDA;
+    GPT2LogitsEdit e = {};
+    if (edit) {
+        // The history is the generation's own: what d_out holds so far, the prompt in front.
+        e = *edit;
+        e.history = d_out;
+        e.history_stride = out_stride;
+        e.max_history = static_cast<int>(std::min<long long>(out_stride, bt->maxT));
+        e.length = bt->pos;  // and one: the token that this step consumes
+        e.prompt = d_plen;
+        if ((rc = edit::check(&e, bt->B, V)) || (rc = edit::prepare(ctx))) return rc;
+        if (!bt->logits && cudaMalloc(&bt->logits, sizeof(__half) * LDL * bt->B) != cudaSuccess) {
+            bt->logits = nullptr;
+            return GPT2_B200_ENOMEM;
+        }
+    }
+    // The graphs bake in the generation buffers; re-capture when they change (all of them: one that is left would run on the old ones).
+    if ((bt->graph[0] || bt->graph[1] || bt->graph[2]) &&
+        (bt->g_prompt != d_prompt || bt->g_plen != d_plen || bt->g_out != d_out || bt->g_ps != prompt_stride || bt->g_os != out_stride ||
+         (edit && bt->graph[2] && std::memcmp(&bt->g_edit, &e, sizeof(e)) != 0))) {
         // earlier replays of these graphs may still be queued: let them finish first
         if (cudaDeviceSynchronize() != cudaSuccess) return GPT2_B200_ECUDA;
         for (cudaGraphExec_t &g : bt->graph)
@@ -362,7 +415,7 @@ int gpt2_b200_batch_generate(gpt2_b200_batch *bt, const int *d_prompt, long long
     bt->g_out = d_out;
     bt->g_ps = prompt_stride;
     bt->g_os = out_stride;
-    const int head_tiles = bt->head_p.p.n_tiles;
+    if (edit) std::memcpy(&bt->g_edit, &e, sizeof(e));
     if (!bt->graph[gi]) {
         cudaStream_t cs;
         if (cudaStreamCreateWithFlags(&cs, cudaStreamNonBlocking) != cudaSuccess)
@@ -372,10 +425,18 @@ int gpt2_b200_batch_generate(gpt2_b200_batch *bt, const int *d_prompt, long long
         if (cudaStreamBeginCapture(cs, cudaStreamCaptureModeThreadLocal) != cudaSuccess) {
             rc = GPT2_B200_ECUDA;
         } else {
-            rc = enqueue_step(bt, bt->tok, bt->pos, nullptr, 0, nullptr, attn_only, cs);
-            const int rc2 = launch(k_advance, bt->B, 128, cs, bt->pdl, bt->tok, bt->pos, d_out,
-                                   out_stride, d_prompt, prompt_stride, d_plen, bt->amax,
-                                   head_tiles, attn_only ? 1 : 0);
+            rc = enqueue_step(bt, bt->tok, bt->pos, edit ? bt->logits : nullptr, edit ? LDL : 0, nullptr, attn_only, cs);
+            int rc2;
+            if (edit) {
+                rc2 = edit::launch(ctx, bt->logits, LDL, bt->logits, LDL, GPT2_BEAM_HALF, bt->B, V, e, 1, bt->chosen, bt->pdl, cs);
+                const int rc3 = launch(k_advance_chosen, (bt->B + 127) / 128, 128, cs, bt->pdl, bt->tok, bt->pos, d_out, out_stride, d_prompt,
+                                       prompt_stride, d_plen, bt->chosen, bt->B);
+                if (rc2 == GPT2_B200_OK) rc2 = rc3;
+            } else {
+                rc2 = launch(k_advance, bt->B, 128, cs, bt->pdl, bt->tok, bt->pos, d_out,
+                             out_stride, d_prompt, prompt_stride, d_plen, bt->amax,
+                             bt->head_keys, attn_only ? 1 : 0);
+            }
             if (rc == GPT2_B200_OK) rc = rc2;
             if (cudaStreamEndCapture(cs, &g) != cudaSuccess && rc == GPT2_B200_OK)
                 rc = GPT2_B200_ECUDA;
@@ -396,6 +457,75 @@ int gpt2_b200_batch_generate(gpt2_b200_batch *bt, const int *d_prompt, long long
     for (int s = 0; s < n_steps; ++s)
         if (cudaGraphLaunch(bt->graph[gi], stream) != cudaSuccess) return GPT2_B200_ECUDA;
     return GPT2_B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gpt2_b200_batch_create(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2KVCache *kvs,
+                           int B) {
+    return batch_new(out, w, nullptr, kvs, B);
+}
+
+int gpt2_b200_batch_create_w4(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B) {
+    if (!q) {
+        if (out) *out = nullptr;
+        return GPT2_B200_EINVAL;
+    }
+    return batch_new(out, w, q, kvs, B);
+}
+
+void gpt2_b200_batch_destroy(gpt2_b200_batch *bt) {
+    if (!bt) return;
+    // replays queued on any stream may still be running: drain the device before releasing them
+    int prev = -1;
+    if (cudaGetDevice(&prev) == cudaSuccess && prev != bt->device) cudaSetDevice(bt->device);
+    cudaDeviceSynchronize();
+    for (cudaGraphExec_t &g : bt->graph)
+        if (g) cudaGraphExecDestroy(g);
+    if (bt->arena) cudaFree(bt->arena);
+    if (bt->logits) cudaFree(bt->logits);
+    if (prev >= 0 && prev != bt->device) cudaSetDevice(prev);
+    delete bt;
+}
+
+int gpt2_b200_batch_step(gpt2_b200_batch *bt, const int *d_tokens, const int *d_pos,
+                         gpt2_half *logits, long long logits_stride, int *d_next,
+                         cudaStream_t stream) {
+    if (!bt || !d_tokens || !d_pos) return GPT2_B200_EINVAL;
+    if (logits && (logits_stride < V || !aligned16(logits))) return GPT2_B200_EINVAL;
+    int rc = check_device(bt);
+    if (rc) return rc;
+    if ((rc = enqueue_step(bt, d_tokens, d_pos, logits, logits_stride, nullptr, false, stream)))
+        return rc;
+    if (d_next) {
+        if ((rc = launch(k_argmax, bt->B, 128, stream, bt->pdl, d_next, bt->amax,
+                         bt->head_keys)) != GPT2_B200_OK)
+            return rc;
+    }
+    return GPT2_B200_OK;
+}
+
+int gpt2_b200_batch_launches_per_step(const gpt2_b200_batch *bt, int flags) {
+    if (!bt) return -1;
+    // attention only: 12 attention launches + the bookkeeping kernel
+    if (flags & GPT2_B200_GEN_ATTENTION_ONLY) return NL + 1;
+    // embed+LN, 12 x (QKV, attention, proj, LN2, FC, proj2, LN), head, bookkeeping
+    return 1 + NL * 7 + 1 + 1;
+}
+
+int gpt2_b200_batch_generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride,
+                             const int *d_plen, int n_steps, int *d_out, long long out_stride,
+                             int flags, cudaStream_t stream) {
+    const bool attn_only = (flags & GPT2_B200_GEN_ATTENTION_ONLY) != 0;
+    return generate(bt, d_prompt, prompt_stride, d_plen, n_steps, d_out, out_stride, attn_only ? 1 : 0, nullptr, stream);
+}
+
+int gpt2_b200_batch_generate_edited(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps, int *d_out,
+                                    long long out_stride, const GPT2LogitsEdit *edit, cudaStream_t stream) {
+    if (!edit || edit->history || edit->length || edit->prompt) return GPT2_B200_EINVAL;
+    return generate(bt, d_prompt, prompt_stride, d_plen, n_steps, d_out, out_stride, 2, edit, stream);
 }
 
 // ---------------------------------------------------------------- the linear layer alone

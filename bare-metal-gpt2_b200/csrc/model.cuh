@@ -118,13 +118,14 @@ int launch(void (*kern)(KArgs...), int grid, int block, cudaStream_t st, bool pd
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-inline bool weights_ok(const GPT2WeightsGPU *w) {
+// linear: the four matmul weights of each layer are needed too (a batch over 4-bit weights has others).
+inline bool weights_ok(const GPT2WeightsGPU *w, bool linear = true) {
     if (!w || !w->wte || !w->wpe || !w->lnf_g || !w->lnf_b || !aligned16(w->wte)) return false;
     for (int L = 0; L < NL; ++L) {
         const GPT2LayerGPU &l = w->layers[L];
-        if (!l.ln1_g || !l.ln1_b || !l.qkv_w || !l.qkv_b || !l.attn_proj_w || !l.attn_proj_b ||
-            !l.ln2_g || !l.ln2_b || !l.fc_w || !l.fc_b || !l.proj_w || !l.proj_b)
-            return false;
+        if (!l.ln1_g || !l.ln1_b || !l.qkv_b || !l.attn_proj_b || !l.ln2_g || !l.ln2_b || !l.fc_b || !l.proj_b) return false;
+        if (!linear) continue;
+        if (!l.qkv_w || !l.attn_proj_w || !l.fc_w || !l.proj_w) return false;
         if (!aligned16(l.qkv_w) || !aligned16(l.attn_proj_w) || !aligned16(l.fc_w) ||
             !aligned16(l.proj_w))
             return false;

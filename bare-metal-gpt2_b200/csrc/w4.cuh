@@ -70,20 +70,44 @@ struct Dest {
     unsigned *status;
 };
 
-struct Plan {
-    GPT2W4 w;
+struct RowParams {
+    const uint8_t *codes;
+    const __half *scale, *least;
+    int K, shift;  // log2 of the group
     const __half *x;
     long long ldx;
+    int tiles, steps, panel;  // tiles; steps of a warp per tile, and those whose x is held at once (a multiple of DEPTH)
     Dest d;
-    bool pdl;
 };
 
-bool shape_ok(const GPT2W4 *w);    // sizes
-bool weight_ok(const GPT2W4 *w);   // and pointers
-int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo);
-int keys_of(const GPT2W4 &w, int B);  // argmax keys per row that a plan of EPI_HEAD writes
-int prepare(const Plan &pl);          // kernel attributes, so that a capture finds them set
-int launch(const Plan &pl, cudaStream_t stream);
+struct TcParams {
+    const __half *scale, *least;
+    int K, shift;            // shift: log2 of the group
+    int stages, cs, tiles;   // per tile; CTAs that share a tile's k; tiles
+    int x_ring, bpad, nacc;  // stages of x in flight; columns; accumulators
+    int push, share;         // split k: sums are pushed to the CTA that adds them (else pulled); columns that each adds
+    Dest d;
+    unsigned long long timeout_ns;
+};
+
+// A launch that was thought out: which kernel, how it is split, its tensor maps.
+struct Plan {
+    CUtensorMap tm_w, tm_x;
+    RowParams rows;  // few: up to 8 rows
+    TcParams tc;     // else
+    Dest d;
+    bool few, pdl;  // pdl: a programmatic dependent of the kernel before it
+    const void *kernel;
+    dim3 grid;
+    int threads, cluster;
+    size_t smem;
+};
+
+bool shape_ok(const GPT2W4 *w);   // sizes
+bool weight_ok(const GPT2W4 *w);  // and pointers
+// resid and ldr: EPI_RESID's. Returns a GPT2_B200_* code; d's fields of EPI_QKV and EPI_HEAD are the caller's to fill in.
+int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo, const __half *resid, long long ldr);
+int launch(Plan &pl, cudaStream_t stream);
 
 }  // namespace w4
 }  // namespace b200

@@ -62,7 +62,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // ---------------------------------------------------------------- few rows
-// B <= 16: bound by reading the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
+// B <= 8: bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
 // feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA, TMEM and
 // their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
 //   - A step is 16 features x 128 k: lane (g, t) = (lane / 4, lane % 4) holds 32 neighbouring k, 16 bytes, of features g and g + 8.
@@ -76,16 +76,6 @@ constexpr int ROW_CTAS = 2;  // per SM
 constexpr int ROWS_MAX_B = 8;
 constexpr int PANEL_BYTES = 88 * 1024;  // of x in shared memory
 
-struct RowParams {
-    const uint8_t *codes;
-    const __half *scale, *least;
-    int K, shift;  // log2 of the group
-    const __half *x;
-    long long ldx;
-    int tiles, steps, panel;  // tiles; steps of a warp per tile, and those whose x is held at once (a multiple of DEPTH)
-    Dest d;
-};
-
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -95,9 +85,9 @@ __device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 __device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
-template <int NT, int WR, bool LEAST>
+template <int WR, bool LEAST>
 __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowParams p) {
-    constexpr int WK = ROW_WARPS / WR, COLS = 8 * NT, FEATURES = 16 * WR;
+    constexpr int WK = ROW_WARPS / WR, COLS = ROWS_MAX_B, FEATURES = 16 * WR;
     extern __shared__ __align__(16) uint8_t xs[];  // [B][panel * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
     __shared__ float red[2][WK][FEATURES][COLS + 1];
     const Dest &d = p.d;
@@ -158,9 +148,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
     };
     fill(0);
     // Rows of x past the last are read as the last: the columns are dropped.
-    const uint8_t *xr[NT];
-#pragma unroll
-    for (int q = 0; q < NT; ++q) xr[q] = xs + min(8 * q + g, d.B - 1) * x_row + kg * 256 + t * 16;
+    const uint8_t *xr = xs + min(g, d.B - 1) * x_row + kg * 256 + t * 16;
 
     // The outputs of this thread: 16 lanes take 16 neighbouring features of a row of x.
     const int sub = tid >> 4, f = tid & 15, units = WR * d.B;
@@ -168,7 +156,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
         const int n0 = tile * FEATURES, next = tile + gridDim.x;
         Extra early = {0.0f, 0.0f};
         if (sub < units && n0 + sub % WR * 16 + f < d.N) early = extra_of(d, sub / WR, n0 + sub % WR * 16 + f);
-        float c[NT][4] = {};
+        float c[4] = {};
         if (next < p.tiles) then = place(next);
         for (int first = 0; first < p.steps; first += p.panel) {
             if (p.panel < p.steps && (first || tile != static_cast<int>(blockIdx.x))) {
@@ -186,12 +174,9 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
                     values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
                     values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
                     const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
-#pragma unroll
-                    for (int m = 0; m < NT; ++m) {
-                        const uint4 xv = *reinterpret_cast<const uint4 *>(xr[m] + x_at + u * (WK * 256) + j * 64);
-                        mma16816(c[m], a0, xv.x, xv.y);
-                        mma16816(c[m], a1, xv.z, xv.w);
-                    }
+                    const uint4 xv = *reinterpret_cast<const uint4 *>(xr + x_at + u * (WK * 256) + j * 64);
+                    mma16816(c, a0, xv.x, xv.y);
+                    mma16816(c, a1, xv.z, xv.w);
                 }
             };
             const auto use = [&](int u) {
@@ -238,9 +223,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
             }
         }
 #pragma unroll
-        for (int q = 0; q < NT; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][8 * q + 2 * t + (i & 1)] = c[q][i];
+        for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][2 * t + (i & 1)] = c[i];
         here = then;
         __syncthreads();  // the other half of red is free: its readers came here
         for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 16) {
@@ -264,7 +247,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
 }
 
 // ---------------------------------------------------------------- many rows
-// B > 16, on tcgen05: 256 features x up to 128 rows of x per CTA, as two MMAs of 128 features that share x; more rows are
+// B > 8, on tcgen05: 256 features x up to 128 rows of x per CTA, as two MMAs of 128 features that share x; more rows are
 // several column blocks. Sums of 128 k at a time:
 //   warp 0       TMA of the codes, 2 x 128 features x 64 bytes (64-byte swizzle), as they lie;
 //   warp 2       TMA of x, 128-byte swizzle, K-major: the MMAs' B operand;
@@ -289,16 +272,6 @@ constexpr int A_COLS = KS / 2;               // TMEM columns of one
 constexpr int TC_THREADS = 640;
 constexpr int CONVERTERS = 16;               // warps
 constexpr size_t TC_SMEM = 226 * 1024;       // the SM for itself: no other CTA's TMEM allocation meets this one's
-
-struct TcParams {
-    const __half *scale, *least;
-    int K, shift;            // shift: log2 of the group
-    int stages, cs, tiles;   // per tile; CTAs that share a tile's k; tiles
-    int x_ring, bpad, nacc;  // stages of x in flight; columns; accumulators
-    int push, share;         // split k: sums are pushed to the CTA that adds them (else pulled); columns that each adds
-    Dest d;
-    unsigned long long timeout_ns;
-};
 
 __device__ __forceinline__ float4 dsmem_ld_v4(uint32_t cluster_saddr) {
     float4 v;
@@ -741,16 +714,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     if (warp == 1) tmem_dealloc(tmem_slot, 512);
 }
 
-}  // namespace
-
-namespace {
-
 typedef void (*TcKernel)(CUtensorMap, CUtensorMap, TcParams);
 template <bool LEAST>
 TcKernel tc_kernel(int group) {
     return group == 128 ? k_w4_tc<1, LEAST> : group == 64 ? k_w4_tc<2, LEAST> : k_w4_tc<4, LEAST>;
 }
-TcKernel tc_kernel(const GPT2W4 &w) { return w.least ? tc_kernel<true>(w.group) : tc_kernel<false>(w.group); }
+typedef void (*RowKernel)(RowParams);
+template <bool LEAST>
+RowKernel row_kernel(int wr) {
+    return wr == 1 ? k_w4_rows<1, LEAST> : wr == 2 ? k_w4_rows<2, LEAST> : wr == 4 ? k_w4_rows<4, LEAST> : k_w4_rows<8, LEAST>;
+}
 
 bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long inner, long long rows, long long row_bytes, int box_inner, int box_rows,
             CUtensorMapSwizzle swizzle) {
@@ -761,6 +734,20 @@ bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
     return fn(m, type, 2, const_cast<void *>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The kernels' shared memory, on the current device once: so that neither a launch nor a capture has to.
+int prepare(DeviceContext *ctx) {
+    if (ctx->w4_attr_done) return GPT2_B200_OK;
+    RelaxedCapture relaxed;
+    for (int wr = 1; wr <= ROW_WARPS; wr *= 2)
+        for (const RowKernel k : {row_kernel<false>(wr), row_kernel<true>(wr)})
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, PANEL_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
+    for (int group = 32; group <= 128; group *= 2)
+        for (const TcKernel k : {tc_kernel<false>(group), tc_kernel<true>(group)})
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
+    ctx->w4_attr_done = true;
+    return GPT2_B200_OK;
 }
 
 // How many clusters of cs CTAs run at once (one CTA per SM), asked once per device.
@@ -779,89 +766,32 @@ int active_clusters(DeviceContext *ctx, int cs) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int got = 0;
-    if (cudaOccupancyMaxActiveClusters(&got, k_w4_tc<1, false>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&got, tc_kernel<false>(128), &cfg) != cudaSuccess) {
         cudaGetLastError();
         return 0;
     }
     return n = got;
 }
 
-int prepare_tc(DeviceContext *ctx) {
-    if (ctx->w4_attr_done) return GPT2_B200_OK;
-    RelaxedCapture relaxed;
-    for (const TcKernel k : {tc_kernel<false>(32), tc_kernel<false>(64), tc_kernel<false>(128), tc_kernel<true>(32), tc_kernel<true>(64), tc_kernel<true>(128)})
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
-    ctx->w4_attr_done = true;
-    return GPT2_B200_OK;
-}
-
-}  // namespace
-
-int keys_of(const GPT2W4 &w, int B) { return B <= ROWS_MAX_B ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * 8; }
-
-int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo) {
-    if (!weight_ok(&w) || !x || (reinterpret_cast<uintptr_t>(x) & 15) || (ldx & 7) || ldx < w.K || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
-    if (epi < EPI_STORE || epi > EPI_HEAD || (epi != EPI_HEAD && !out) || (out && ldo < w.N) ||
-        ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1))
-        return GPT2_B200_EINVAL;
-    DeviceContext *ctx = device_context();
-    if (!ctx) return GPT2_B200_ECUDA;
-    *pl = Plan{};
-    pl->w = w;
-    pl->x = x;
-    pl->ldx = ldx;
-    pl->d.epi = epi;
-    pl->d.B = B;
-    pl->d.N = w.N;
-    pl->d.bias = bias;
-    pl->d.out = out;
-    pl->d.ldo = ldo;
-    pl->d.keys = keys_of(w, B);
-    pl->d.status = ctx->status;
-    return GPT2_B200_OK;
-}
-
-namespace {
-
-typedef void (*RowKernel)(RowParams);
-template <int NT, bool LEAST>
-RowKernel row_kernel(int wr) {
-    return wr == 1 ? k_w4_rows<NT, 1, LEAST> : wr == 2 ? k_w4_rows<NT, 2, LEAST> : wr == 4 ? k_w4_rows<NT, 4, LEAST> : k_w4_rows<NT, 8, LEAST>;
-}
-
-int prepare_rows(DeviceContext *ctx) {
-    if (ctx->w4_rows_attr_done) return GPT2_B200_OK;
-    RelaxedCapture relaxed;
-    for (int wr = 1; wr <= 8; wr *= 2)
-        for (const RowKernel k : {row_kernel<1, false>(wr), row_kernel<1, true>(wr), row_kernel<2, false>(wr), row_kernel<2, true>(wr)})
-            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, PANEL_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
-    ctx->w4_rows_attr_done = true;
-    return GPT2_B200_OK;
-}
-
-int launch_rows(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
-    const int rc = prepare_rows(ctx);
-    if (rc != GPT2_B200_OK) return rc;
-    const GPT2W4 &w = pl.w;
-    const int B = pl.d.B, nt = B <= 8 ? 1 : 2, chunks = (w.K + CHUNK - 1) / CHUNK, slots = ROW_CTAS * ctx->num_sms;
-    RowParams p = {};
+int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, long long ldx) {
+    const int B = pl->d.B, chunks = (w.K + CHUNK - 1) / CHUNK, slots = ROW_CTAS * ctx->num_sms;
+    RowParams &p = pl->rows;
     p.codes = static_cast<const uint8_t *>(w.codes);
     p.scale = w.scale;
     p.least = w.least;
     p.K = w.K;
     p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
-    p.x = pl.x;
-    p.ldx = pl.ldx;
-    p.d = pl.d;
+    p.x = x;
+    p.ldx = ldx;
     // Tile height: the fewest steps of the busiest CTA, a tile's end counted as one.
-    int wr = 1;
+    int wr = 0;
     long long best = 0;
     for (int h = 1; h <= ROW_WARPS; h *= 2) {
         const long long tiles = (static_cast<long long>(w.N) + 16 * h - 1) / (16 * h), rounds = (tiles + slots - 1) / slots;
         const int wk = ROW_WARPS / h, steps = (chunks + wk - 1) / wk;
         const long long cost = rounds * (steps + 1);
         if ((PANEL_BYTES / B - 64) / (256 * wk) < DEPTH) continue;  // x has room for a round of the buffers
-        if (!best || cost < best) {
+        if (!wr || cost < best) {
             best = cost;
             wr = h;
             p.tiles = static_cast<int>(tiles);
@@ -870,25 +800,16 @@ int launch_rows(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     }
     const int wk = ROW_WARPS / wr, fit = (PANEL_BYTES / B - 64) / (256 * wk);  // steps whose x fits
     p.panel = std::min((p.steps + DEPTH - 1) / DEPTH, fit / DEPTH) * DEPTH;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tiles, slots)), 1, 1);
-    cfg.blockDim = dim3(ROW_WARPS * 32, 1, 1);
-    cfg.dynamicSmemBytes = static_cast<size_t>(B) * (p.panel * wk * 256 + 64);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pl.pdl ? 1 : 0;
-    const RowKernel k = nt == 1 ? (w.least ? row_kernel<1, true>(wr) : row_kernel<1, false>(wr)) : (w.least ? row_kernel<2, true>(wr) : row_kernel<2, false>(wr));
-    return cudaLaunchKernelEx(&cfg, k, p) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    pl->grid = dim3(static_cast<unsigned>(std::min(p.tiles, slots)), 1, 1);
+    pl->threads = ROW_WARPS * 32;
+    pl->smem = static_cast<size_t>(B) * (p.panel * wk * 256 + 64);
+    pl->kernel = reinterpret_cast<const void *>(w.least ? row_kernel<true>(wr) : row_kernel<false>(wr));
+    return GPT2_B200_OK;
 }
 
-int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
-    const int rc = prepare_tc(ctx);
-    if (rc != GPT2_B200_OK) return rc;
-    const GPT2W4 &w = pl.w;
-    TcParams p = {};
+int plan_tc(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, long long ldx) {
+    const Dest &d = pl->d;
+    TcParams &p = pl->tc;
     p.scale = w.scale;
     p.least = w.least;
     p.K = w.K;
@@ -901,12 +822,12 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     // cheaper than adding wide sums (64 x 2304 x 768).
     int blocks = 0;
     long long best = 0;
-    for (int n = (pl.d.B + MAX_COLS - 1) / MAX_COLS; n <= (pl.d.B + 15) / 16; ++n) {
-        const int cols = ((pl.d.B + n - 1) / n + 15) / 16 * 16;
-        if ((pl.d.B + cols - 1) / cols != n) continue;  // an empty block
+    for (int n = (d.B + MAX_COLS - 1) / MAX_COLS; n <= (d.B + 15) / 16; ++n) {
+        const int cols = ((d.B + n - 1) / n + 15) / 16 * 16;
+        if ((d.B + cols - 1) / cols != n) continue;  // an empty block
         const long long stage = std::max(1000, 8 * cols);
         for (int c = 1; c <= std::min(lin::MAX_CLUSTER, p.stages); ++c) {
-            if (c > 1 && (pl.d.epi == EPI_HEAD || p.tiles > active_clusters(ctx, c) / n)) continue;
+            if (c > 1 && (d.epi == EPI_HEAD || p.tiles > active_clusters(ctx, c) / n)) continue;
             const long long each = std::max(1, ctx->num_sms / n), rounds = c > 1 ? 1 : (p.tiles + each - 1) / each;
             const long long cost = 3300 + rounds * ((p.stages + c - 1) / c * stage + (c > 1 ? 2000 + 90 * cols : 40 * cols));
             if (!blocks || cost < best) {
@@ -918,26 +839,60 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
         }
     }
     p.nacc = p.bpad <= 64 ? 2 : 1;
-    p.d = pl.d;
     p.timeout_ns = wait_timeout_ns();
     p.share = (p.bpad + p.cs - 1) / p.cs;
     p.push = p.cs > 1 && p.bpad <= PUSH_COLS;
     const size_t rest = TC_SMEM - 1024 - CODE_RING * CODE_BYTES - (p.push ? static_cast<size_t>(p.cs) * p.share * FEATURES * 4 : 0);
     p.x_ring = std::min<int>(MAX_X_RING, static_cast<int>(rest / (p.bpad * 2 * KS)));
-    CUtensorMap tm_w, tm_x;
-    if (!encode(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, w.K / 2, w.N, w.K / 2, KS / 2, BM, CU_TENSOR_MAP_SWIZZLE_64B) ||
-        !encode(&tm_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, pl.x, w.K, pl.d.B, pl.ldx * 2, 64, p.bpad, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (!encode(&pl->tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, w.K / 2, w.N, w.K / 2, KS / 2, BM, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !encode(&pl->tm_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, w.K, d.B, ldx * 2, 64, p.bpad, CU_TENSOR_MAP_SWIZZLE_128B))
         return GPT2_B200_EDEVICE;
+    pl->cluster = p.cs;
+    pl->grid = dim3(static_cast<unsigned>(p.cs > 1 ? p.tiles * p.cs : std::min(p.tiles, std::max(1, ctx->num_sms / blocks))), blocks, 1);
+    pl->threads = TC_THREADS;
+    pl->smem = TC_SMEM;
+    pl->kernel = reinterpret_cast<const void *>(w.least ? tc_kernel<true>(w.group) : tc_kernel<false>(w.group));
+    return GPT2_B200_OK;
+}
+
+}  // namespace
+
+int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo, const __half *resid, long long ldr) {
+    if (!weight_ok(&w) || !x || (reinterpret_cast<uintptr_t>(x) & 15) || (ldx & 7) || ldx < w.K || B < 1 || B > lin::MAX_BPAD) return GPT2_B200_EINVAL;
+    if (epi < EPI_STORE || epi > EPI_HEAD || (epi != EPI_HEAD && !out) || (out && ldo < w.N) || (epi == EPI_RESID && (!resid || ldr < w.N)) ||
+        ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(resid)) & 1))
+        return GPT2_B200_EINVAL;
+    DeviceContext *ctx = device_context();
+    if (!ctx) return GPT2_B200_ECUDA;
+    const int rc = prepare(ctx);
+    if (rc != GPT2_B200_OK) return rc;
+    *pl = Plan{};
+    pl->d.epi = epi;
+    pl->d.B = B;
+    pl->d.N = w.N;
+    pl->d.bias = bias;
+    pl->d.out = out;
+    pl->d.ldo = ldo;
+    pl->d.resid = resid;
+    pl->d.ldr = ldr;
+    pl->few = B <= ROWS_MAX_B;
+    pl->d.keys = pl->few ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * (FEATURES / 32);
+    pl->d.status = ctx->status;
+    pl->cluster = 1;
+    return pl->few ? plan_rows(ctx, pl, w, x, ldx) : plan_tc(ctx, pl, w, x, ldx);
+}
+
+int launch(Plan &pl, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.cs > 1 ? p.tiles * p.cs : std::min(p.tiles, std::max(1, ctx->num_sms / blocks))), blocks, 1);
-    cfg.blockDim = dim3(TC_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = TC_SMEM;
+    cfg.gridDim = pl.grid;
+    cfg.blockDim = dim3(pl.threads, 1, 1);
+    cfg.dynamicSmemBytes = pl.smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int na = 0;
-    if (p.cs > 1) {
+    if (pl.cluster > 1) {
         attr[na].id = cudaLaunchAttributeClusterDimension;
-        attr[na].val.clusterDim.x = static_cast<unsigned>(p.cs);
+        attr[na].val.clusterDim.x = static_cast<unsigned>(pl.cluster);
         attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
         ++na;
     }
@@ -948,21 +903,9 @@ int launch_tc(DeviceContext *ctx, const Plan &pl, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    return cudaLaunchKernelEx(&cfg, tc_kernel(w), tm_w, tm_x, p) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
-}
-
-}  // namespace
-
-int prepare(const Plan &pl) {
-    DeviceContext *ctx = device_context();
-    if (!ctx) return GPT2_B200_ECUDA;
-    return pl.d.B <= ROWS_MAX_B ? prepare_rows(ctx) : prepare_tc(ctx);
-}
-
-int launch(const Plan &pl, cudaStream_t stream) {
-    DeviceContext *ctx = device_context();
-    if (!ctx) return GPT2_B200_ECUDA;
-    return pl.d.B <= ROWS_MAX_B ? launch_rows(ctx, pl, stream) : launch_tc(ctx, pl, stream);
+    pl.rows.d = pl.tc.d = pl.d;
+    void *few[1] = {&pl.rows}, *many[3] = {&pl.tm_w, &pl.tm_x, &pl.tc};
+    return cudaLaunchKernelExC(&cfg, pl.kernel, pl.few ? few : many) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
 }  // namespace w4
@@ -972,12 +915,9 @@ using namespace b200;
 
 extern "C" int gpt2_w4_linear_b200(gpt2_half *C, long long ldc, const gpt2_half *A, long long lda, const GPT2W4 *w, const gpt2_half *bias, const gpt2_half *R,
                                    long long ldr, int B, int epi, cudaStream_t stream) {
-    if (!w || !C || epi < GPT2_B200_LINEAR_STORE || epi > GPT2_B200_LINEAR_RESID || (epi == GPT2_B200_LINEAR_RESID && (!R || (reinterpret_cast<uintptr_t>(R) & 1) || ldr < w->N)))
-        return GPT2_B200_EINVAL;
+    if (!w || !C || epi < GPT2_B200_LINEAR_STORE || epi > GPT2_B200_LINEAR_RESID) return GPT2_B200_EINVAL;
+    const int e = epi == GPT2_B200_LINEAR_STORE ? lin::EPI_STORE : epi == GPT2_B200_LINEAR_GELU ? lin::EPI_GELU : lin::EPI_RESID;
     w4::Plan pl;
-    const int rc = w4::plan(&pl, epi == GPT2_B200_LINEAR_STORE ? lin::EPI_STORE : epi == GPT2_B200_LINEAR_GELU ? lin::EPI_GELU : lin::EPI_RESID, *w, A, lda, B, bias, C, ldc);
-    if (rc != GPT2_B200_OK) return rc;
-    pl.d.resid = R;
-    pl.d.ldr = ldr;
-    return w4::launch(pl, stream);
+    const int rc = w4::plan(&pl, e, *w, A, lda, B, bias, C, ldc, e == lin::EPI_RESID ? R : nullptr, ldr);
+    return rc == GPT2_B200_OK ? w4::launch(pl, stream) : rc;
 }

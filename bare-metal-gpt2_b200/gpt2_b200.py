@@ -107,6 +107,12 @@ class GPT2LogitsEdit(ctypes.Structure):
                 ("mask_rows", ctypes.c_int), ("mask_row", ctypes.c_void_p)]
 
 
+class GPT2W4Weights(ctypes.Structure):
+    """GPT-2-124M's matmul weights in 4 bits (include/gpt2_b200.h)."""
+
+    _fields_ = [(n, GPT2W4 * N_LAYER) for n in ("qkv", "attn_proj", "fc", "proj")] + [("head", GPT2W4)]
+
+
 class GPT2LayerGPU(ctypes.Structure):
     """Same layout as GPT2LayerGPU in the reference's cuda/kernels.cuh:19-23."""
 
@@ -186,6 +192,8 @@ _SIGS = {
     "gpt2_w4_dequantize_b200": (_ci, [_vp, _cll, _w4p, _vp]),
     "gpt2_w4_linear_b200": (_ci, [_vp, _cll, _vp, _cll, _w4p, _vp, _vp, _cll, _ci, _ci, _vp]),
     "gpt2_logits_edit_b200": (_ci, [_vp, _cll, _vp, _cll, _ci, _ci, _ci, _edp, _vp, _vp]),
+    "gpt2_b200_batch_create_w4": (_ci, [ctypes.POINTER(_vp), _wp, ctypes.POINTER(GPT2W4Weights), _kvp, _ci]),
+    "gpt2_b200_batch_generate_edited": (_ci, [_vp, _vp, _cll, _vp, _ci, _vp, _cll, _edp, _vp]),
     "gpt2_b200_compose_backend": (None, [ctypes.POINTER(GPT2Backend), ctypes.POINTER(GPT2Backend)]),
     "gpt2_b200_reserve": (_ci, [_ci, _ci, _ci]),
     "gpt2_b200_status": (_cu, [_ci]),
@@ -508,7 +516,7 @@ class LogitsEdit:
         tensors = (repetition, frequency, presence, history, length, prompt, bias_token, bias, n_bias, mask, mask_row)
         some = [t for t in tensors if t is not None]
         self.lib, self.rows, self.vocab, self.tensors = lib, rows, vocab, tensors
-        self._at = some[0].device if some else None
+        self._at = self.device = some[0].device if some else None
         i32, f32, self._kinds, _ = _types()
         e = GPT2LogitsEdit()
         for name, t, kind in (("repetition", repetition, f32), ("frequency", frequency, f32), ("presence", presence, f32), ("length", length, i32),
@@ -608,20 +616,44 @@ class ModelWeights:
         self.struct = w
 
 
+class W4ModelWeights:
+    """The matmul weights of a ModelWeights in 4 bits (GPT2W4Weights): `layers` holds a W4Weight per layer and name, `head` the tied
+    head's, or None with head=False (the fp16 embedding is the head then)."""
+
+    NAMES = (("qkv", "qkv_w"), ("attn_proj", "attn_proj_w"), ("fc", "fc_w"), ("proj", "proj_w"))
+
+    def __init__(self, lib: "Lib", torch, weights: ModelWeights, group: int = 64, least: bool = False, head: bool = True, stream: int = 0):
+        self.struct = GPT2W4Weights()
+        self.layers = []
+        for L in range(N_LAYER):
+            q = {n: W4Weight.pack(lib, torch, weights.t[f"h{L}.{t}"], group, least, stream) for n, t in self.NAMES}
+            for n, _ in self.NAMES:
+                getattr(self.struct, n)[L] = q[n].c
+            self.layers.append(q)
+        self.head = W4Weight.pack(lib, torch, weights.t["wte"], group, least, stream) if head else None
+        if head:
+            self.struct.head = self.head.c
+
+
 class DecodeBatch:
     """B sequences of GPT-2-124M decoded together (the gpt2_b200_batch_* entry points).
 
     caches: a torch fp16 tensor [B][12][2][12][maxT][64] (each sequence's arena in the reference
     layout) that stays alive as long as the batch. step() consumes one token per sequence at its
     position; generate() runs lock-step greedy generation (prompt tokens first) in a CUDA graph.
+    w4: the matmuls run over these 4-bit weights instead of the weights' own.
     """
 
-    def __init__(self, lib: "Lib", weights: ModelWeights, caches):
-        self.lib, self.weights, self.caches = lib, weights, caches
+    def __init__(self, lib: "Lib", weights: ModelWeights, caches, w4: "W4ModelWeights | None" = None):
+        self.lib, self.weights, self.caches, self.w4 = lib, weights, caches, w4
         self.B, max_t = int(caches.shape[0]), int(caches.shape[4])
         self.kvs = (GPT2KVCache * self.B)(*[cache_view(caches[b].data_ptr(), N_LAYER, max_t)
                                              for b in range(self.B)])
         self.h = ctypes.c_void_p()
+        if w4 is not None:
+            lib.check(lib.gpt2_b200_batch_create_w4(ctypes.byref(self.h), ctypes.byref(weights.struct), ctypes.byref(w4.struct),
+                                                    self.kvs, self.B), "gpt2_b200_batch_create_w4")
+            return
         lib.check(lib.gpt2_b200_batch_create(ctypes.byref(self.h), ctypes.byref(weights.struct),
                                              self.kvs, self.B), "gpt2_b200_batch_create")
 
@@ -635,8 +667,22 @@ class DecodeBatch:
             next_tokens.data_ptr() if next_tokens is not None else None, stream),
             "gpt2_b200_batch_step")
 
-    def generate(self, prompt, prompt_len, n_steps: int, out, stream: int = 0) -> None:
-        """prompt: int32 [B][P]; prompt_len: int32 [B] (1..P); out: int32 [B][>= n_steps+1]."""
+    def generate(self, prompt, prompt_len, n_steps: int, out, stream: int = 0, edit: "LogitsEdit | None" = None) -> None:
+        """prompt: int32 [B][P]; prompt_len: int32 [B] (1..P); out: int32 [B][>= n_steps+1]. edit: made for B rows of VOCAB
+        logits without a history; every choice is made of the logits so edited, out and prompt_len being the history."""
+        if edit is not None:
+            if edit.rows != self.B or edit.vocab != VOCAB or edit.c.history:
+                raise ValueError("generate: edit is for the batch's rows of VOCAB logits, without a history of its own")
+            i32, at = _types()[0], self.caches.device
+            for t in (prompt, out):
+                if t.dim() != 2 or t.dtype is not i32 or t.shape[0] != self.B or t.shape[1] < 1 or t.stride(1) != 1 or t.device != at:
+                    raise ValueError("generate: prompt is int32 [B][P], out int32 [B][>= n_steps + 1], on the caches' device")
+            if out.shape[1] <= n_steps or (edit.device is not None and edit.device != at):
+                raise ValueError("generate: out is too narrow, or the edit is on another device")
+            self.lib.check(self.lib.gpt2_b200_batch_generate_edited(
+                self.h, prompt.data_ptr(), prompt.stride(0), _vector("generate", prompt_len, i32, self.B, at), n_steps, out.data_ptr(), out.stride(0),
+                edit.ref_c, stream), "gpt2_b200_batch_generate_edited")
+            return
         self.lib.check(self.lib.gpt2_b200_batch_generate(
             self.h, prompt.data_ptr(), prompt.stride(0), prompt_len.data_ptr(), n_steps,
             out.data_ptr(), out.stride(0), 0, stream), "gpt2_b200_batch_generate")

@@ -469,6 +469,22 @@ typedef struct {
 int gpt2_logits_edit_b200(void *out, long long ldo, const void *logits, long long ld, int type, int rows, int V, const GPT2LogitsEdit *edit,
                           int *d_next, cudaStream_t stream);
 
+/* The decode step over 4-bit weights: gpt2_b200_batch_create with every layer's four matmul weights, and the head's if head.codes is not
+ * NULL (else the fp16 wte is the head), in 4 bits: qkv [2304][768], attn_proj [768][768], fc [FFN][768], proj [768][FFN], head
+ * [50257][768]. w gives the embeddings, LayerNorms and biases; its matmul weights may be NULL. The 4-bit weights stay owned by the caller.
+ * All gpt2_b200_batch_* calls take such a batch. Each output is rounded once, behind bias, GELU or residual. */
+typedef struct {
+    GPT2W4 qkv[12], attn_proj[12], fc[12], proj[12], head;
+} GPT2W4Weights;
+int gpt2_b200_batch_create_w4(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B);
+
+/* gpt2_b200_batch_generate with every step's logits edited before the choice, in the same graph: sequence b's history is what d_out[b]
+ * holds so far, its first d_plen[b] tokens the prompt, so edit's history, length and prompt are NULL; the other arrays have
+ * a row per sequence and may be changed between steps by work ordered on the stream. A sequence with nothing left to choose gets -1 in
+ * d_out (status bits) and goes on from token 0. The first call of a batch allocates its logits. */
+int gpt2_b200_batch_generate_edited(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps, int *d_out,
+                                    long long out_stride, const GPT2LogitsEdit *edit, cudaStream_t stream);
+
 /* ================================================================ backend, status, set-up */
 
 /* Composes a backend the reference's way (cuda/kernels_fused.cu:157-164): copies *base and installs

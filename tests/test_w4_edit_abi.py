@@ -128,3 +128,53 @@ def test_edit_wrappers(lib, torch, monkeypatch):
     assert not made
     e.apply(x, x), e.apply(x.half(), x.half(), torch.zeros(3, **i32))
     assert len(made) == 2
+
+
+def _weights():
+    w = G.GPT2WeightsGPU()
+    for name in ("data", "wte", "wpe", "lnf_g", "lnf_b"):
+        setattr(w, name, 4096)
+    for L in range(12):
+        for name, _ in G.LAYER_TENSORS:
+            setattr(w.layers[L], name, 4096 if not name.endswith("_w") else None)  # the matmuls' own weights are not needed
+    return w
+
+
+def _four_bits():
+    q = G.GPT2W4Weights()
+    for name, N, K in (("qkv", 2304, 768), ("attn_proj", 768, 768), ("fc", 4 * 768, 768), ("proj", 768, 4 * 768)):
+        for L in range(12):
+            getattr(q, name)[L] = weight(N=N, K=K)
+    return q
+
+
+def test_a_batch_refuses_4_bit_weights_of_another_shape(lib):
+    h, w, kv = ctypes.c_void_p(), _weights(), G.cache_view(4096, 12, 32)
+    create = lib.gpt2_b200_batch_create_w4
+
+    def refused(q, w=w, kv=kv, B=1):
+        h.value = 5
+        return create(ctypes.byref(h), ctypes.byref(w), ctypes.byref(q) if q else None, ctypes.byref(kv), B) == G.EINVAL and not h.value
+
+    assert refused(None)
+    for name in ("qkv", "attn_proj", "fc", "proj"):
+        for bad in (dict(N=767), dict(K=704), dict(codes=None), dict(scale=None), dict(codes=4104), dict(group=48)):
+            q = _four_bits()
+            good = getattr(q, name)[7]
+            getattr(q, name)[7] = weight(**{**dict(N=good.N, K=good.K), **bad})
+            assert refused(q), (name, bad)
+    q = _four_bits()
+    q.head = weight(N=50256, K=768)
+    assert refused(q)
+    bad = _weights()
+    bad.layers[3].qkv_b = None
+    assert refused(_four_bits(), w=bad) and refused(_four_bits(), B=0) and refused(_four_bits(), B=257)
+    assert refused(_four_bits(), kv=G.cache_view(4096, 11, 32))
+    assert create(None, ctypes.byref(w), ctypes.byref(_four_bits()), ctypes.byref(kv), 1) == G.EINVAL
+
+
+def test_edited_generation_refuses_a_history_of_its_own(lib):
+    gen = lib.gpt2_b200_batch_generate_edited
+    for bad in (None, edit(history=16), edit(length=16), edit(prompt=16)):
+        assert gen(16, 16, 4, 16, 3, 16, 4, ctypes.byref(bad) if bad else None, None) == G.EINVAL
+    assert gen(None, 16, 4, 16, 3, 16, 4, ctypes.byref(edit()), None) == G.EINVAL
