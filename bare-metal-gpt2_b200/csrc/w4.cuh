@@ -77,6 +77,7 @@ struct RowParams {
     const __half *x;
     long long ldx;
     int tiles, steps, panel;  // tiles; steps of a warp per tile, and those whose x is held at once (a multiple of DEPTH)
+    int ahead;                // codes are fetched before x
     Dest d;
 };
 
@@ -93,7 +94,7 @@ struct TcParams {
 // A launch that was thought out: which kernel, how it is split, its tensor maps.
 struct Plan {
     CUtensorMap tm_w, tm_x;
-    RowParams rows;  // few: up to 8 rows
+    RowParams rows;  // few
     TcParams tc;     // else
     Dest d;
     bool few, pdl;  // pdl: a programmatic dependent of the kernel before it

@@ -62,7 +62,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // ---------------------------------------------------------------- few rows
-// B <= 8: bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
+// B <= 8, and up to 16 for small weights (rows_do): bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
 // feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA, TMEM and
 // their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
 //   - A step is 16 features x 128 k: lane (g, t) = (lane / 4, lane % 4) holds 32 neighbouring k, 16 bytes, of features g and g + 8.
@@ -73,7 +73,7 @@ constexpr int CHUNK = 128;
 constexpr int ROW_WARPS = 8;
 constexpr int DEPTH = 4;
 constexpr int ROW_CTAS = 2;  // per SM
-constexpr int ROWS_MAX_B = 8;
+constexpr int ROWS_MAX_B = 16;
 constexpr int PANEL_BYTES = 88 * 1024;  // of x in shared memory
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
@@ -85,9 +85,10 @@ __device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 __device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
-template <int WR, bool LEAST>
+// NT: instructions side by side, 8 rows of x each.
+template <int NT, int WR, bool LEAST>
 __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowParams p) {
-    constexpr int WK = ROW_WARPS / WR, COLS = ROWS_MAX_B, FEATURES = 16 * WR;
+    constexpr int WK = ROW_WARPS / WR, COLS = 8 * NT, FEATURES = 16 * WR;
     extern __shared__ __align__(16) uint8_t xs[];  // [B][panel * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
     __shared__ float red[2][WK][FEATURES][COLS + 1];
     const Dest &d = p.d;
@@ -111,11 +112,11 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
         return Place{p.codes + (static_cast<long long>(n) * p.K + k_first) / 2, p.codes + (static_cast<long long>(m) * p.K + k_first) / 2, s + 2ll * n, s + 2ll * m};
     };
     constexpr int Q_STEP = CHUNK * WK / 2;
-    const int s_step = ((CHUNK * WK) >> p.shift) * d.N * 2;
+    const long long s_step = ((CHUNK * WK) >> p.shift) * 2ll * d.N;
     const long long to_least = (p.least - p.scale) * 2;
     const auto fetch = [&](int u, const Place &at, int step) {
         step = min(step, last);
-        const long long s = static_cast<long long>(step) * s_step;
+        const long long s = step * s_step;
         ld_codes(qa[u], at.qa + static_cast<long long>(step) * Q_STEP);
         ld_codes(qb[u], at.qb + static_cast<long long>(step) * Q_STEP);
         ld_scale(sa[u], at.sa + s);
@@ -128,27 +129,43 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
     const int full = p.K / (CHUNK * WK);  // steps that are whole for every lane
     int tile = blockIdx.x;
     Place here = place(tile), then = here;
+    const auto fetch_first = [&] {
 #pragma unroll
-    for (int u = 0; u < DEPTH; ++u) {
-        la[u] = lb[u] = 0;
-        fetch(u, here, u);
-    }
-    grid_dependency_wait();
-    grid_launch_dependents();
-
+        for (int u = 0; u < DEPTH; ++u) {
+            la[u] = lb[u] = 0;
+            fetch(u, here, u);
+        }
+    };
     const auto fill = [&](int first) {
-        const int chunk0 = first * WK, held = min(p.panel, p.steps - first) * WK;  // zeros behind the last k
-        for (int b = 0; b < d.B; ++b)
-            for (int i = tid; i < held * 16; i += ROW_WARPS * 32) {
-                const int k = chunk0 * CHUNK + i * 8;  // piece i & 15 = 4 t + j of its chunk goes to place 4 j + t
-                cp_async16(xs + b * x_row + (i >> 4) * 256 + ((i & 3) * 4 + (i >> 2 & 3)) * 16, p.x + b * p.ldx + min(k, p.K - 8), k < p.K);
+        const int k0 = first * WK * CHUNK, per = min(p.panel, p.steps - first) * WK * 16;  // pieces of 8 k per row; zeros behind the last k
+        int b = 0, i = tid;
+        while (true) {
+            while (i >= per) {
+                i -= per;
+                ++b;
             }
+            if (b >= d.B) break;
+            const int k = k0 + i * 8;  // piece i & 15 = 4 t + j of its chunk goes to place 4 j + t
+            cp_async16(xs + b * x_row + (i >> 4) * 256 + ((i & 3) * 4 + (i >> 2 & 3)) * 16, p.x + b * p.ldx + min(k, p.K - 8), k < p.K);
+            i += ROW_WARPS * 32;
+        }
+    };
+    const auto filled = [] {
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
     };
+    // Behind another kernel the codes go first, since they need not wait for it. Otherwise x does: behind the codes of all CTAs, which
+    // fill HBM's queues, it takes 4000 to 8000 cycles to come, without them 1500.
+    if (p.ahead) fetch_first();
+    grid_dependency_wait();
+    grid_launch_dependents();
     fill(0);
+    if (!p.ahead) fetch_first();
+    filled();
     // Rows of x past the last are read as the last: the columns are dropped.
-    const uint8_t *xr = xs + min(g, d.B - 1) * x_row + kg * 256 + t * 16;
+    const uint8_t *xr[NT];
+#pragma unroll
+    for (int q = 0; q < NT; ++q) xr[q] = xs + min(8 * q + g, d.B - 1) * x_row + kg * 256 + t * 16;
 
     // The outputs of this thread: 16 lanes take 16 neighbouring features of a row of x.
     const int sub = tid >> 4, f = tid & 15, units = WR * d.B;
@@ -156,12 +173,13 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
         const int n0 = tile * FEATURES, next = tile + gridDim.x;
         Extra early = {0.0f, 0.0f};
         if (sub < units && n0 + sub % WR * 16 + f < d.N) early = extra_of(d, sub / WR, n0 + sub % WR * 16 + f);
-        float c[4] = {};
+        float c[NT][4] = {};
         if (next < p.tiles) then = place(next);
         for (int first = 0; first < p.steps; first += p.panel) {
             if (p.panel < p.steps && (first || tile != static_cast<int>(blockIdx.x))) {
                 __syncthreads();
                 fill(first);
+                filled();
             }
             const int end = min(p.steps, first + p.panel);
             int x_at = 0, i0 = first;
@@ -174,9 +192,12 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
                     values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
                     values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
                     const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
-                    const uint4 xv = *reinterpret_cast<const uint4 *>(xr + x_at + u * (WK * 256) + j * 64);
-                    mma16816(c, a0, xv.x, xv.y);
-                    mma16816(c, a1, xv.z, xv.w);
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        const uint4 xv = *reinterpret_cast<const uint4 *>(xr[m] + x_at + u * (WK * 256) + j * 64);
+                        mma16816(c[m], a0, xv.x, xv.y);
+                        mma16816(c[m], a1, xv.z, xv.w);
+                    }
                 }
             };
             const auto use = [&](int u) {
@@ -188,7 +209,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
             // Whole rounds whose next fetches are of this tile and all there: no checks, addresses a constant apart.
             if (i0 + 2 * DEPTH <= full) {
                 const uint8_t *pa = here.qa + static_cast<long long>(i0 + DEPTH) * Q_STEP, *pb = here.qb + static_cast<long long>(i0 + DEPTH) * Q_STEP;
-                const uint8_t *ps = here.sa + static_cast<long long>(i0 + DEPTH) * s_step;
+                const uint8_t *ps = here.sa + (i0 + DEPTH) * s_step;
                 const long long other = here.sb - here.sa;
                 for (; i0 < end && i0 + 2 * DEPTH <= full; i0 += DEPTH) {
 #pragma unroll
@@ -223,7 +244,9 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][2 * t + (i & 1)] = c[i];
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][8 * q + 2 * t + (i & 1)] = c[q][i];
         here = then;
         __syncthreads();  // the other half of red is free: its readers came here
         for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 16) {
@@ -247,7 +270,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
 }
 
 // ---------------------------------------------------------------- many rows
-// B > 8, on tcgen05: 256 features x up to 128 rows of x per CTA, as two MMAs of 128 features that share x; more rows are
+// The rest, on tcgen05: 256 features x up to 128 rows of x per CTA, as two MMAs of 128 features that share x; more rows are
 // several column blocks. Sums of 128 k at a time:
 //   warp 0       TMA of the codes, 2 x 128 features x 64 bytes (64-byte swizzle), as they lie;
 //   warp 2       TMA of x, 128-byte swizzle, K-major: the MMAs' B operand;
@@ -719,10 +742,18 @@ template <bool LEAST>
 TcKernel tc_kernel(int group) {
     return group == 128 ? k_w4_tc<1, LEAST> : group == 64 ? k_w4_tc<2, LEAST> : k_w4_tc<4, LEAST>;
 }
+// Which of the two. Up to 8 rows k_w4_rows. Up to 16, two MMAs per weight are cheaper than what k_w4_tc takes
+// to start, as long as the weights are few and x is held at once. Rows against tcgen05, us at B = 16: 768 x 768 4.9 against 6.5, 2304 x 768
+// 5.4 against 6.5, 4096 x 1024 6.8 against 6.9; 768 x 4 * 768 (two panels of x) 9.7 against 7.8, 4096 x 4096 14.8 against 10.0.
+bool rows_do(int B, int N, int K) { return B <= 8 || (B <= ROWS_MAX_B && K <= 2048 && static_cast<long long>(N) * K <= 1 << 22); }
+
 typedef void (*RowKernel)(RowParams);
-template <bool LEAST>
+template <int NT, bool LEAST>
 RowKernel row_kernel(int wr) {
-    return wr == 1 ? k_w4_rows<1, LEAST> : wr == 2 ? k_w4_rows<2, LEAST> : wr == 4 ? k_w4_rows<4, LEAST> : k_w4_rows<8, LEAST>;
+    return wr == 1 ? k_w4_rows<NT, 1, LEAST> : wr == 2 ? k_w4_rows<NT, 2, LEAST> : wr == 4 ? k_w4_rows<NT, 4, LEAST> : k_w4_rows<NT, 8, LEAST>;
+}
+RowKernel row_kernel(int B, int wr, bool least) {
+    return B <= 8 ? (least ? row_kernel<1, true>(wr) : row_kernel<1, false>(wr)) : (least ? row_kernel<2, true>(wr) : row_kernel<2, false>(wr));
 }
 
 bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long inner, long long rows, long long row_bytes, int box_inner, int box_rows,
@@ -741,7 +772,7 @@ int prepare(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
     for (int wr = 1; wr <= ROW_WARPS; wr *= 2)
-        for (const RowKernel k : {row_kernel<false>(wr), row_kernel<true>(wr)})
+        for (const RowKernel k : {row_kernel(1, wr, false), row_kernel(1, wr, true), row_kernel(ROWS_MAX_B, wr, false), row_kernel(ROWS_MAX_B, wr, true)})
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, PANEL_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
     for (int group = 32; group <= 128; group *= 2)
         for (const TcKernel k : {tc_kernel<false>(group), tc_kernel<true>(group)})
@@ -803,7 +834,7 @@ int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, lo
     pl->grid = dim3(static_cast<unsigned>(std::min(p.tiles, slots)), 1, 1);
     pl->threads = ROW_WARPS * 32;
     pl->smem = static_cast<size_t>(B) * (p.panel * wk * 256 + 64);
-    pl->kernel = reinterpret_cast<const void *>(w.least ? row_kernel<true>(wr) : row_kernel<false>(wr));
+    pl->kernel = reinterpret_cast<const void *>(row_kernel(B, wr, w.least != nullptr));
     return GPT2_B200_OK;
 }
 
@@ -875,7 +906,7 @@ int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int
     pl->d.ldo = ldo;
     pl->d.resid = resid;
     pl->d.ldr = ldr;
-    pl->few = B <= ROWS_MAX_B;
+    pl->few = rows_do(B, w.N, w.K);
     pl->d.keys = pl->few ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * (FEATURES / 32);
     pl->d.status = ctx->status;
     pl->cluster = 1;
@@ -904,6 +935,7 @@ int launch(Plan &pl, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = na;
     pl.rows.d = pl.tc.d = pl.d;
+    pl.rows.ahead = pl.pdl;
     void *few[1] = {&pl.rows}, *many[3] = {&pl.tm_w, &pl.tm_x, &pl.tc};
     return cudaLaunchKernelExC(&cfg, pl.kernel, pl.few ? few : many) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
