@@ -12,6 +12,7 @@
 // Rows may start anywhere: a row is cut at the 16-byte boundaries of its input; the vectors at its ends are taken element by
 // element, and so are stores to an output that is aligned otherwise.
 #include <algorithm>
+#include <type_traits>
 
 #include "linear.cuh"
 #include "logits_edit.cuh"
@@ -108,6 +109,18 @@ __device__ __forceinline__ float edited(float x, uint32_t word, const Row &r) {
     return x;
 }
 
+// One more of a token in the prompt, or behind it; what its word was (1 if neither). Both under predicates: as branches they take three times
+// the instructions, and the history is looked at token by token.
+__device__ __forceinline__ uint32_t counted(uint32_t word, bool seen, bool count) {
+    uint32_t before = 1;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 p, %2, 0;\nsetp.ne.u32 q, %3, 0;\n@p atom.shared.or.b32 %0, [%1], %4;\n@q atom.shared.add.u32 %0, [%1], 1;\n}"
+        : "+r"(before)
+        : "r"(word), "r"(static_cast<uint32_t>(seen)), "r"(static_cast<uint32_t>(count)), "n"(SEEN)
+        : "memory");
+    return before;
+}
+
 // MASK, NEXT: there is a mask, a choice is asked for.
 template <typename T, bool MASK, bool NEXT>
 __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
@@ -116,7 +129,6 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
     extern __shared__ __align__(16) uint32_t words[];  // a segment's words, bits, mask and list, the bias list
     __shared__ unsigned long long best[NT / 32], row_best[MAX_CLUSTER];
     __shared__ int dups, n_touched;
-    __shared__ uint32_t gather[NT / 32][32 * AHEAD];
     const long long row = blockIdx.x / p.cluster;
     const int rank = static_cast<int>(blockIdx.x % p.cluster);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -213,45 +225,63 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
         uint32_t allowed[BATCH];
         const uint4 *src = reinterpret_cast<const uint4 *>(in - shift);
         const int place32 = (d0 - base) * VEC & 31;  // the same for all vectors of a thread
-        const auto fetch = [&](int v) {
+        const auto fetch = [&](int v, auto whole) {
             const uint32_t *mine = allow + ((v - base) * VEC >> 5);
+            const uint4 *sv = src + v;
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                if (v + j * NT >= d1) break;
+                if (!whole && v + j * NT >= d1) break;
                 if (MASK) allowed[j] = mine[j * (NT * VEC / 32)] >> place32 & ALL;
-                if (!MASK || allowed[j]) x[j] = src[v + j * NT];
+                if (!MASK || allowed[j]) x[j] = sv[j * NT];
             }
         };
-        if (dense) fetch(d0);
-        const auto dense_pass = [&](int n_edit) {
-            for (int v = d0; v < d1; v += NT * BATCH) {
-                if (v != d0) fetch(v);
+        const int last_whole = d1 - (BATCH - 1) * NT;  // a batch that starts before has no end in it
+        const auto fetch_any = [&](int v) {
+            if (!NEXT && v < last_whole)
+                fetch(v, std::true_type());
+            else
+                fetch(v, std::false_type());
+        };
+        if (dense) fetch_any(d0);
+        const bool simple = same && !p.in_place;
+        const auto finish = [&](int v, int n_edit, auto whole) {
+            uint4 *ov = reinterpret_cast<uint4 *>(out - shift) + v;
 #pragma unroll
-                for (int j = 0; j < BATCH; ++j) {
-                    const int u = v + j * NT, t = u * VEC - shift;
-                    if (u >= d1) break;
-                    if (MASK) cut(x[j], allowed[j], T());
-                    if (!p.in_place || (MASK && allowed[j] != ALL)) {
-                        if (same) {
-                            reinterpret_cast<uint4 *>(out - shift)[u] = x[j];
-                        } else {
+            for (int j = 0; j < BATCH; ++j) {
+                const int u = v + j * NT, t = u * VEC - shift;
+                if (!whole && u >= d1) break;
+                if (MASK) cut(x[j], allowed[j], T());
+                if (whole) {
+                    ov[j * NT] = x[j];
+                } else if (!p.in_place || (MASK && allowed[j] != ALL)) {
+                    if (same) {
+                        ov[j * NT] = x[j];
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) out[t + i] = reinterpret_cast<const T *>(&x[j])[i];
-                        }
+                        for (int i = 0; i < VEC; ++i) out[t + i] = reinterpret_cast<const T *>(&x[j])[i];
                     }
-                    if (NEXT && (!MASK || allowed[j]) && top_of(x[j], T()) > top) {
-                        const int w = t - t0;
-                        const uint32_t skip = n_edit ? bits[w >> 5] >> (w & 31) : 0u;
+                }
+                if (NEXT && (!MASK || allowed[j]) && top_of(x[j], T()) > top) {
+                    const int w = t - t0;
+                    const uint32_t skip = n_edit ? bits[w >> 5] >> (w & 31) : 0u;
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            const float y = to_f(reinterpret_cast<const T *>(&x[j])[i]);
-                            if (y > top && !(skip >> i & 1)) {
-                                top = y;
-                                at = t + i;
-                            }
+                    for (int i = 0; i < VEC; ++i) {
+                        const float y = to_f(reinterpret_cast<const T *>(&x[j])[i]);
+                        if (y > top && !(skip >> i & 1)) {
+                            top = y;
+                            at = t + i;
                         }
                     }
                 }
+            }
+        };
+        const auto dense_pass = [&](int n_edit) {
+            for (int v = d0; v < d1; v += NT * BATCH) {
+                if (v != d0) fetch_any(v);
+                if (!NEXT && simple && v < last_whole)
+                    finish(v, n_edit, std::true_type());
+                else
+                    finish(v, n_edit, std::false_type());
             }
             // the tokens of a row's first and last vector where those are not whole
             const int t = tid < VEC ? tid - shift : f1 * VEC - shift + tid - VEC;
@@ -266,50 +296,43 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
         // Without a choice the pass needs nothing of the history, whose loads it then covers.
         if (!NEXT && dense) dense_pass(0);
 
-        // Marks a token; the first to do so puts it on the list. The whole warp comes here.
-        const auto mark = [&](bool in_here, int w, uint32_t before) {
-            const bool first = in_here && before == 0;
-            const unsigned all = __ballot_sync(0xFFFFFFFFu, first);
-            if (!all) return;
-            int place = 0;
-            if (lane == 0) place = atomicAdd(&n_touched, __popc(all));
-            place = __shfl_sync(0xFFFFFFFFu, place, 0) + __popc(all & ((1u << lane) - 1));
-            if (first) {
-                touched[place] = static_cast<uint16_t>(w);
-                if (NEXT) atomicOr(&bits[w >> 5], 1u << (w & 31));
-            }
+        const unsigned below = (1u << lane) - 1;
+        const uint32_t word0 = smem_u32(words);
+        const auto listed = [&](int place, int w) {
+            touched[place] = static_cast<uint16_t>(w);
+            if (NEXT) atomicOr(&bits[w >> 5], 1u << (w & 31));
         };
         for (int i0 = warp * 32; i0 < r.nb; i0 += NT) {
             const int i = i0 + lane, t = i < r.nb ? btok[i] : -1;
-            const bool here = inside(t);
-            uint32_t before = 0;
-            if (here) before = atomicMax(&words[t - t0], static_cast<uint32_t>(MAX_BIAS - i) << BIAS_AT);
-            if (before) dups = 1;
-            mark(here, t - t0, before);
+            if (!inside(t)) continue;
+            if (atomicMax(&words[t - t0], static_cast<uint32_t>(MAX_BIAS - i) << BIAS_AT))
+                dups = 1;
+            else
+                listed(atomicAdd(&n_touched, 1), t - t0);
         }
         if (r.nb) __syncthreads();  // the counts go below the entries
-        // Of the history, a warp first gathers what lies in the segment: with 8 CTAs to a row that is an eighth.
-        uint32_t *gathered = gather[warp];
         for (int i0 = warp * 32; i0 < n; i0 += NT * AHEAD) {
             if (i0 != warp * 32) tokens(i0);
-            int got = 0;
+            unsigned first[AHEAD];
+            int many = 0;
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k) {
-                const bool here = inside(h[k]);
-                const unsigned all = __ballot_sync(0xFFFFFFFFu, here);
-                if (here) gathered[got + __popc(all & ((1u << lane) - 1))] = static_cast<uint32_t>(h[k] - t0) | (i0 + k * NT + lane < from ? SEEN : 0u);
-                got += __popc(all);
+                first[k] = 0;
+                if (i0 + k * NT >= n) continue;
+                const bool here = inside(h[k]), early = i0 + k * NT + lane < from;
+                const uint32_t before = counted(word0 + 4 * (h[k] - t0), here && early, here && !early);
+                first[k] = __ballot_sync(0xFFFFFFFFu, before == 0);
+                many += __popc(first[k]);
             }
-            __syncwarp();
-            for (int i = 0; i < got; i += 32) {
-                const bool here = i + lane < got;
-                const uint32_t g = here ? gathered[i + lane] : 0u;
-                const int w = static_cast<int>(g & ~SEEN);
-                uint32_t before = 0;
-                if (here) before = g & SEEN ? atomicOr(&words[w], SEEN) : atomicAdd(&words[w], 1u);
-                mark(here, w, before);
+            if (!many) continue;
+            int place = 0;
+            if (lane == 0) place = atomicAdd(&n_touched, many);
+            place = __shfl_sync(0xFFFFFFFFu, place, 0);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                if (first[k] >> lane & 1) listed(place + __popc(first[k] & below), h[k] - t0);
+                place += __popc(first[k]);
             }
-            __syncwarp();
         }
         __syncthreads();
         const int n_edit = n_touched;
