@@ -76,7 +76,7 @@ struct RowParams {
     int K, shift;  // log2 of the group
     const __half *x;
     long long ldx;
-    int tiles, steps, panel;  // tiles; steps of a warp per tile, and those whose x is held at once (a multiple of DEPTH)
+    int tiles, steps;  // tiles; steps of a warp per tile
     int ahead;                // codes are fetched before x
     Dest d;
 };

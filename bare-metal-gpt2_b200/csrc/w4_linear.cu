@@ -62,19 +62,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // ---------------------------------------------------------------- few rows
-// B <= 8, and up to 16 for small weights (rows_do): bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their use, and
-// feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA, TMEM and
-// their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
+// B <= 8 (rows_do): bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their
+// use, and feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA,
+// TMEM and their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
 //   - A step is 16 features x 128 k: lane (g, t) = (lane / 4, lane % 4) holds 32 neighbouring k, 16 bytes, of features g and g + 8.
 //     The sum over k may be taken in any order, so 4 of a lane's k serve as its share of each instruction's 16.
-//   - A CTA's 8 warps are WR rows of 16 features x WK = 8 / WR pieces of k, whose sums are added through shared memory in their order. CTAs
+//   - A CTA's W warps are WR rows of 16 features x WK = W / WR pieces of k, whose sums are added through shared memory in their order. CTAs
 //     stay and take tile after tile: x is there, and the next tile's codes are on their way while a tile's sums are put together.
+//   - One CTA per SM: each has all of x, and x costs the L2 0.3 us per MB beside the codes. (Two of 8 warps: 4096 x 4096 at B = 8 13.6 us
+//     against 9.6, 8192 x 2048 10.9 against 8.5.) L1 holds the loads in flight: less of it for more shared memory is 10% slower.
 constexpr int CHUNK = 128;
-constexpr int ROW_WARPS = 8;
 constexpr int DEPTH = 4;
-constexpr int ROW_CTAS = 2;  // per SM
-constexpr int ROWS_MAX_B = 16;
-constexpr int PANEL_BYTES = 88 * 1024;  // of x in shared memory
+constexpr int ROWS_MAX_B = 8;  // an instruction's columns
+constexpr int MAX_X = 1 << 15;      // elements of x
+constexpr int X_BYTES = 2 * (MAX_X + ROWS_MAX_B * 16 * CHUNK) + ROWS_MAX_B * 64;  // in shared memory: rows in whole steps of 16 pieces, half a line more
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
@@ -85,16 +86,16 @@ __device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 __device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
-// NT: instructions side by side, 8 rows of x each.
-template <int NT, int WR, bool LEAST>
-__global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowParams p) {
-    constexpr int WK = ROW_WARPS / WR, COLS = 8 * NT, FEATURES = 16 * WR;
-    extern __shared__ __align__(16) uint8_t xs[];  // [B][panel * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
+// W warps, WR of them side by side.
+template <int W, int WR, bool LEAST>
+__global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
+    constexpr int WK = W / WR, COLS = ROWS_MAX_B, FEATURES = 16 * WR;
+    extern __shared__ __align__(16) uint8_t xs[];  // [B][steps * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
     __shared__ float red[2][WK][FEATURES][COLS + 1];
     const Dest &d = p.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int wr = warp % WR, kg = warp / WR;
-    const int x_row = p.panel * WK * 256 + 64;  // the odd half line keeps neighbouring rows on different banks
+    const int x_row = p.steps * WK * 256 + 64;  // the odd half line keeps neighbouring rows on different banks
 
     uint4 qa[DEPTH], qb[DEPTH];
     uint32_t sa[DEPTH], sb[DEPTH], la[DEPTH], lb[DEPTH];
@@ -136,36 +137,32 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
             fetch(u, here, u);
         }
     };
-    const auto fill = [&](int first) {
-        const int k0 = first * WK * CHUNK, per = min(p.panel, p.steps - first) * WK * 16;  // pieces of 8 k per row; zeros behind the last k
-        int b = 0, i = tid;
-        while (true) {
+    const auto fill = [&] {
+        const unsigned per = p.steps * WK * 16, all = d.B * per;  // pieces of 8 k per row; zeros behind the last k
+        // Each CTA starts elsewhere: all that read the same lines in the same order meet at one part of the L2 after another.
+        const unsigned start = (blockIdx.x * 8u * 37u + tid) % all;
+        unsigned b = start / per, i = start % per;
+        for (unsigned done = tid; done < all; done += W * 32) {
+            const int k = i * 8;  // piece i & 15 = 4 t + j of its chunk goes to place 4 j + t
+            cp_async16(xs + b * x_row + (i >> 4) * 256 + ((i & 3) * 4 + (i >> 2 & 3)) * 16, p.x + b * p.ldx + min(k, p.K - 8), k < p.K);
+            i += W * 32;
             while (i >= per) {
                 i -= per;
-                ++b;
+                if (++b == d.B) b = 0;
             }
-            if (b >= d.B) break;
-            const int k = k0 + i * 8;  // piece i & 15 = 4 t + j of its chunk goes to place 4 j + t
-            cp_async16(xs + b * x_row + (i >> 4) * 256 + ((i & 3) * 4 + (i >> 2 & 3)) * 16, p.x + b * p.ldx + min(k, p.K - 8), k < p.K);
-            i += ROW_WARPS * 32;
         }
-    };
-    const auto filled = [] {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
     };
     // Behind another kernel the codes go first, since they need not wait for it. Otherwise x does: behind the codes of all CTAs, which
     // fill HBM's queues, it takes 4000 to 8000 cycles to come, without them 1500.
     if (p.ahead) fetch_first();
     grid_dependency_wait();
     grid_launch_dependents();
-    fill(0);
+    fill();
     if (!p.ahead) fetch_first();
-    filled();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     // Rows of x past the last are read as the last: the columns are dropped.
-    const uint8_t *xr[NT];
-#pragma unroll
-    for (int q = 0; q < NT; ++q) xr[q] = xs + min(8 * q + g, d.B - 1) * x_row + kg * 256 + t * 16;
+    const uint8_t *xr = xs + min(g, d.B - 1) * x_row + kg * 256 + t * 16;
 
     // The outputs of this thread: 16 lanes take 16 neighbouring features of a row of x.
     const int sub = tid >> 4, f = tid & 15, units = WR * d.B;
@@ -173,83 +170,70 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, ROW_CTAS) k_w4_rows(const RowP
         const int n0 = tile * FEATURES, next = tile + gridDim.x;
         Extra early = {0.0f, 0.0f};
         if (sub < units && n0 + sub % WR * 16 + f < d.N) early = extra_of(d, sub / WR, n0 + sub % WR * 16 + f);
-        float c[NT][4] = {};
+        float c[4] = {};
         if (next < p.tiles) then = place(next);
-        for (int first = 0; first < p.steps; first += p.panel) {
-            if (p.panel < p.steps && (first || tile != static_cast<int>(blockIdx.x))) {
-                __syncthreads();
-                fill(first);
-                filled();
+        int x_at = 0, i0 = 0;
+        const auto products = [&](int u, auto any_big) {
+            constexpr bool BIG = decltype(any_big)::value;
+            const Scale ka = scale_of<LEAST, BIG>(sa[u], la[u]), kb = scale_of<LEAST, BIG>(sb[u], lb[u]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t va[4], vb[4];
+                values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
+                values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
+                const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
+                const uint4 xv = *reinterpret_cast<const uint4 *>(xr + x_at + u * (WK * 256) + j * 64);
+                mma16816(c, a0, xv.x, xv.y);
+                mma16816(c, a1, xv.z, xv.w);
             }
-            const int end = min(p.steps, first + p.panel);
-            int x_at = 0, i0 = first;
-            const auto products = [&](int u, auto any_big) {
-                constexpr bool BIG = decltype(any_big)::value;
-                const Scale ka = scale_of<LEAST, BIG>(sa[u], la[u]), kb = scale_of<LEAST, BIG>(sb[u], lb[u]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t va[4], vb[4];
-                    values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
-                    values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
-                    const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
-#pragma unroll
-                    for (int m = 0; m < NT; ++m) {
-                        const uint4 xv = *reinterpret_cast<const uint4 *>(xr[m] + x_at + u * (WK * 256) + j * 64);
-                        mma16816(c[m], a0, xv.x, xv.y);
-                        mma16816(c[m], a1, xv.z, xv.w);
-                    }
-                }
-            };
-            const auto use = [&](int u) {
-                if (__any_sync(0xFFFFFFFFu, big_scale(max(sa[u], sb[u]))))
-                    products(u, std::true_type());
-                else
-                    products(u, std::false_type());
-            };
-            // Whole rounds whose next fetches are of this tile and all there: no checks, addresses a constant apart.
-            if (i0 + 2 * DEPTH <= full) {
-                const uint8_t *pa = here.qa + static_cast<long long>(i0 + DEPTH) * Q_STEP, *pb = here.qb + static_cast<long long>(i0 + DEPTH) * Q_STEP;
-                const uint8_t *ps = here.sa + (i0 + DEPTH) * s_step;
-                const long long other = here.sb - here.sa;
-                for (; i0 < end && i0 + 2 * DEPTH <= full; i0 += DEPTH) {
-#pragma unroll
-                    for (int u = 0; u < DEPTH; ++u) {
-                        use(u);
-                        ld_codes(qa[u], pa + u * Q_STEP);
-                        ld_codes(qb[u], pb + u * Q_STEP);
-                        ld_scale(sa[u], ps);
-                        ld_scale(sb[u], ps + other);
-                        if (LEAST) {
-                            ld_scale(la[u], ps + to_least);
-                            ld_scale(lb[u], ps + to_least + other);
-                        }
-                        ps += s_step;
-                    }
-                    pa += DEPTH * Q_STEP;
-                    pb += DEPTH * Q_STEP;
-                    x_at += DEPTH * WK * 256;
-                }
-            }
-            for (; i0 < end; i0 += DEPTH, x_at += DEPTH * WK * 256) {
+        };
+        const auto use = [&](int u) {
+            if (__any_sync(0xFFFFFFFFu, big_scale(max(sa[u], sb[u]))))
+                products(u, std::true_type());
+            else
+                products(u, std::false_type());
+        };
+        // Whole rounds whose next fetches are of this tile and all there: no checks, addresses a constant apart.
+        if (i0 + 2 * DEPTH <= full) {
+            const uint8_t *pa = here.qa + static_cast<long long>(i0 + DEPTH) * Q_STEP, *pb = here.qb + static_cast<long long>(i0 + DEPTH) * Q_STEP;
+            const uint8_t *ps = here.sa + (i0 + DEPTH) * s_step;
+            const long long other = here.sb - here.sa;
+            for (; i0 + 2 * DEPTH <= full; i0 += DEPTH) {
 #pragma unroll
                 for (int u = 0; u < DEPTH; ++u) {
-                    const int i = i0 + u;
-                    if (i >= end) break;
                     use(u);
-                    if (i + DEPTH < p.steps)
-                        fetch(u, here, i + DEPTH);
-                    else if (next < p.tiles)
-                        fetch(u, then, u);
+                    ld_codes(qa[u], pa + u * Q_STEP);
+                    ld_codes(qb[u], pb + u * Q_STEP);
+                    ld_scale(sa[u], ps);
+                    ld_scale(sb[u], ps + other);
+                    if (LEAST) {
+                        ld_scale(la[u], ps + to_least);
+                        ld_scale(lb[u], ps + to_least + other);
+                    }
+                    ps += s_step;
                 }
+                pa += DEPTH * Q_STEP;
+                pb += DEPTH * Q_STEP;
+                x_at += DEPTH * WK * 256;
+            }
+        }
+        for (; i0 < p.steps; i0 += DEPTH, x_at += DEPTH * WK * 256) {
+#pragma unroll
+            for (int u = 0; u < DEPTH; ++u) {
+                const int i = i0 + u;
+                if (i >= p.steps) break;
+                use(u);
+                if (i + DEPTH < p.steps)
+                    fetch(u, here, i + DEPTH);
+                else if (next < p.tiles)
+                    fetch(u, then, u);
             }
         }
 #pragma unroll
-        for (int q = 0; q < NT; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][8 * q + 2 * t + (i & 1)] = c[q][i];
+        for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][2 * t + (i & 1)] = c[i];
         here = then;
         __syncthreads();  // the other half of red is free: its readers came here
-        for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 16) {
+        for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 2 * W) {
             const int b = unit / WR, n = unit % WR * 16 + f;
             unsigned long long key = 0;
             const bool in = unit < units && n0 + n < d.N;
@@ -742,18 +726,19 @@ template <bool LEAST>
 TcKernel tc_kernel(int group) {
     return group == 128 ? k_w4_tc<1, LEAST> : group == 64 ? k_w4_tc<2, LEAST> : k_w4_tc<4, LEAST>;
 }
-// Which of the two. Up to 8 rows k_w4_rows. Up to 16, two MMAs per weight are cheaper than what k_w4_tc takes
-// to start, as long as the weights are few and x is held at once. Rows against tcgen05, us at B = 16: 768 x 768 4.9 against 6.5, 2304 x 768
-// 5.4 against 6.5, 4096 x 1024 6.8 against 6.9; 768 x 4 * 768 (two panels of x) 9.7 against 7.8, 4096 x 4096 14.8 against 10.0.
-bool rows_do(int B, int N, int K) { return B <= 8 || (B <= ROWS_MAX_B && K <= 2048 && static_cast<long long>(N) * K <= 1 << 22); }
+// Which of the two. k_w4_rows copies all of x into every SM and has an instruction of 8 columns, k_w4_tc takes 3 us to start and
+// then does not mind the rows. us, rows against tcgen05: 2304 x 768 4.7 against 6.4 at B = 1, 5.3 against 6.6 at 8; 50257 x 768 11.0
+// against 13.8, 13.1 against 13.9; 4096 x 4096 7.5 against 10.0, 9.6 against 10.2; 8192 x 8192 15.4 against 17.9 at B = 1, 16.8 at 4, and
+// with 96 KB of x and more 19.0 against 17.9 at 6, 21.0 at 8. Two instructions for 9 to 16 rows gained 0.9 us at 9 x 2304 x 768, lost 1.4 at
+// 9 x 50257 x 768 and were slower in a decode step.
+bool rows_do(int B, int K) { return B <= ROWS_MAX_B && B * static_cast<long long>(K) <= MAX_X; }
 
 typedef void (*RowKernel)(RowParams);
-template <int NT, bool LEAST>
-RowKernel row_kernel(int wr) {
-    return wr == 1 ? k_w4_rows<NT, 1, LEAST> : wr == 2 ? k_w4_rows<NT, 2, LEAST> : wr == 4 ? k_w4_rows<NT, 4, LEAST> : k_w4_rows<NT, 8, LEAST>;
-}
-RowKernel row_kernel(int B, int wr, bool least) {
-    return B <= 8 ? (least ? row_kernel<1, true>(wr) : row_kernel<1, false>(wr)) : (least ? row_kernel<2, true>(wr) : row_kernel<2, false>(wr));
+template <bool LEAST>
+RowKernel row_kernel(int warps, int wr) {
+    if (warps == 8) return k_w4_rows<8, 1, LEAST>;
+    return wr == 1 ? k_w4_rows<16, 1, LEAST> : wr == 2 ? k_w4_rows<16, 2, LEAST> : wr == 4 ? k_w4_rows<16, 4, LEAST>
+           : wr == 8 ? k_w4_rows<16, 8, LEAST> : k_w4_rows<16, 16, LEAST>;
 }
 
 bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long inner, long long rows, long long row_bytes, int box_inner, int box_rows,
@@ -771,9 +756,9 @@ bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long
 int prepare(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
-    for (int wr = 1; wr <= ROW_WARPS; wr *= 2)
-        for (const RowKernel k : {row_kernel(1, wr, false), row_kernel(1, wr, true), row_kernel(ROWS_MAX_B, wr, false), row_kernel(ROWS_MAX_B, wr, true)})
-            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, PANEL_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
+    for (int wr = 0; wr <= 16; wr = wr ? 2 * wr : 1)  // 0: of 8 warps
+        for (const RowKernel k : {row_kernel<false>(wr ? 16 : 8, wr), row_kernel<true>(wr ? 16 : 8, wr)})
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
     for (int group = 32; group <= 128; group *= 2)
         for (const TcKernel k : {tc_kernel<false>(group), tc_kernel<true>(group)})
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
@@ -805,7 +790,7 @@ int active_clusters(DeviceContext *ctx, int cs) {
 }
 
 int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, long long ldx) {
-    const int B = pl->d.B, chunks = (w.K + CHUNK - 1) / CHUNK, slots = ROW_CTAS * ctx->num_sms;
+    const int B = pl->d.B, chunks = (w.K + CHUNK - 1) / CHUNK, sms = ctx->num_sms;
     RowParams &p = pl->rows;
     p.codes = static_cast<const uint8_t *>(w.codes);
     p.scale = w.scale;
@@ -814,27 +799,26 @@ int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, lo
     p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.x = x;
     p.ldx = ldx;
-    // Tile height: the fewest steps of the busiest CTA, a tile's end counted as one.
+    // 8 warps where every tile of 16 features has an SM, which all take a piece of k each. Else 16, and the tile height with the fewest steps
+    // of the busiest CTA, a tile's end counted as one. us, 8 against 16 warps at B = 1: 768 x 768 3.2 against 4.0, 768 x 4 * 768 4.4 against
+    // 5.1, but 4096 x 1024 6.2 (two CTAs per SM, each with its x) against 5.2.
+    const int warps = (w.N + 15) / 16 <= sms ? 8 : 16;
     int wr = 0;
     long long best = 0;
-    for (int h = 1; h <= ROW_WARPS; h *= 2) {
-        const long long tiles = (static_cast<long long>(w.N) + 16 * h - 1) / (16 * h), rounds = (tiles + slots - 1) / slots;
-        const int wk = ROW_WARPS / h, steps = (chunks + wk - 1) / wk;
+    for (int h = 1; h <= (warps == 8 ? 1 : warps); h *= 2) {
+        const long long tiles = (static_cast<long long>(w.N) + 16 * h - 1) / (16 * h), rounds = (tiles + sms - 1) / sms;
+        const int wk = warps / h, steps = (chunks + wk - 1) / wk;
         const long long cost = rounds * (steps + 1);
-        if ((PANEL_BYTES / B - 64) / (256 * wk) < DEPTH) continue;  // x has room for a round of the buffers
-        if (!wr || cost < best) {
-            best = cost;
-            wr = h;
-            p.tiles = static_cast<int>(tiles);
-            p.steps = steps;
-        }
+        if (wr && cost >= best) continue;
+        best = cost;
+        wr = h;
+        p.tiles = static_cast<int>(tiles);
+        p.steps = steps;
     }
-    const int wk = ROW_WARPS / wr, fit = (PANEL_BYTES / B - 64) / (256 * wk);  // steps whose x fits
-    p.panel = std::min((p.steps + DEPTH - 1) / DEPTH, fit / DEPTH) * DEPTH;
-    pl->grid = dim3(static_cast<unsigned>(std::min(p.tiles, slots)), 1, 1);
-    pl->threads = ROW_WARPS * 32;
-    pl->smem = static_cast<size_t>(B) * (p.panel * wk * 256 + 64);
-    pl->kernel = reinterpret_cast<const void *>(row_kernel(B, wr, w.least != nullptr));
+    pl->grid = dim3(static_cast<unsigned>(std::min(p.tiles, sms)), 1, 1);
+    pl->threads = warps * 32;
+    pl->smem = static_cast<size_t>(B) * (p.steps * (warps / wr) * 256 + 64);
+    pl->kernel = reinterpret_cast<const void *>(w.least ? row_kernel<true>(warps, wr) : row_kernel<false>(warps, wr));
     return GPT2_B200_OK;
 }
 
@@ -906,7 +890,7 @@ int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int
     pl->d.ldo = ldo;
     pl->d.resid = resid;
     pl->d.ldr = ldr;
-    pl->few = rows_do(B, w.N, w.K);
+    pl->few = rows_do(B, w.K);
     pl->d.keys = pl->few ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * (FEATURES / 32);
     pl->d.status = ctx->status;
     pl->cluster = 1;
