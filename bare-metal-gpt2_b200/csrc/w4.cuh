@@ -104,8 +104,7 @@ struct Plan {
     size_t smem;
 };
 
-bool shape_ok(const GPT2W4 *w);   // sizes
-bool weight_ok(const GPT2W4 *w);  // and pointers
+bool weight_ok(const GPT2W4 *w);  // sizes and pointers
 // resid and ldr: EPI_RESID's. Returns a GPT2_B200_* code; d's fields of EPI_QKV and EPI_HEAD are the caller's to fill in.
 int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo, const __half *resid, long long ldr);
 int launch(Plan &pl, cudaStream_t stream);

@@ -155,11 +155,10 @@ bool matrix_ok(const __half *W, long long ldw, const GPT2W4 *w) {
 
 }  // namespace
 
-bool shape_ok(const GPT2W4 *w) {
-    return w && (w->group == 32 || w->group == 64 || w->group == 128) && w->N >= 1 && w->K >= w->group && w->K % w->group == 0 && w->K <= (1 << 24);
-}
+// N: a feature's number, rounded up to a tile, is an int.
 bool weight_ok(const GPT2W4 *w) {
-    return shape_ok(w) && w->codes && aligned(w->codes, 16) && w->scale && aligned(w->scale, 2) && aligned(w->least, 2);
+    return w && (w->group == 32 || w->group == 64 || w->group == 128) && w->N >= 1 && w->N <= (1 << 30) && w->K >= w->group && w->K % w->group == 0 &&
+           w->K <= (1 << 24) && w->codes && aligned(w->codes, 16) && w->scale && aligned(w->scale, 2) && aligned(w->least, 2);
 }
 
 }  // namespace w4

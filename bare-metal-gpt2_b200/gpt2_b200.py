@@ -527,7 +527,10 @@ class LogitsEdit:
         def table(name, t, kind, n):
             if t.dim() != 2 or t.dtype is not kind or t.shape[0] != n or t.device != self._at or (t.shape[1] > 1 and t.stride(1) != 1):
                 raise ValueError(f"LogitsEdit: {name} is {kind} with {n} rows of neighbouring values on the others' device")
-            return t.data_ptr(), (t.stride(0) if t.stride(0) >= t.shape[1] or t.stride(0) == 0 else t.shape[1]), t.shape[1]
+            stride = t.stride(0) if n > 1 else t.shape[1]
+            if 0 < stride < t.shape[1]:
+                raise ValueError(f"LogitsEdit: the rows of {name} overlap")
+            return t.data_ptr(), stride, t.shape[1]
 
         if history is not None:
             e.history, e.history_stride, e.max_history = table("history", history, i32, rows)
@@ -542,10 +545,14 @@ class LogitsEdit:
             e.bias = table("bias", bias, f32, rows)[0]
         if mask is not None:
             n = mask.shape[0]
-            e.mask, e.mask_stride, words = table("mask", mask, i32, n)
+            e.mask, stride, words = table("mask", mask, i32, n)
+            if n > 1 and stride == 0:  # the same for all rows
+                if mask_row is not None or n != rows:
+                    raise ValueError("LogitsEdit: mask_row names rows of their own")
+                n = 1
             if words < (vocab + 31) // 32 or (mask_row is None and n not in (1, rows)):
                 raise ValueError("LogitsEdit: a mask has a bit for each token, and one row, as many as the edit, or mask_row")
-            e.mask_rows, e.mask_stride = n, max(e.mask_stride, words)
+            e.mask_rows, e.mask_stride = n, stride or words
         elif mask_row is not None:
             raise ValueError("LogitsEdit: mask_row belongs to a mask")
         self.c, self.ref_c = e, ctypes.byref(e)

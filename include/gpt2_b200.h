@@ -412,7 +412,8 @@ int gpt2_b200_beam_generate(gpt2_b200_beam *bm, const int *d_prompt, long long p
  *   scale : [K/group][N], one per `group` (32, 64 or 128) neighbouring k of a row;
  *   least : [K/group][N], or NULL.
  * A code c of 0..15 stands for fp16(c * scale + least), without least for fp16((c - 8) * scale), rounded once. K is a multiple of
- * group, at most 2^24. No call allocates, synchronises or keeps anything of its arguments, so all may be captured. */
+ * group, at most 2^24, N at most 2^30; scales and leasts are finite. No call allocates, synchronises or keeps anything of its
+ * arguments, so all may be captured. */
 typedef struct {
     void *codes;
     gpt2_half *scale, *least;
@@ -429,8 +430,8 @@ int gpt2_w4_dequantize_b200(gpt2_half *W, long long ldw, const GPT2W4 *w, cudaSt
 
 /* gpt2_b200_linear with a 4-bit weight: C[b, n] = e(sum_k A[b, k] * value(n, k) + bias[n]) for b < B (1..256), sums in fp32, e and one
  * rounding to fp16 behind them: GPT2_B200_LINEAR_STORE the sum, _GELU gelu_new of it, _RESID R[b, n] + the sum (R: rows of stride
- * ldr >= N, may be C itself; not read otherwise, may be NULL). bias may be NULL. A 16-byte aligned, lda a multiple of 8, ldc >= N;
- * C must not overlap A. */
+ * ldr >= N, may be C itself with ldr = ldc; not read otherwise, may be NULL). bias may be NULL. A 16-byte aligned, lda a multiple of 8, ldc >= N;
+ * C must not overlap A, nor R but as said. */
 int gpt2_w4_linear_b200(gpt2_half *C, long long ldc, const gpt2_half *A, long long lda, const GPT2W4 *w, const gpt2_half *bias,
                         const gpt2_half *R, long long ldr, int B, int epi, cudaStream_t stream);
 

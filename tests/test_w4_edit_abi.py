@@ -14,7 +14,7 @@ def weight(**other):
     return w
 
 
-BAD = [dict(codes=None), dict(codes=4104), dict(scale=None), dict(scale=8193), dict(least=8193), dict(N=0), dict(N=-1), dict(K=0), dict(K=32), dict(K=250),
+BAD = [dict(codes=None), dict(codes=4104), dict(scale=None), dict(scale=8193), dict(least=8193), dict(N=0), dict(N=-1), dict(N=2**30 + 1), dict(K=0), dict(K=32), dict(K=250),
        dict(K=2**24 + 64), dict(group=0), dict(group=16), dict(group=48), dict(group=256), dict(group=-64)]
 
 
@@ -31,7 +31,7 @@ def test_calls_refuse_bad_arguments(lib):
     for call in (lambda W, ld: lib.gpt2_w4_quantize_b200(p, W, ld, None), lambda W, ld: lib.gpt2_w4_dequantize_b200(W, ld, p, None)):
         assert call(None, 256) == call(8, 256) == call(16, 248) == call(16, 257) == call(16, -256) == G.EINVAL
     assert lib.gpt2_w4_quantize_b200(None, 16, 256, None) == lib.gpt2_w4_dequantize_b200(16, 256, None, None) == G.EINVAL
-    big = ctypes.byref(weight(N=2**31 - 1, K=2**24))  # more tiles than a grid has
+    big = ctypes.byref(weight(N=2**30, K=2**24))  # more tiles than a grid has
     assert lib.gpt2_w4_quantize_b200(big, 16, 2**24, None) == G.EINVAL
 
     def linear(C=16, ldc=64, A=16, lda=256, w=p, bias=None, R=None, ldr=0, B=1, epi=G.LINEAR_STORE):
@@ -114,7 +114,8 @@ def test_edit_wrappers(lib, torch, monkeypatch):
     for bad in (dict(repetition=torch.ones(2)), dict(repetition=torch.ones(3, dtype=torch.float64)), dict(history=torch.zeros(3, 8)), dict(history=torch.zeros(2, 8, **i32)),
                 dict(history=torch.zeros(8, 3, **i32).t()), dict(history=None), dict(length=torch.zeros(3)), dict(bias=None), dict(bias_token=None), dict(bias=torch.zeros(3, 5)),
                 dict(bias=torch.zeros(3, 8)[:, :4]), dict(mask=torch.zeros(2, 3, **i32)), dict(mask=torch.zeros(2, 4)), dict(mask_row=None), dict(mask=None),
-                dict(n_bias=torch.zeros(4, **i32)), dict(mask_row=torch.zeros(3, dtype=torch.int64)), dict(prompt=torch.zeros(3, device="meta", **i32))):
+                dict(history=torch.zeros(20, **i32).as_strided((3, 8), (4, 1))), dict(mask=torch.zeros(1, 4, **i32).expand(2, 4)),
+                dict(mask=torch.zeros(9, **i32).as_strided((2, 4), (2, 1))), dict(n_bias=torch.zeros(4, **i32)), dict(mask_row=torch.zeros(3, dtype=torch.int64)), dict(prompt=torch.zeros(3, device="meta", **i32))):
         with pytest.raises(ValueError):
             G.LogitsEdit(lib, torch, rows, vocab, **{**good, **bad})
     e = G.LogitsEdit(lib, torch, rows, vocab, **good)
@@ -128,6 +129,15 @@ def test_edit_wrappers(lib, torch, monkeypatch):
     assert not made
     e.apply(x, x), e.apply(x.half(), x.half(), torch.zeros(3, **i32))
     assert len(made) == 2
+
+
+def test_an_edit_over_tables_that_all_rows_share(lib, torch):
+    i32 = dict(dtype=torch.int32)
+    one = torch.zeros(1, 4, **i32)
+    e = G.LogitsEdit(lib, torch, 3, 100, mask=one.expand(3, 4), history=one.expand(3, 4), bias_token=one.expand(3, 4), bias=torch.zeros(1, 4).expand(3, 4)).c
+    assert (e.mask_rows, e.mask_stride, e.history_stride, e.max_history, e.bias_stride, e.max_bias) == (1, 4, 0, 4, 0, 4)
+    e = G.LogitsEdit(lib, torch, 1, 100, mask=one, history=torch.zeros(4, 1, **i32).t()).c  # the stride of a single row says nothing
+    assert (e.mask_rows, e.mask_stride, e.history_stride, e.max_history) == (1, 4, 4, 4)
 
 
 def _weights():
