@@ -62,7 +62,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // ---------------------------------------------------------------- few rows
-// B <= 8 (rows_do): bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their
+// Few rows of x (rows_do): bound by reading and converting the weights. Warps stream codes from global memory into registers, DEPTH steps ahead of their
 // use, and feed mma.sync with them; nothing but x goes through shared memory, and nothing in the loop waits for another warp. (Through TMA,
 // TMEM and their barriers, a stage of 8 KB of codes takes longer to hand over than to read.)
 //   - A step is 16 features x 128 k: lane (g, t) = (lane / 4, lane % 4) holds 32 neighbouring k, 16 bytes, of features g and g + 8.
@@ -73,8 +73,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 //     against 9.6, 8192 x 2048 10.9 against 8.5.) L1 holds the loads in flight: less of it for more shared memory is 10% slower.
 constexpr int CHUNK = 128;
 constexpr int DEPTH = 4;
-constexpr int ROWS_MAX_B = 8;  // an instruction's columns
-constexpr int MAX_X = 1 << 15;      // elements of x
+constexpr int ROWS_MAX_B = 16;
+constexpr int MAX_X = 3 << 14;      // elements of x
 constexpr int X_BYTES = 2 * (MAX_X + ROWS_MAX_B * 16 * CHUNK) + ROWS_MAX_B * 64;  // in shared memory: rows in whole steps of 16 pieces, half a line more
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
@@ -86,10 +86,10 @@ __device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 __device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
-// W warps, WR of them side by side.
-template <int W, int WR, bool LEAST>
+// W warps, WR of them side by side; NT instructions of 8 rows each.
+template <int W, int WR, int NT, bool LEAST>
 __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
-    constexpr int WK = W / WR, COLS = ROWS_MAX_B, FEATURES = 16 * WR;
+    constexpr int WK = W / WR, COLS = 8 * NT, FEATURES = 16 * WR;
     extern __shared__ __align__(16) uint8_t xs[];  // [B][steps * WK * 256 + 64]: x, 16-byte pieces ordered for the loop
     __shared__ float red[2][WK][FEATURES][COLS + 1];
     const Dest &d = p.d;
@@ -162,7 +162,9 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     // Rows of x past the last are read as the last: the columns are dropped.
-    const uint8_t *xr = xs + min(g, d.B - 1) * x_row + kg * 256 + t * 16;
+    const uint8_t *xr[NT];
+#pragma unroll
+    for (int q = 0; q < NT; ++q) xr[q] = xs + min(8 * q + g, d.B - 1) * x_row + kg * 256 + t * 16;
 
     // The outputs of this thread: 16 lanes take 16 neighbouring features of a row of x.
     const int sub = tid >> 4, f = tid & 15, units = WR * d.B;
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
         const int n0 = tile * FEATURES, next = tile + gridDim.x;
         Extra early = {0.0f, 0.0f};
         if (sub < units && n0 + sub % WR * 16 + f < d.N) early = extra_of(d, sub / WR, n0 + sub % WR * 16 + f);
-        float c[4] = {};
+        float c[NT][4] = {};
         if (next < p.tiles) then = place(next);
         int x_at = 0, i0 = 0;
         const auto products = [&](int u, auto any_big) {
@@ -182,9 +184,12 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
                 values_of<LEAST, BIG>((&qa[u].x)[j], ka, va);
                 values_of<LEAST, BIG>((&qb[u].x)[j], kb, vb);
                 const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
-                const uint4 xv = *reinterpret_cast<const uint4 *>(xr + x_at + u * (WK * 256) + j * 64);
-                mma16816(c, a0, xv.x, xv.y);
-                mma16816(c, a1, xv.z, xv.w);
+#pragma unroll
+                for (int q = 0; q < NT; ++q) {
+                    const uint4 xv = *reinterpret_cast<const uint4 *>(xr[q] + x_at + u * (WK * 256) + j * 64);
+                    mma16816(c[q], a0, xv.x, xv.y);
+                    mma16816(c[q], a1, xv.z, xv.w);
+                }
             }
         };
         const auto use = [&](int u) {
@@ -230,7 +235,9 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][2 * t + (i & 1)] = c[i];
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[turn][kg][wr * 16 + g + 8 * (i >> 1)][8 * q + 2 * t + (i & 1)] = c[q][i];
         here = then;
         __syncthreads();  // the other half of red is free: its readers came here
         for (int unit = sub; unit < (units + 1) / 2 * 2; unit += 2 * W) {
@@ -726,19 +733,26 @@ template <bool LEAST>
 TcKernel tc_kernel(int group) {
     return group == 128 ? k_w4_tc<1, LEAST> : group == 64 ? k_w4_tc<2, LEAST> : k_w4_tc<4, LEAST>;
 }
-// Which of the two. k_w4_rows copies all of x into every SM and has an instruction of 8 columns, k_w4_tc takes 3 us to start and
-// then does not mind the rows. us, rows against tcgen05: 2304 x 768 4.7 against 6.4 at B = 1, 5.3 against 6.6 at 8; 50257 x 768 11.0
-// against 13.8, 13.1 against 13.9; 4096 x 4096 7.5 against 10.0, 9.6 against 10.2; 8192 x 8192 15.4 against 17.9 at B = 1, 16.8 at 4, and
-// with 96 KB of x and more 19.0 against 17.9 at 6, 21.0 at 8. Two instructions for 9 to 16 rows gained 0.9 us at 9 x 2304 x 768, lost 1.4 at
-// 9 x 50257 x 768 and were slower in a decode step.
-bool rows_do(int B, int K) { return B <= ROWS_MAX_B && B * static_cast<long long>(K) <= MAX_X; }
+// Which of the two. k_w4_rows copies all of x into every SM and has instructions of 8 columns, k_w4_tc takes 3 us to start and
+// then does not mind the rows. us, rows against tcgen05: 2304 x 768 4.7 against 6.4 at B = 1, 5.3 against 6.6 at 8, 6.1 against 6.6 at 16;
+// 768 x 4 * 768 7.7 against 7.7 at 16; 4096 x 1024 6.7 against 7.1 at 16; 50257 x 768 11.0 against 13.8 at 1, 13.0 against 13.9 at 8, but 15.0
+// against 13.8 at 9; 8192 x 2048 9.5 against 9.2 at 9; 4096 x 4096 7.5 against 10.0 at 1, 9.6 against 10.2 at 8; 8192 x 8192 15.4 against
+// 17.9 at 1, 16.8 at 4, and with 96 KB of x and more 19.0 against 17.9 at 6. A decode step of 9 sequences 300 against 377, of 16 370 against 387.
+bool rows_do(int B, int N, int K) {
+    const long long x = static_cast<long long>(B) * K, weight = static_cast<long long>(N) * K;
+    return (B <= 8 && x <= 1 << 15) || (B <= ROWS_MAX_B && x <= MAX_X && weight <= 1 << 22);
+}
 
 typedef void (*RowKernel)(RowParams);
-template <bool LEAST>
+template <int NT, bool LEAST>
 RowKernel row_kernel(int warps, int wr) {
-    if (warps == 8) return k_w4_rows<8, 1, LEAST>;
-    return wr == 1 ? k_w4_rows<16, 1, LEAST> : wr == 2 ? k_w4_rows<16, 2, LEAST> : wr == 4 ? k_w4_rows<16, 4, LEAST>
-           : wr == 8 ? k_w4_rows<16, 8, LEAST> : k_w4_rows<16, 16, LEAST>;
+    if (warps == 8) return k_w4_rows<8, 1, NT, LEAST>;
+    return wr == 1 ? k_w4_rows<16, 1, NT, LEAST> : wr == 2 ? k_w4_rows<16, 2, NT, LEAST> : wr == 4 ? k_w4_rows<16, 4, NT, LEAST>
+           : wr == 8 ? k_w4_rows<16, 8, NT, LEAST> : k_w4_rows<16, 16, NT, LEAST>;
+}
+RowKernel row_kernel(int B, bool least, int warps, int wr) {
+    return B <= 8 ? (least ? row_kernel<1, true>(warps, wr) : row_kernel<1, false>(warps, wr))
+                  : (least ? row_kernel<2, true>(warps, wr) : row_kernel<2, false>(warps, wr));
 }
 
 bool encode(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, long long inner, long long rows, long long row_bytes, int box_inner, int box_rows,
@@ -757,8 +771,8 @@ int prepare(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
     for (int wr = 0; wr <= 16; wr = wr ? 2 * wr : 1)  // 0: of 8 warps
-        for (const RowKernel k : {row_kernel<false>(wr ? 16 : 8, wr), row_kernel<true>(wr ? 16 : 8, wr)})
-            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
+        for (int i = 0; i < 4; ++i)
+            if (cudaFuncSetAttribute(row_kernel(i & 1 ? 1 : ROWS_MAX_B, i & 2, wr ? 16 : 8, wr), cudaFuncAttributeMaxDynamicSharedMemorySize, X_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
     for (int group = 32; group <= 128; group *= 2)
         for (const TcKernel k : {tc_kernel<false>(group), tc_kernel<true>(group)})
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
@@ -818,7 +832,7 @@ int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, lo
     pl->grid = dim3(static_cast<unsigned>(std::min(p.tiles, sms)), 1, 1);
     pl->threads = warps * 32;
     pl->smem = static_cast<size_t>(B) * (p.steps * (warps / wr) * 256 + 64);
-    pl->kernel = reinterpret_cast<const void *>(w.least ? row_kernel<true>(warps, wr) : row_kernel<false>(warps, wr));
+    pl->kernel = reinterpret_cast<const void *>(row_kernel(B, w.least != nullptr, warps, wr));
     return GPT2_B200_OK;
 }
 
@@ -890,7 +904,7 @@ int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int
     pl->d.ldo = ldo;
     pl->d.resid = resid;
     pl->d.ldr = ldr;
-    pl->few = rows_do(B, w.K);
+    pl->few = rows_do(B, w.N, w.K);
     pl->d.keys = pl->few ? (w.N + 15) / 16 : (w.N + FEATURES - 1) / FEATURES * (FEATURES / 32);
     pl->d.status = ctx->status;
     pl->cluster = 1;

@@ -136,7 +136,8 @@ def test_quantise_values_that_are_not_finite_and_the_types_ends(lib, cuda, least
 LINEAR = [(1, 1, 32, 32), (1, 768, 768, 64), (2, 5, 64, 64), (3, 130, 96, 32), (5, 300, 1024, 128), (8, 2304, 768, 64), (9, 17, 4096, 128),
           (15, 999, 224, 32), (16, 256, 2048, 64), (17, 128, 160, 32), (31, 640, 1152, 128), (33, 700, 96, 32), (64, 2304, 768, 64), (65, 129, 320, 64),
           (100, 1111, 416, 32), (128, 768, 768, 64), (129, 260, 2080, 32), (200, 77, 32, 32), (256, 520, 1024, 128), (256, 1, 64, 64),
-          (12, 4100, 1056, 32), (13, 2048, 2048, 128), (16, 2049, 2048, 64), (16, 100, 2080, 32), (16, 2304, 768, 64), (11, 9001, 96, 32)]
+          (12, 4100, 1056, 32), (13, 2048, 2048, 128), (16, 2049, 2048, 64), (16, 100, 2080, 32), (16, 2304, 768, 64), (11, 9001, 96, 32),
+          (13, 1100, 3776, 64), (10, 70, 4896, 32)]
 
 
 @pytest.mark.parametrize("epi", ["store", "gelu", "resid"])
