@@ -5,7 +5,8 @@
 // extremes of a group among its 4, 8 or 16 lanes, and writes one word of codes per lane. At HBM's rate a warp has about 28 cycles
 // of an SM for its 256 weights, so instructions count: extremes are found in packed fp16 (exact), the divisions of 4 rows are
 // done once, in different lanes, and a product becomes a whole number by adding 1.5 * 2^23 to it. Scales are laid out by row, so they are
-// collected in shared memory and leave as runs of 32 rows.
+// collected in shared memory and leave as runs of 32 rows. 8192 x 8192 with least, both ways: 68 us, 5.0 TB/s (floor 52); quantising issues at
+// 85% of the slots.
 #include "w4.cuh"
 
 namespace b200 {
