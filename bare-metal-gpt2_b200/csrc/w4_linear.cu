@@ -751,8 +751,8 @@ typedef void (*RowKernel)(RowParams);
 template <int NT, bool LEAST>
 RowKernel row_kernel(int warps, int wr) {
     if (warps == 8) return k_w4_rows<8, 1, NT, LEAST>;
-    return wr == 1 ? k_w4_rows<16, 1, NT, LEAST> : wr == 2 ? k_w4_rows<16, 2, NT, LEAST> : wr == 4 ? k_w4_rows<16, 4, NT, LEAST>
-           : wr == 8 ? k_w4_rows<16, 8, NT, LEAST> : k_w4_rows<16, 16, NT, LEAST>;
+    if (NT == 1 && wr == 1) return k_w4_rows<16, 1, 1, LEAST>;
+    return wr == 2 ? k_w4_rows<16, 2, NT, LEAST> : wr == 4 ? k_w4_rows<16, 4, NT, LEAST> : wr == 8 ? k_w4_rows<16, 8, NT, LEAST> : k_w4_rows<16, 16, NT, LEAST>;
 }
 RowKernel row_kernel(int B, bool least, int warps, int wr) {
     return B <= 8 ? (least ? row_kernel<1, true>(warps, wr) : row_kernel<1, false>(warps, wr))
@@ -775,8 +775,10 @@ int prepare(DeviceContext *ctx) {
     if (ctx->w4_attr_done) return GPT2_B200_OK;
     RelaxedCapture relaxed;
     for (int wr = 0; wr <= 16; wr = wr ? 2 * wr : 1)  // 0: of 8 warps
-        for (int i = 0; i < 4; ++i)
-            if (cudaFuncSetAttribute(row_kernel(i & 1 ? 1 : ROWS_MAX_B, i & 2, wr ? 16 : 8, wr), cudaFuncAttributeMaxDynamicSharedMemorySize, X_BYTES) != cudaSuccess) return GPT2_B200_ECUDA;
+        for (int i = wr == 1 ? 1 : 0; i < 4; i += wr == 1 ? 2 : 1)
+            if (cudaFuncSetAttribute(row_kernel(i & 1 ? 1 : ROWS_MAX_B, i & 2, wr ? 16 : 8, wr), cudaFuncAttributeMaxDynamicSharedMemorySize, X_BYTES) !=
+                cudaSuccess)
+                return GPT2_B200_ECUDA;
     for (int group = 32; group <= 128; group *= 2)
         for (const TcKernel k : {tc_kernel<false>(group), tc_kernel<true>(group)})
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TC_SMEM)) != cudaSuccess) return GPT2_B200_ECUDA;
@@ -823,7 +825,8 @@ int plan_rows(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, lo
     const int warps = (w.N + 15) / 16 <= sms ? 8 : 16;
     int wr = 0;
     long long best = 0;
-    for (int h = 1; h <= (warps == 8 ? 1 : warps); h *= 2) {
+    // (More than 8 rows of weights that small never have so many k that 16 warps would share them.)
+    for (int h = warps == 16 && B > 8 ? 2 : 1; h <= (warps == 8 ? 1 : warps); h *= 2) {
         const long long tiles = (static_cast<long long>(w.N) + 16 * h - 1) / (16 * h), rounds = (tiles + sms - 1) / sms;
         const int wk = warps / h, steps = (chunks + wk - 1) / wk;
         const long long cost = rounds * (steps + 1);

@@ -137,7 +137,10 @@ LINEAR = [(1, 1, 32, 32), (1, 768, 768, 64), (2, 5, 64, 64), (3, 130, 96, 32), (
           (15, 999, 224, 32), (16, 256, 2048, 64), (17, 128, 160, 32), (31, 640, 1152, 128), (33, 700, 96, 32), (64, 2304, 768, 64), (65, 129, 320, 64),
           (100, 1111, 416, 32), (128, 768, 768, 64), (129, 260, 2080, 32), (200, 77, 32, 32), (256, 520, 1024, 128), (256, 1, 64, 64),
           (12, 4100, 1056, 32), (13, 2048, 2048, 128), (16, 2049, 2048, 64), (16, 100, 2080, 32), (16, 2304, 768, 64), (11, 9001, 96, 32),
-          (13, 1100, 3776, 64), (10, 70, 4896, 32)]
+          (13, 1100, 3776, 64), (10, 70, 4896, 32),
+          # few rows of many features: every tile height, one and several tiles per CTA, whole rounds of the buffers and their ends
+          (1, 7104, 6144, 128), (2, 4700, 1248, 32), (4, 2400, 8192, 64), (8, 9472, 1024, 64), (3, 16380, 352, 32), (5, 14000, 128, 64), (7, 40001, 192, 64),
+          (1, 60000, 64, 32), (6, 2369, 5152, 32), (10, 4000, 1024, 128), (16, 2400, 1696, 32), (12, 16000, 256, 64), (9, 50000, 64, 32), (14, 30000, 128, 32)]
 
 
 @pytest.mark.parametrize("epi", ["store", "gelu", "resid"])
@@ -168,6 +171,30 @@ def test_linear(lib, cuda, B, N, K, group, epi):
     if epi == "resid":
         want, magnitude = want + c0.astype(np.float64), magnitude + np.abs(c0.astype(np.float64))
     close(got[:, :N], want, magnitude, K, epi == "gelu")
+    assert lib.status() == 0
+
+
+@pytest.mark.parametrize("B,N,K,group", [(1, 7104, 16384, 128), (4, 40000, 2048, 32), (8, 50257, 768, 64), (2, 20001, 4096, 64), (15, 50257, 768, 64),
+                                         (64, 9000, 8192, 128), (250, 20000, 2080, 32)])
+def test_linear_of_many_tiles(lib, cuda, B, N, K, group):
+    """Large weights, several tiles per CTA, against the values that dequantize gives (compared bit by bit above) in 64 bits."""
+    torch = cuda
+    g = torch.Generator(device="cuda")
+    g.manual_seed(N + B)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scale = (0.01 * torch.exp(0.5 * torch.randn(K // group, N, generator=g, device="cuda"))).half()
+    least = (-7.5 * scale.float() * (1 + 0.2 * torch.randn(K // group, N, generator=g, device="cuda"))).half() if B % 2 == 0 else None
+    w = G.W4Weight(lib, torch, codes, scale, least)
+    v = torch.empty(N, K, dtype=torch.float16, device="cuda")
+    w.dequantize(v)
+    x = torch.randn(B, K, generator=g, device="cuda", dtype=torch.float16)
+    out = torch.full((B, N), float("nan"), dtype=torch.float16, device="cuda")
+    w.linear(out, x)
+    want, magnitude = torch.empty(B, N, dtype=torch.float64, device="cuda"), torch.empty(B, N, dtype=torch.float64, device="cuda")
+    for n in range(0, N, 4096):
+        part = v[n:n + 4096].double().t()
+        want[:, n:n + 4096], magnitude[:, n:n + 4096] = x.double() @ part, x.double().abs() @ part.abs()
+    close(out.cpu().numpy(), want.cpu().numpy(), magnitude.cpu().numpy(), K)
     assert lib.status() == 0
 
 
