@@ -96,7 +96,8 @@ def handle(lib, torch, p, device="cuda"):
 
 
 CASES = [(1, 1, 1, 0, None), (1, 9, 3, 2, 1), (2, 33, 40, 5, 2), (3, 100, 0, 7, None), (5, 1000, 100, 0, 3), (1, 50257, 300, 0, None), (1, 50257, 1000, 1024, 1),
-         (64, 50257, 1023, 16, 8), (7, 20001, 5000, 300, 4), (2, 262145, 700, 33, 2), (300, 511, 64, 3, 300), (700, 4097, 20, 1, 5), (600, 40001, 3, 2, None)]
+         (64, 50257, 1023, 16, 8), (7, 20001, 5000, 300, 4), (2, 262145, 700, 33, 2), (300, 511, 64, 3, 300), (700, 4097, 20, 1, 5), (600, 40001, 3, 2, None),
+         (2, 262145, 9000, 33, 2), (3, 50, 6000, 1024, 1), (2, 1000, 20000, 3, 2), (150, 70001, 4097, 1, None)]
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
