@@ -284,3 +284,28 @@ def test_two_streams_at_once(lib, cuda):
     for _, v, x, out, _ in jobs:
         x64 = x.cpu().numpy().astype(np.float64)
         close(out.cpu().numpy(), x64 @ v.T, np.abs(x64) @ np.abs(v).T, 1024)
+
+
+@pytest.mark.parametrize("B", [12, 64, 200])
+def test_beside_the_fp16_products(lib, cuda, B):
+    """Both kinds of products hold tensor memory: on two streams at once each gives the bits that it gives alone."""
+    torch = cuda
+    d, _ = make(torch, 2304, 768, 64, False, B)
+    w = G.W4Weight(lib, torch, *d)
+    v = torch.empty(2304, 768, dtype=torch.float16, device="cuda")
+    w.dequantize(v)
+    x = torch.randn(B, 768, device="cuda", dtype=torch.float16)
+    out = torch.empty(2, 2, B, 2304, device="cuda", dtype=torch.float16)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def both(o, first, second, times):
+        for _ in range(times):
+            w.linear(o[0], x, stream=first)
+            lib.check(lib.gpt2_b200_linear(o[1].data_ptr(), 2304, x.data_ptr(), 768, v.data_ptr(), None, B, 2304, 768, G.LINEAR_STORE, second), "linear")
+        torch.cuda.synchronize()
+
+    both(out[0], one.cuda_stream, one.cuda_stream, 1)
+    both(out[1], one.cuda_stream, two.cuda_stream, 30)
+    assert torch.equal(out[0], out[1])
+    assert lib.status() == 0
