@@ -458,8 +458,17 @@ class W4Weight:
 
     @classmethod
     def pack(cls, lib: "Lib", torch, w, group: int = 64, least: bool = False, stream: int = 0) -> "W4Weight":
-        """The fp16 weight w [N][K] in 4 bits."""
+        """The fp16 weight w [N][K] in 4 bits. `stream` first waits for torch's current stream, on which w was made and the weight's
+        memory comes from the allocator."""
         q = cls.create(lib, torch, w.shape[0], w.shape[1], group, least, w.device)
+        if w.device.type == "cuda":
+            current = torch.cuda.current_stream(w.device)
+            if stream != current.cuda_stream:
+                st = torch.cuda.ExternalStream(stream, w.device) if stream else torch.cuda.default_stream(w.device)
+                st.wait_stream(current)
+                for t in (w, q.codes, q.scale, q.least):
+                    if t is not None:
+                        t.record_stream(st)
         q.quantize(w, stream)
         return q
 
