@@ -476,7 +476,7 @@ class W4Weight:
         if w.dtype != self._half or w.dim() != 2 or w.shape != (self.N, self.K) or w.stride(1) != 1 or w.device != self._at:
             raise ValueError(f"{what}: expected fp16 [{self.N}][{self.K}] on the weight's device")
         self._current(what)
-        return w.data_ptr(), w.stride(0) if self.N > 1 else max(w.stride(0), self.K)
+        return w.data_ptr(), w.stride(0) if self.N > 1 else self.K
 
     def quantize(self, w, stream: int = 0) -> None:
         """Writes the codes, scales and least values of the fp16 weight w [N][K]."""
@@ -493,14 +493,14 @@ class W4Weight:
         (None: what out holds)."""
         shape, os_, xs, half, at = out.shape, out.stride(), x.stride(), self._half, self._at
         B = shape[0] if len(shape) == 2 else 0
-        if B < 1 or shape[1] != self.N or x.shape != (B, self.K) or xs[1] != 1 or os_[1] != 1 or x.dtype is not half or \
+        if B < 1 or shape[1] != self.N or x.shape != (B, self.K) or xs[1] != 1 or (os_[1] != 1 and self.N > 1) or x.dtype is not half or \
                 out.dtype is not half or x.device != at or out.device != at:
             raise ValueError("linear: out is fp16 [B][N] and x fp16 [B][K] on the weight's device")
         rp, rs = None, 0
         if epi == LINEAR_RESID:
             r = out if residual is None else residual
             rs = r.stride()
-            if r.shape != shape or rs[1] != 1 or r.dtype is not half or r.device != at:
+            if r.shape != shape or (rs[1] != 1 and self.N > 1) or r.dtype is not half or r.device != at:
                 raise ValueError("linear: residual is fp16 [B][N] on the weight's device")
             rp, rs = r.data_ptr(), rs[0] if B > 1 else self.N
         self._current("linear")
