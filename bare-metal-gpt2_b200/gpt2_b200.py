@@ -696,12 +696,12 @@ class DecodeBatch:
             if out.shape[1] <= n_steps or (edit.device is not None and edit.device != at):
                 raise ValueError("generate: out is too narrow, or the edit is on another device")
             self.lib.check(self.lib.gpt2_b200_batch_generate_edited(
-                self.h, prompt.data_ptr(), prompt.stride(0), _vector("generate", prompt_len, i32, self.B, at), n_steps, out.data_ptr(), out.stride(0),
-                edit.ref_c, stream), "gpt2_b200_batch_generate_edited")
+                self.h, prompt.data_ptr(), _row_stride(prompt), _vector("generate", prompt_len, i32, self.B, at), n_steps, out.data_ptr(),
+                _row_stride(out), edit.ref_c, stream), "gpt2_b200_batch_generate_edited")
             return
         self.lib.check(self.lib.gpt2_b200_batch_generate(
-            self.h, prompt.data_ptr(), prompt.stride(0), prompt_len.data_ptr(), n_steps,
-            out.data_ptr(), out.stride(0), 0, stream), "gpt2_b200_batch_generate")
+            self.h, prompt.data_ptr(), _row_stride(prompt), prompt_len.data_ptr(), n_steps,
+            out.data_ptr(), _row_stride(out), 0, stream), "gpt2_b200_batch_generate")
 
     def close(self) -> None:
         """Destroys the batch (the library synchronises the device first); safe to call twice."""
@@ -733,11 +733,11 @@ class BeamDecoder:
         for t, n in ((prompt, self.B), (out, rows)):
             if t.dim() != 2 or t.dtype is not i32 or t.shape[0] != n or t.shape[1] < 1 or t.stride(1) != 1 or t.device != at:
                 raise ValueError("generate: prompt is int32 [B][P], out int32 [B * W][>= n_steps + 1], on the cache's device")
-        if out.shape[1] <= n_steps < out.stride(0):  # a view whose rows end early: the library sees the stride alone
+        if out.shape[1] <= n_steps < _row_stride(out):  # a view whose rows end early: the library sees the stride alone
             raise ValueError("generate: out is too narrow")
         self.lib.check(self.lib.gpt2_b200_beam_generate(
-            self.h, prompt.data_ptr(), prompt.stride(0), _vector(what, prompt_len, i32, self.B, at), n_steps, eos, out.data_ptr(),
-            out.stride(0), _vector(what, score, f32, rows, at) if score is not None else None, stream), "gpt2_b200_beam_generate")
+            self.h, prompt.data_ptr(), _row_stride(prompt), _vector(what, prompt_len, i32, self.B, at), n_steps, eos, out.data_ptr(),
+            _row_stride(out), _vector(what, score, f32, rows, at) if score is not None else None, stream), "gpt2_b200_beam_generate")
 
     def close(self) -> None:
         """Destroys the decoder (the library synchronises the device first); safe to call twice."""
@@ -762,6 +762,11 @@ def _current(torch, device):
         if get() != index:
             raise ValueError(f"{what}: the tensors are on {device}, the current device is cuda:{get()}")
     return check
+
+
+def _row_stride(t) -> int:
+    """The elements from a matrix's row to the next; of a single row its width, since its stride may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _vector(what, t, dtype, n, device):
