@@ -765,8 +765,8 @@ def _current(torch, device):
 
 
 def _row_stride(t) -> int:
-    """The elements from a matrix's row to the next; of a single row its width, since its stride may be anything."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """The elements from a matrix's row to the next; of a single row, whose stride may be anything, its width at least."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[-1])
 
 
 def _vector(what, t, dtype, n, device):
