@@ -445,7 +445,7 @@ class W4Weight:
         c.N, c.K, c.group = N, K, group
         self.c, self.ref_c = c, ctypes.byref(c)
         self._at, self._half, self._current = codes.device, torch.float16, _current(torch, codes.device)
-        self._linear = lib.lib.gpt2_w4_linear_b200
+        self._linear = _entry(lib.lib.gpt2_w4_linear_b200, codes.device)
 
     @classmethod
     def create(cls, lib: "Lib", torch, N: int, K: int, group: int = 64, least: bool = False, device="cuda") -> "W4Weight":
@@ -475,6 +475,7 @@ class W4Weight:
     def _matrix(self, what, w):
         if w.dtype != self._half or w.dim() != 2 or w.shape != (self.N, self.K) or w.stride(1) != 1 or w.device != self._at:
             raise ValueError(f"{what}: expected fp16 [{self.N}][{self.K}] on the weight's device")
+        _on_gpu(what, self._at)
         self._current(what)
         return w.data_ptr(), w.stride(0) if self.N > 1 else self.K
 
@@ -565,8 +566,8 @@ class LogitsEdit:
         elif mask_row is not None:
             raise ValueError("LogitsEdit: mask_row belongs to a mask")
         self.c, self.ref_c = e, ctypes.byref(e)
-        self._current = _current(torch, self._at) if some else None
-        self._edit = lib.lib.gpt2_logits_edit_b200
+        self._torch, self._current = torch, _current(torch, self._at) if some else None
+        self._edit = _entry(lib.lib.gpt2_logits_edit_b200, self._at)
 
     def apply(self, out, logits, next_tokens=None, stream: int = 0) -> None:
         """out [rows][vocab] = the edited logits (fp16 or fp32 rows, strided ones are fine; out may be logits); next_tokens int32
@@ -578,6 +579,9 @@ class LogitsEdit:
             raise ValueError("apply: logits and out are fp16 or fp32 [rows][vocab] of one type, on the edit's device")
         if self._current is not None:
             self._current("apply")
+        else:  # no tensors of its own: the logits say where
+            _on_gpu("apply", at)
+            _current(self._torch, at)("apply")
         rc = self._edit(out.data_ptr(), os_[0] if rows > 1 else vocab, logits.data_ptr(), ls[0] if rows > 1 else vocab, kind, rows, vocab, self.ref_c,
                         _vector("apply", next_tokens, _types()[0], rows, at) if next_tokens is not None else None, stream)
         if rc:
@@ -762,6 +766,18 @@ def _current(torch, device):
         if get() != index:
             raise ValueError(f"{what}: the tensors are on {device}, the current device is cuda:{get()}")
     return check
+
+
+def _on_gpu(what, device) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"{what}: the tensors are on {device}, the library takes those of a GPU")
+
+
+def _entry(call, device):
+    """The library's call; where the tensors are not on a GPU, one that refuses their addresses. device None: not known yet."""
+    if device is None or device.type == "cuda":
+        return call
+    return lambda *a: _on_gpu(call.__name__, device)
 
 
 def _row_stride(t) -> int:
