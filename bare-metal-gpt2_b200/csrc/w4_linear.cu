@@ -88,6 +88,10 @@ __device__ __forceinline__ void ld_codes(uint4 &v, const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 __device__ __forceinline__ void ld_scale(uint32_t &v, const uint8_t *p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); }
+// The same, or 0.
+__device__ __forceinline__ void ld_scale_if(uint32_t &v, const uint8_t *p, bool in) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\nmov.u32 %0, 0;\n@p ld.global.nc.u16 %0, [%1];\n}" : "=&r"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
+}
 // W warps, WR of them side by side; NT instructions of 8 rows each.
 template <int W, int WR, int NT, bool LEAST>
 __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
@@ -102,13 +106,13 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
     uint4 qa[DEPTH], qb[DEPTH];
     uint32_t sa[DEPTH], sb[DEPTH], la[DEPTH], lb[DEPTH];
     // A lane's place in a tile: its first codes and scales of feature g, and the way to those of the other feature. Nothing outside is
-    // read: features past the last are read as the last and dropped, steps past the last k as the lane's last one and multiplied
-    // by zeros.
+    // read: features past the last are read as the last and dropped, steps past the last k as the lane's last one (or k = 0) under scales
+    // of 0, since x is 0 there and a value may be infinite.
     struct Place {
         const uint8_t *qa, *qb, *sa, *sb;
     };
     const int k_lane = kg * CHUNK + 32 * t;
-    const int k_first = k_lane < p.K ? k_lane : 0, last = k_lane < p.K ? (p.K - 1 - k_lane) / (CHUNK * WK) : 0;
+    const int k_first = k_lane < p.K ? k_lane : 0, last = k_lane < p.K ? (p.K - 1 - k_lane) / (CHUNK * WK) : -1;
     const auto place = [&](int tile) {
         const int n = min(tile * FEATURES + wr * 16 + g, d.N - 1), m = min(tile * FEATURES + wr * 16 + g + 8, d.N - 1);
         const uint8_t *s = reinterpret_cast<const uint8_t *>(p.scale + static_cast<long long>(k_first >> p.shift) * d.N);
@@ -118,15 +122,16 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
     const long long s_step = ((CHUNK * WK) >> p.shift) * 2ll * d.N;
     const long long to_least = (p.least - p.scale) * 2;
     const auto fetch = [&](int u, const Place &at, int step) {
-        step = min(step, last);
+        const bool in = step <= last;
+        step = in ? step : max(last, 0);
         const long long s = step * s_step;
         ld_codes(qa[u], at.qa + static_cast<long long>(step) * Q_STEP);
         ld_codes(qb[u], at.qb + static_cast<long long>(step) * Q_STEP);
-        ld_scale(sa[u], at.sa + s);
-        ld_scale(sb[u], at.sb + s);
+        ld_scale_if(sa[u], at.sa + s, in);
+        ld_scale_if(sb[u], at.sb + s, in);
         if (LEAST) {
-            ld_scale(la[u], at.sa + s + to_least);
-            ld_scale(lb[u], at.sb + s + to_least);
+            ld_scale_if(la[u], at.sa + s + to_least, in);
+            ld_scale_if(lb[u], at.sb + s + to_least, in);
         }
     };
     const int full = p.K / (CHUNK * WK);  // steps that are whole for every lane
