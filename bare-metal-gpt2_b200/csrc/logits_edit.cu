@@ -47,7 +47,7 @@ struct Params {
     int V, cluster;
     int seg;      // tokens per segment
     int list;     // touched tokens of a segment at most
-    int len_add;  // added to every length (the decoder's positions)
+    int len_add;  // added to every length; not 0: the decoder's positions, of which those within a prompt are left alone
     int in_place;
     GPT2LogitsEdit e;
     int *next;
@@ -158,6 +158,10 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
         n = e.length ? e.length[row] + p.len_add : e.max_history;
         if (e.prompt) from = e.prompt[row];
     }
+    if (NEXT && p.len_add && n < from) {  // the decoder within a prompt: its next token is there, nothing is chosen or reported
+        if (p.cluster > 1) cluster_wait();
+        return;
+    }
     Row r;
     r.rep = e.repetition ? e.repetition[row] : 1.0f;
     r.freq = e.frequency ? e.frequency[row] : 0.0f;
@@ -182,7 +186,7 @@ __global__ void __launch_bounds__(NT, 2) k_logits_edit(const Params p) {
     // The dense pass has something to do unless the logits stay in place and nothing asks for the mask or the largest.
     const bool dense = MASK || NEXT || !p.in_place;
     n = clamped(n, 0, hist ? e.max_history : 0, tell, p.status);
-    from = p.len_add ? min(max(from, 0), n) : clamped(from, 0, n, tell, p.status);  // the decoder edits within the prompt too
+    from = p.len_add ? min(max(from, 0), n) : clamped(from, 0, n, tell, p.status);
     r.nb = clamped(r.nb, 0, e.max_bias, tell, p.status);
     int h[AHEAD];
     const auto tokens = [&](int i0) {

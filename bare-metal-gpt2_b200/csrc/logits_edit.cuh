@@ -9,7 +9,8 @@ namespace edit {
 int check(const GPT2LogitsEdit *e, int rows, int V);
 // Kernel attributes on the current device (before a capture).
 int prepare(DeviceContext *ctx);
-// gpt2_logits_edit_b200 with len_add added to every length; pdl: a programmatic dependent of the kernel before it.
+// gpt2_logits_edit_b200 with len_add added to every length. With len_add and next, a row whose length is below its prompt's is left as it
+// is, next too. pdl: a programmatic dependent of the kernel before it.
 int launch(DeviceContext *ctx, void *out, long long ldo, const void *in, long long ld, int type, int rows, int V, const GPT2LogitsEdit &e, int len_add, int *next,
            bool pdl, cudaStream_t stream);
 

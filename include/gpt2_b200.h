@@ -479,7 +479,7 @@ typedef struct {
 } GPT2W4Weights;
 int gpt2_b200_batch_create_w4(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B);
 
-/* gpt2_b200_batch_generate with every step's logits edited before the choice, in the same graph: sequence b's history is what d_out[b]
+/* gpt2_b200_batch_generate with the logits of every step behind the prompt edited before the choice, in the same graph: sequence b's history is what d_out[b]
  * holds so far, its first d_plen[b] tokens the prompt, so edit's history, length and prompt are NULL; the other arrays have
  * a row per sequence and may be changed between steps by work ordered on the stream. A sequence with nothing left to choose gets -1 in
  * d_out (status bits) and goes on from token 0. The first call of a batch allocates its logits. */
