@@ -689,7 +689,8 @@ class DecodeBatch:
 
     def generate(self, prompt, prompt_len, n_steps: int, out, stream: int = 0, edit: "LogitsEdit | None" = None) -> None:
         """prompt: int32 [B][P]; prompt_len: int32 [B] (1..P); out: int32 [B][>= n_steps+1]. edit: made for B rows of VOCAB
-        logits without a history; every choice is made of the logits so edited, out and prompt_len being the history."""
+        logits without a history; every choice is made of the logits so edited, out and prompt_len being the history. All steps are enqueued
+        here: what the edit's tensors hold is the same for all of them."""
         if edit is not None:
             if edit.rows != self.B or edit.vocab != VOCAB or edit.c.history:
                 raise ValueError("generate: edit is for the batch's rows of VOCAB logits, without a history of its own")

@@ -479,10 +479,12 @@ typedef struct {
 } GPT2W4Weights;
 int gpt2_b200_batch_create_w4(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2W4Weights *q, const GPT2KVCache *kvs, int B);
 
-/* gpt2_b200_batch_generate with the logits of every step behind the prompt edited before the choice, in the same graph: sequence b's history is what d_out[b]
- * holds so far, its first d_plen[b] tokens the prompt, so edit's history, length and prompt are NULL; the other arrays have
- * a row per sequence and may be changed between steps by work ordered on the stream. A sequence with nothing left to choose gets -1 in
- * d_out (status bits) and goes on from token 0. The first call of a batch allocates its logits. */
+/* gpt2_b200_batch_generate with the logits of every step behind the prompt edited before the choice, in the same graph: sequence b's
+ * history is what d_out[b] holds so far, its first d_plen[b] tokens the prompt, so edit's history, length and prompt are NULL; the other
+ * arrays have a row per sequence and are the same for all steps of a call, which enqueues them all: work ordered on the stream may change them
+ * between calls. (A mask that follows the tokens, a grammar's, needs gpt2_b200_batch_step and gpt2_logits_edit_b200 for each.) A sequence with
+ * nothing left to choose gets -1 in d_out (status bits) and goes on from token 0. The first call of a batch allocates its logits. A step
+ * makes one launch more than gpt2_b200_batch_launches_per_step says. */
 int gpt2_b200_batch_generate_edited(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps, int *d_out,
                                     long long out_stride, const GPT2LogitsEdit *edit, cudaStream_t stream);
 
