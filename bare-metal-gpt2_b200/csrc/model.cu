@@ -24,8 +24,8 @@
 // agree to fp32 rounding before the fp16 store.
 #include <algorithm>
 #include <cstdlib>
-#include <cstring>
 #include <new>
+#include <tuple>
 
 #include "common.cuh"
 #include "logits_edit.cuh"
@@ -372,6 +372,15 @@ int check_device(const gpt2_b200_batch *bt) {
     return dev == bt->device ? GPT2_B200_OK : GPT2_B200_EINVAL;
 }
 
+// The same launch. Field by field: the padding between them is the caller's and may hold anything.
+bool same(const GPT2LogitsEdit &a, const GPT2LogitsEdit &b) {
+    const auto fields = [](const GPT2LogitsEdit &e) {
+        return std::tie(e.repetition, e.frequency, e.presence, e.history, e.history_stride, e.max_history, e.length, e.prompt, e.bias_token, e.bias, e.bias_stride,
+                        e.max_bias, e.n_bias, e.mask, e.mask_stride, e.mask_rows, e.mask_row);
+    };
+    return fields(a) == fields(b);
+}
+
 // Lock-step generation with graph gi: 0 greedy, 1 the attention alone, 2 with edited logits.
 int generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, const int *d_plen, int n_steps, int *d_out, long long out_stride, int gi,
              const GPT2LogitsEdit *edit, cudaStream_t stream) {
@@ -401,7 +410,7 @@ int generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, 
     // The graphs bake in the generation buffers; re-capture when they change (all of them: one that is left would run on the old ones).
     if ((bt->graph[0] || bt->graph[1] || bt->graph[2]) &&
         (bt->g_prompt != d_prompt || bt->g_plen != d_plen || bt->g_out != d_out || bt->g_ps != prompt_stride || bt->g_os != out_stride ||
-         (edit && bt->graph[2] && std::memcmp(&bt->g_edit, &e, sizeof(e)) != 0))) {
+         (edit && bt->graph[2] && !same(bt->g_edit, e)))) {
         // earlier replays of these graphs may still be queued: let them finish first
         if (cudaDeviceSynchronize() != cudaSuccess) return GPT2_B200_ECUDA;
         for (cudaGraphExec_t &g : bt->graph)
@@ -415,7 +424,7 @@ int generate(gpt2_b200_batch *bt, const int *d_prompt, long long prompt_stride, 
     bt->g_out = d_out;
     bt->g_ps = prompt_stride;
     bt->g_os = out_stride;
-    if (edit) std::memcpy(&bt->g_edit, &e, sizeof(e));
+    if (edit) bt->g_edit = e;
     if (!bt->graph[gi]) {
         cudaStream_t cs;
         if (cudaStreamCreateWithFlags(&cs, cudaStreamNonBlocking) != cudaSuccess)
