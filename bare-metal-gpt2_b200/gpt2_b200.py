@@ -700,6 +700,7 @@ class DecodeBatch:
                     raise ValueError("generate: prompt is int32 [B][P], out int32 [B][>= n_steps + 1], on the caches' device")
             if out.shape[1] <= n_steps or (edit.device is not None and edit.device != at):
                 raise ValueError("generate: out is too narrow, or the edit is on another device")
+            self.edit = edit  # its tensors are read by steps that run behind this call
             self.lib.check(self.lib.gpt2_b200_batch_generate_edited(
                 self.h, prompt.data_ptr(), _row_stride(prompt), _vector("generate", prompt_len, i32, self.B, at), n_steps, out.data_ptr(),
                 _row_stride(out), edit.ref_c, stream), "gpt2_b200_batch_generate_edited")
