@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     __shared__ uint64_t c_full[CODE_RING], c_empty[CODE_RING], x_full[MAX_X_RING], x_empty[MAX_X_RING], a_full[TILES][A_BUFS], a_empty[TILES][A_BUFS], acc_full[2],
         acc_empty[2], last_full;
     __shared__ uint32_t tmem_slot;
-    __shared__ int bad;  // a wait gave up: nothing more is written
+    __shared__ int bad;  // a wait gave up here, or in a CTA that shares the tile: nothing more is written
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const x_smem = smem + CODE_RING * CODE_BYTES;
     const int x_bytes = p.bpad * 2 * KS;
@@ -683,6 +683,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     }
     __syncwarp();
     if (p.cs > 1) {
+        // A CTA that gave up left no sums, or not all: the others may not add them. The warp that gave up sees its own mark here.
+        if (*reinterpret_cast<volatile int *>(&bad) && lane < p.cs)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dsmem_addr(smem_u32(&bad), static_cast<uint32_t>(lane))), "r"(1) : "memory");
+        __syncwarp();
         // Every CTA of the cluster has `share` of the columns, and adds them over the ranks in their order: 4 features a thread.
         const int f = tid % (FEATURES / 4) * 4, n = first_tile * FEATURES + f, c0 = rank * p.share + tid / (FEATURES / 4);
         const int c1 = min(min(p.d.B - b0, p.bpad), (rank + 1) * p.share);
