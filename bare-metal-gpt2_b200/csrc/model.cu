@@ -167,8 +167,9 @@ int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half
         int rc;
         if (!attention_only) {
             if (bt->w4) {
-                bt->qkv_4[L].d.d_pos = d_pos;
-                rc = w4::launch(bt->qkv_4[L], st);
+                w4::Dest d = bt->qkv_4[L].d;
+                d.d_pos = d_pos;
+                rc = w4::launch(bt->qkv_4[L], d, st);
             } else {
                 lin::Plan p = bt->qkv_p[L];
                 p.p.d_pos = d_pos;
@@ -208,9 +209,10 @@ int enqueue_step(gpt2_b200_batch *bt, const int *d_tok, const int *d_pos, __half
         return GPT2_B200_ECUDA;
     int rc;
     if (bt->w4_head) {
-        bt->head_4.d.out = logits;
-        bt->head_4.d.ldo = logits_stride;
-        rc = w4::launch(bt->head_4, st);
+        w4::Dest d = bt->head_4.d;
+        d.out = logits;
+        d.ldo = logits_stride;
+        rc = w4::launch(bt->head_4, d, st);
     } else {
         lin::Plan hp = bt->head_p;
         hp.p.out = logits;

@@ -107,7 +107,9 @@ struct Plan {
 bool weight_ok(const GPT2W4 *w);  // sizes and pointers
 // resid and ldr: EPI_RESID's. Returns a GPT2_B200_* code; d's fields of EPI_QKV and EPI_HEAD are the caller's to fill in.
 int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int B, const __half *bias, __half *out, long long ldo, const __half *resid, long long ldr);
-int launch(Plan &pl, cudaStream_t stream);
+// d: the plan's own, or it with other pointers. The plan stays as it is.
+int launch(const Plan &pl, const Dest &d, cudaStream_t stream);
+inline int launch(const Plan &pl, cudaStream_t stream) { return launch(pl, pl.d, stream); }
 
 }  // namespace w4
 }  // namespace b200

@@ -927,7 +927,7 @@ int plan(Plan *pl, int epi, const GPT2W4 &w, const __half *x, long long ldx, int
     return pl->few ? plan_rows(ctx, pl, w, x, ldx) : plan_tc(ctx, pl, w, x, ldx);
 }
 
-int launch(Plan &pl, cudaStream_t stream) {
+int launch(const Plan &pl, const Dest &d, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = pl.grid;
     cfg.blockDim = dim3(pl.threads, 1, 1);
@@ -948,10 +948,20 @@ int launch(Plan &pl, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    pl.rows.d = pl.tc.d = pl.d;
-    pl.rows.ahead = pl.pdl;
-    void *few[1] = {&pl.rows}, *many[3] = {&pl.tm_w, &pl.tm_x, &pl.tc};
-    return cudaLaunchKernelExC(&cfg, pl.kernel, pl.few ? few : many) == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
+    cudaError_t err;
+    if (pl.few) {
+        RowParams p = pl.rows;
+        p.d = d;
+        p.ahead = pl.pdl;
+        void *args[1] = {&p};
+        err = cudaLaunchKernelExC(&cfg, pl.kernel, args);
+    } else {
+        TcParams p = pl.tc;
+        p.d = d;
+        void *args[3] = {const_cast<CUtensorMap *>(&pl.tm_w), const_cast<CUtensorMap *>(&pl.tm_x), &p};
+        err = cudaLaunchKernelExC(&cfg, pl.kernel, args);
+    }
+    return err == cudaSuccess ? GPT2_B200_OK : GPT2_B200_ECUDA;
 }
 
 }  // namespace w4

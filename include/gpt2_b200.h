@@ -235,7 +235,8 @@ void gpt2_decode_step_b200(const GPT2Backend *be, const GPT2WeightsGPU *w, GPT2K
 
 /* A batch of B (1..256) sequences decoded together, sequence b over the cache kvs[b] (host array of
  * B caches in the reference layout, all with the GPT-2-124M shape and the same maxT). Holds its own
- * activations, tensor maps and launch plans; the weights and caches stay owned by the caller. */
+ * activations, tensor maps and launch plans; the weights and caches stay owned by the caller. Its calls share the
+ * activations: they come from one host thread at a time, on one stream or on streams ordered behind one another. */
 typedef struct gpt2_b200_batch gpt2_b200_batch;
 int gpt2_b200_batch_create(gpt2_b200_batch **out, const GPT2WeightsGPU *w, const GPT2KVCache *kvs,
                            int B);
