@@ -437,13 +437,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
     constexpr uint32_t tm_a = 0, tm_acc = A_BUFS * TILES * A_COLS;
     grid_launch_dependents();
 
+    bool gave_up = false;  // this warp did (lane 0 knows)
     const auto fail = [&] {
+        gave_up = true;
         if (lane == 0) {
             bad = 1;
             atomicOr(p.d.status, ST_LINEAR_TIMEOUT);
         }
     };
-    if (tid == 0 && tmem_slot != 0) bad = 1;  // cannot be
+    if (tid == 0 && tmem_slot != 0) bad = gave_up = true;  // cannot be
     // Each role counts slots, phases, stages and tiles by hand: one warp's divisions by run-time numbers take longer than a stage.
     if (warp == 0) {
         const bool leader = elect_one();
@@ -681,12 +683,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_w4_tc(const __grid_constant__
         __syncwarp();
         if (p.cs > 1) cluster_wait();
     }
+    // A CTA that gave up left no sums, or not all: the others may not add them. (Kept in a register: every warp's look at `bad` here
+    // takes 0.1 us.)
+    if (__builtin_expect(gave_up, 0) && p.cs > 1 && lane == 0) {
+#pragma unroll 1
+        for (int q = 0; q < p.cs; ++q) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dsmem_addr(smem_u32(&bad), static_cast<uint32_t>(q))), "r"(1) : "memory");
+    }
     __syncwarp();
     if (p.cs > 1) {
-        // A CTA that gave up left no sums, or not all: the others may not add them. The warp that gave up sees its own mark here.
-        if (*reinterpret_cast<volatile int *>(&bad) && lane < p.cs)
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dsmem_addr(smem_u32(&bad), static_cast<uint32_t>(lane))), "r"(1) : "memory");
-        __syncwarp();
         // Every CTA of the cluster has `share` of the columns, and adds them over the ranks in their order: 4 features a thread.
         const int f = tid % (FEATURES / 4) * 4, n = first_tile * FEATURES + f, c0 = rank * p.share + tid / (FEATURES / 4);
         const int c1 = min(min(p.d.B - b0, p.bpad), (rank + 1) * p.share);
