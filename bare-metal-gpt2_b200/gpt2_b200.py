@@ -445,7 +445,8 @@ class W4Weight:
         c.N, c.K, c.group = N, K, group
         self.c, self.ref_c = c, ctypes.byref(c)
         self._at, self._half, self._current = codes.device, torch.float16, _current(torch, codes.device)
-        self._linear = _entry(lib.lib.gpt2_w4_linear_b200, codes.device)
+        self._quantize, self._dequantize, self._linear = (_entry(call, codes.device) for call in (
+            lib.lib.gpt2_w4_quantize_b200, lib.lib.gpt2_w4_dequantize_b200, lib.lib.gpt2_w4_linear_b200))
 
     @classmethod
     def create(cls, lib: "Lib", torch, N: int, K: int, group: int = 64, least: bool = False, device="cuda") -> "W4Weight":
@@ -475,19 +476,18 @@ class W4Weight:
     def _matrix(self, what, w):
         if w.dtype != self._half or w.dim() != 2 or w.shape != (self.N, self.K) or w.stride(1) != 1 or w.device != self._at:
             raise ValueError(f"{what}: expected fp16 [{self.N}][{self.K}] on the weight's device")
-        _on_gpu(what, self._at)
         self._current(what)
         return w.data_ptr(), w.stride(0) if self.N > 1 else self.K
 
     def quantize(self, w, stream: int = 0) -> None:
         """Writes the codes, scales and least values of the fp16 weight w [N][K]."""
         p, ld = self._matrix("quantize", w)
-        self.lib.check(self.lib.gpt2_w4_quantize_b200(self.ref_c, p, ld, stream), "gpt2_w4_quantize_b200")
+        self.lib.check(self._quantize(self.ref_c, p, ld, stream), "gpt2_w4_quantize_b200")
 
     def dequantize(self, w, stream: int = 0) -> None:
         """Writes the fp16 values that the codes stand for to w [N][K]."""
         p, ld = self._matrix("dequantize", w)
-        self.lib.check(self.lib.gpt2_w4_dequantize_b200(p, ld, self.ref_c, stream), "gpt2_w4_dequantize_b200")
+        self.lib.check(self._dequantize(p, ld, self.ref_c, stream), "gpt2_w4_dequantize_b200")
 
     def linear(self, out, x, bias=None, epi: int = LINEAR_STORE, residual=None, stream: int = 0) -> None:
         """out [B][N] = e(x [B][K] W^T + bias [N]), fp16 rows (strided ones are fine); epi LINEAR_RESID adds residual [B][N]
