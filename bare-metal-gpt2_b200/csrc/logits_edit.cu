@@ -10,7 +10,7 @@
 // CTAs shares a row when there are few rows.
 //
 // 256 x 131072 fp32 with 8192 of history, a mask and 300 biases: 89 us (floor 42.7), without any 42.6. The history is looked through by each of a
-// row's 8 CTAs, and its tokens' logits are single reads and writes: 30 us. 64 x 50257 fp16 with 1023 of history and a choice: 11.7 us, most of it
+// row's 8 CTAs, and its tokens' logits are single reads and writes: 30 us. 64 x 50257 fp16 with 1023 of history and a choice: 12.0 us, most of it
 // barriers between short passes.
 //
 // Rows may start anywhere: a row is cut at the 16-byte boundaries of its input; the vectors at its ends are taken element by

@@ -71,8 +71,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 //     stay and take tile after tile: x is there, and the next tile's codes are on their way while a tile's sums are put together.
 //   - One CTA per SM: each has all of x, and x costs the L2 0.3 us per MB beside the codes. (Two of 8 warps: 4096 x 4096 at B = 8 13.6 us
 //     against 9.6, 8192 x 2048 10.9 against 8.5.) L1 holds the loads in flight: less of it for more shared memory is 10% slower.
-// 1 x 8192 x 8192 with least 15.3 us (2.3 TB/s), 8 x 50257 x 768 13.0 us: 5 us of launch and first bytes, then the conversions of 4 warps
-// per scheduler (IPC 1.7, issue slots 45 to 52%). 1 x 131072 x 4096 73 us (3.9 TB/s).
+// 1 x 8192 x 8192 with least 15.2 us (2.4 TB/s), 8 x 50257 x 768 13.0 us: 5 us of launch and first bytes, then 4 warps per scheduler
+// that wait for loads and for their own conversions (IPC 1.65 and 1.80 of 4: 41 and 45% of the issue slots). 1 x 131072 x 4096 73 us (3.9 TB/s).
 constexpr int CHUNK = 128;
 constexpr int DEPTH = 4;
 constexpr int ROWS_MAX_B = 16;
@@ -278,8 +278,9 @@ __global__ void __launch_bounds__(W * 32, 1) k_w4_rows(const RowParams p) {
 // A hand-over through an mbarrier costs each role 200 to 400 cycles, and HBM delivers the codes of a stage in 700: so a stage is 32768
 // codes and each role passes one barrier per stage. Two tiles of features per x halve what x costs the L2: at 128 rows of x, 16 KB
 // of codes come with 32 KB of x (one tile of 128 x 256: 8 with 64, 10 TB/s from the L2 and no more).
-// 64 x 8192 x 8192 20.1 us (bytes 5.8), bound by the conversion; 256 x 16384 x 8192 61.9 us, 1111 TFLOP/s of the 1680 measured for cuBLAS, by the
-// MMAs and their hand-overs.
+// 64 x 8192 x 8192 20.0 us (bytes 5.8): 16 stages of 1250 cycles, of which the conversion needs 610 to 800 and the hand-overs the rest, and
+// 10 us of launch, start and the cluster's sums; 256 x 16384 x 8192 61 us, 1125 TFLOP/s of the 1680 measured for cuBLAS, by the MMAs and
+// their hand-overs.
 // A few features and a long k: the CTAs of a cluster share a tile's k and add their sums through distributed shared memory, in rank order.
 constexpr int BM = 128;                      // features of an MMA, one TMEM lane each
 constexpr int TILES = 2;                     // MMAs side by side
@@ -865,8 +866,10 @@ int plan_tc(DeviceContext *ctx, Plan *pl, const GPT2W4 &w, const __half *x, long
     p.shift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.stages = (w.K + KS - 1) / KS;
     p.tiles = (w.N + FEATURES - 1) / FEATURES;
-    // Column blocks and CTAs per tile, by the cycles that they are seen to take: 3300 to the first codes, 1000 a stage (or the MMAs, 8 a
-    // column), 2000 and 90 a column for the sums of a cluster, 40 a column for a tile's outputs without one. Blocks read the weights
+    // Column blocks and CTAs per tile, by the cycles that they take in a model that is near enough to choose by: 3300 to the first codes, 1000
+    // a stage (or the MMAs, 8 a column), 2000 and 90 a column for the sums of a cluster, 40 a column for a tile's outputs without one. (Seen
+    // at 64 columns and 1965 MHz: 1250 a stage, and a cluster's sums take 4600 to 4800 longer than outputs without, 8192 x 8192 against
+    // 32768 x 2048.) Blocks read the weights
     // again, from the L2, and convert them again, on SMs that have nothing else to do: with a few features and a short k that is
     // cheaper than adding wide sums (64 x 2304 x 768).
     int blocks = 0;
