@@ -665,6 +665,8 @@ class DecodeBatch:
     """
 
     def __init__(self, lib: "Lib", weights: ModelWeights, caches, w4: "W4ModelWeights | None" = None):
+        if w4 is not None and any(q.codes.device != caches.device for q in [*(q for layer in w4.layers for q in layer.values()), w4.head] if q is not None):
+            raise ValueError(f"DecodeBatch: the 4-bit weights are on another device than the caches, {caches.device}")
         self.lib, self.weights, self.caches, self.w4 = lib, weights, caches, w4
         self.B, max_t = int(caches.shape[0]), int(caches.shape[4])
         self.kvs = (GPT2KVCache * self.B)(*[cache_view(caches[b].data_ptr(), N_LAYER, max_t)
